@@ -20,7 +20,7 @@ ERRORS = {
     -5: "API version mismatch",
     -6: "device status error",
 }
-LB_F32, LB_BF16, LB_I8, LB_F16 = 0, 1, 2, 3
+LB_F32, LB_BF16, LB_I8, LB_F16, LB_E4M3 = 0, 1, 2, 3, 4
 LB_INPUT_PCM, LB_INPUT_MEL = 0, 1
 REASONS = ("continue", "reset", "gap_or_cursor_mismatch", "identity_reset")
 
@@ -31,6 +31,9 @@ DEV_BAD_HANDLE = 1 << 3
 DEV_STALE_COMMIT = 1 << 4
 DEV_BAD_ROW_COUNT = 1 << 5
 DEV_INGRESS_OVERFLOW = 1 << 6
+DEV_PAGES_EXHAUSTED = 1 << 7
+DEV_BAD_PAGE = 1 << 8
+DEV_NONFINITE = 1 << 9
 INGRESS_JOIN, INGRESS_LEAVE, INGRESS_PAUSE, INGRESS_RESUME = 0, 1, 2, 3
 
 
@@ -75,6 +78,7 @@ class LbCounters(ctypes.Structure):
 P = ctypes.c_void_p
 I = ctypes.c_int
 I64 = ctypes.c_int64
+F = ctypes.c_float
 
 # name -> (restype, argtypes); every symbol include/listener_b200.h declares
 SIGNATURES: dict[str, tuple] = {
@@ -117,6 +121,13 @@ SIGNATURES: dict[str, tuple] = {
     "lb_op_gemm_splitk_scratch": (I, [P, I, I, P, I, P, P, I, I, P, I, I, I, P, P]),
     "lb_snapshot_ready_rows": (I, [I, P, P, P, P, P, P, P, I64, P, P, P, P, P]),
     "lb_order_ready_heads": (I, [I, P, P, P, I64, I64, I, P, P, P, P]),
+    "lb_plan_pages": (I, [I, P, P, I, I, I, I, P, P, P, I, P, P, P, P, P, P, P, P]),
+    "lb_commit_pages": (I, [I, P, I, I, I, I, P, P, P, P, P, P, P]),
+    "lb_release_pages": (I, [I, P, I, I, I, I, P, P, P, P, P]),
+    "lb_op_kv8_append": (I, [P, I64, I64, P, I64, I64, I, I, I, I, P, P, P, P, P, I, I, P, P]),
+    "lb_op_kv8_attention": (I, [P, I64, I64, I, I, I, I, I, I, P, P, P, P, I, I, P, I, P, P, F, I, F, P, P, P, P]),
+    "lb_op_rms_norm8": (I, [P, I64, P, I64, I, P, I, I, I, F, I, I, P, P, P, P]),
+    "lb_op_w4_matvec": (I, [P, I64, I, P, I, I, P, P, I, I, I, P, I64, I, P]),
 }
 
 

@@ -48,7 +48,10 @@ enum lb_device_status_bits {
   LB_DEV_BAD_HANDLE = 1 << 3,
   LB_DEV_STALE_COMMIT = 1 << 4,
   LB_DEV_BAD_ROW_COUNT = 1 << 5,
-  LB_DEV_INGRESS_OVERFLOW = 1 << 6 /* a frame found its session's ingress ring full (refused) */
+  LB_DEV_INGRESS_OVERFLOW = 1 << 6, /* a frame found its session's ingress ring full (refused) */
+  LB_DEV_PAGES_EXHAUSTED = 1 << 7,  /* a page plan asks for more pages than are free, or a row for more than its table holds */
+  LB_DEV_BAD_PAGE = 1 << 8,         /* a page or slot outside the cache (skipped) */
+  LB_DEV_NONFINITE = 1 << 9         /* a key or value that was written is infinite or NaN */
 };
 
 /* Session events of the GPU ingress (lb_ingress_events_async). */
@@ -59,8 +62,9 @@ enum lb_ingress_event {
   LB_INGRESS_RESUME = 3
 };
 
-/* Tensor element types for lb_set_tensor. */
-enum lb_dtype { LB_F32 = 0, LB_BF16 = 1, LB_I8 = 2, LB_F16 = 3 };
+/* Tensor element types (lb_set_tensor takes the first four; LB_E4M3 is an
+ * 8-bit activation of the text-decoder operators). */
+enum lb_dtype { LB_F32 = 0, LB_BF16 = 1, LB_I8 = 2, LB_F16 = 3, LB_E4M3 = 4 };
 
 /* Weight formats of the dense contractions. */
 enum lb_weight_format {
@@ -405,6 +409,101 @@ int lb_op_gemm_splitk_scratch(const void* x, int x_ld, int m, const void* w, int
                               const void* w_scale, const float* bias, int out_features, int k,
                               void* out, int ld_out, int act, int splits, int* status_dev,
                               void* stream);
+
+/* ----------------------------------------------------------------------
+ * Text-decoder operators: what a decoder block needs to consume the soft
+ * tokens.  The reference's decoder keeps a private K/V cache per session
+ * (native/gemma4_listener/gemma4_listener_cache.cu:34-42) in 16 bits; here the
+ * caches of all sessions share one pool of pages of 8-bit codes.  Device
+ * pointers; asynchronous on `stream`; nothing is allocated; capturable.
+ * ---------------------------------------------------------------------- */
+
+/* Plans the pages of one step on the GPU: block tables, token positions and
+ * cache slots from the request lengths.  Row i adds new_tokens[i] >= 0 tokens to
+ * session sessions[i] of a directory of n_sessions: tables int32
+ * [n_sessions][max_pages] (page ids), lengths int32 [n_sessions] (tokens held) and
+ * used, one bit per page (int32 words, page p is bit p & 31 of word p >> 5).  The
+ * k-th page that the rows need, in row order, is the k-th lowest free page.
+ * The directory is only read; lb_commit_pages installs the plan.  Outputs, all
+ * written whole: row_tables int32 [n][max_pages] (-1 past a row's last page),
+ * kv_len int32 [n] (lengths after the step), cu_tokens int32 [n+1], and for the
+ * tokens of the rows in order slots int64 (page * page_tokens + offset),
+ * positions int32 and token_rows int32 [max_tokens] (-1 past the last token).
+ * *status: 0, or LB_DEV_* bits of a refused plan (a session twice or out of
+ * range, a negative count, more tokens than max_tokens, no page left); a
+ * refused plan has no tokens (kv_len 0, tables and slots -1) and is not committed.
+ * n <= 8192, n_sessions <= 262144, max_tokens <= 2^26, page_tokens a multiple of 16
+ * up to 256. */
+int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int n_sessions, int max_pages,
+                  int n_pages, int page_tokens, const int32_t* tables, const int32_t* lengths,
+                  const int32_t* used, int max_tokens, int32_t* row_tables, int32_t* kv_len,
+                  int32_t* cu_tokens, int64_t* slots, int32_t* positions, int32_t* token_rows,
+                  int32_t* status, void* stream);
+/* Installs a plan whose *status is 0: the rows' new pages, lengths and used bits. */
+int lb_commit_pages(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,
+                    const int32_t* row_tables, const int32_t* kv_len, const int32_t* status, int32_t* tables,
+                    int32_t* lengths, int32_t* used, void* stream);
+/* Gives the pages of n distinct sessions back; a session out of range sets
+ * LB_DEV_BAD_HANDLE in *status and is skipped. */
+int lb_release_pages(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,
+                     int32_t* tables, int32_t* lengths, int32_t* used, int32_t* status, void* stream);
+
+/* Writes n_tokens keys and values into the 8-bit cache: k_codes / v_codes int8
+ * [n_pages][kv_heads][page_tokens][dim], k_scale / v_scale f32 [n_pages][kv_heads]
+ * (value = code * scale).  slots int64 [n_tokens] as lb_plan_pages writes them
+ * (negative: skipped); the tokens of one page follow one another, in order.  A
+ * page's scale is the running max |x| / 127 over its tokens: where new tokens
+ * raise it, the codes before them are rounded again to the new scale; a token at
+ * offset 0 begins the page afresh.  k, v: [n_tokens][kv_heads][dim] of dtype (LB_F32,
+ * LB_BF16, LB_F16), strides in elements, the last dimension contiguous.  Infinite
+ * values take the code +-127 and NaN the code 0, neither counts for the scale, and
+ * LB_DEV_NONFINITE is OR-ed into *status (may be NULL), as is LB_DEV_BAD_PAGE for a
+ * slot past the cache (skipped).  dim a multiple of 16, at most 512; page_tokens a
+ * multiple of 16, at most 256; codes 16-byte aligned. */
+int lb_op_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                     int64_t v_token_stride, int64_t v_head_stride, int dtype, int n_tokens, int kv_heads, int dim,
+                     const int64_t* slots, int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale,
+                     int n_pages, int page_tokens, int32_t* status, void* stream);
+
+/* Attention of the step's tokens over that cache.  Row r holds the tokens
+ * [cu_tokens[r], cu_tokens[r+1]), the last of the kv_len[r] tokens of its session:
+ * token i is at position kv_len - new + i and sees the keys j <= position, with
+ * window > 0 only those with j > position - window.  q [n_tokens][heads][dim]
+ * (LB_BF16 or LB_F16, strides in elements), heads a multiple of kv_heads; scores
+ * are scale * q.k, with softcap > 0 softcap * tanh(score / softcap).  out
+ * [n_tokens][heads][dim] of q's type, contiguous; lse f32 [n_tokens][heads] (natural
+ * log-sum-exp) or NULL.  A token that sees no key, and one in no row, has out 0 and
+ * lse -inf.  dim 64, 128 or 256; page_tokens a multiple of 16, at most 256.  A page id
+ * out of range counts as unseen keys and sets LB_DEV_BAD_PAGE in *status (may be NULL). */
+int lb_op_kv8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_dtype, int n_tokens,
+                        int n_rows, int heads, int kv_heads, int dim, const int8_t* k_codes,
+                        const int8_t* v_codes, const float* k_scale, const float* v_scale, int n_pages,
+                        int page_tokens, const int32_t* row_tables, int max_pages, const int32_t* kv_len,
+                        const int32_t* cu_tokens, float scale, int window, float softcap, void* out, float* lse,
+                        int32_t* status, void* stream);
+
+/* h = x + residual; y = h * rsqrt(mean(h^2) + eps) * weight, written as 8-bit codes
+ * (out_dtype LB_E4M3: top 448, LB_I8: top 127) with scales max |y| / top for each
+ * row (group 0) or each `group` columns.  x, residual and hidden of dtype (LB_F32,
+ * LB_BF16, LB_F16), x_ld / residual_ld elements between rows; weight LB_F32 or
+ * dtype; residual may be NULL (h = x), hidden may be NULL (h is not stored), else
+ * [rows][dim].  codes [rows][dim]; scales f32 [rows][dim / group].  A group whose y is
+ * all zero has scale 0 and codes 0; one that holds a NaN has scale NaN and codes 0.
+ * dim <= 16384. */
+int lb_op_rms_norm8(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int dtype,
+                    const void* weight, int weight_dtype, int rows, int dim, float eps, int group, int out_dtype,
+                    void* codes, float* scales, void* hidden, void* stream);
+
+/* out[m][o] = sum_k x[m][k] * (n[o][k] - 8) * w_scale[o][k / group] with 4-bit codes n:
+ * codes uint8 [out_features][k / 2], the low four bits are the even k; w_scale f16
+ * [out_features][k / group], group 32, 64 or 128, k a multiple of it.  x [m][k] of
+ * x_dtype (LB_BF16, LB_F16, or LB_E4M3 / LB_I8 with x_scale f32 [m][k / x_group];
+ * x_group 0: one scale a row, else a multiple of 128), x_ld elements between rows;
+ * out of out_dtype (LB_F32, LB_BF16, LB_F16), ld_out elements between rows.  codes
+ * 16-byte aligned. */
+int lb_op_w4_matvec(const void* x, int64_t x_ld, int x_dtype, const float* x_scale, int x_group, int m,
+                    const void* codes, const void* w_scale, int group, int out_features, int k, void* out,
+                    int64_t ld_out, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }
