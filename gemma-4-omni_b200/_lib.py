@@ -125,8 +125,8 @@ SIGNATURES: dict[str, tuple] = {
     "lb_commit_pages": (I, [I, P, I, I, I, I, P, P, P, P, P, P, P]),
     "lb_release_pages": (I, [I, P, I, I, I, I, P, P, P, P, P]),
     "lb_op_kv8_append": (I, [P, I64, I64, P, I64, I64, I, I, I, I, P, P, P, P, P, I, I, P, P]),
-    "lb_op_kv8_attention": (I, [P, I64, I64, I, I, I, I, I, I, P, P, P, P, I, I, P, I, P, P, F, I, F, P, P, P, P, P]),
-    "lb_kv8_attention_workspace": (I64, [I]),
+    "lb_op_kv8_attention": (I, [P, I64, I64, I, I, I, I, I, I, P, P, P, P, I, I, P, I, P, P, I, F, I, F, P, P, P, P, P]),
+    "lb_kv8_attention_workspace": (I64, [I, I, I, I]),
     "lb_op_rms_norm8": (I, [P, I64, P, I64, I, P, I, I, I, F, I, I, P, P, P, P]),
     "lb_op_w4_matvec": (I, [P, I64, I, P, I, I, P, P, I, I, I, P, I64, I, P]),
 }

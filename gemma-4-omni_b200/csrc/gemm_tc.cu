@@ -615,6 +615,21 @@ int make_tensor_map_2d(CUtensorMap* map, const void* base, int elem_bytes, uint6
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
+int make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t span,
+                       uint32_t box_outer) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return -1;
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {inner};
+  cuuint32_t box[2] = {span, box_outer};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   span == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
 int gemm_token_tile(int O, int m_cap, int num_sms) {
   if (m_cap <= 32) return 32;
   if (m_cap <= 64) return 64;

@@ -55,6 +55,10 @@ struct GemmPlan {
 int make_tensor_map_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t inner,
                        uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner,
                        uint32_t box_outer, bool swizzle128, bool f16 = false);
+// Contiguous 8-bit rows [outer][inner], read in boxes of box_outer rows of `span`
+// (128 or 64) bytes, swizzled over that span.
+int make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t span,
+                       uint32_t box_outer);
 // Token tile (UMMA N) for an [m_cap x O] output: 32/64/128/256 up to 256
 // tokens, beyond that the multiple of 16 in [128, 256] that fills whole waves.
 int gemm_token_tile(int O, int m_cap, int num_sms);

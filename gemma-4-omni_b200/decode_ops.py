@@ -246,10 +246,10 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, row_tables: torch.Tensor, kv
     lse = torch.empty((t, heads), dtype=torch.float32, device=dev) if return_lse else None
     if t:
         kc, vc, ks, vs = cache._where
-        space = torch.empty(_lib.load().lb_kv8_attention_workspace(dim), dtype=torch.uint8, device=dev)
+        space = torch.empty(_lib.load().lb_kv8_attention_workspace(dim, heads, cache.kv_heads, max_new), dtype=torch.uint8, device=dev)
         _call(dev, "lb_op_kv8_attention", q.data_ptr(), q.stride(0), q.stride(1), DTYPE_CODES[q.dtype], t, n, heads,
               cache.kv_heads, dim, kc, vc, ks, vs, cache.pages, cache.page_tokens, row_tables.data_ptr(), max_pages,
-              kv_len.data_ptr(), cu_tokens.data_ptr(), dim ** -0.5 if scale is None else scale, window, softcap,
+              kv_len.data_ptr(), cu_tokens.data_ptr(), max_new, dim ** -0.5 if scale is None else scale, window, softcap,
               out.data_ptr(), lse.data_ptr() if return_lse else None, cache.status_word.data_ptr(),
               space.data_ptr())
     return (out, lse) if return_lse else out

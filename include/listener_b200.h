@@ -475,16 +475,17 @@ int lb_op_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_strid
  * log-sum-exp) or NULL.  A token that sees no key, and one in no row, has out 0 and
  * lse -inf.  dim 64, 128 or 256; page_tokens a multiple of 16, at most 256.  A page id
  * out of range counts as unseen keys and sets LB_DEV_BAD_PAGE in *status (may be NULL).
- * workspace: lb_kv8_attention_workspace(dim) bytes. */
+ * max_new: the most tokens of a row, on which the split of the work goes (rows with
+ * more are right, but slower).  workspace: lb_kv8_attention_workspace bytes. */
 int lb_op_kv8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_dtype, int n_tokens,
                         int n_rows, int heads, int kv_heads, int dim, const int8_t* k_codes,
                         const int8_t* v_codes, const float* k_scale, const float* v_scale, int n_pages,
                         int page_tokens, const int32_t* row_tables, int max_pages, const int32_t* kv_len,
-                        const int32_t* cu_tokens, float scale, int window, float softcap, void* out, float* lse,
-                        int32_t* status, void* workspace, void* stream);
+                        const int32_t* cu_tokens, int max_new, float scale, int window, float softcap, void* out,
+                        float* lse, int32_t* status, void* workspace, void* stream);
 /* Bytes of the attention's workspace (16-byte aligned, contents of no account; calls
  * that overlap on the GPU need one each), or LB_ERR_INVALID_ARGUMENT. */
-int64_t lb_kv8_attention_workspace(int dim);
+int64_t lb_kv8_attention_workspace(int dim, int heads, int kv_heads, int max_new);
 
 /* h = x + residual; y = h * rsqrt(mean(h^2) + eps) * weight, written as 8-bit codes
  * (out_dtype LB_E4M3: top 448, LB_I8: top 127) with scales max |y| / top for each

@@ -36,11 +36,12 @@ def test_append_entry(lib):
 
 
 def test_attention_entry(lib):
-    good = [P, 64, 64, 1, 1, 1, 4, 2, 64, P, P, P, P, 4, 16, P, 2, P, P, 0.1, 0, 0.0, P, None, None, P, None]
+    good = [P, 64, 64, 1, 1, 1, 4, 2, 64, P, P, P, P, 4, 16, P, 2, P, P, 1, 0.1, 0, 0.0, P, None, None, P, None]
     refused(lib, "lb_op_kv8_attention", good, [(0, None), (3, 0), (3, 2), (4, 0), (5, 0), (7, 3), (8, 96), (9, P + 4), (13, 0),
-                                               (14, 8), (15, None), (16, 0), (20, -1), (21, -1.0), (21, float("nan")),
-                                               (22, None), (25, None), (25, P + 4)])
-    assert lib.lb_kv8_attention_workspace(96) == -1 and lib.lb_kv8_attention_workspace(128) > 0
+                                               (14, 8), (15, None), (16, 0), (19, 0), (21, -1), (22, -1.0),
+                                               (22, float("nan")), (23, None), (26, None), (26, P + 4)])
+    assert lib.lb_kv8_attention_workspace(96, 4, 2, 1) == -1 and lib.lb_kv8_attention_workspace(64, 3, 2, 1) == -1
+    assert 0 < lib.lb_kv8_attention_workspace(128, 4, 2, 1) < lib.lb_kv8_attention_workspace(128, 4, 2, 100)
 
 
 def test_norm_entry(lib):
