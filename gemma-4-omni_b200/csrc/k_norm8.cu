@@ -3,7 +3,13 @@
 //   h = x + r;  y = h * rsqrt(mean(h^2) + eps) * w;  s_g = max_g |y| / top;
 //   code = round(y / s_g)  (top 448 for e4m3, 127 for int8; g a row or `group` columns)
 //
-// A CTA a row; the row's h stays in shared memory between its three uses.
+// The bytes bound it: 7 an element in 16 bits (x, r, the stored h, the code).  So a row is
+// read once and stays in registers between its three uses, T threads a row with
+// C pieces of 8 columns each: with many rows a warp a row (T = 32 up to 2048 columns: 16
+// loads of 16 bytes in flight a lane and no block barrier), with few rows as many
+// threads as there are pieces, since then the latency of one row is all there is.  Rows that
+// are not 16-byte aligned, odd widths and groups that are no power of two of pieces take the
+// plain kernel at the end.
 #include <cuda_fp8.h>
 
 #include "../../include/listener_b200.h"
@@ -12,7 +18,15 @@
 namespace lb {
 namespace {
 
-constexpr int kThreads = 256;
+struct NormArgs {
+  const void *x, *res, *w;
+  long long x_ld, r_ld;
+  int dtype, w_f32, rows, dim, group, e4m3;
+  float eps;
+  uint8_t* codes;
+  float* scales;
+  void* hidden;
+};
 
 __device__ __forceinline__ float load_as_float(const void* p, int dtype, long long i) {
   if (dtype == LB_F32) return static_cast<const float*>(p)[i];
@@ -25,6 +39,42 @@ __device__ __forceinline__ void store_from_float(void* p, int dtype, long long i
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// 8 columns
+template <typename T>
+struct Piece {
+  uint4 raw[sizeof(T) == 4 ? 2 : 1];
+};
+template <typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T* p) {
+  Piece<T> v;
+  v.raw[0] = reinterpret_cast<const uint4*>(p)[0];
+  if constexpr (sizeof(T) == 4) v.raw[1] = reinterpret_cast<const uint4*>(p)[1];
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Piece<T>& v, float (&f)[8]) {
+  const T* e = reinterpret_cast<const T*>(v.raw);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (__is_same(T, float)) f[i] = e[i];
+    else if constexpr (__is_same(T, __half)) f[i] = __half2float(e[i]);
+    else f[i] = __bfloat162float(e[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T* p, const float (&f)[8]) {
+  Piece<T> v;
+  T* e = reinterpret_cast<T*>(v.raw);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (__is_same(T, float)) e[i] = f[i];
+    else if constexpr (__is_same(T, __half)) e[i] = __float2half_rn(f[i]);
+    else e[i] = __float2bfloat16_rn(f[i]);
+  }
+  reinterpret_cast<uint4*>(p)[0] = v.raw[0];
+  if constexpr (sizeof(T) == 4) reinterpret_cast<uint4*>(p)[1] = v.raw[1];
+}
+
 // max that keeps a NaN of either side
 __device__ __forceinline__ float max_nan(float a, float b) { return (a > b || isnan(a)) ? a : b; }
 
@@ -34,19 +84,141 @@ __device__ __forceinline__ float warp_max_nan(float v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kThreads) rms_norm8_kernel(const void* x, long long x_ld, const void* res,
-                                                             long long r_ld, int dtype, const void* w, int w_dtype,
-                                                             int dim, float eps, int group, int e4m3, uint8_t* codes,
-                                                             float* scales, void* hidden) {
+__device__ __forceinline__ uint8_t code_of(float q, bool e4m3) {
+  if (e4m3) return __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
+  return static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(fminf(fmaxf(q, -127.0f), 127.0f))));
+}
+
+// The codes of 8 columns.  One multiplication by the inverse (its rounding moves a code only where
+// y / s is within 2^-22 of halfway), a division where the inverse is not finite.
+__device__ __forceinline__ uint2 codes_of(const float (&y)[8], float s, bool e4m3) {
+  uint32_t w[2] = {0, 0};
+  if (!(s > 0.0f)) return make_uint2(0, 0);  // all zero, or a NaN: the scale says so
+  const float inv = 1.0f / s;
+  const bool divide = !(inv < INFINITY);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float a = divide ? y[i] / s : y[i] * inv, b = divide ? y[i + 1] / s : y[i + 1] * inv;
+    uint32_t pair;
+    if (e4m3) pair = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    else pair = code_of(a, false) | static_cast<uint32_t>(code_of(b, false)) << 8;
+    w[i / 4] |= pair << (8 * (i & 3));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+template <typename T, int kT, int C>
+__global__ void __launch_bounds__(kT < 256 ? 256 : kT) norm_rows_kernel(const NormArgs a) {
+  constexpr int kBlock = kT < 256 ? 256 : kT, kRowsBlock = kBlock / kT, kWarpsRow = kT / 32;
+  __shared__ float part[kBlock / 32];
+  const int in_row = threadIdx.x % kT, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = static_cast<long long>(blockIdx.x) * kRowsBlock + threadIdx.x / kT;
+  const bool live = row < a.rows;
+  const int pieces = a.dim / 8;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+  const T* res = static_cast<const T*>(a.res) + row * a.r_ld;
+  float h[C][8];
+  Piece<T> px[C], pr[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int i = in_row + c * kT;
+    if (live && i < pieces) {
+      px[c] = load_piece<T>(x + i * 8);
+      if (a.res) pr[c] = load_piece<T>(res + i * 8);
+    }
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int i = in_row + c * kT;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[c][e] = 0.0f;
+    if (live && i < pieces) {
+      widen<T>(px[c], h[c]);
+      if (a.res) {
+        float r[8];
+        widen<T>(pr[c], r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[c][e] += r[e];
+      }
+      if (a.hidden) store_piece<T>(static_cast<T*>(a.hidden) + row * a.dim + i * 8, h[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(h[c][e], h[c][e], sum);
+    }
+  }
+  sum = warp_sum(sum);
+  if constexpr (kWarpsRow > 1) {
+    if (lane == 0) part[warp] = sum;
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWarpsRow; ++k) sum += part[warp / kWarpsRow * kWarpsRow + k];
+  }
+  const float r = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+  const float top = a.e4m3 ? 448.0f : 127.0f;
+  float m[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int i = in_row + c * kT;
+    m[c] = 0.0f;
+    if (live && i < pieces) {
+      float w[8];
+      if (a.w_f32) widen<float>(load_piece<float>(static_cast<const float*>(a.w) + i * 8), w);
+      else widen<T>(load_piece<T>(static_cast<const T*>(a.w) + i * 8), w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[c][e] = h[c][e] * r * w[e];
+        m[c] = max_nan(m[c], fabsf(h[c][e]));
+      }
+    }
+  }
+  if (a.group) {
+    // a group's pieces are neighbouring lanes
+    const int width = a.group / 8;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      for (int o = 1; o < width; o <<= 1) m[c] = max_nan(m[c], __shfl_xor_sync(0xffffffffu, m[c], o));
+      const int i = in_row + c * kT;
+      if (live && i < pieces) {
+        const float s = m[c] / top;
+        if ((i & (width - 1)) == 0) a.scales[row * (pieces / width) + i / width] = s;
+        *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], s, a.e4m3);
+      }
+    }
+    return;
+  }
+  float most = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) most = max_nan(most, m[c]);
+  most = warp_max_nan(most);
+  if constexpr (kWarpsRow > 1) {
+    __syncthreads();  // the sums have been read
+    if (lane == 0) part[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kWarpsRow; ++k) most = max_nan(most, part[warp / kWarpsRow * kWarpsRow + k]);
+  }
+  const float s = most / top;
+  if (live && in_row == 0) a.scales[row] = s;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int i = in_row + c * kT;
+    if (live && i < pieces) *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], s, a.e4m3);
+  }
+}
+
+// Any width, alignment and group: a CTA a row, the row in shared memory.
+constexpr int kThreads = 256;
+__global__ void __launch_bounds__(kThreads) norm_any_kernel(const NormArgs a) {
   extern __shared__ float row_smem[];
   __shared__ float part[kThreads / 32];
   const long long row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = a.dim;
   float sum = 0.0f;
   for (int i = tid; i < dim; i += kThreads) {
-    float h = load_as_float(x, dtype, row * x_ld + i);
-    if (res) h += load_as_float(res, dtype, row * r_ld + i);
-    if (hidden) store_from_float(hidden, dtype, row * dim + i, h);
+    float h = load_as_float(a.x, a.dtype, row * a.x_ld + i);
+    if (a.res) h += load_as_float(a.res, a.dtype, row * a.r_ld + i);
+    if (a.hidden) store_from_float(a.hidden, a.dtype, row * dim + i, h);
     row_smem[i] = h;
     sum = fmaf(h, h, sum);
   }
@@ -55,25 +227,41 @@ __global__ void __launch_bounds__(kThreads) rms_norm8_kernel(const void* x, long
   __syncthreads();
   sum = 0.0f;
   for (int i = 0; i < kThreads / 32; ++i) sum += part[i];
-  const float r = rsqrtf(sum / static_cast<float>(dim) + eps);
-  for (int i = tid; i < dim; i += kThreads) row_smem[i] = row_smem[i] * r * load_as_float(w, w_dtype, i);
+  const float r = rsqrtf(sum / static_cast<float>(dim) + a.eps);
+  for (int i = tid; i < dim; i += kThreads) row_smem[i] = row_smem[i] * r * load_as_float(a.w, a.w_f32 ? LB_F32 : a.dtype, i);
   __syncthreads();
-  const int width = group ? group : dim, n_groups = dim / width;
-  const float top = e4m3 ? 448.0f : 127.0f;
-  for (int g = group ? warp : 0; g < n_groups; g += group ? kThreads / 32 : 1) {
+  const int width = a.group ? a.group : dim, n_groups = dim / width;
+  const float top = a.e4m3 ? 448.0f : 127.0f;
+  for (int g = a.group ? warp : 0; g < n_groups; g += a.group ? kThreads / 32 : 1) {
     // a warp a group; for one scale a row every warp finds the row's maximum
     float m = 0.0f;
     for (int i = lane; i < width; i += 32) m = max_nan(m, fabsf(row_smem[g * width + i]));
     const float s = warp_max_nan(m) / top;
-    if (lane == 0 && (group || warp == 0)) scales[row * n_groups + g] = s;
-    for (int i = group ? lane : tid; i < width; i += group ? 32 : kThreads) {
-      const float q = s > 0.0f ? row_smem[g * width + i] / s : 0.0f;
-      uint8_t c;
-      if (e4m3) c = __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-      else c = static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(fminf(fmaxf(q, -127.0f), 127.0f))));
-      codes[row * dim + g * width + i] = c;
-    }
+    if (lane == 0 && (a.group || warp == 0)) a.scales[row * n_groups + g] = s;
+    for (int i = a.group ? lane : tid; i < width; i += a.group ? 32 : kThreads)
+      a.codes[row * dim + g * width + i] = s > 0.0f ? code_of(row_smem[g * width + i] / s, a.e4m3) : uint8_t(0);
   }
+}
+
+template <typename T, int kT, int C>
+cudaError_t launch(const NormArgs& a, cudaStream_t s) {
+  constexpr int kBlock = kT < 256 ? 256 : kT, kRowsBlock = kBlock / kT;
+  norm_rows_kernel<T, kT, C><<<(a.rows + kRowsBlock - 1) / kRowsBlock, kBlock, 0, s>>>(a);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch(const NormArgs& a, cudaStream_t s) {
+  const int pieces = a.dim / 8;
+  if (a.rows < 148 * 8) {  // fewer than a warp a row would fill the SMs with: a piece a thread
+    if (pieces <= 256) return launch<T, 256, 1>(a, s);
+    return pieces <= 1024 ? launch<T, 1024, 1>(a, s) : launch<T, 1024, 2>(a, s);
+  }
+  if (pieces <= 32) return launch<T, 32, 1>(a, s);
+  if (pieces <= 64) return launch<T, 32, 2>(a, s);
+  if (pieces <= 128) return launch<T, 32, 4>(a, s);
+  if (pieces <= 256) return launch<T, 32, 8>(a, s);
+  if (pieces <= 512) return launch<T, 128, 4>(a, s);
+  return pieces <= 1024 ? launch<T, 256, 4>(a, s) : launch<T, 512, 4>(a, s);
 }
 
 }  // namespace
@@ -89,12 +277,27 @@ extern "C" int lb_op_rms_norm8(const void* x, int64_t x_ld, const void* residual
   if ((dtype != LB_F32 && dtype != LB_BF16 && dtype != LB_F16) || (weight_dtype != LB_F32 && weight_dtype != dtype) ||
       (out_dtype != LB_E4M3 && out_dtype != LB_I8))
     return LB_ERR_INVALID_ARGUMENT;
-  const size_t smem = sizeof(float) * dim;
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(rms_norm8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               16384 * static_cast<int>(sizeof(float))) != cudaSuccess)
-    return LB_ERR_CUDA;
-  rms_norm8_kernel<<<rows, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
-      x, x_ld, residual, residual_ld, dtype, weight, weight_dtype, dim, eps, group, out_dtype == LB_E4M3,
-      static_cast<uint8_t*>(codes), scales, hidden);
-  return cudaGetLastError() == cudaSuccess ? LB_OK : LB_ERR_CUDA;
+  const NormArgs a{x, residual, weight, x_ld, residual_ld, dtype, weight_dtype == LB_F32, rows, dim, group,
+                   out_dtype == LB_E4M3, eps, static_cast<uint8_t*>(codes), scales, hidden};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t size = dtype == LB_F32 ? 4 : 2;
+  const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const int width = group / 8;  // a group's pieces
+  const bool vec = dim % 8 == 0 && aligned(x) && aligned(residual) && aligned(weight) && aligned(hidden) &&
+                   reinterpret_cast<uintptr_t>(codes) % 8 == 0 && x_ld * size % 16 == 0 && residual_ld * size % 16 == 0 &&
+                   (group == 0 || (group % 8 == 0 && width <= 32 && (width & (width - 1)) == 0));
+  cudaError_t e;
+  if (vec) {
+    e = dtype == LB_F32 ? launch<float>(a, s) : dtype == LB_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
+  } else {
+    const size_t smem = sizeof(float) * dim;
+    e = smem > 40 * 1024 ? cudaFuncSetAttribute(norm_any_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                16384 * static_cast<int>(sizeof(float)))
+                         : cudaSuccess;
+    if (e == cudaSuccess) {
+      norm_any_kernel<<<rows, kThreads, smem, s>>>(a);
+      e = cudaGetLastError();
+    }
+  }
+  return e == cudaSuccess ? LB_OK : LB_ERR_CUDA;
 }
