@@ -23,8 +23,6 @@
 namespace lb {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kTileO = 32;          // outputs of a stage
 constexpr int kBlockK = 128;        // k of a stage
 constexpr int kCodeBytes = kTileO * kBlockK / 2;
@@ -57,18 +55,25 @@ __device__ __forceinline__ void cp_async_wait_pending(int n) {  // at most n gro
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <bool kBf16>
+// kFirst: a sum begins (c is only written)
+template <bool kBf16, bool kFirst>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (kBf16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+#define LB_MMA(type, c0)                                                                                        \
+  "mma.sync.aligned.m16n8k16.row.col.f32." type "." type ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " c0 ";"
+#define LB_IN "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1)
+  if constexpr (kFirst) {
+    if constexpr (kBf16)
+      asm volatile(LB_MMA("bf16", "{%10,%10,%10,%10}") : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : LB_IN, "f"(0.0f));
+    else
+      asm volatile(LB_MMA("f16", "{%10,%10,%10,%10}") : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : LB_IN, "f"(0.0f));
+  } else {
+    if constexpr (kBf16)
+      asm volatile(LB_MMA("bf16", "{%0,%1,%2,%3}") : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : LB_IN);
+    else
+      asm volatile(LB_MMA("f16", "{%0,%1,%2,%3}") : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : LB_IN);
+  }
+#undef LB_IN
+#undef LB_MMA
 }
 
 template <typename H>
@@ -126,12 +131,13 @@ __device__ __forceinline__ uint4 load_x8(const W4Args& a, int row, int k) {
 }
 
 // kXShared: x lies in shared memory; otherwise (k too large for it) every fragment is read from x itself.
-template <bool kBf16, int NT, bool kXShared>
-__global__ void __launch_bounds__(kThreads) w4_kernel(const W4Args a) {
+template <bool kBf16, int NT, bool kXShared, int kWarps, int kGroup>
+__global__ void __launch_bounds__(kWarps * 32) w4_kernel(const W4Args a) {
   extern __shared__ __align__(128) unsigned char w4_smem[];
+  constexpr int kThreads = kWarps * 32, kPerBlock = kBlockK / kGroup;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int blocks = (a.k + kBlockK - 1) / kBlockK, groups = a.k / a.group, per_block = kBlockK / a.group;
-  const int x_row = blocks * kBlockK * 2 + kXPad, group_log = 31 - __clz(a.group);
+  const int blocks = (a.k + kBlockK - 1) / kBlockK, groups = a.k / kGroup;
+  const int x_row = blocks * kBlockK * 2 + kXPad;
   unsigned char* x_s = w4_smem;                                                // [8 NT][x_row]
   unsigned char* ring = x_s + (kXShared ? 8 * NT * x_row : 0) + warp * a.stages * kStageBytes;
   float* sums = reinterpret_cast<float*>(w4_smem + (kXShared ? 8 * NT * x_row : 0));  // the rings, between tiles
@@ -156,34 +162,43 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const W4Args a) {
     pend_slot = -1;
   };
   int iss_tile = first, iss_b = 0, iss_slot = 0, issued = 0;
+  const uint8_t* from = nullptr;      // this lane's 16 bytes of the unit's first row group
+  const uint16_t* scale_from = nullptr;
+  unsigned rows_there = 0;            // bit i: row 8 i + lane / 4 of the tile exists; bit 4: row `lane` does
+  const uint32_t lane_dst = (lane >> 2) * 64;
+  const auto aim = [&]() {            // at the first unit of iss_tile
+    const int o0 = iss_tile * kTileO;
+    from = a.codes + static_cast<long long>(o0 + (lane >> 2)) * (a.k / 2) + b0 * (kBlockK / 2) + 16 * (lane & 3);
+    scale_from = reinterpret_cast<const uint16_t*>(a.w_scale) + static_cast<long long>(o0 + lane) * groups + b0 * kPerBlock;
+    rows_there = o0 + lane < a.out_features ? 16u : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows_there |= o0 + 8 * i + (lane >> 2) < a.out_features ? 1u << i : 0u;
+  };
+  if (n_units > 0) aim();
   const auto issue = [&]() {
     flush_scales();
     if (issued < n_units) {
-      const int o0 = iss_tile * kTileO, k0 = (b0 + iss_b) * kBlockK;
-      const uint32_t dst = ring_at + iss_slot * kStageBytes;
+      const int k0 = (b0 + iss_b) * kBlockK;
+      const uint32_t dst = ring_at + iss_slot * kStageBytes + lane_dst;
+      const bool k_there = k0 + 32 * (lane & 3) < a.k;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2), c = lane & 3;
-        if (o0 + r < a.out_features && k0 + 32 * c < a.k)
-          cp_async16(dst + r * 64 + ((c ^ ((r >> 1) & 3)) << 4),
-                     a.codes + static_cast<long long>(o0 + r) * (a.k / 2) + k0 / 2 + 16 * c);
-      }
+      for (int i = 0; i < 4; ++i)
+        if (k_there && (rows_there >> i & 1u))
+          cp_async16(dst + i * 512 + (((lane & 3) ^ (((lane >> 2) >> 1) & 3)) << 4), from + static_cast<long long>(i) * 4 * a.k);
       uint32_t s[4] = {0, 0, 0, 0};
-      if (o0 + lane < a.out_features) {
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(a.w_scale) + static_cast<long long>(o0 + lane) * groups;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int gi = (k0 >> group_log) + i;
-          if (i < per_block && gi < groups) s[i] = p[gi];
-        }
-      }
+      for (int i = 0; i < kPerBlock; ++i)
+        if ((rows_there & 16u) && (k0 / kGroup + i) < groups) s[i] = scale_from[i];
       pend[0] = s[0] | s[1] << 16;
       pend[1] = s[2] | s[3] << 16;
       pend_slot = iss_slot;
       ++issued;
+      from += kBlockK / 2;
+      scale_from += kPerBlock;
       if (++iss_b == nb) {
         iss_b = 0;
         iss_tile += step;
+        if (issued < n_units) aim();
       }
       if (++iss_slot == a.stages) iss_slot = 0;
     }
@@ -200,6 +215,11 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const W4Args a) {
     __syncthreads();
   }
 
+  // a lane's words of a stage: the same place in each of the rows g, g + 8, g + 16, g + 24
+  int word_at[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) word_at[j] = g * 64 + ((j ^ ((g >> 1) & 3)) << 4) + 4 * t;
+  const unsigned char* x_lane = x_s + g * x_row + b0 * (kBlockK * 2) + t * 16;
   int slot = 0;
   for (int pass = 0; pass < passes; ++pass) {
     float acc[2][NT][4] = {};
@@ -211,14 +231,14 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const W4Args a) {
         const unsigned char* st = ring + slot * kStageBytes;
         if (++slot == a.stages) slot = 0;
         const int k0 = (b0 + b) * kBlockK;
-        float part[2][NT][4] = {};
+        float part[2][NT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint4 xb[NT];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             if constexpr (kXShared) {
-              xb[n] = *reinterpret_cast<const uint4*>(x_s + (8 * n + g) * x_row + (k0 + 32 * j + 8 * t) * 2);
+              xb[n] = *reinterpret_cast<const uint4*>(x_lane + 8 * n * x_row + b * (kBlockK * 2) + j * 64);
             } else {
               const int k = k0 + 32 * j + 8 * t;
               xb[n] = 8 * n + g < m_live && k < a.k ? load_x8(a, m0 + 8 * n + g, k) : make_uint4(0, 0, 0, 0);
@@ -227,38 +247,43 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const W4Args a) {
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
             uint32_t lo[4], hi[4];
-            const int r = 16 * mt + g;
-            widen8<kBf16>(*reinterpret_cast<const uint32_t*>(st + r * 64 + ((j ^ ((r >> 1) & 3)) << 4) + 4 * t), lo);
-            widen8<kBf16>(*reinterpret_cast<const uint32_t*>(st + (r + 8) * 64 + ((j ^ (((r + 8) >> 1) & 3)) << 4) + 4 * t), hi);
+            widen8<kBf16>(*reinterpret_cast<const uint32_t*>(st + word_at[j] + mt * 1024), lo);
+            widen8<kBf16>(*reinterpret_cast<const uint32_t*>(st + word_at[j] + mt * 1024 + 512), hi);
             const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma_16816<kBf16>(part[mt][n], a0, xb[n].x, xb[n].y);
-              mma_16816<kBf16>(part[mt][n], a1, xb[n].z, xb[n].w);
+              if ((32 * j) % kGroup == 0) mma_16816<kBf16, true>(part[mt][n], a0, xb[n].x, xb[n].y);
+              else mma_16816<kBf16, false>(part[mt][n], a0, xb[n].x, xb[n].y);
+              mma_16816<kBf16, false>(part[mt][n], a1, xb[n].z, xb[n].w);
             }
           }
-          const int done = 32 * (j + 1);
-          if ((done & (a.group - 1)) == 0) {  // a group ends: its sum takes its scale (and x's, of a group of 128 or more)
-            const __half* sc = reinterpret_cast<const __half*>(st + kCodeBytes) + (done >> group_log) - 1;
+          if ((32 * (j + 1)) % kGroup == 0) {  // a group ends: its sum takes its scale (and x's, of a group of 128 or more)
+            const __half* sc = reinterpret_cast<const __half*>(st + kCodeBytes) + 32 * (j + 1) / kGroup - 1;
             float xs[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) xs[n][0] = xs[n][1] = 1.0f;
+            if (a.x_group) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int row = 8 * n + 2 * t + e;
-                xs[n][e] = a.x_group && row < m_live && k0 < a.k
-                               ? a.x_scale[static_cast<long long>(m0 + row) * (a.k / a.x_group) + k0 / a.x_group] : 1.0f;
-              }
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int row = 8 * n + 2 * t + e;
+                  if (row < m_live) xs[n][e] = a.x_scale[static_cast<long long>(m0 + row) * (a.k / a.x_group) + k0 / a.x_group];
+                }
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) part[mt][n][e] *= xs[n][e & 1];
+            }
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
               const float s0 = __half2float(sc[(16 * mt + g) * 4]), s1 = __half2float(sc[(16 * mt + g + 8) * 4]);
 #pragma unroll
               for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  acc[mt][n][e] = fmaf(part[mt][n][e], (e < 2 ? s0 : s1) * xs[n][e & 1], acc[mt][n][e]);
-                  part[mt][n][e] = 0.0f;
-                }
+                for (int e = 0; e < 4; ++e) acc[mt][n][e] = fmaf(part[mt][n][e], e < 2 ? s0 : s1, acc[mt][n][e]);
             }
           }
         }
@@ -308,20 +333,27 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const W4Args a) {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <bool kBf16, int NT, bool kXShared>
+template <bool kBf16, int NT, bool kXShared, int kWarps, int kGroup>
 cudaError_t launch(const W4Args& a, int grid, size_t smem, cudaStream_t s) {
+  const auto kernel = w4_kernel<kBf16, NT, kXShared, kWarps, kGroup>;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(w4_kernel<kBf16, NT, kXShared>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kMaxSmem);
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), kMaxSmem);
     if (e != cudaSuccess) return e;
   }
-  w4_kernel<kBf16, NT, kXShared><<<grid, kThreads, smem, s>>>(a);
+  kernel<<<grid, kWarps * 32, smem, s>>>(a);
   return cudaGetLastError();
 }
-template <bool kBf16>
-cudaError_t launch(const W4Args& a, int nt, bool shared, int grid, size_t smem, cudaStream_t s) {
-  if (nt == 1) return shared ? launch<kBf16, 1, true>(a, grid, smem, s) : launch<kBf16, 1, false>(a, grid, smem, s);
-  return shared ? launch<kBf16, 2, true>(a, grid, smem, s) : launch<kBf16, 2, false>(a, grid, smem, s);
+template <bool kBf16, int NT, bool kXShared, int kWarps>
+cudaError_t launch(const W4Args& a, int grid, size_t smem, cudaStream_t s) {
+  if (a.group == 32) return launch<kBf16, NT, kXShared, kWarps, 32>(a, grid, smem, s);
+  if (a.group == 64) return launch<kBf16, NT, kXShared, kWarps, 64>(a, grid, smem, s);
+  return launch<kBf16, NT, kXShared, kWarps, 128>(a, grid, smem, s);
+}
+template <bool kBf16, int NT>
+cudaError_t launch(const W4Args& a, int warps, bool shared, int grid, size_t smem, cudaStream_t s) {
+  if (!shared) return launch<kBf16, NT, false, 8>(a, grid, smem, s);
+  return warps == 8 ? launch<kBf16, NT, true, 8>(a, grid, smem, s) : launch<kBf16, NT, true, 16>(a, grid, smem, s);
 }
 
 }  // namespace
@@ -344,31 +376,40 @@ extern "C" int lb_op_w4_matvec(const void* x, int64_t x_ld, int x_dtype, const f
 
   const int blocks = (k + kBlockK - 1) / kBlockK, tiles = (out_features + kTileO - 1) / kTileO;
   const size_t x_row = static_cast<size_t>(blocks) * kBlockK * 2 + kXPad;
-  constexpr size_t kRing = static_cast<size_t>(kWarps) * kStageBytes;  // of one stage
-  // 16 rows of x a pass where they fit beside a ring of four stages, else 8, else none of them
+  constexpr size_t kLimit = kMaxSmem, kRing8 = 8 * kStageBytes, kRing16 = 16 * kStageBytes;  // of one stage
+  // 16 rows of x a pass where they fit beside rings of four stages, else 8, else x stays where it is
   int nt = m > 8 ? 2 : 1;
-  if (8 * nt * x_row + 4 * kRing > kMaxSmem) nt = 1;
-  const bool shared = 8 * nt * x_row + 4 * kRing <= kMaxSmem;
+  if (8 * nt * x_row + 4 * kRing8 > kLimit) nt = 1;
+  const bool shared = 8 * nt * x_row + 4 * kRing8 <= kLimit;
   if (!shared) nt = m > 8 ? 2 : 1;
   const int m_tiles = (m + 8 * nt - 1) / (8 * nt);
-  // K split among a CTA's warps until the tiles give every SM sixteen warps
-  int splits = 1;
-  while (splits < kWarps && splits < blocks && static_cast<long long>(tiles) * m_tiles * splits < 148 * 16) splits *= 2;
   const size_t x_bytes = shared ? 8 * nt * x_row : 0;
-  // two CTAs an SM where x leaves the room; a split tile's sums take the rings' place
-  int stages = x_bytes + 4 * kRing <= kMaxSmem / 2 ? static_cast<int>((kMaxSmem / 2 - x_bytes) / kRing)
-                                                   : static_cast<int>((kMaxSmem - x_bytes) / kRing);
-  stages = stages > 8 ? 8 : stages;
-  const size_t smem = x_bytes + stages * kRing;
-  const int rows = kWarps / splits, tile_ctas = (tiles + rows - 1) / rows;
-  const int resident = 148 * (smem <= kMaxSmem / 2 ? 2 : 1);
-  int grid = tile_ctas;
-  if (splits == 1 && static_cast<long long>(grid) * m_tiles > resident) grid = resident / m_tiles > 0 ? resident / m_tiles : 1;
-  if (static_cast<long long>(grid) * m_tiles > 0x7fffffffll) return LB_ERR_CAPACITY;
-  W4Args a{x, x_ld, ld_out, x_scale, x_dtype, x_group, m, group, out_features, k, out_dtype, splits, stages, tiles, m_tiles,
-           static_cast<const uint8_t*>(codes), static_cast<const __half*>(w_scale), out};
+  // Small products: CTAs of 8 warps, two an SM, with K split among a CTA's warps as far as one wave of
+  // CTAs goes.  Large ones: 16 warps an SM (each SM loads x once) that walk over the tiles.
+  const bool two = x_bytes + 4 * kRing8 <= kLimit / 2;
+  const long long wave = 148ll * (two ? 2 : 1);
+  int warps = 8, splits = 1;
+  const auto ctas = [&](int w, int sp) { return static_cast<long long>((tiles + w / sp - 1) / (w / sp)) * m_tiles; };
+  while (splits < 8 && splits < blocks && ctas(8, 2 * splits) <= wave) splits *= 2;
+  if (ctas(8, splits) > wave && shared && x_bytes + 4 * kRing16 <= kLimit) {
+    warps = 16;
+    while (splits < 16 && splits < blocks && ctas(16, 2 * splits) <= 148) splits *= 2;
+  }
+  const size_t ring = warps == 8 ? kRing8 : kRing16, room = (warps == 8 && two ? kLimit / 2 : kLimit) - x_bytes;
+  const int stages = room / ring > 8 ? 8 : static_cast<int>(room / ring);
+  const size_t smem = x_bytes + stages * ring;
+  // a split tile's CTA makes one pass (its sums take the rings' place)
+  const long long all = (tiles + warps / splits - 1) / (warps / splits), fit = wave / (warps == 16 && two ? 2 : 1) / m_tiles;
+  const long long grid = splits > 1 || all <= fit ? all : fit > 0 ? fit : 1;
+  if (grid * m_tiles > 0x7fffffffll) return LB_ERR_CAPACITY;
+  const W4Args a{x, x_ld, ld_out, x_scale, x_dtype, x_group, m, group, out_features, k, out_dtype, splits, stages, tiles, m_tiles,
+                 static_cast<const uint8_t*>(codes), static_cast<const __half*>(w_scale), out};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = x_dtype == LB_BF16 ? launch<true>(a, nt, shared, grid * m_tiles, smem, s)
-                                           : launch<false>(a, nt, shared, grid * m_tiles, smem, s);
+  const int n = static_cast<int>(grid * m_tiles);
+  cudaError_t e;
+  if (x_dtype == LB_BF16)
+    e = nt == 1 ? launch<true, 1>(a, warps, shared, n, smem, s) : launch<true, 2>(a, warps, shared, n, smem, s);
+  else
+    e = nt == 1 ? launch<false, 1>(a, warps, shared, n, smem, s) : launch<false, 2>(a, warps, shared, n, smem, s);
   return e == cudaSuccess ? LB_OK : LB_ERR_CUDA;
 }
