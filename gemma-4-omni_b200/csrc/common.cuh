@@ -8,6 +8,7 @@
 // hanging the GPU.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <utility>
 #include <cuda.h>
@@ -61,6 +62,18 @@ inline cudaError_t launch_kernel(bool pdl, void (*kernel)(KArgs...), dim3 grid, 
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Raises a kernel's dynamic shared-memory limit, once per device and kernel (`done`: a
+// static of the caller's, a bit per device; setting it twice does no harm).
+inline cudaError_t ensure_smem(std::atomic<unsigned long long>& done, const void* kernel, int bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+  if ((done.load(std::memory_order_acquire) >> dev) & 1ull) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(1ull << dev, std::memory_order_acq_rel);
+  return e;
 }
 
 // Upper bound for any single spin-wait: 2 s of wall time on the device clock.

@@ -850,7 +850,8 @@ int rows_of(int max_new, int group) {
 template <typename T, int D, int R>
 cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
   using S = Shape<D, R>;
-  cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(attend_kernel<T, D, R>), S::kSmem);
   if (e != cudaSuccess) return e;
   attend_kernel<T, D, R><<<kSms, kThreads, S::kSmem, s>>>(a, k_map, v_map);
   e = cudaGetLastError();

@@ -262,9 +262,9 @@ int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int
              reinterpret_cast<long long*>(slots)};
   const size_t smem = sizeof(int) * (3 * static_cast<size_t>(n) + 1 + kPlanThreads + (n_sessions + 31) / 32);
   constexpr size_t kMost = sizeof(int) * (3 * kMaxPlanRows + 1 + kPlanThreads + kMaxPlanSessions / 32);
+  static std::atomic<unsigned long long> done{0};
   if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMost)) !=
-          cudaSuccess)
+      ensure_smem(done, reinterpret_cast<const void*>(plan_kernel), static_cast<int>(kMost)) != cudaSuccess)
     return LB_ERR_CUDA;
   // a CTA for each 4096 values written, at most one per SM
   const long long values = static_cast<long long>(n) * max_pages + 3ll * max_tokens;

@@ -39,25 +39,27 @@ MAX_PLAN_TOKENS = 1 << 26
 def _call(device: torch.device, name: str, *args) -> None:
     """Runs one C entry on the current stream of ``device`` (appended to the arguments)."""
     fn = getattr(_lib.load(), name)
-    if device.index is not None and device.index != torch.cuda.current_device():
+    # the raw handle of torch.cuda.current_stream(device), without an object around it
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, stream)
     else:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        rc = fn(*args, stream)
     if rc != _lib.LB_OK:
         _lib.check(name, rc)
 
 
 def _need(t: torch.Tensor, name: str, dtype, shape: tuple, device: torch.device) -> None:
     """Refuses a tensor that is not contiguous, of this type and shape, on this device."""
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}")
 
 
 def _cuda(device: torch.device, what: str) -> torch.device:
     if device.type != "cuda":
         raise ValueError(f"{what} runs on a CUDA device (no CPU fallback)")
-    return device
+    return device  # of a tensor: it has an index
 
 
 @dataclass
@@ -99,6 +101,7 @@ class PageDirectory:
         self.tables, self.lengths, self.used = tables, lengths, used
         self.pages, self.page_tokens = int(pages), int(page_tokens)
         self._released = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._where = (tables.data_ptr(), lengths.data_ptr(), used.data_ptr())
 
     @classmethod
     def create(cls, *, sessions: int, max_pages: int, pages: int, page_tokens: int,
@@ -121,20 +124,21 @@ class PageDirectory:
             raise ValueError(f"max_tokens must be between 1 and {MAX_PLAN_TOKENS}")
         _need(sessions, "sessions", torch.int32, (n,), dev)
         _need(new_tokens, "new_tokens", torch.int32, (n,), dev)
-        # one allocation: the 64-bit slots first, then the 32-bit arrays
-        slots = torch.empty(2 * max_tokens + (n * self.max_pages + 2 * n + 2) // 2 + 1, dtype=torch.int64, device=dev)
-        rest = slots[max_tokens:].view(torch.int32)
-        tables, positions, rows, kv_len, cu, status, _ = rest.split(
-            (n * self.max_pages, max_tokens, max_tokens, n, n + 1, 1,
-             rest.numel() - n * self.max_pages - 2 * max_tokens - 2 * n - 2))
-        base = slots.data_ptr()
-        at = base + 8 * max_tokens
-        step = 4 * n * self.max_pages
-        _call(dev, "lb_plan_pages", n, sessions.data_ptr(), new_tokens.data_ptr(), self.sessions, self.max_pages,
-              self.pages, self.page_tokens, self.tables.data_ptr(), self.lengths.data_ptr(), self.used.data_ptr(),
-              max_tokens, at, at + step + 8 * max_tokens, at + step + 8 * max_tokens + 4 * n, base, at + step,
-              at + step + 4 * max_tokens, at + step + 8 * max_tokens + 8 * n + 4)
-        return PagePlan(sessions, tables.view(n, self.max_pages), kv_len, cu, slots[:max_tokens], positions, rows, status)
+        # one allocation: the 64-bit slots, then the 32-bit arrays
+        mp = self.max_pages
+        words = 2 * max_tokens, n * mp, max_tokens, max_tokens, n, n + 1, 1
+        buf = torch.empty(sum(words), dtype=torch.int32, device=dev)
+        slots, tables, positions, rows, kv_len, cu, status = buf.split(words)
+        p_slots = buf.data_ptr()
+        p_tables = p_slots + 8 * max_tokens
+        p_pos = p_tables + 4 * n * mp
+        p_rows = p_pos + 4 * max_tokens
+        p_len = p_rows + 4 * max_tokens
+        p_cu = p_len + 4 * n
+        _call(dev, "lb_plan_pages", n, sessions.data_ptr(), new_tokens.data_ptr(), self.sessions, mp, self.pages,
+              self.page_tokens, self._where[0], self._where[1], self._where[2], max_tokens, p_tables, p_len, p_cu,
+              p_slots, p_pos, p_rows, p_cu + 4 * n + 4)
+        return PagePlan(sessions, tables.view(n, mp), kv_len, cu, slots.view(torch.int64), positions, rows, status)
 
     def commit(self, plan: PagePlan) -> None:
         """Installs a plan made from the directory as it is now (a refused plan changes nothing)."""
@@ -197,7 +201,7 @@ class Kv8Cache:
         if k.dtype not in FLOAT_INPUTS or v.dtype != k.dtype:
             raise ValueError("k and v must both be float32, bfloat16 or float16")
         for name, t in (("k", k), ("v", v)):
-            if tuple(t.shape) != (n, self.kv_heads, self.dim) or t.device != self.device or t.stride(2) != 1:
+            if t.shape != (n, self.kv_heads, self.dim) or t.device != self.device or t.stride(2) != 1:
                 raise ValueError(f"{name} must be [{n}, {self.kv_heads}, {self.dim}] on {self.device}, its rows contiguous")
         _need(slots, "slots", torch.int64, (n,), self.device)
         if n == 0:
@@ -228,19 +232,19 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, row_tables: torch.Tensor, kv
         raise ValueError(f"q must be [tokens, heads, {cache.dim}] on {dev}, its rows contiguous")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("q must be bfloat16 or float16")
-    t, heads, dim = (int(v) for v in q.shape)
+    t, heads, dim = q.shape
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError("heads must be a positive multiple of the cache's kv_heads")
     if row_tables.dim() != 2 or row_tables.shape[0] < 1:
         raise ValueError("row_tables must be [rows, max_pages]")
-    n, max_pages = (int(v) for v in row_tables.shape)
+    n, max_pages = row_tables.shape
     _need(row_tables, "row_tables", torch.int32, (n, max_pages), dev)
     _need(kv_len, "kv_len", torch.int32, (n,), dev)
     _need(cu_tokens, "cu_tokens", torch.int32, (n + 1,), dev)
     if window < 0 or softcap < 0.0 or max_new < 1:
         raise ValueError("window and softcap must not be negative, max_new must be positive")
     if out is None:
-        out = torch.empty((t, heads, dim), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _need(out, "out", q.dtype, (t, heads, dim), dev)
     lse = torch.empty((t, heads), dtype=torch.float32, device=dev) if return_lse else None
@@ -265,7 +269,7 @@ def rms_norm8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor |
     if x.dim() != 2 or x.dtype not in FLOAT_INPUTS or (x.numel() and x.stride(1) != 1):
         raise ValueError("x must be a float32, bfloat16 or float16 [rows, dim] tensor, its rows contiguous")
     dev = _cuda(x.device, "rms_norm8")
-    rows, dim = (int(v) for v in x.shape)
+    rows, dim = x.shape
     if not 0 < dim <= 16384 or group < 0 or (group and dim % group):
         raise ValueError("dim must be at most 16384 and a multiple of group")
     if dtype not in (torch.float8_e4m3fn, torch.int8):
@@ -276,9 +280,9 @@ def rms_norm8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor |
     if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape or residual.device != dev
                                  or (x.numel() and residual.stride(1) != 1)):
         raise ValueError("residual must be like x")
-    codes = torch.empty((rows, dim), dtype=dtype, device=dev)
+    codes = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
     scales = torch.empty((rows, dim // group if group else 1), dtype=torch.float32, device=dev)
-    hidden = x if residual is None else torch.empty((rows, dim), dtype=x.dtype, device=dev)
+    hidden = x if residual is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     if rows:
         _call(dev, "lb_op_rms_norm8", x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(),
               0 if residual is None else residual.stride(0), DTYPE_CODES[x.dtype], weight.data_ptr(),
@@ -350,7 +354,7 @@ def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | No
         if out_dtype not in FLOAT_INPUTS:
             raise ValueError("out_dtype must be float32, bfloat16 or float16")
         out = torch.empty((rows, weight.out_features), dtype=out_dtype, device=dev)
-    elif out.dtype not in FLOAT_INPUTS or tuple(out.shape) != (rows, weight.out_features) or out.device != dev or (
+    elif out.dtype not in FLOAT_INPUTS or out.shape != (rows, weight.out_features) or out.device != dev or (
             out.numel() and out.stride(1) != 1):
         raise ValueError(f"out must be [{rows}, {weight.out_features}] on {dev}, its rows contiguous")
     if rows:
