@@ -25,13 +25,13 @@
 // depend on which CTA finishes first.
 //
 // Warp roles: 0 loads (TMA boxes of 64 keys, or of the largest power of two that divides a
-// page: an issued box costs the warp about 120 cycles whatever its size), 1 issues the MMAs of
-// the scores, 14 those of the outputs (a thread that waits on a barrier before each tile's MMAs
-// loses some 500 cycles to it, so the two do not share one), 2-5 and 6-9 turn the scores of
-// even and of odd tiles into digits of p (a thread a key: tensor memory's lanes), each
-// with a running sum of its own, 10-13 add up the outputs (a thread a column).
-// Scores, digits and outputs have two buffers each, so neighbouring tiles overlap; the
-// ring of K and V tiles takes the rest of the shared memory.
+// page), 1 issues the MMAs of the scores, 14 those of the outputs (a thread that waits on a
+// barrier before each tile's MMAs loses some 500 cycles to it, so the two do not share one),
+// 15 splits the next task's q into digits while the present one runs, 2-5 and 6-9 turn scores
+// into digits of p (a thread a key: tensor memory's lanes), 8 queries at a time (more of them unrolled
+// outgrow the instruction cache: 16 took 6.9 thousand cycles a tile, 8 take 2.5), 10-13 add up the
+// outputs (a thread a column).  K and V lie in one ring of units of 128 keys, K freed by its
+// scores, V by its outputs; scores, digits, outputs and q have two buffers each.
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 #include "kernels.h"
@@ -39,9 +39,12 @@
 namespace lb {
 namespace {
 
-constexpr int kThreads = 480;
+constexpr int kThreads = 512;
 constexpr int kTile = 128;   // keys of a tile: the lanes of the tensor memory
 constexpr int kBoxes = 8;    // most TMA boxes of a tile (pages are multiples of 16)
+constexpr int kQueries = 8;    // queries of a score warpgroup's turn
+constexpr int kTasks = 8;      // tasks that the loading warp may be ahead
+constexpr int kInfo = 16;      // tiles whose scales are kept: more than the ring's units reach ahead
 constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -79,12 +82,13 @@ struct Shape {
   static constexpr int kOutBuffers = 2 * kS + 2 * kHalves * kN2 <= 512 ? 2 : 1;
   static constexpr int kColumns = 2 * kS + kOutBuffers * kHalves * kN2;
   static constexpr int kAlloc = kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
-  static constexpr int kQBytes = kHalves * kN1 * kRow;
+  static constexpr int kQBytes = (kHalves * kN1 * kRow + 1023) / 1024 * 1024;
   static constexpr int kPBytes = kN2 * kTile;
-  static constexpr int kFixedBytes = (kQBytes + 1023) / 1024 * 1024 + 2 * kPBytes + 1024;
-  static constexpr int kStages = (225 * 1024 - 8192 - kFixedBytes) / (2 * kSide) < 8
-                                     ? (225 * 1024 - 8192 - kFixedBytes) / (2 * kSide) : 8;
-  static constexpr int kSmem = kFixedBytes + kStages * 2 * kSide;
+  static constexpr int kFixedBytes = 2 * kQBytes + 2 * kPBytes + 1024;
+  static constexpr int kRoom = (217 * 1024 - kFixedBytes) / kSide;
+  static constexpr int kUnits = kRoom < kInfo ? kRoom : kInfo;  // (a tile's scales outlive its units)
+  static constexpr int kSmem = kFixedBytes + kUnits * kSide;
+  static constexpr int kTurns = R / kQueries;  // of the score warpgroups, a tile
   static constexpr int kPart = R * D + 2 * R;
 };
 
@@ -122,7 +126,6 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t off) {
 template <int C>
 __device__ __forceinline__ void tmem_ld3(uint32_t a0, uint32_t a1, uint32_t a2, int (&x)[C], int (&y)[C], int (&z)[C]);
 #define LB_R8(v) "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-#define LB_R16(v) LB_R8(v), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
 template <>
 __device__ __forceinline__ void tmem_ld3<8>(uint32_t a0, uint32_t a1, uint32_t a2, int (&x)[8], int (&y)[8], int (&z)[8]) {
   asm volatile(
@@ -134,25 +137,40 @@ __device__ __forceinline__ void tmem_ld3<8>(uint32_t a0, uint32_t a1, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2)
       : "memory");
 }
-template <>
-__device__ __forceinline__ void tmem_ld3<16>(uint32_t a0, uint32_t a1, uint32_t a2, int (&x)[16], int (&y)[16],
-                                             int (&z)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%48];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%49];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47}, [%50];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : LB_R16(x), LB_R16(y), LB_R16(z)
-      : "r"(a0), "r"(a1), "r"(a2)
-      : "memory");
-}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Waits for a phase, at most kWaitLimitNs (common.cuh).  One copy for all roles: the kernel's code has to
+// stay small, since sixteen warps in six roles share the SM's instruction cache.  try_wait sleeps in
+// hardware, so a waiting warp takes few issue slots.
+__device__ __noinline__ bool wait_phase(uint32_t bar, uint32_t parity, int* status) {
+  const unsigned long long start = globaltimer_ns();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(20000u)
+        : "memory");
+    if (done) return true;
+    if (globaltimer_ns() - start > kWaitLimitNs) {
+      if (status) atomicOr(status, kStatusWaitTimeout);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, int* status) {
+  return mbar_try_wait(bar, parity) || wait_phase(smem_u32(bar), parity, status);
+}
+// by a whole warp: the same answer for every lane
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* status) {
+  return __all_sync(0xffffffffu, wait_one(bar, parity, status));
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) { return (a > b || isnan(a)) ? a : b; }
 // the largest of the warp's values, a NaN if there is one
 __device__ __forceinline__ float warp_top(float x) {
@@ -203,18 +221,19 @@ __device__ __forceinline__ long long warp_prefix(long long v) {  // inclusive
   return v;
 }
 
-// A CTA's part of a task.
+// A CTA's part of a task, as the loading warp hands it to the others (n 0: there are no more).
 struct Task {
-  Row w;
-  int row, hk, qt, rows, tile0, tile1;
-  int pos_low, pos_high;  // positions of its first and last token
-  int start, stop;        // keys that any of its tokens sees
-  long long next;         // the line's tile after it
-  __device__ __forceinline__ bool from_start() const { return tile0 == 0; }
-  __device__ __forceinline__ bool to_end() const { return tile1 == w.tiles; }
+  int n;                    // tiles
+  int tile0, low;           // its first tile; key 0 of tile 0
+  int rows, hk, qt, begin;  // query rows; kv head, query tile; the batch row's first token
+  int pos_low, pos_high;    // positions of its first and last token
+  int start, stop;          // keys that any of its tokens sees
+  int row, q_tiles;
+  int from_start, to_end;   // whether the task's first and last tiles are among these
+  int last_cta;             // of a task that goes on after them: the CTA that has its last tile
 };
 
-// Walks the tasks of a CTA's share [x, x_end) of the line; a warp at a time, every role for itself.
+// Walks the tasks of a CTA's share [x, x_end) of the line (a warp together).
 template <int R>
 struct Walk {
   long long x, x_end, base, upto;
@@ -233,9 +252,13 @@ struct Walk {
     held = row_of<R>(a, win + (threadIdx.x & 31));
     upto = warp_prefix(row_work(a, held));
   }
-  __device__ __forceinline__ bool next(const AttendArgs& a, Task& t) {
-    if (x >= x_end) return false;
+  __device__ __forceinline__ bool next(const AttendArgs& a, long long line, long long n_ctas, Task& t) {
+    if (x >= x_end) {
+      t.n = 0;
+      return false;
+    }
     unsigned after = __ballot_sync(0xffffffffu, base + upto > x);
+#pragma unroll 1
     while (after == 0) {
       base += __shfl_sync(0xffffffffu, upto, 31);
       win += 32;
@@ -244,27 +267,33 @@ struct Walk {
       after = __ballot_sync(0xffffffffu, base + upto > x);
     }
     const int at = __ffs(after) - 1;
+    Row w;
     t.row = win + at;
-    t.w.begin = __shfl_sync(0xffffffffu, held.begin, at);
-    t.w.count = __shfl_sync(0xffffffffu, held.count, at);
-    t.w.len = __shfl_sync(0xffffffffu, held.len, at);
-    t.w.low = __shfl_sync(0xffffffffu, held.low, at);
-    t.w.tiles = __shfl_sync(0xffffffffu, held.tiles, at);
-    t.w.q_tiles = __shfl_sync(0xffffffffu, held.q_tiles, at);
-    const long long y = x - (base + __shfl_sync(0xffffffffu, upto, at) - row_work(a, t.w));
-    const int task = static_cast<int>(y / t.w.tiles);
-    t.tile0 = static_cast<int>(y - static_cast<long long>(task) * t.w.tiles);
-    t.hk = task / t.w.q_tiles;
-    t.qt = task - t.hk * t.w.q_tiles;
-    t.tile1 = static_cast<int>(min(static_cast<long long>(t.w.tiles), t.tile0 + (x_end - x)));
-    x += t.tile1 - t.tile0;
-    t.next = x;
+    w.begin = __shfl_sync(0xffffffffu, held.begin, at);
+    w.count = __shfl_sync(0xffffffffu, held.count, at);
+    w.len = __shfl_sync(0xffffffffu, held.len, at);
+    w.low = __shfl_sync(0xffffffffu, held.low, at);
+    w.tiles = __shfl_sync(0xffffffffu, held.tiles, at);
+    w.q_tiles = __shfl_sync(0xffffffffu, held.q_tiles, at);
+    const long long y = x - (base + __shfl_sync(0xffffffffu, upto, at) - row_work(a, w));
+    const int task = static_cast<int>(y / w.tiles);
+    t.tile0 = static_cast<int>(y - static_cast<long long>(task) * w.tiles);
+    t.hk = task / w.q_tiles;
+    t.qt = task - t.hk * w.q_tiles;
+    t.n = static_cast<int>(min(static_cast<long long>(w.tiles - t.tile0), x_end - x));
+    x += t.n;
+    t.from_start = t.tile0 == 0;
+    t.to_end = t.tile0 + t.n == w.tiles;
+    t.last_cta = static_cast<int>(((x + (w.tiles - t.tile0 - t.n)) * n_ctas - 1) / line);
     const int G = a.heads / a.kv_heads;
-    t.rows = min(R, t.w.count * G - t.qt * R);
-    t.pos_low = t.w.len - t.w.count + t.qt * R / G;
-    t.pos_high = t.w.len - t.w.count + (t.qt * R + t.rows - 1) / G;
-    t.stop = min(min(max(t.w.len, 0), a.max_pages * a.page_tokens), t.pos_high + 1);
-    t.start = a.window ? max(t.w.low, t.pos_low + 1 - a.window) : 0;
+    t.low = w.low;
+    t.begin = w.begin;
+    t.q_tiles = w.q_tiles;
+    t.rows = min(R, w.count * G - t.qt * R);
+    t.pos_low = w.len - w.count + t.qt * R / G;
+    t.pos_high = w.len - w.count + (t.qt * R + t.rows - 1) / G;
+    t.stop = min(min(max(w.len, 0), a.max_pages * a.page_tokens), t.pos_high + 1);
+    t.start = a.window ? max(w.low, t.pos_low + 1 - a.window) : 0;
     return true;
   }
 };
@@ -276,20 +305,22 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   using S = Shape<D, R>;
   extern __shared__ unsigned char attend_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(attend_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* ring = smem;                                  // [stage][K, V][half][128 keys][kRow]
-  unsigned char* q_digits = ring + S::kStages * 2 * S::kSide;  // [half][digit * R + query][kRow]
-  unsigned char* p_digits = q_digits + (S::kQBytes + 1023) / 1024 * 1024;  // [buffer][digit * R + query][128 keys]
-  __shared__ uint64_t full[S::kStages], empty[S::kStages], s_full[2], s_empty[2], p_full[2], p_empty[2], o_full[2], o_empty[2];
-  __shared__ uint64_t q_full, q_empty, f_full[4], tops[2], l_full, l_empty;
+  unsigned char* ring = smem;                                  // [unit][half][128 keys][kRow]
+  unsigned char* q_digits = ring + S::kUnits * S::kSide;       // [buffer][half][digit * R + query][kRow]
+  unsigned char* p_digits = q_digits + 2 * S::kQBytes;         // [buffer][digit * R + query][128 keys]
+  __shared__ uint64_t full[S::kUnits], empty[S::kUnits], s_full[2], s_empty[2], p_full[2], p_empty[2], o_full[2], o_empty[2];
+  __shared__ uint64_t g_full[kInfo], q_full[2], q_empty[2], f_full[4], tops[2], l_full, l_empty;
+  __shared__ uint64_t task_full[kTasks], task_empty[kTasks];
+  __shared__ Task tasks[kTasks];
   __shared__ uint32_t tmem_slot;
   __shared__ long long pre[kThreads + 1];
   __shared__ long long warp_total[kThreads / 32];
-  __shared__ float g_ks[S::kStages][kBoxes], g_vs[S::kStages][kBoxes], g_top[S::kStages];
-  __shared__ unsigned g_there[S::kStages];
-  __shared__ __align__(16) float fac_s[R];       // a query: its factor to log2 scores, and the keys that it sees
-  __shared__ int last_s[R], first_s[R];
-  __shared__ __align__(16) float tops_s[2][4][R];  // a tile's largest scores, by warp
-  __shared__ __align__(16) float top_s[8][R], beta_s[8][R];
+  __shared__ float g_ks[kInfo][kBoxes], g_vs[kInfo][kBoxes], g_top[kInfo];
+  __shared__ unsigned g_there[kInfo];
+  __shared__ __align__(16) float fac_s[2][R];    // a query: its factor to log2 scores, and the keys that it sees
+  __shared__ int last_s[2][R], first_s[2][R];
+  __shared__ float tops_s[2][2][4][kQueries];    // [warpgroup][turn]: a turn's largest scores, by warp
+  __shared__ __align__(16) float top_s[8][kQueries], beta_s[8][kQueries];
   __shared__ float mx_ring[4][R], v_ring[4];     // a tile's largest scores and largest V scale
   __shared__ __align__(16) float out_f[4][R];
   __shared__ float l_part[8][R], m_ref[2][R];
@@ -297,395 +328,528 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   const int G = a.heads / a.kv_heads, P = a.page_tokens;
 
   // ---- set-up, and this CTA's share of the line of tiles
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, S::kAlloc);
+    tmem_relinquish();
+  }
   if (tid == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < S::kUnits; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&s_empty[b], 4);
-      mbar_init(&p_full[b], 4);
+      mbar_init(&s_empty[b], 4 * S::kTurns);
+      mbar_init(&p_full[b], 4 * S::kTurns);
       mbar_init(&p_empty[b], 1);
       mbar_init(&o_full[b], 1);
       mbar_init(&o_empty[b], 4);
       mbar_init(&tops[b], 4);
+      mbar_init(&q_full[b], 1);
+      mbar_init(&q_empty[b], 9);
     }
-    for (int b = 0; b < 4; ++b) mbar_init(&f_full[b], 1);
-    mbar_init(&q_full, 8);
-    mbar_init(&q_empty, 1);
+    for (int b = 0; b < 4; ++b) mbar_init(&f_full[b], S::kTurns);
+    for (int b = 0; b < kInfo; ++b) mbar_init(&g_full[b], 1);
+    for (int b = 0; b < kTasks; ++b) {
+      mbar_init(&task_full[b], 1);
+      mbar_init(&task_empty[b], 15);
+    }
     mbar_init(&l_full, 8);
     mbar_init(&l_empty, 4);
     fence_barrier_init();
     a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
   }
+  const int first_token = min(max(a.cu_tokens[0], 0), a.n_tokens);
+  const int last_token = min(max(a.cu_tokens[a.n_rows], 0), a.n_tokens);
   const int each = (a.n_rows + kThreads - 1) / kThreads;
   long long mine = 0;
+#pragma unroll 2
   for (int r = tid * each; r < min(a.n_rows, (tid + 1) * each); ++r) mine += row_work(a, row_of<R>(a, r));
   long long sum = warp_prefix(mine);
   if (lane == 31) warp_total[warp] = sum;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) sum += warp_total[w];
-  pre[tid + 1] = sum;
-  if (tid == 0) pre[0] = 0;
   if constexpr (R == 8) {  // rows of padding: zero once
-    for (int i = tid; i < S::kHalves * 8 * S::kRow / 4; i += kThreads) {
-      const int h = i / (8 * S::kRow / 4), o = i - h * (8 * S::kRow / 4);
-      reinterpret_cast<uint32_t*>(q_digits + h * S::kN1 * S::kRow + 24 * S::kRow)[o] = 0u;
+    for (int i = tid; i < 2 * S::kHalves * 8 * S::kRow / 4; i += kThreads) {
+      const int buf = i / (S::kHalves * 8 * S::kRow / 4), j = i - buf * (S::kHalves * 8 * S::kRow / 4);
+      const int h = j / (8 * S::kRow / 4), o = j - h * (8 * S::kRow / 4);
+      reinterpret_cast<uint32_t*>(q_digits + buf * S::kQBytes + h * S::kN1 * S::kRow + 24 * S::kRow)[o] = 0u;
     }
     fence_proxy_async_smem();
-  }
-  // tokens of no row
-  {
-    const int first = min(max(a.cu_tokens[0], 0), a.n_tokens);
-    const int last = min(max(a.cu_tokens[a.n_rows], 0), a.n_tokens);
-    const long long pieces = static_cast<long long>(a.heads) * D / 8;
-    if (first != 0 || last != a.n_tokens)
-      for (long long i = static_cast<long long>(blockIdx.x) * kThreads + tid; i < a.n_tokens * pieces;
-           i += static_cast<long long>(gridDim.x) * kThreads) {
-        const long long tok = i / pieces;
-        if (tok >= first && tok < last) continue;
-        reinterpret_cast<int4*>(a.out)[i] = make_int4(0, 0, 0, 0);
-        if (a.lse && i % (D / 8) == 0) a.lse[i / (D / 8)] = -INFINITY;
-      }
-  }
-  __syncthreads();
-  const long long W = pre[kThreads];
-  const long long n_ctas = min(static_cast<long long>(gridDim.x), W);
-  const long long b = blockIdx.x;
-  if (b >= n_ctas) return;
-  Walk<R> walk;
-  walk.begin(a, pre, each, W * b / n_ctas, W * (b + 1) / n_ctas);
-  if (warp == 1) {
-    tmem_alloc(&tmem_slot, S::kAlloc);
-    tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+#pragma unroll 1
+  for (int w = 0; w < warp; ++w) sum += warp_total[w];
+  pre[tid + 1] = sum;
+  if (tid == 0) pre[0] = 0;
+  // tokens of no row
+  if (first_token != 0 || last_token != a.n_tokens) {
+    const long long pieces = static_cast<long long>(a.heads) * D / 8;
+    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + tid; i < a.n_tokens * pieces;
+         i += static_cast<long long>(gridDim.x) * kThreads) {
+      const long long tok = i / pieces;
+      if (tok >= first_token && tok < last_token) continue;
+      reinterpret_cast<int4*>(a.out)[i] = make_int4(0, 0, 0, 0);
+      if (a.lse && i % (D / 8) == 0) a.lse[i / (D / 8)] = -INFINITY;
+    }
+  }
+  __syncthreads();
   const uint32_t tmem = tmem_slot;
   const uint32_t tmem_o = tmem + 2 * S::kS;
-  bool ok = true;
-  Task t;
+  const long long W = pre[kThreads];
+  const long long n_ctas = min(static_cast<long long>(gridDim.x), W);
+  const long long b = blockIdx.x;
+  bool ok = b < n_ctas;
+  // The next task, for the warps that do not load: false when there is none, or the wait ran out.
+  int task = 0;
+  const auto next = [&]() {
+    ok = wait_warp(&task_full[task % kTasks], (task / kTasks) & 1, a.status);
+    return ok && tasks[task % kTasks].n > 0;
+  };
+  const auto done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&task_empty[task % kTasks]);
+    ++task;
+  };
 
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
-    int i = 0;  // tiles so far
+    int i = 0, last = 0;  // tiles so far; tile i has the units 2 i (K) and 2 i + 1 (V); units issued
     const uint64_t once = l2_policy_evict_first();
-    const int nb = kTile / a.box, batch = 32 / nb;  // boxes of a tile, tiles of a batch
-    const int own_tile = lane / nb, k = lane - own_tile * nb;
-    while (ok && walk.next(a, t)) {
-      const int* table = a.row_tables + static_cast<long long>(t.row) * a.max_pages;
-      // the boxes of some tiles at a time, a lane each: where they lie and their scales
-      for (int tile = t.tile0; ok && tile < t.tile1; tile += batch) {
-        const int key = t.w.low + tile * kTile + lane * a.box;
-        int where = -1;
-        float ks = 0.0f, vs = 0.0f;
-        if (key < t.stop && key + a.box > t.start && tile + own_tile < t.tile1) {
-          const int c = key / P, page = table[c];
-          if (page >= 0 && page < a.n_pages) {
-            const int ph = page * a.kv_heads + t.hk;
-            where = ph * P + (key - c * P);
-            ks = a.k_scale[ph];
-            vs = a.v_scale[ph];
-          } else if (a.status) {
-            atomicOr(a.status, static_cast<int>(LB_DEV_BAD_PAGE));
-          }
+    uint64_t again;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(again));
+    const int nb = kTile / a.box;                            // boxes of a tile
+    const int own_tile = lane / nb, k = lane - own_tile * nb;  // a lane's box among those of a batch of tiles
+    const int batch = nb == 2 ? 8 : 32 / nb;
+    Walk<R> walk;
+    if (ok) walk.begin(a, pre, each, W * b / n_ctas, W * (b + 1) / n_ctas);
+    int known = 0;  // tasks made known
+    // Three batches are in hand, so that no load is waited for: the tables of the third, the scales of the second
+    // and the boxes of the first are under way together.  n 0: there are no more tasks.
+    struct Batch {
+      int task, tile, n;
+    };
+    const auto following = [&](const Batch& c) {
+      Batch d{c.task, c.tile + batch, c.n};
+      if (c.task >= 0 && (c.n == 0 || d.tile < c.n)) return d;
+      d.task = c.task + 1;
+      d.tile = 0;
+      if (d.task == known) {
+        Task t;
+        walk.next(a, W, n_ctas, t);
+        if (known >= kTasks) ok = wait_warp(&task_empty[known % kTasks], (known / kTasks - 1) & 1, a.status) && ok;
+        if (!ok) t.n = 0;
+        if (ok && lane == 0) {
+          tasks[known % kTasks] = t;
+          mbar_arrive(&task_full[known % kTasks]);
         }
-        const unsigned there = __ballot_sync(0xffffffffu, where >= 0);
-        float v_top = fabsf(vs);
-        for (int o = 1; o < nb; o <<= 1) v_top = max_nan(v_top, __shfl_xor_sync(0xffffffffu, v_top, o));
-        for (int j = 0; j < batch && tile + j < t.tile1; ++j, ++i) {
-          const int s = i % S::kStages;
-          if (i >= S::kStages) ok = mbar_wait(&empty[s], ((i / S::kStages) - 1) & 1, a.status);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const bool own = own_tile == j;
-          const unsigned mask = (there >> (j * nb)) & ((1u << nb) - 1u);
-          if (own) {
-            g_ks[s][k] = ks;
-            g_vs[s][k] = vs;
-            if (k == 0) {
-              g_there[s] = mask;
-              g_top[s] = v_top;
-            }
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(mask) * (2 * a.box * D));
-          __syncwarp();
-          if (own && where >= 0) {
-            unsigned char* kd = ring + s * 2 * S::kSide + k * a.box * S::kRow;
+        __syncwarp();
+        ++known;
+        d.n = t.n;
+      }
+      return d;
+    };
+    const auto box_key = [&](const Batch& c) {  // the first key of this lane's box, -1 where it has none
+      const Task& t = tasks[c.task % kTasks];
+      if (own_tile >= batch || c.tile + own_tile >= c.n) return -1;
+      const int key = t.low + (t.tile0 + c.tile) * kTile + lane * a.box;
+      return key < t.stop && key + a.box > t.start ? key : -1;
+    };
+    const auto page_at = [&](const Batch& c) {
+      const int key = box_key(c);
+      if (key < 0) return -1;
+      const int page = a.row_tables[static_cast<long long>(tasks[c.task % kTasks].row) * a.max_pages + key / P];
+      if (page >= 0 && page < a.n_pages) return page;
+      if (a.status) atomicOr(a.status, static_cast<int>(LB_DEV_BAD_PAGE));
+      return -1;
+    };
+    struct Where {
+      int at;  // row of the cache, -1: not there
+      float ks, vs;
+    };
+    const auto scales_at = [&](const Batch& c, int page) {
+      Where w{-1, 0.0f, 0.0f};
+      if (page >= 0) {
+        const int ph = page * a.kv_heads + tasks[c.task % kTasks].hk;
+        w.at = ph * P + box_key(c) % P;
+        w.ks = a.k_scale[ph];
+        w.vs = a.v_scale[ph];
+      }
+      return w;
+    };
+    Batch b0{-1, 0, 0}, b1;
+    int page1 = -1;
+    Where w0{-1, 0.0f, 0.0f};
+    if (ok) {
+      b0 = following(b0);
+      const int page0 = page_at(b0);
+      b1 = following(b0);
+      page1 = page_at(b1);
+      w0 = scales_at(b0, page0);
+    }
+#pragma unroll 1
+    while (ok && b0.n > 0) {
+      const Batch b2 = following(b1);
+      const int page2 = page_at(b2);
+      const Where w1 = scales_at(b1, page1);
+      const int tiles = min(batch, b0.n - b0.tile);
+      const uint64_t policy = tasks[b0.task % kTasks].q_tiles > 1 ? again : once;  // other query tiles read the same keys
+      const unsigned there = __ballot_sync(0xffffffffu, w0.at >= 0);
+      float v_top = fabsf(w0.vs);
+#pragma unroll 1
+      for (int o = 1; o < nb; o <<= 1) v_top = max_nan(v_top, __shfl_xor_sync(0xffffffffu, v_top, o));
+#pragma unroll 1
+      for (int j = 0; ok && j < tiles; ++j, ++i) {
+        const int info = i % kInfo;
+        const bool own = own_tile == j;
+        const unsigned mask = (there >> (j * nb)) & ((1u << nb) - 1u);
 #pragma unroll
-            for (int h = 0; h < S::kHalves; ++h) {
-              tma_load_2d(kd + h * S::kHalfBytes, &k_map, &full[s], h * 128, where, once);
-              tma_load_2d(kd + S::kSide + h * S::kHalfBytes, &v_map, &full[s], h * 128, where, once);
+        for (int side = 0; side < 2; ++side) {
+          const int u = 2 * i + side, s = u % S::kUnits;
+          if (ok && u >= S::kUnits) ok = wait_warp(&empty[s], (u / S::kUnits - 1) & 1, a.status);
+          if (!ok) break;
+          if (side == 0 && own) {
+            g_ks[info][k] = w0.ks;
+            g_vs[info][k] = w0.vs;
+            if (k == 0) {
+              g_there[info] = mask;
+              g_top[info] = v_top;
             }
           }
           __syncwarp();
+          if (lane == 0) {
+            if (side == 0) mbar_arrive(&g_full[info]);
+            mbar_arrive_expect_tx(&full[s], __popc(mask) * (a.box * D));
+          }
+          __syncwarp();
+          if (own && w0.at >= 0) {
+            unsigned char* d = ring + s * S::kSide + k * a.box * S::kRow;
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+              tma_load_2d(d + h * S::kHalfBytes, side ? &v_map : &k_map, &full[s], h * 128, w0.at, policy);
+          }
+          last = u + 1;
         }
       }
+      b0 = b1;
+      w0 = w1;
+      b1 = b2;
+      page1 = page2;
     }
     // loads that nobody waited for (after a wait that ran out) end before the CTA does
-    if (!ok)
-      for (int k = max(0, i - S::kStages); k < i; ++k) mbar_wait(&full[k % S::kStages], (k / S::kStages) & 1, a.status);
+    if (!ok && lane == 0)
+#pragma unroll 1
+      for (int u = max(0, last - S::kUnits); u < last; ++u) wait_one(&full[u % S::kUnits], (u / S::kUnits) & 1, a.status);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs of the scores: one thread
     constexpr uint32_t id = idesc_i8(128, S::kN1, false);
-    int i = 0, task = 0;
-    while (ok && walk.next(a, t)) {
+    int i = 0;
+    while (ok && next()) {
+      const int n_tiles = tasks[task % kTasks].n;
       if (lane == 0) {
-        const uint32_t q = smem_u32(q_digits);
-        ok = mbar_wait(&q_full, task & 1, a.status);
-        for (int tile = t.tile0; ok && tile < t.tile1; ++tile, ++i) {
-          const int s = i % S::kStages, buf = i & 1;
-          if (i >= 2) ok = mbar_wait(&s_empty[buf], ((i >> 1) - 1) & 1, a.status);
-          if (!ok || !(ok = mbar_wait(&full[s], (i / S::kStages) & 1, a.status))) break;
+        const uint32_t q = smem_u32(q_digits + (task & 1) * S::kQBytes);
+        ok = wait_one(&q_full[task & 1], (task >> 1) & 1, a.status);
+#pragma unroll 1
+        for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
+          const int u = 2 * i, s = u % S::kUnits, buf = i & 1;
+          if (i >= 2) ok = wait_one(&s_empty[buf], ((i >> 1) - 1) & 1, a.status);
+          if (!ok || !(ok = wait_one(&full[s], (u / S::kUnits) & 1, a.status))) break;
           tc_fence_after();
-          const uint32_t k = smem_u32(ring + s * 2 * S::kSide);
-#pragma unroll
-          for (int h = 0; h < S::kHalves; ++h)
-#pragma unroll
-            for (int n = 0; n < S::kRow / 32; ++n)
-              umma_i8(tmem + buf * S::kS, smem_desc<S::kRow>(k + h * S::kHalfBytes + n * 32),
-                      smem_desc<S::kRow>(q + h * S::kN1 * S::kRow + n * 32), id, h > 0 || n > 0);
+          uint64_t k = smem_desc<S::kRow>(smem_u32(ring + s * S::kSide)), qd = smem_desc<S::kRow>(q);
+#pragma unroll 1
+          for (int n = 0; n < D / 32; ++n) {  // 32 columns a step; every 128 the next half
+            umma_i8(tmem + buf * S::kS, k, qd, id, n > 0);
+            const bool next = S::kHalves > 1 && n % 4 == 3;
+            k += (next ? S::kHalfBytes - 96 : 32) >> 4;
+            qd += (next ? S::kN1 * S::kRow - 96 : 32) >> 4;
+          }
           umma_commit(&s_full[buf]);
+          umma_commit(&empty[s]);
         }
-        if (ok) umma_commit(&q_empty);
+        if (ok) umma_commit(&q_empty[task & 1]);
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
-      ++task;
+      done();
     }
   } else if (warp == 14) {
     // ---------------------------------------------------------------- MMAs of the outputs: one thread
     constexpr uint32_t id = idesc_i8(128, S::kN2, true);
     constexpr int B = S::kOutBuffers;
     int i = 0;
-    while (ok && walk.next(a, t)) {
+    while (ok && next()) {
+      const int n_tiles = tasks[task % kTasks].n;
       if (lane == 0) {
-        for (int tile = t.tile0; ok && tile < t.tile1; ++tile, ++i) {
-          const int s = i % S::kStages, buf = i & 1, ob = i % B;
-          if (i >= B) ok = mbar_wait(&o_empty[ob], (i / B - 1) & 1, a.status);
-          if (ok) ok = mbar_wait(&full[s], (i / S::kStages) & 1, a.status);
-          if (!ok || !(ok = mbar_wait(&p_full[buf], (i >> 1) & 1, a.status))) break;
+#pragma unroll 1
+        for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
+          const int u = 2 * i + 1, s = u % S::kUnits, buf = i & 1, ob = i % B;
+          if (i >= B) ok = wait_one(&o_empty[ob], (i / B - 1) & 1, a.status);
+          if (ok) ok = wait_one(&full[s], (u / S::kUnits) & 1, a.status);
+          if (!ok || !(ok = wait_one(&p_full[buf], (i >> 1) & 1, a.status))) break;
           tc_fence_after();
-          const uint32_t v = smem_u32(ring + s * 2 * S::kSide + S::kSide), p = smem_u32(p_digits + buf * S::kPBytes);
-#pragma unroll
-          for (int h = 0; h < S::kHalves; ++h)
-#pragma unroll
-            for (int n = 0; n < kTile / 32; ++n)
-              umma_i8(tmem_o + (ob * S::kHalves + h) * S::kN2,
-                      smem_desc<S::kRow>(v + h * S::kHalfBytes + n * 32 * S::kRow), smem_desc<128>(p + n * 32), id, n > 0);
+          uint64_t v = smem_desc<S::kRow>(smem_u32(ring + s * S::kSide));
+          const uint64_t p = smem_desc<128>(smem_u32(p_digits + buf * S::kPBytes));
+#pragma unroll 1
+          for (int n = 0; n < 4 * S::kHalves; ++n, v += 32 * S::kRow >> 4)  // 32 keys a step; the halves are neighbours
+            umma_i8(tmem_o + (ob * S::kHalves + n / 4) * S::kN2, v, p + (n % 4) * 2, id, n % 4 > 0);
           umma_commit(&o_full[ob]);
           umma_commit(&p_empty[buf]);
           umma_commit(&empty[s]);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
+      done();
     }
-  } else if (warp < 10) {
-    // ---------------------------------------------------------------- scores -> digits of p
-    const int side = (warp - 2) >> 2, wq = (warp - 2) & 3, sub = warp & 3, key_row = sub * 32 + lane;
-    const uint32_t scores = tmem + side * S::kS + (static_cast<uint32_t>(sub * 32) << 16);
-    unsigned char* p = p_digits + side * S::kPBytes;
-    constexpr int C = R < 16 ? R : 16;
-    int i = 0, task = 0;
-    while (ok && walk.next(a, t)) {
-      // ---- the task's q, in digits: kPer threads a query, four columns at a time
-      if (task > 0) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty, (task - 1) & 1, a.status));
+  } else if (warp == 15) {
+    // ---------------------------------------------------------------- q -> digits, a task ahead
+    constexpr int kE = D / 32;  // columns a lane
+    struct alignas(16) Columns {
+      uint16_t v[kE];
+    };
+    while (ok && next()) {
+      const Task t = tasks[task % kTasks];
+      const int buf = task & 1;
+      if (task >= 2) ok = wait_warp(&q_empty[buf], ((task >> 1) - 1) & 1, a.status);
       if (!ok) break;
-      constexpr int kPer = 256 / R < D / 4 ? 256 / R : D / 4, kE = D / kPer;
-      const int qi = (tid - 64) / kPer, d0 = (tid - 64) % kPer * kE;
-      if (qi < R) {  // whole warps: kPer divides 32, R * kPer is a multiple of 32
-        const int qr = t.qt * R + qi;
-        const bool live = qi < t.rows;
-        const int tok = live ? qr / G : 0;
-        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (t.w.begin + tok) * a.q_token_stride +
-                              (t.hk * G + (live ? qr - tok * G : 0)) * a.q_head_stride + d0;
-        const auto four = [&](int e, float (&v)[4]) {
-          uint16_t raw[4];
-          if (a.q_vec) {
-            const uint2 w = *reinterpret_cast<const uint2*>(src + e);
-            raw[0] = static_cast<uint16_t>(w.x);
-            raw[1] = static_cast<uint16_t>(w.x >> 16);
-            raw[2] = static_cast<uint16_t>(w.y);
-            raw[3] = static_cast<uint16_t>(w.y >> 16);
+      unsigned char* digits = q_digits + buf * S::kQBytes + (lane * kE / 128) * (S::kN1 * S::kRow);
+      const int col = lane * kE % 128;
+      int tok = t.qt * R / G, head = t.qt * R - tok * G;  // of the next row to load
+      const auto load = [&](int q) {
+        Columns c{};
+        if (q < t.rows) {
+          const uint16_t* src = static_cast<const uint16_t*>(a.q) + (t.begin + tok) * a.q_token_stride +
+                                (t.hk * G + head) * a.q_head_stride + lane * kE;
+          if (!a.q_vec) {
+#pragma unroll
+            for (int e = 0; e < kE; ++e) c.v[e] = src[e];
+          } else if constexpr (kE == 8) {
+            *reinterpret_cast<uint4*>(c.v) = *reinterpret_cast<const uint4*>(src);
+          } else if constexpr (kE == 4) {
+            *reinterpret_cast<uint2*>(c.v) = *reinterpret_cast<const uint2*>(src);
           } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) raw[c] = src[e + c];
+            *reinterpret_cast<uint32_t*>(c.v) = *reinterpret_cast<const uint32_t*>(src);
           }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) v[c] = to_f<T>(raw[c]);
-        };
-        float top = 0.0f;
-#pragma unroll 2
-        for (int e = 0; e < kE; e += 4) {
-          float v[4];
-          four(e, v);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) top = max_nan(top, fabsf(v[c]));
         }
+        if (++head == G) {
+          head = 0;
+          ++tok;
+        }
+        return c;
+      };
+      int pos = t.pos_low, left = G - head;  // of the row in hand, and rows of its token still to come
+      Columns r0 = load(0), r1 = load(1), r2 = load(2);  // three rows' loads are under way
+#pragma unroll 1
+      for (int qi = 0; qi < R; ++qi) {
+        const Columns raw = r0;
+        r0 = r1;
+        r1 = r2;
+        r2 = load(qi + 3);
+        uint32_t size = 0;  // absolute values by their bits: a NaN is above all
 #pragma unroll
-        for (int o = 1; o < kPer; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const bool use = live && top < INFINITY;  // no NaN either
+        for (int e = 0; e < kE; ++e) size = max(size, __float_as_uint(to_f<T>(raw.v[e])) & 0x7fffffffu);
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, size));
+        const bool fine = top < INFINITY;
         // 2^ex brings the maximum to [2^21, 2^22); in two factors, each inside the floating range
-        const int ex = use && top > 0.0f ? 21 + 127 - max(1, __float_as_int(top) >> 23) : 0;
+        const int ex = fine && top > 0.0f ? 21 + 127 - max(1, __float_as_int(top) >> 23) : 0;
         const int e1 = ex / 2, e2 = ex - e1;
         const float up1 = __int_as_float((127 + e1) << 23), up2 = __int_as_float((127 + e2) << 23);
-        if (d0 == 0) {
+        if (lane == 0) {
           const float down = __int_as_float((127 - e1) << 23) * (a.softcap > 0.0f ? a.scale / a.softcap : a.scale * kLog2e);
-          fac_s[qi] = top < INFINITY ? down * __int_as_float((127 - e2) << 23) : NAN;
-          const int pos = t.w.len - t.w.count + qr / G;
-          last_s[qi] = live ? min(pos, t.stop - 1) : t.stop - 1;
-          first_s[qi] = live && a.window ? pos - a.window + 1 : 0;
+          fac_s[buf][qi] = fine ? down * __int_as_float((127 - e2) << 23) : NAN;
+          last_s[buf][qi] = min(qi < t.rows ? pos : 0x7fffffff, t.stop - 1);
+          first_s[buf][qi] = qi < t.rows && a.window ? pos - a.window + 1 : 0;
         }
-#pragma unroll 1
-        for (int e = 0; e < kE; e += 4) {
-          float f[4];
-          four(e, f);
-          uint32_t w0 = 0, w1 = 0, w2 = 0;
+        if (--left == 0) {
+          left = G;
+          ++pos;
+        }
+        uint32_t w[3][kE / 4 > 0 ? kE / 4 : 1] = {};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int v = use ? __float2int_rn(f[c] * up1 * up2) : 0;
-            const uint32_t digits = (v + 0x8080) ^ 0x8080;  // bytes 0, 1, 2 (see the digits of p below)
-            w0 |= ((digits >> 16) & 0xff) << (8 * c);
-            w1 |= ((digits >> 8) & 0xff) << (8 * c);
-            w2 |= (digits & 0xff) << (8 * c);
-          }
-          const int d = d0 + e, h = d / 128, col = d - h * 128;
-          unsigned char* q = q_digits + h * S::kN1 * S::kRow;
-          *reinterpret_cast<uint32_t*>(q + swizzled<S::kRow>(qi * S::kRow + col)) = w0;
-          *reinterpret_cast<uint32_t*>(q + swizzled<S::kRow>((R + qi) * S::kRow + col)) = w1;
-          *reinterpret_cast<uint32_t*>(q + swizzled<S::kRow>((2 * R + qi) * S::kRow + col)) = w2;
+        for (int e = 0; e < kE; ++e) {
+          const int v = fine ? __float2int_rn(to_f<T>(raw.v[e]) * up1 * up2) : 0;
+          const uint32_t d = (v + 0x8080) ^ 0x8080;  // bytes 0, 1, 2 (see the digits of p below)
+#pragma unroll
+          for (int c = 0; c < 3; ++c) w[c][e / 4] |= ((d >> (16 - 8 * c)) & 0xffu) << (8 * (e & 3));
+        }
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+          unsigned char* to = digits + swizzled<S::kRow>((c * R + qi) * S::kRow + col);
+          if constexpr (kE == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[c][0], w[c][1]);
+          else if constexpr (kE == 4) *reinterpret_cast<uint32_t*>(to) = w[c][0];
+          else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(w[c][0]);
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
-      ok = __all_sync(0xffffffffu, mbar_wait(&q_full, task & 1, a.status));  // what the other warps know of the queries
-
-      float l[R];
+      if (lane == 0) mbar_arrive(&q_full[buf]);
+      done();
+    }
+  } else if (warp < 10) {
+    // ---------------------------------------------------------------- scores -> digits of p
+    // A turn is 8 queries of a tile; the two warpgroups take turns: with 8 query rows a tile each,
+    // with more a tile's queries.
+    const int side = (warp - 2) >> 2, wq = (warp - 2) & 3, sub = warp & 3, key_row = sub * 32 + lane;
+    const uint32_t lane_at = static_cast<uint32_t>(sub * 32) << 16;
+    constexpr int C = kQueries, kOwn = S::kTurns > 2 ? S::kTurns / 2 : 1;  // a warpgroup's turns of a tile
+    int i = 0, turn = 0;
+    while (ok && next()) {
+      const Task& t = tasks[task % kTasks];
+      const int n_tiles = t.n, first_key = t.low + t.tile0 * kTile;
+      const int plain_stop = min(t.pos_low + 1, t.stop), plain_start = a.window ? t.pos_high - a.window + 1 : 0;  // keys all queries see
+      const int qb = task & 1;
+      ok = wait_warp(&q_full[qb], (task >> 1) & 1, a.status);  // what is known of the queries
+      float l[kOwn][C];
+      float ref[kOwn];  // lane q: the reference maximum of query q (the four warps keep the same)
 #pragma unroll
-      for (int q = 0; q < R; ++q) l[q] = 0.0f;
-      float ref = -INFINITY;  // lane q: the reference maximum of query q (the four warps keep the same)
-      for (int tile = t.tile0; ok && tile < t.tile1; ++tile, ++i) {
-        if ((i & 1) != side) continue;
-        const int s = i % S::kStages, phase = (i >> 1) & 1;
-        ok = mbar_wait(&full[s], (i / S::kStages) & 1, a.status);
-        if (ok) ok = mbar_wait(&s_full[side], phase, a.status);
+      for (int k = 0; k < kOwn; ++k) {
+        ref[k] = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < C; ++q) l[k][q] = 0.0f;
+      }
+#pragma unroll 1
+      for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
+        if (S::kTurns == 1 && (i & 1) != side) continue;
+        const int buf = i & 1, phase = (i >> 1) & 1, info = i % kInfo;
+        ok = wait_one(&g_full[info], (i / kInfo) & 1, a.status);  // the tile's scales
+        ok = wait_warp(&s_full[buf], phase, a.status) && ok;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         const int grp = key_row / a.box;
-        const float ks = g_ks[s][grp], vs = g_vs[s][grp], v_top = g_top[s];
-        const bool there = (g_there[s] >> grp) & 1u;
-        float x[R];
-#pragma unroll
-        for (int c0 = 0; c0 < R; c0 += C) {
-          int d2[C], d1[C], dd[C];
-          tmem_ld3<C>(scores + c0, scores + R + c0, scores + 2 * R + c0, d2, d1, dd);
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-            x[c0 + c] = fmaf(__int2float_rn(d2[c]), 65536.0f, __int2float_rn(d1[c] * 256 + dd[c])) * (ks * fac_s[c0 + c]);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[side]);
-        if (a.softcap > 0.0f) {
-#pragma unroll
-          for (int q = 0; q < R; ++q)  // tanh(u) = 1 - 2 / (1 + e^2u)
-            x[q] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + exp2_fast(x[q] * (2.0f * kLog2e))));
-        }
-        const int key0 = t.w.low + tile * kTile, key = key0 + key_row;
-        if (key0 + kTile > min(t.pos_low + 1, t.stop) || (a.window && key0 <= t.pos_high - a.window) ||
-            __any_sync(0xffffffffu, !there)) {
-#pragma unroll
-          for (int q = 0; q < R; ++q)
-            if (!there || key > last_s[q] || key < first_s[q]) x[q] = -INFINITY;
-        }
-        // the tile's largest score of each query: warp, then the four warps
-        float mx = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < R; ++q) {
-          const float m = warp_top(x[q]);
-          if (lane == q) mx = m;
-        }
-        if (lane < R) tops_s[side][wq][lane] = mx;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tops[side]);
-        ok = mbar_wait(&tops[side], phase, a.status);
-        if (ok && i >= 2) ok = mbar_wait(&p_empty[side], phase ^ 1, a.status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        float alpha = 1.0f;
-        if (lane < R) {
-          mx = max_nan(max_nan(tops_s[side][0][lane], tops_s[side][1][lane]),
-                       max_nan(tops_s[side][2][lane], tops_s[side][3][lane]));
-          if (ref == -INFINITY) {
-            ref = mx;
-          } else if (mx > ref + kSlack) {
-            alpha = exp2_fast(ref - mx);
-            ref = mx;
-          }
-          top_s[warp - 2][lane] = mx == -INFINITY ? 0.0f : mx;
-          beta_s[warp - 2][lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref);
-          if (wq == 0) mx_ring[i & 3][lane] = mx;
-        }
-        if (wq == 0 && lane == 0) v_ring[i & 3] = v_top;
-        const bool moved = __any_sync(0xffffffffu, alpha != 1.0f);
-        __syncwarp();
-        if (wq == 0 && lane == 0) mbar_arrive(&f_full[i & 3]);
-        if (moved) {
-#pragma unroll
-          for (int q = 0; q < R; ++q) l[q] *= __shfl_sync(0xffffffffu, alpha, q);
-        }
+        const float ks = g_ks[info][grp], vs = g_vs[info][grp], v_top = g_top[info];
+        const bool there = (g_there[info] >> grp) & 1u;
+        const int key0 = first_key + tile * kTile, key = key0 + key_row;
+        const bool masked = key0 + kTile > plain_stop || key0 < plain_start || __any_sync(0xffffffffu, !there);
         const float to_fixed = v_top > 0.0f ? __fdividef(vs, v_top) * kFixed : 0.0f;
+        unsigned char* p = p_digits + buf * S::kPBytes;
 #pragma unroll
-        for (int q = 0; q < R; ++q) {
-          const float e = exp2_fast(x[q] - top_s[warp - 2][q]);
-          l[q] = fmaf(e, beta_s[warp - 2][q], l[q]);
-          // v = rint(e * to_fixed) by a sum with 1.5 * 2^23.  With 128 added to each of the two lower
-          // digits' places, the bytes of v are its signed digits, the lower two with the sign bit turned over.
-          const uint32_t v = __float_as_uint(fmaf(e, to_fixed, 12582912.0f)) - 0x4B400000u;
-          const uint32_t digits = (v + 0x8080u) ^ 0x8080u;
-          p[swizzled<128>(q * kTile + key_row)] = static_cast<unsigned char>(digits >> 16);
-          p[swizzled<128>((R + q) * kTile + key_row)] = static_cast<unsigned char>(digits >> 8);
-          p[swizzled<128>((2 * R + q) * kTile + key_row)] = static_cast<unsigned char>(digits);
+        for (int k = 0; k < kOwn; ++k, ++turn) {
+          const int c0 = S::kTurns == 1 ? 0 : (2 * k + side) * C;  // the turn's first query
+          float x[C];
+          {
+            int d2[C], d1[C], dd[C];
+            const uint32_t at = tmem + buf * S::kS + lane_at + c0;
+            tmem_ld3<C>(at, at + R, at + 2 * R, d2, d1, dd);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+              x[c] = fmaf(__int2float_rn(d2[c]), 65536.0f, __int2float_rn(d1[c] * 256 + dd[c])) * (ks * fac_s[qb][c0 + c]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[buf]);
+          if (a.softcap > 0.0f) {
+#pragma unroll
+            for (int q = 0; q < C; ++q)  // tanh(u) = 1 - 2 / (1 + e^2u)
+              x[q] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + exp2_fast(x[q] * (2.0f * kLog2e))));
+          }
+          if (masked) {
+#pragma unroll
+            for (int q = 0; q < C; ++q)
+              if (!there || key > last_s[qb][c0 + q] || key < first_s[qb][c0 + q]) x[q] = -INFINITY;
+          }
+          // the turn's largest score of each query: warp, then the four warps
+          float mx = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < C; ++q) {
+            const float m = warp_top(x[q]);
+            if (lane == q) mx = m;
+          }
+          if (lane < C) tops_s[side][turn & 1][wq][lane] = mx;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tops[side]);
+          if (k == 0 && i >= 2) ok = wait_one(&p_empty[buf], phase ^ 1, a.status);
+          ok = wait_warp(&tops[side], turn & 1, a.status) && ok;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          float alpha = 1.0f;
+          if (lane < C) {
+            const float* w0 = tops_s[side][turn & 1][0];
+            mx = max_nan(max_nan(w0[lane], w0[C + lane]), max_nan(w0[2 * C + lane], w0[3 * C + lane]));
+            if (ref[k] == -INFINITY) {
+              ref[k] = mx;
+            } else if (mx > ref[k] + kSlack) {
+              alpha = exp2_fast(ref[k] - mx);
+              ref[k] = mx;
+            }
+            top_s[warp - 2][lane] = mx == -INFINITY ? 0.0f : mx;
+            beta_s[warp - 2][lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref[k]);
+            if (wq == 0) mx_ring[i & 3][c0 + lane] = mx;
+          }
+          if (wq == 0 && lane == 0 && c0 == 0) v_ring[i & 3] = v_top;
+          const bool moved = __any_sync(0xffffffffu, alpha != 1.0f);
+          __syncwarp();
+          if (wq == 0 && lane == 0) mbar_arrive(&f_full[i & 3]);
+          if (moved) {
+#pragma unroll
+            for (int q = 0; q < C; ++q) l[k][q] *= __shfl_sync(0xffffffffu, alpha, q);
+          }
+#pragma unroll
+          for (int q = 0; q < C; ++q) {
+            const float e = exp2_fast(x[q] - top_s[warp - 2][q]);
+            l[k][q] = fmaf(e, beta_s[warp - 2][q], l[k][q]);
+            // v = rint(e * to_fixed) by a sum with 1.5 * 2^23.  With 128 added to each of the two lower
+            // digits' places, the bytes of v are its signed digits, the lower two with the sign bit turned over.
+            const uint32_t v = __float_as_uint(fmaf(e, to_fixed, 12582912.0f)) - 0x4B400000u;
+            const uint32_t digits = (v + 0x8080u) ^ 0x8080u;
+            unsigned char* to = p + swizzled<128>(q * kTile + key_row) + c0 * kTile;  // (c0 is a multiple of 8 rows)
+            to[0] = static_cast<unsigned char>(digits >> 16);
+            to[R * kTile] = static_cast<unsigned char>(digits >> 8);
+            to[2 * R * kTile] = static_cast<unsigned char>(digits);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[buf]);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[side]);
       }
       // ---- the task's sums
-      if (ok && task > 0) ok = mbar_wait(&l_empty, (task - 1) & 1, a.status);
-      ok = __all_sync(0xffffffffu, ok);
+      if (ok && task > 0) ok = wait_warp(&l_empty, (task - 1) & 1, a.status);
       if (!ok) break;
 #pragma unroll
-      for (int q = 0; q < R; ++q) {
-        const float v = warp_sum(l[q]);
-        if (lane == q) l_part[warp - 2][q] = v;
+      for (int k = 0; k < kOwn; ++k) {
+        const int c0 = S::kTurns == 1 ? 0 : (2 * k + side) * C;
+        // eight sums over the warp at once: a half of them, by a bit of the lane, goes on at each step
+#pragma unroll
+        for (int o = 16; o >= 4; o >>= 1) {
+          const bool high = lane & o;
+#pragma unroll
+          for (int q = 0; q < o / 4; ++q) {
+            const float give = high ? l[k][q] : l[k][q + o / 4], keep = high ? l[k][q + o / 4] : l[k][q];
+            l[k][q] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+        }
+        float sum_q = l[k][0] + __shfl_xor_sync(0xffffffffu, l[k][0], 2);
+        sum_q += __shfl_xor_sync(0xffffffffu, sum_q, 1);
+        if ((lane & 3) == 0) l_part[warp - 2][c0 + lane / 4] = sum_q;
+        if (wq == 0 && lane < C) m_ref[side][c0 + lane] = ref[k];
       }
-      if (wq == 0 && lane < R) m_ref[side][lane] = ref;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&l_full);
-      ++task;
+      if (lane == 0) {
+        mbar_arrive(&q_empty[qb]);
+        mbar_arrive(&l_full);
+      }
+      done();
     }
   } else {
     // ---------------------------------------------------------------- outputs
     const int sub = warp & 3, col = sub * 32 + lane;
     const uint32_t lane_at = static_cast<uint32_t>(sub * 32) << 16;
-    constexpr int C = R < 16 ? R : 16;
+    constexpr int C = kQueries;
     float* factor = out_f[sub];
-    int i = 0, task = 0;
-    while (ok && walk.next(a, t)) {
+    int i = 0;
+    while (ok && next()) {
+      const Task& t = tasks[task % kTasks];
+      const int n_tiles = t.n;
       float o[S::kHalves][R];
 #pragma unroll
       for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
         for (int q = 0; q < R; ++q) o[h][q] = 0.0f;
       float ref = -INFINITY;  // lane q: the reference maximum of query q
-      for (int tile = t.tile0; ok && tile < t.tile1; ++tile, ++i) {
+#pragma unroll 1
+      for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
         const int buf = i % S::kOutBuffers;
-        ok = __all_sync(0xffffffffu, mbar_wait(&f_full[i & 3], (i >> 2) & 1, a.status));
+        ok = wait_warp(&f_full[i & 3], (i >> 2) & 1, a.status);
         if (!ok) break;
         float alpha = 1.0f;
         if (lane < R) {
@@ -707,7 +871,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
             for (int h = 0; h < S::kHalves; ++h) o[h][q] *= f;
           }
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[buf], (i / S::kOutBuffers) & 1, a.status));
+        ok = wait_warp(&o_full[buf], (i / S::kOutBuffers) & 1, a.status);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -726,24 +890,25 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_empty[buf]);
       }
-      if (ok) ok = mbar_wait(&l_full, task & 1, a.status);
-      ok = __all_sync(0xffffffffu, ok);
+      if (ok) ok = wait_warp(&l_full, task & 1, a.status);
       if (!ok) break;
       // lane q: the query's sum, its inverse, where it goes
       float l = 0.0f;
-      long long to = 0;
+      int to = 0;  // (the entry refuses more than 2^31 rows)
       if (lane < t.rows) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
+          if (S::kTurns > 1 && k != ((lane / C) & 1)) continue;  // the query's own warpgroup
           const float part = l_part[4 * k][lane] + l_part[4 * k + 1][lane] + l_part[4 * k + 2][lane] + l_part[4 * k + 3][lane];
           if (part != 0.0f) l += part * exp2_fast(m_ref[k][lane] - ref);
         }
         const int qr = t.qt * R + lane;
-        to = static_cast<long long>(t.w.begin + qr / G) * a.heads + t.hk * G + qr % G;
+        to = (t.begin + qr / G) * a.heads + t.hk * G + qr % G;
       }
-      const bool whole = t.from_start() && t.to_end();
-      float* part = a.parts + (2 * b + (t.from_start() ? 1 : 0)) * S::kPart;
-      if (lane < t.rows && sub == 0) {
+      const int rows = t.rows;
+      const bool whole = t.from_start && t.to_end;
+      float* part = a.parts + (2 * b + (t.from_start ? 1 : 0)) * S::kPart;
+      if (lane < rows && sub == 0) {
         if (!whole) {
           part[R * D + lane] = ref;
           part[R * D + R + lane] = l;
@@ -751,28 +916,32 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
           a.lse[to] = l != 0.0f ? (ref + log2f(l)) * kLn2 : -INFINITY;
         }
       }
-      const float inv = whole ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+      if (whole) {
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + col;
 #pragma unroll
-      for (int q = 0; q < R; ++q) {
-        if (q >= t.rows) break;
-        const float f = __shfl_sync(0xffffffffu, inv, q);
-        const long long at = __shfl_sync(0xffffffffu, to, q);
-        if (col < D) {
+        for (int q = 0; q < R; ++q) {
+          const float f = __shfl_sync(0xffffffffu, inv, q);
+          uint16_t* d = out + static_cast<long long>(__shfl_sync(0xffffffffu, to, q)) * D;
+          if (q < rows && col < D) {
 #pragma unroll
-          for (int h = 0; h < S::kHalves; ++h) {
-            if (whole) static_cast<uint16_t*>(a.out)[at * D + h * 128 + col] = to_bits<T>(o[h][q] * f);
-            else part[q * D + h * 128 + col] = o[h][q];
+            for (int h = 0; h < S::kHalves; ++h) d[h * 128] = to_bits<T>(o[h][q] * f);
+          }
+        }
+      } else if (col < D) {
+        float* d = part + col;
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+          if (q < rows) {
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h) d[q * D + h * 128] = o[h][q];
           }
         }
       }
-      if (t.from_start() && !t.to_end() && sub == 0 && lane == 0) {
-        // the last CTA of the task: the one whose share holds its last tile
-        const long long last = t.next + (t.w.tiles - t.tile1) - 1;
-        a.cuts[b] = make_int4(t.row, t.hk, t.qt, static_cast<int>(((last + 1) * n_ctas - 1) / W));
-      }
+      if (t.from_start && !t.to_end && sub == 0 && lane == 0) a.cuts[b] = make_int4(t.row, t.hk, t.qt, t.last_cta);
       __syncwarp();
       if (lane == 0) mbar_arrive(&l_empty);
-      ++task;
+      done();
     }
   }
   __syncwarp();
@@ -785,51 +954,59 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
 }
 
 // Joins the parts of the task that is cut at the end of CTA blockIdx.x: query row
-// blockIdx.y.  Lanes over columns, the groups of lanes over parts, then the groups' sums in order.
+// blockIdx.y.  First the parts' weights, a thread each, then groups of lanes (over columns) over the
+// parts, then the groups' sums in order.
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(256) combine_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(512) combine_kernel(const AttendArgs a) {
   using S = Shape<D, R>;
-  constexpr int kLanes = D / 4, kParts = 256 / kLanes;
+  constexpr int kLanes = D / 4, kParts = 512 / kLanes;
   __shared__ float4 sum_o[kParts][kLanes];
-  __shared__ float sum_l[kParts], sum_m[kParts];
+  __shared__ float weight[kSms];
+  __shared__ float top_w[8], sum_w[8];
   pdl_wait();
   const int4 cut = a.cuts[blockIdx.x];
   if (cut.x < 0) return;
-  const int G = a.heads / a.kv_heads, r = blockIdx.y, qr = cut.z * R + r;
+  const int G = a.heads / a.kv_heads, r = blockIdx.y, qr = cut.z * R + r, tid = threadIdx.x;
   const Row w = row_of<R>(a, cut.x);
   if (qr >= w.count * G) return;
-  const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const int first = blockIdx.x, n = cut.w - first + 1;
+  const int first = blockIdx.x, n = cut.w - first + 1;  // at most kSms parts
+  const auto part = [&](int i) { return a.parts + (2ll * (first + i) + (i == 0 ? 1 : 0)) * S::kPart; };
+  // a thread a part: its maximum and sum, then its weight
   float m = -INFINITY, l = 0.0f;
+  if (tid < n) {
+    m = part(tid)[R * D + r];
+    l = part(tid)[R * D + R + r];
+  }
+  float top = warp_max(m);
+  if ((tid & 31) == 0 && tid < 256) top_w[tid >> 5] = top;
+  __syncthreads();
+  top = top_w[0];
+#pragma unroll
+  for (int k = 1; k < (kSms + 31) / 32; ++k) top = fmaxf(top, top_w[k]);
+  const float f = tid < n && !(m == -INFINITY && l == 0.0f) ? exp2_fast(m - top) : 0.0f;
+  if (tid < n) weight[tid] = f;
+  l = warp_sum(f != 0.0f ? l * f : 0.0f);
+  if ((tid & 31) == 0 && tid < 256) sum_w[tid >> 5] = l;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < (kSms + 31) / 32; ++k) l += sum_w[k];
+  const int lane = tid % kLanes, grp = tid / kLanes;
   float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
   for (int i = grp; i < n; i += kParts) {
-    const float* part = a.parts + (2ll * (first + i) + (i == 0 ? 1 : 0)) * S::kPart;
-    const float pm = part[R * D + r], pl = part[R * D + R + r];
-    const float4 z = *reinterpret_cast<const float4*>(part + r * D + lane * 4);
-    if (pm == -INFINITY && pl == 0.0f) continue;
-    const float top = fmaxf(m, pm);
-    const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top), pf = exp2_fast(pm - top);
-    l = l * f + pl * pf;
-    y = make_float4(y.x * f + z.x * pf, y.y * f + z.y * pf, y.z * f + z.z * pf, y.w * f + z.w * pf);
-    m = top;
+    const float4 z = *reinterpret_cast<const float4*>(part(i) + r * D + lane * 4);
+    const float c = weight[i];
+    if (c != 0.0f) y = make_float4(fmaf(z.x, c, y.x), fmaf(z.y, c, y.y), fmaf(z.z, c, y.z), fmaf(z.w, c, y.w));
   }
   sum_o[grp][lane] = y;
-  if (lane == 0) {
-    sum_m[grp] = m;
-    sum_l[grp] = l;
-  }
   __syncthreads();
   if (grp != 0) return;
-  float top = -INFINITY;
-  for (int k = 0; k < kParts; ++k) top = fmaxf(top, sum_m[k]);
-  l = 0.0f;
   y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
   for (int k = 0; k < kParts; ++k) {
-    if (sum_m[k] == -INFINITY && sum_l[k] == 0.0f) continue;
-    const float f = exp2_fast(sum_m[k] - top);
     const float4 z = sum_o[k][lane];
-    l += sum_l[k] * f;
-    y = make_float4(y.x + z.x * f, y.y + z.y * f, y.z + z.z * f, y.w + z.w * f);
+    y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
   }
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   const long long to = static_cast<long long>(w.begin + qr / G) * a.heads + cut.y * G + qr % G;
@@ -856,7 +1033,7 @@ cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensor
   attend_kernel<T, D, R><<<kSms, kThreads, S::kSmem, s>>>(a, k_map, v_map);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return launch_kernel(true, combine_kernel<T, D, R>, dim3(kSms, R), dim3(256), 0, s, a);
+  return launch_kernel(true, combine_kernel<T, D, R>, dim3(kSms, R), dim3(512), 0, s, a);
 }
 template <typename T, int D>
 cudaError_t launch(const AttendArgs& a, int rows, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
