@@ -27,7 +27,7 @@
 // Warp roles: 0 loads (TMA boxes of 64 keys, or of the largest power of two that divides a
 // page), 1 issues the MMAs of the scores, 14 those of the outputs (a thread that waits on a
 // barrier before each tile's MMAs loses some 500 cycles to it, so the two do not share one),
-// 15 splits the next task's q into digits while the present one runs, 2-5 and 6-9 turn scores
+// 3 splits the next task's q into digits while the present one runs, 2-5 and 6-9 turn scores
 // into digits of p (a thread a key: tensor memory's lanes), 8 queries at a time (more of them unrolled
 // outgrow the instruction cache: 16 took 6.9 thousand cycles a tile, 8 take 2.5), 10-13 add up the
 // outputs (a thread a column).  K and V lie in one ring of units of 128 keys, K freed by its
@@ -43,6 +43,9 @@ constexpr int kThreads = 512;
 constexpr int kTile = 128;   // keys of a tile: the lanes of the tensor memory
 constexpr int kBoxes = 8;    // most TMA boxes of a tile (pages are multiples of 16)
 constexpr int kQueries = 8;    // queries of a score warpgroup's turn
+constexpr int kScorers = 2;    // score warpgroups
+constexpr int kFirstScorer = 4, kFirstOutput = 12;  // warps
+constexpr int kRing = 8;       // tiles whose largest scores are kept: more than the digits' and outputs' buffers together
 constexpr int kTasks = 8;      // tasks that the loading warp may be ahead
 constexpr int kInfo = 16;      // tiles whose scales are kept: more than the ring's units reach ahead
 constexpr int kSms = 148;
@@ -62,7 +65,7 @@ struct AttendArgs {
   const int *row_tables, *kv_len, *cu_tokens;
   float scale, softcap;
   int window, q_vec;
-  int box;  // keys of a TMA box: 16, 32 or 64, a divisor of page_tokens
+  int box, box_log;  // keys of a TMA box: 16, 32 or 64, a divisor of page_tokens
   void* out;
   float* lse;
   int* status;
@@ -79,16 +82,18 @@ struct Shape {
   static constexpr int kN1 = R == 8 ? 32 : 3 * R;           // score columns: three digits (8 rows: and 8 of padding)
   static constexpr int kN2 = kN1;                           // output columns: three digits
   static constexpr int kS = (kN1 + 31) / 32 * 32;           // tensor-memory columns of a score buffer
-  static constexpr int kOutBuffers = 2 * kS + 2 * kHalves * kN2 <= 512 ? 2 : 1;
-  static constexpr int kColumns = 2 * kS + kOutBuffers * kHalves * kN2;
+  static constexpr int kBuffers = 4 * kS + 2 * kHalves * kN2 <= 512 ? 4 : 2;  // of scores and of digits of p
+  static constexpr int kColumns = kBuffers * kS + 2 * kHalves * kN2;
+  static_assert(kColumns <= 512, "tensor memory");
   static constexpr int kAlloc = kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
   static constexpr int kQBytes = (kHalves * kN1 * kRow + 1023) / 1024 * 1024;
   static constexpr int kPBytes = kN2 * kTile;
-  static constexpr int kFixedBytes = 2 * kQBytes + 2 * kPBytes + 1024;
-  static constexpr int kRoom = (217 * 1024 - kFixedBytes) / kSide;
+  static constexpr int kFixedBytes = 2 * kQBytes + kBuffers * kPBytes + 1024;
+  static constexpr int kRoom = (213 * 1024 - kFixedBytes) / kSide;  // (up to 14 KB are declared beside it)
   static constexpr int kUnits = kRoom < kInfo ? kRoom : kInfo;  // (a tile's scales outlive its units)
   static constexpr int kSmem = kFixedBytes + kUnits * kSide;
-  static constexpr int kTurns = R / kQueries;  // of the score warpgroups, a tile
+  static constexpr int kTurns = R / kQueries;             // of the score warpgroups, a tile
+  static constexpr int kEvery = kScorers / kTurns;        // a warpgroup takes its turn in every so many tiles
   static constexpr int kPart = R * D + 2 * R;
 };
 
@@ -142,33 +147,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Waits for a phase, at most kWaitLimitNs (common.cuh).  One copy for all roles: the kernel's code has to
-// stay small, since sixteen warps in six roles share the SM's instruction cache.  try_wait sleeps in
-// hardware, so a waiting warp takes few issue slots.
-__device__ __noinline__ bool wait_phase(uint32_t bar, uint32_t parity, int* status) {
-  const unsigned long long start = globaltimer_ns();
-  while (true) {
+// Waits for a phase.  Bounded by the number of polls: try_wait sleeps in hardware, for up to the 20 us
+// that it is given, so the limit is at most 2.6 s.  Kept short, because all roles
+// together are bound by the instructions they issue.
+constexpr int kPolls = 1 << 17;
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_u32(bar);
+#pragma unroll 1
+  for (int n = 0; n < kPolls; ++n) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
-        : "r"(bar), "r"(parity), "r"(20000u)
+        : "r"(at), "r"(parity), "r"(20000u)
         : "memory");
     if (done) return true;
-    if (globaltimer_ns() - start > kWaitLimitNs) {
-      if (status) atomicOr(status, kStatusWaitTimeout);
-      return false;
-    }
   }
-}
-__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, int* status) {
-  return mbar_try_wait(bar, parity) || wait_phase(smem_u32(bar), parity, status);
+  return false;
 }
 // by a whole warp: the same answer for every lane
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* status) {
-  return __all_sync(0xffffffffu, wait_one(bar, parity, status));
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_one(bar, parity));
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) { return (a > b || isnan(a)) ? a : b; }
@@ -252,7 +253,7 @@ struct Walk {
     held = row_of<R>(a, win + (threadIdx.x & 31));
     upto = warp_prefix(row_work(a, held));
   }
-  __device__ __forceinline__ bool next(const AttendArgs& a, long long line, long long n_ctas, Task& t) {
+  __device__ __noinline__ bool next(const AttendArgs& a, long long line, long long n_ctas, Task& t) {
     if (x >= x_end) {
       t.n = 0;
       return false;
@@ -304,12 +305,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
                                                              const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D, R>;
   extern __shared__ unsigned char attend_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(attend_raw) + 1023) & ~uintptr_t(1023));
+  // 1024-byte aligned (an offset, not a cast of the address: the accesses stay shared-memory ones)
+  unsigned char* smem = attend_raw + ((1024 - (smem_u32(attend_raw) & 1023)) & 1023);
   unsigned char* ring = smem;                                  // [unit][half][128 keys][kRow]
   unsigned char* q_digits = ring + S::kUnits * S::kSide;       // [buffer][half][digit * R + query][kRow]
   unsigned char* p_digits = q_digits + 2 * S::kQBytes;         // [buffer][digit * R + query][128 keys]
-  __shared__ uint64_t full[S::kUnits], empty[S::kUnits], s_full[2], s_empty[2], p_full[2], p_empty[2], o_full[2], o_empty[2];
-  __shared__ uint64_t g_full[kInfo], q_full[2], q_empty[2], f_full[4], tops[2], l_full, l_empty;
+  __shared__ uint64_t full[S::kUnits], empty[S::kUnits], o_full[2], o_empty[2];
+  __shared__ uint64_t s_full[S::kBuffers], s_empty[S::kBuffers], p_full[S::kBuffers], p_empty[S::kBuffers];
+  __shared__ uint64_t q_full[2], q_empty[2], tops[kScorers], l_full, l_empty;
   __shared__ uint64_t task_full[kTasks], task_empty[kTasks];
   __shared__ Task tasks[kTasks];
   __shared__ uint32_t tmem_slot;
@@ -319,11 +322,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   __shared__ unsigned g_there[kInfo];
   __shared__ __align__(16) float fac_s[2][R];    // a query: its factor to log2 scores, and the keys that it sees
   __shared__ int last_s[2][R], first_s[2][R];
-  __shared__ float tops_s[2][2][4][kQueries];    // [warpgroup][turn]: a turn's largest scores, by warp
-  __shared__ __align__(16) float top_s[8][kQueries], beta_s[8][kQueries];
-  __shared__ float mx_ring[4][R], v_ring[4];     // a tile's largest scores and largest V scale
+  __shared__ float tops_s[kScorers][2][4][kQueries];  // a turn's largest scores, by warp
+  __shared__ __align__(16) float top_s[4 * kScorers][kQueries], beta_s[4 * kScorers][kQueries];
+  __shared__ __align__(16) float factor_s[4 * kScorers][kQueries];
+  __shared__ float mx_ring[kRing][R], v_ring[kRing];  // a tile's largest scores and largest V scale
   __shared__ __align__(16) float out_f[4][R];
-  __shared__ float l_part[8][R], m_ref[2][R];
+  __shared__ float l_part[4 * kScorers][kQueries], m_ref[kScorers][kQueries];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.heads / a.kv_heads, P = a.page_tokens;
 
@@ -337,24 +341,24 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&s_full[b], 1);
+    for (int b = 0; b < S::kBuffers; ++b) {
+      mbar_init(&s_full[b], 2);  // the MMAs, and the thread that saw the tile's scales
       mbar_init(&s_empty[b], 4 * S::kTurns);
       mbar_init(&p_full[b], 4 * S::kTurns);
       mbar_init(&p_empty[b], 1);
-      mbar_init(&o_full[b], 1);
-      mbar_init(&o_empty[b], 4);
-      mbar_init(&tops[b], 4);
-      mbar_init(&q_full[b], 1);
-      mbar_init(&q_empty[b], 9);
     }
-    for (int b = 0; b < 4; ++b) mbar_init(&f_full[b], S::kTurns);
-    for (int b = 0; b < kInfo; ++b) mbar_init(&g_full[b], 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&o_full[b], 2);  // the MMAs, and the thread that saw the tile's largest scores
+      mbar_init(&o_empty[b], 4);
+      mbar_init(&q_full[b], 1);
+      mbar_init(&q_empty[b], 1 + 4 * kScorers);
+    }
+    for (int b = 0; b < kScorers; ++b) mbar_init(&tops[b], 4);
     for (int b = 0; b < kTasks; ++b) {
       mbar_init(&task_full[b], 1);
-      mbar_init(&task_empty[b], 15);
+      mbar_init(&task_empty[b], 3 + 4 * kScorers + 4);
     }
-    mbar_init(&l_full, 8);
+    mbar_init(&l_full, 4 * kScorers);
     mbar_init(&l_empty, 4);
     fence_barrier_init();
     a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   }
   __syncthreads();
   const uint32_t tmem = tmem_slot;
-  const uint32_t tmem_o = tmem + 2 * S::kS;
+  const uint32_t tmem_o = tmem + S::kBuffers * S::kS;
   const long long W = pre[kThreads];
   const long long n_ctas = min(static_cast<long long>(gridDim.x), W);
   const long long b = blockIdx.x;
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   // The next task, for the warps that do not load: false when there is none, or the wait ran out.
   int task = 0;
   const auto next = [&]() {
-    ok = wait_warp(&task_full[task % kTasks], (task / kTasks) & 1, a.status);
+    ok = wait_warp(&task_full[task % kTasks], (task / kTasks) & 1);
     return ok && tasks[task % kTasks].n > 0;
   };
   const auto done = [&]() {
@@ -417,6 +421,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     int i = 0, last = 0;  // tiles so far; tile i has the units 2 i (K) and 2 i + 1 (V); units issued
+    int s = 0;  // the next unit, and the phase of the ring's turn before
+    uint32_t turn = 1;
     const uint64_t once = l2_policy_evict_first();
     uint64_t again;
     asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(again));
@@ -439,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       if (d.task == known) {
         Task t;
         walk.next(a, W, n_ctas, t);
-        if (known >= kTasks) ok = wait_warp(&task_empty[known % kTasks], (known / kTasks - 1) & 1, a.status) && ok;
+        if (known >= kTasks) ok = wait_warp(&task_empty[known % kTasks], (known / kTasks - 1) & 1) && ok;
         if (!ok) t.n = 0;
         if (ok && lane == 0) {
           tasks[known % kTasks] = t;
@@ -507,8 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         const unsigned mask = (there >> (j * nb)) & ((1u << nb) - 1u);
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-          const int u = 2 * i + side, s = u % S::kUnits;
-          if (ok && u >= S::kUnits) ok = wait_warp(&empty[s], (u / S::kUnits - 1) & 1, a.status);
+          if (ok && last >= S::kUnits) ok = wait_warp(&empty[s], turn);
           if (!ok) break;
           if (side == 0 && own) {
             g_ks[info][k] = w0.ks;
@@ -520,7 +525,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
           }
           __syncwarp();
           if (lane == 0) {
-            if (side == 0) mbar_arrive(&g_full[info]);
             mbar_arrive_expect_tx(&full[s], __popc(mask) * (a.box * D));
           }
           __syncwarp();
@@ -530,7 +534,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
             for (int h = 0; h < S::kHalves; ++h)
               tma_load_2d(d + h * S::kHalfBytes, side ? &v_map : &k_map, &full[s], h * 128, w0.at, policy);
           }
-          last = u + 1;
+          ++last;
+          if (++s == S::kUnits) {
+            s = 0;
+            turn ^= 1;
+          }
         }
       }
       b0 = b1;
@@ -541,21 +549,25 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
     // loads that nobody waited for (after a wait that ran out) end before the CTA does
     if (!ok && lane == 0)
 #pragma unroll 1
-      for (int u = max(0, last - S::kUnits); u < last; ++u) wait_one(&full[u % S::kUnits], (u / S::kUnits) & 1, a.status);
+      for (int u = max(0, last - S::kUnits); u < last; ++u) wait_one(&full[u % S::kUnits], (u / S::kUnits) & 1);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs of the scores: one thread
     constexpr uint32_t id = idesc_i8(128, S::kN1, false);
-    int i = 0;
+    int i = 0, s = 0;  // s: the tile's unit
+    uint32_t turn = 0;
     while (ok && next()) {
       const int n_tiles = tasks[task % kTasks].n;
       if (lane == 0) {
         const uint32_t q = smem_u32(q_digits + (task & 1) * S::kQBytes);
-        ok = wait_one(&q_full[task & 1], (task >> 1) & 1, a.status);
+        ok = wait_one(&q_full[task & 1], (task >> 1) & 1);
 #pragma unroll 1
         for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
-          const int u = 2 * i, s = u % S::kUnits, buf = i & 1;
-          if (i >= 2) ok = wait_one(&s_empty[buf], ((i >> 1) - 1) & 1, a.status);
-          if (!ok || !(ok = wait_one(&full[s], (u / S::kUnits) & 1, a.status))) break;
+          const int buf = i % S::kBuffers;
+          // (scores that are there say that their digits' buffer is free as well)
+          if (i >= S::kBuffers)
+            ok = wait_one(&s_empty[buf], (i / S::kBuffers - 1) & 1) &&
+                 wait_one(&p_empty[buf], (i / S::kBuffers - 1) & 1);
+          if (!ok || !(ok = wait_one(&full[s], turn))) break;
           tc_fence_after();
           uint64_t k = smem_desc<S::kRow>(smem_u32(ring + s * S::kSide)), qd = smem_desc<S::kRow>(q);
 #pragma unroll 1
@@ -566,27 +578,32 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
             qd += (next ? S::kN1 * S::kRow - 96 : 32) >> 4;
           }
           umma_commit(&s_full[buf]);
+          mbar_arrive(&s_full[buf]);
           umma_commit(&empty[s]);
+          if ((s += 2) >= S::kUnits) {
+            s -= S::kUnits;
+            turn ^= 1;
+          }
         }
         if (ok) umma_commit(&q_empty[task & 1]);
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       done();
     }
-  } else if (warp == 14) {
+  } else if (warp == 2) {
     // ---------------------------------------------------------------- MMAs of the outputs: one thread
     constexpr uint32_t id = idesc_i8(128, S::kN2, true);
-    constexpr int B = S::kOutBuffers;
-    int i = 0;
+    int i = 0, s = 1;
+    uint32_t turn = 0;
     while (ok && next()) {
       const int n_tiles = tasks[task % kTasks].n;
       if (lane == 0) {
 #pragma unroll 1
         for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
-          const int u = 2 * i + 1, s = u % S::kUnits, buf = i & 1, ob = i % B;
-          if (i >= B) ok = wait_one(&o_empty[ob], (i / B - 1) & 1, a.status);
-          if (ok) ok = wait_one(&full[s], (u / S::kUnits) & 1, a.status);
-          if (!ok || !(ok = wait_one(&p_full[buf], (i >> 1) & 1, a.status))) break;
+          const int buf = i % S::kBuffers, ob = i & 1;
+          if (i >= 2) ok = wait_one(&o_empty[ob], ((i >> 1) - 1) & 1);
+          if (ok) ok = wait_one(&full[s], turn);
+          if (!ok || !(ok = wait_one(&p_full[buf], (i / S::kBuffers) & 1))) break;
           tc_fence_after();
           uint64_t v = smem_desc<S::kRow>(smem_u32(ring + s * S::kSide));
           const uint64_t p = smem_desc<128>(smem_u32(p_digits + buf * S::kPBytes));
@@ -594,14 +611,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
           for (int n = 0; n < 4 * S::kHalves; ++n, v += 32 * S::kRow >> 4)  // 32 keys a step; the halves are neighbours
             umma_i8(tmem_o + (ob * S::kHalves + n / 4) * S::kN2, v, p + (n % 4) * 2, id, n % 4 > 0);
           umma_commit(&o_full[ob]);
+          mbar_arrive(&o_full[ob]);
           umma_commit(&p_empty[buf]);
           umma_commit(&empty[s]);
+          if ((s += 2) >= S::kUnits) {
+            s -= S::kUnits;
+            turn ^= 1;
+          }
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       done();
     }
-  } else if (warp == 15) {
+  } else if (warp == 3) {
     // ---------------------------------------------------------------- q -> digits, a task ahead
     constexpr int kE = D / 32;  // columns a lane
     struct alignas(16) Columns {
@@ -610,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
     while (ok && next()) {
       const Task t = tasks[task % kTasks];
       const int buf = task & 1;
-      if (task >= 2) ok = wait_warp(&q_empty[buf], ((task >> 1) - 1) & 1, a.status);
+      if (task >= 2) ok = wait_warp(&q_empty[buf], ((task >> 1) - 1) & 1);
       if (!ok) break;
       unsigned char* digits = q_digits + buf * S::kQBytes + (lane * kE / 128) * (S::kN1 * S::kRow);
       const int col = lane * kE % 128;
@@ -653,10 +675,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         // 2^ex brings the maximum to [2^21, 2^22); in two factors, each inside the floating range
         const int ex = fine && top > 0.0f ? 21 + 127 - max(1, __float_as_int(top) >> 23) : 0;
         const int e1 = ex / 2, e2 = ex - e1;
-        const float up1 = __int_as_float((127 + e1) << 23), up2 = __int_as_float((127 + e2) << 23);
+        const float up1 = copysignf(__int_as_float((127 + e1) << 23), a.scale), up2 = __int_as_float((127 + e2) << 23);
         if (lane == 0) {
-          const float down = __int_as_float((127 - e1) << 23) * (a.softcap > 0.0f ? a.scale / a.softcap : a.scale * kLog2e);
-          fac_s[buf][qi] = fine ? down * __int_as_float((127 - e2) << 23) : NAN;
+          // positive (a negative scale turns the digits over) and not zero, so that masked scores stay at -inf
+          const float down = __int_as_float((127 - e1) << 23) * (fabsf(a.scale) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e)) *
+                             __int_as_float((127 - e2) << 23);
+          fac_s[buf][qi] = !fine ? NAN : down < 0x1p-126f ? 0x1p-126f : down;
           last_s[buf][qi] = min(qi < t.rows ? pos : 0x7fffffff, t.stop - 1);
           first_s[buf][qi] = qi < t.rows && a.window ? pos - a.window + 1 : 0;
         }
@@ -685,144 +709,135 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       if (lane == 0) mbar_arrive(&q_full[buf]);
       done();
     }
-  } else if (warp < 10) {
+  } else if (warp < kFirstOutput) {
     // ---------------------------------------------------------------- scores -> digits of p
-    // A turn is 8 queries of a tile; the two warpgroups take turns: with 8 query rows a tile each,
-    // with more a tile's queries.
-    const int side = (warp - 2) >> 2, wq = (warp - 2) & 3, sub = warp & 3, key_row = sub * 32 + lane;
-    const uint32_t lane_at = static_cast<uint32_t>(sub * 32) << 16;
-    constexpr int C = kQueries, kOwn = S::kTurns > 2 ? S::kTurns / 2 : 1;  // a warpgroup's turns of a tile
+    // A turn is 8 queries of a tile: with 8 query rows the two warpgroups take a tile each in turn, with
+    // 16 half of a tile's queries each.
+    const int side = (warp - kFirstScorer) >> 2, wq = warp & 3, key_row = wq * 32 + lane;
+    const uint32_t lane_at = static_cast<uint32_t>(wq * 32) << 16;
+    constexpr int C = kQueries;
+    const int c0 = side % S::kTurns * C;  // the warpgroup's first query
+    float* own_top = top_s[warp - kFirstScorer];
+    float* own_beta = beta_s[warp - kFirstScorer];
+    float* own_fac = factor_s[warp - kFirstScorer];
     int i = 0, turn = 0;
     while (ok && next()) {
       const Task& t = tasks[task % kTasks];
       const int n_tiles = t.n, first_key = t.low + t.tile0 * kTile;
       const int plain_stop = min(t.pos_low + 1, t.stop), plain_start = a.window ? t.pos_high - a.window + 1 : 0;  // keys all queries see
       const int qb = task & 1;
-      ok = wait_warp(&q_full[qb], (task >> 1) & 1, a.status);  // what is known of the queries
-      float l[kOwn][C];
-      float ref[kOwn];  // lane q: the reference maximum of query q (the four warps keep the same)
+      ok = wait_warp(&q_full[qb], (task >> 1) & 1);  // what is known of the queries
+      float l[C];
 #pragma unroll
-      for (int k = 0; k < kOwn; ++k) {
-        ref[k] = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < C; ++q) l[k][q] = 0.0f;
-      }
+      for (int q = 0; q < C; ++q) l[q] = 0.0f;
+      float ref = -INFINITY;  // lane q: the reference maximum of query q (the four warps keep the same)
+      // (a capped score has its factor already)
+      if (lane < C) own_fac[lane] = a.softcap > 0.0f ? 1.0f : fac_s[qb][c0 + lane];
+      __syncwarp();
 #pragma unroll 1
       for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
-        if (S::kTurns == 1 && (i & 1) != side) continue;
-        const int buf = i & 1, phase = (i >> 1) & 1, info = i % kInfo;
-        ok = wait_one(&g_full[info], (i / kInfo) & 1, a.status);  // the tile's scales
-        ok = wait_warp(&s_full[buf], phase, a.status) && ok;
-        ok = __all_sync(0xffffffffu, ok);
+        if (i % S::kEvery != side / S::kTurns) continue;
+        const int buf = i % S::kBuffers, phase = (i / S::kBuffers) & 1, info = i % kInfo;
+        ok = wait_warp(&s_full[buf], phase);
         if (!ok) break;
         tc_fence_after();
-        const int grp = key_row / a.box;
+        const int grp = key_row >> a.box_log;
         const float ks = g_ks[info][grp], vs = g_vs[info][grp], v_top = g_top[info];
         const bool there = (g_there[info] >> grp) & 1u;
         const int key0 = first_key + tile * kTile, key = key0 + key_row;
         const bool masked = key0 + kTile > plain_stop || key0 < plain_start || __any_sync(0xffffffffu, !there);
         const float to_fixed = v_top > 0.0f ? __fdividef(vs, v_top) * kFixed : 0.0f;
         unsigned char* p = p_digits + buf * S::kPBytes;
+        float x[C];
+        {
+          int d2[C], d1[C], dd[C];
+          const uint32_t at = tmem + buf * S::kS + lane_at + c0;
+          tmem_ld3<C>(at, at + R, at + 2 * R, d2, d1, dd);
 #pragma unroll
-        for (int k = 0; k < kOwn; ++k, ++turn) {
-          const int c0 = S::kTurns == 1 ? 0 : (2 * k + side) * C;  // the turn's first query
-          float x[C];
-          {
-            int d2[C], d1[C], dd[C];
-            const uint32_t at = tmem + buf * S::kS + lane_at + c0;
-            tmem_ld3<C>(at, at + R, at + 2 * R, d2, d1, dd);
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-              x[c] = fmaf(__int2float_rn(d2[c]), 65536.0f, __int2float_rn(d1[c] * 256 + dd[c])) * (ks * fac_s[qb][c0 + c]);
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_empty[buf]);
-          if (a.softcap > 0.0f) {
-#pragma unroll
-            for (int q = 0; q < C; ++q)  // tanh(u) = 1 - 2 / (1 + e^2u)
-              x[q] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + exp2_fast(x[q] * (2.0f * kLog2e))));
-          }
-          if (masked) {
-#pragma unroll
-            for (int q = 0; q < C; ++q)
-              if (!there || key > last_s[qb][c0 + q] || key < first_s[qb][c0 + q]) x[q] = -INFINITY;
-          }
-          // the turn's largest score of each query: warp, then the four warps
-          float mx = -INFINITY;
-#pragma unroll
-          for (int q = 0; q < C; ++q) {
-            const float m = warp_top(x[q]);
-            if (lane == q) mx = m;
-          }
-          if (lane < C) tops_s[side][turn & 1][wq][lane] = mx;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&tops[side]);
-          if (k == 0 && i >= 2) ok = wait_one(&p_empty[buf], phase ^ 1, a.status);
-          ok = wait_warp(&tops[side], turn & 1, a.status) && ok;
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          float alpha = 1.0f;
-          if (lane < C) {
-            const float* w0 = tops_s[side][turn & 1][0];
-            mx = max_nan(max_nan(w0[lane], w0[C + lane]), max_nan(w0[2 * C + lane], w0[3 * C + lane]));
-            if (ref[k] == -INFINITY) {
-              ref[k] = mx;
-            } else if (mx > ref[k] + kSlack) {
-              alpha = exp2_fast(ref[k] - mx);
-              ref[k] = mx;
-            }
-            top_s[warp - 2][lane] = mx == -INFINITY ? 0.0f : mx;
-            beta_s[warp - 2][lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref[k]);
-            if (wq == 0) mx_ring[i & 3][c0 + lane] = mx;
-          }
-          if (wq == 0 && lane == 0 && c0 == 0) v_ring[i & 3] = v_top;
-          const bool moved = __any_sync(0xffffffffu, alpha != 1.0f);
-          __syncwarp();
-          if (wq == 0 && lane == 0) mbar_arrive(&f_full[i & 3]);
-          if (moved) {
-#pragma unroll
-            for (int q = 0; q < C; ++q) l[k][q] *= __shfl_sync(0xffffffffu, alpha, q);
-          }
-#pragma unroll
-          for (int q = 0; q < C; ++q) {
-            const float e = exp2_fast(x[q] - top_s[warp - 2][q]);
-            l[k][q] = fmaf(e, beta_s[warp - 2][q], l[k][q]);
-            // v = rint(e * to_fixed) by a sum with 1.5 * 2^23.  With 128 added to each of the two lower
-            // digits' places, the bytes of v are its signed digits, the lower two with the sign bit turned over.
-            const uint32_t v = __float_as_uint(fmaf(e, to_fixed, 12582912.0f)) - 0x4B400000u;
-            const uint32_t digits = (v + 0x8080u) ^ 0x8080u;
-            unsigned char* to = p + swizzled<128>(q * kTile + key_row) + c0 * kTile;  // (c0 is a multiple of 8 rows)
-            to[0] = static_cast<unsigned char>(digits >> 16);
-            to[R * kTile] = static_cast<unsigned char>(digits >> 8);
-            to[2 * R * kTile] = static_cast<unsigned char>(digits);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[buf]);
+          for (int c = 0; c < C; ++c)
+            x[c] = fmaf(__int2float_rn(d2[c]), 65536.0f, __int2float_rn(d1[c] * 256 + dd[c])) * ks;
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[buf]);
+        if (a.softcap > 0.0f) {
+#pragma unroll
+          for (int q = 0; q < C; ++q)  // tanh(u) = 1 - 2 / (1 + e^2u)
+            x[q] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + exp2_fast(x[q] * fac_s[qb][c0 + q] * (2.0f * kLog2e))));
+        }
+        if (masked) {
+#pragma unroll
+          for (int q = 0; q < C; ++q)
+            if (!there || key > last_s[qb][c0 + q] || key < first_s[qb][c0 + q]) x[q] = -INFINITY;
+        }
+        // the turn's largest score of each query, still without its (positive) factor: warp, then the four warps
+        float mx = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < C; ++q) {
+          const float m = warp_top(x[q]);
+          if (lane == q) mx = m;
+        }
+        if (lane < C) tops_s[side][turn & 1][wq][lane] = mx;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tops[side]);
+        ok = wait_warp(&tops[side], turn & 1);
+        if (!ok) break;
+        float alpha = 1.0f;
+        if (lane < C) {
+          const float* w0 = tops_s[side][turn & 1][0];
+          mx = max_nan(max_nan(w0[lane], w0[C + lane]), max_nan(w0[2 * C + lane], w0[3 * C + lane])) * own_fac[lane];
+          if (ref == -INFINITY) {
+            ref = mx;
+          } else if (mx > ref + kSlack) {
+            alpha = exp2_fast(ref - mx);
+            ref = mx;
+          }
+          own_top[lane] = mx == -INFINITY ? 0.0f : mx;
+          own_beta[lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref);
+          if (wq == 0) mx_ring[i % kRing][c0 + lane] = mx;
+        }
+        if (wq == 0 && lane == 0 && c0 == 0) v_ring[i % kRing] = v_top;
+        const bool moved = __any_sync(0xffffffffu, alpha != 1.0f);
+        __syncwarp();
+        if (moved) {
+#pragma unroll
+          for (int q = 0; q < C; ++q) l[q] *= __shfl_sync(0xffffffffu, alpha, q);
+        }
+#pragma unroll
+        for (int q = 0; q < C; ++q) {
+          const float e = exp2_fast(fmaf(x[q], own_fac[q], -own_top[q]));
+          l[q] = fmaf(e, own_beta[q], l[q]);
+          // v = rint(e * to_fixed) by a sum with 1.5 * 2^23.  With 128 added to each of the two lower
+          // digits' places, the bytes of v are its signed digits, the lower two with the sign bit turned over.
+          const uint32_t v = __float_as_uint(fmaf(e, to_fixed, 12582912.0f)) - 0x4B400000u;
+          const uint32_t digits = (v + 0x8080u) ^ 0x8080u;
+          unsigned char* to = p + swizzled<128>(q * kTile + key_row) + c0 * kTile;  // (c0 is a multiple of 8 rows)
+          to[0] = static_cast<unsigned char>(digits >> 16);
+          to[R * kTile] = static_cast<unsigned char>(digits >> 8);
+          to[2 * R * kTile] = static_cast<unsigned char>(digits);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
+        ++turn;
       }
       // ---- the task's sums
-      if (ok && task > 0) ok = wait_warp(&l_empty, (task - 1) & 1, a.status);
+      if (ok && task > 0) ok = wait_warp(&l_empty, (task - 1) & 1);
       if (!ok) break;
+      // eight sums over the warp at once: a half of them, by a bit of the lane, goes on at each step
 #pragma unroll
-      for (int k = 0; k < kOwn; ++k) {
-        const int c0 = S::kTurns == 1 ? 0 : (2 * k + side) * C;
-        // eight sums over the warp at once: a half of them, by a bit of the lane, goes on at each step
+      for (int o = 16; o >= 4; o >>= 1) {
+        const bool high = lane & o;
 #pragma unroll
-        for (int o = 16; o >= 4; o >>= 1) {
-          const bool high = lane & o;
-#pragma unroll
-          for (int q = 0; q < o / 4; ++q) {
-            const float give = high ? l[k][q] : l[k][q + o / 4], keep = high ? l[k][q + o / 4] : l[k][q];
-            l[k][q] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-          }
+        for (int q = 0; q < o / 4; ++q) {
+          const float give = high ? l[q] : l[q + o / 4], keep = high ? l[q + o / 4] : l[q];
+          l[q] = keep + __shfl_xor_sync(0xffffffffu, give, o);
         }
-        float sum_q = l[k][0] + __shfl_xor_sync(0xffffffffu, l[k][0], 2);
-        sum_q += __shfl_xor_sync(0xffffffffu, sum_q, 1);
-        if ((lane & 3) == 0) l_part[warp - 2][c0 + lane / 4] = sum_q;
-        if (wq == 0 && lane < C) m_ref[side][c0 + lane] = ref[k];
       }
+      float sum_q = l[0] + __shfl_xor_sync(0xffffffffu, l[0], 2);
+      sum_q += __shfl_xor_sync(0xffffffffu, sum_q, 1);
+      if ((lane & 3) == 0) l_part[warp - kFirstScorer][lane / 4] = sum_q;
+      if (wq == 0 && lane < C) m_ref[side][lane] = ref;
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&q_empty[qb]);
@@ -848,19 +863,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       float ref = -INFINITY;  // lane q: the reference maximum of query q
 #pragma unroll 1
       for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
-        const int buf = i % S::kOutBuffers;
-        ok = wait_warp(&f_full[i & 3], (i >> 2) & 1, a.status);
+        const int buf = i & 1;
+        ok = wait_warp(&o_full[buf], (i >> 1) & 1);
         if (!ok) break;
+        tc_fence_after();
         float alpha = 1.0f;
         if (lane < R) {
-          const float mx = mx_ring[i & 3][lane];
+          const float mx = mx_ring[i % kRing][lane];
           if (ref == -INFINITY) {
             ref = mx;
           } else if (mx > ref + kSlack) {
             alpha = exp2_fast(ref - mx);
             ref = mx;
           }
-          factor[lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref) * v_ring[i & 3] * (1.0f / kFixed);
+          factor[lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref) * v_ring[i % kRing] * (1.0f / kFixed);
         }
         __syncwarp();
         if (__any_sync(0xffffffffu, alpha != 1.0f)) {
@@ -871,9 +887,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
             for (int h = 0; h < S::kHalves; ++h) o[h][q] *= f;
           }
         }
-        ok = wait_warp(&o_full[buf], (i / S::kOutBuffers) & 1, a.status);
-        if (!ok) break;
-        tc_fence_after();
 #pragma unroll
         for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
@@ -890,17 +903,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_empty[buf]);
       }
-      if (ok) ok = wait_warp(&l_full, task & 1, a.status);
+      if (ok) ok = wait_warp(&l_full, task & 1);
       if (!ok) break;
       // lane q: the query's sum, its inverse, where it goes
       float l = 0.0f;
       int to = 0;  // (the entry refuses more than 2^31 rows)
       if (lane < t.rows) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (S::kTurns > 1 && k != ((lane / C) & 1)) continue;  // the query's own warpgroup
-          const float part = l_part[4 * k][lane] + l_part[4 * k + 1][lane] + l_part[4 * k + 2][lane] + l_part[4 * k + 3][lane];
-          if (part != 0.0f) l += part * exp2_fast(m_ref[k][lane] - ref);
+        for (int k = 0; k < S::kEvery; ++k) {  // the query's warpgroups
+          const int w = lane / C + k * S::kTurns, q = lane % C;
+          const float part = l_part[4 * w][q] + l_part[4 * w + 1][q] + l_part[4 * w + 2][q] + l_part[4 * w + 3][q];
+          if (part != 0.0f) l += part * exp2_fast(m_ref[w][q] - ref);
         }
         const int qr = t.qt * R + lane;
         to = (t.begin + qr / G) * a.heads + t.hk * G + qr % G;
@@ -944,6 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       done();
     }
   }
+  if (!ok && b < n_ctas && a.status) atomicOr(a.status, static_cast<int>(kStatusWaitTimeout));
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -1017,12 +1031,9 @@ __global__ void __launch_bounds__(512) combine_kernel(const AttendArgs a) {
   if (a.lse && lane == 0) a.lse[to] = l != 0.0f ? (top + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// Query rows of a task: as few as hold the rows of most requests, so that the tensor
-// memory's columns and the threads' work are not spent on padding.
-int rows_of(int max_new, int group) {
-  const long long rows = static_cast<long long>(max_new) * group;
-  return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-}
+// Query rows of a task: as few as hold the rows of most requests, so that the tensor memory's columns
+// and the threads' work are not spent on padding; at most what two score warpgroups' turns hold.
+int rows_of(int max_new, int group) { return static_cast<long long>(max_new) * group <= 8 ? 8 : 16; }
 
 template <typename T, int D, int R>
 cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
@@ -1038,8 +1049,7 @@ cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensor
 template <typename T, int D>
 cudaError_t launch(const AttendArgs& a, int rows, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
   if (rows == 8) return launch<T, D, 8>(a, k_map, v_map, s);
-  if (rows == 16) return launch<T, D, 16>(a, k_map, v_map, s);
-  return launch<T, D, 32>(a, k_map, v_map, s);
+  return launch<T, D, 16>(a, k_map, v_map, s);
 }
 template <typename T>
 cudaError_t launch(const AttendArgs& a, int dim, int rows, const CUtensorMap& k_map, const CUtensorMap& v_map,
@@ -1085,7 +1095,7 @@ extern "C" int lb_op_kv8_attention(const void* q, int64_t q_token_stride, int64_
   const int box = page_tokens % 64 == 0 ? 64 : page_tokens % 32 == 0 ? 32 : 16;
   int4* cuts = static_cast<int4*>(workspace);
   AttendArgs a{q, q_token_stride, q_head_stride, n_tokens, n_rows, heads, kv_heads, k_scale, v_scale, n_pages,
-               page_tokens, max_pages, row_tables, kv_len, cu_tokens, scale, softcap, window, q_vec, box, out, lse, status,
+               page_tokens, max_pages, row_tables, kv_len, cu_tokens, scale, softcap, window, q_vec, box, 31 - __builtin_clz(box), out, lse, status,
                reinterpret_cast<float*>(cuts + kSms), cuts};
   const uint64_t cache_rows = static_cast<uint64_t>(n_pages) * kv_heads * page_tokens;
   const uint32_t span = dim < 128 ? dim : 128;
