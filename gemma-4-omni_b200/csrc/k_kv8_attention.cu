@@ -16,8 +16,9 @@
 //
 // A task is R query rows of one (row, kv head): the tokens of the row times the
 // query heads that share the kv head, so the cache is read once for all of them.
-// Its keys are walked in tiles of 128, and all tasks' tiles in one line are dealt out
-// evenly to one CTA per SM: rows of any lengths, many or one, keep every SM busy.
+// Its keys are walked in tiles of 128, and all tasks' tiles in one line (a few more for a task's
+// set-up: without them the CTAs with the short rows took up to 1.5 times as long as the rest) are dealt
+// out evenly to one CTA per SM: rows of any lengths, many or one, keep every SM busy.
 // A CTA finds its share from prefix sums over the rows' lengths (on the device: the
 // lengths may change under a captured graph).  Where a task is cut between
 // CTAs, each leaves an unnormalised part with its reference maximum in the workspace, and
@@ -48,6 +49,7 @@ constexpr int kFirstScorer = 4, kFirstOutput = 12;  // warps
 constexpr int kRing = 8;       // tiles whose largest scores are kept: more than the digits' and outputs' buffers together
 constexpr int kTasks = 8;      // tasks that the loading warp may be ahead
 constexpr int kInfo = 16;      // tiles whose scales are kept: more than the ring's units reach ahead
+constexpr int kTaskCost = 6;   // a task's set-up in tiles, as the line counts it (measured: 2 and 8 are slower for one case each)
 constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -209,8 +211,9 @@ __device__ __forceinline__ Row row_of(const AttendArgs& a, int r) {
   w.q_tiles = (w.count * (a.heads / a.kv_heads) + R - 1) / R;
   return w;
 }
+// in the line's units
 __device__ __forceinline__ long long row_work(const AttendArgs& a, const Row& w) {
-  return static_cast<long long>(w.tiles) * w.q_tiles * a.kv_heads;
+  return static_cast<long long>(w.tiles + kTaskCost) * w.q_tiles * a.kv_heads;
 }
 __device__ __forceinline__ long long warp_prefix(long long v) {  // inclusive
   const int lane = threadIdx.x & 31;
@@ -254,38 +257,44 @@ struct Walk {
     upto = warp_prefix(row_work(a, held));
   }
   __device__ __noinline__ bool next(const AttendArgs& a, long long line, long long n_ctas, Task& t) {
-    if (x >= x_end) {
-      t.n = 0;
-      return false;
-    }
-    unsigned after = __ballot_sync(0xffffffffu, base + upto > x);
-#pragma unroll 1
-    while (after == 0) {
-      base += __shfl_sync(0xffffffffu, upto, 31);
-      win += 32;
-      held = row_of<R>(a, win + (threadIdx.x & 31));
-      upto = warp_prefix(row_work(a, held));
-      after = __ballot_sync(0xffffffffu, base + upto > x);
-    }
-    const int at = __ffs(after) - 1;
     Row w;
-    t.row = win + at;
-    w.begin = __shfl_sync(0xffffffffu, held.begin, at);
-    w.count = __shfl_sync(0xffffffffu, held.count, at);
-    w.len = __shfl_sync(0xffffffffu, held.len, at);
-    w.low = __shfl_sync(0xffffffffu, held.low, at);
-    w.tiles = __shfl_sync(0xffffffffu, held.tiles, at);
-    w.q_tiles = __shfl_sync(0xffffffffu, held.q_tiles, at);
-    const long long y = x - (base + __shfl_sync(0xffffffffu, upto, at) - row_work(a, w));
-    const int task = static_cast<int>(y / w.tiles);
-    t.tile0 = static_cast<int>(y - static_cast<long long>(task) * w.tiles);
-    t.hk = task / w.q_tiles;
-    t.qt = task - t.hk * w.q_tiles;
-    t.n = static_cast<int>(min(static_cast<long long>(w.tiles - t.tile0), x_end - x));
-    x += t.n;
+    do {  // (the share may end, or begin, in a task's set-up: a part without tiles is passed over)
+      if (x >= x_end) {
+        t.n = 0;
+        return false;
+      }
+      unsigned after = __ballot_sync(0xffffffffu, base + upto > x);
+#pragma unroll 1
+      while (after == 0) {
+        base += __shfl_sync(0xffffffffu, upto, 31);
+        win += 32;
+        held = row_of<R>(a, win + (threadIdx.x & 31));
+        upto = warp_prefix(row_work(a, held));
+        after = __ballot_sync(0xffffffffu, base + upto > x);
+      }
+      const int at = __ffs(after) - 1;
+      t.row = win + at;
+      w.begin = __shfl_sync(0xffffffffu, held.begin, at);
+      w.count = __shfl_sync(0xffffffffu, held.count, at);
+      w.len = __shfl_sync(0xffffffffu, held.len, at);
+      w.low = __shfl_sync(0xffffffffu, held.low, at);
+      w.tiles = __shfl_sync(0xffffffffu, held.tiles, at);
+      w.q_tiles = __shfl_sync(0xffffffffu, held.q_tiles, at);
+      const int length = w.tiles + kTaskCost;
+      const long long y = x - (base + __shfl_sync(0xffffffffu, upto, at) - row_work(a, w));
+      const int task = static_cast<int>(y / length);
+      const int from = static_cast<int>(y - static_cast<long long>(task) * length);
+      const int to = static_cast<int>(min(static_cast<long long>(length), from + (x_end - x)));
+      t.hk = task / w.q_tiles;
+      t.qt = task - t.hk * w.q_tiles;
+      t.tile0 = max(0, from - kTaskCost);
+      t.n = max(0, to - kTaskCost) - t.tile0;
+      x += to - from;
+      // the CTA whose share holds the task's last tile
+      t.last_cta = static_cast<int>(((x + (length - to)) * n_ctas - 1) / line);
+    } while (t.n == 0);
     t.from_start = t.tile0 == 0;
     t.to_end = t.tile0 + t.n == w.tiles;
-    t.last_cta = static_cast<int>(((x + (w.tiles - t.tile0 - t.n)) * n_ctas - 1) / line);
     const int G = a.heads / a.kv_heads;
     t.low = w.low;
     t.begin = w.begin;
