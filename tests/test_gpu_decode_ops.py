@@ -497,3 +497,96 @@ def test_refusals(ops):
     assert ops.w4_matvec(torch.zeros(0, 128, device="cuda").to(BF16), w).shape == (0, 8)
     assert ops.rms_norm8(torch.zeros(0, 128, device="cuda"), ones)[0].shape == (0, 128)
     cache.append(x[:0], x[:0], slots[:0])
+
+
+# ------------------------------------------------------------------ the paths that sizes choose
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,dim,group", [(1184, 8, 0), (1200, 256, 128), (2000, 512, 0), (1300, 1024, 64), (1190, 2048, 128),
+                                            (1185, 2056, 8), (1200, 4096, 256), (1184, 8192, 0), (1200, 16384, 128)])
+def test_norm_with_a_row_for_every_scheduler(ops, dtype, rows, dim, group):
+    g = gen(rows + dim)
+    x = torch.randn(rows, dim, generator=g, device="cuda").to(dtype)
+    res = torch.randn(rows, dim, generator=g, device="cuda").to(dtype)
+    w = 1 + 0.3 * torch.randn(dim, generator=g, device="cuda")
+    for out in (E4M3, I8):
+        codes, scales, hidden = ops.rms_norm8(x, w, residual=res, group=group, dtype=out)
+        h, y = decode_ref.rms_norm(x, res, w, eps=1e-6)
+        assert ((hidden.double() - h).abs() <= HALF_ULP[dtype] * (1 + 1e-3) * h.abs() + 1e-9).all()
+        y = y.view(rows, -1, group or dim)
+        want = y.abs().amax(2) / (448 if out is E4M3 else 127)
+        torch.testing.assert_close(scales.double(), want, rtol=4e-6, atol=1e-44)
+        s = want[..., None]
+        near = 0.5 * s if out is I8 else torch.maximum(2.0 ** -4 * y.abs(), 2.0 ** -10 * s)
+        got = codes.double().view(y.shape) * scales.double()[..., None]
+        assert ((got - y).abs() <= near * (1 + 1e-3) + 1e-5 * y.abs()).all()
+
+
+def test_norm_of_values_near_the_ends_of_the_range(ops):
+    x = torch.randn(3, 256, generator=gen(11), device="cuda")
+    x[1] *= 1e-30  # with eps the row is tiny: its scale is far below 2^-100
+    x[2] *= 1e15
+    codes, scales, _ = ops.rms_norm8(x, torch.full((256,), 1e-3, device="cuda"), eps=1e-6, dtype=I8)
+    _, y = decode_ref.rms_norm(x, None, torch.full((256,), 1e-3, device="cuda"), eps=1e-6)
+    got = codes.double() * scales.double()
+    assert ((got - y).abs() <= 0.5 * scales.double() * (1 + 1e-3) + 1e-5 * y.abs()).all()
+
+
+@pytest.mark.parametrize("rows,out,k,kind", [(16, 20000, 256, BF16), (1, 40000, 128, F16), (16, 160, 8192, BF16), (7, 64, 16384, F16),
+                                             (12, 96, 16384, I8), (2, 4700, 1024, E4M3), (33, 9000, 512, BF16)])
+def test_w4_products_in_every_arrangement(ops, rows, out, k, kind):
+    g = gen(out + k)
+    codes = torch.randint(0, 256, (out, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (0.01 * (0.1 + torch.rand(out, k // 64, generator=g, device="cuda"))).to(F16)
+    weight = ops.Int4Weight(codes, scales)
+    x, xs = torch.randn(rows, k, generator=g, device="cuda"), None
+    if kind in (E4M3, I8):
+        x, xs, _ = ops.rms_norm8(x, torch.ones(k, device="cuda"), dtype=kind)
+    else:
+        x = x.to(kind)
+    y = ops.w4_matvec(x, weight, x_scale=xs, out_dtype=F32)
+    ref, spread = decode_ref.w4_product(x, xs, codes, scales)
+    assert ((y.double() - ref).abs() <= k * 2.0 ** -23 * spread + 2.0 ** -23 * ref.abs() + 1e-9).all()
+
+
+@pytest.mark.parametrize("rows,lens,new", [(700, 40, 1), (300, 5, 2), (1, 16300, 1), (2, 9000, 40)])
+def test_attention_over_many_rows_and_long_ones(ops, rows, lens, new):
+    rng, g = random.Random(rows), gen(rows)
+    n = [rng.randint(new, lens) if rows > 2 else lens for _ in range(rows)]
+    cache, tables = random_cache(ops, g, rng, n, 64, 1, 128)
+    q = torch.randn(rows * new, 8, 128, generator=g, device="cuda").to(F16)
+    check_attention(ops, cache, tables, q, n, [new * i for i in range(rows + 1)], max_new=new)
+
+
+def test_attention_scale_signs_and_inputs_that_are_not_finite(ops):
+    rng, g = random.Random(12), gen(12)
+    cache, tables = random_cache(ops, g, rng, [200], 32, 1, 64)
+    q = torch.randn(1, 4, 64, generator=g, device="cuda").to(BF16)
+    check_attention(ops, cache, tables, -q, [200], [0, 1], max_new=1, scale=0.2)
+    plain = ops.kv8_attention(-q, cache, tables, ints([200]), ints([0, 1]), max_new=1, scale=0.2)
+    turned = ops.kv8_attention(q, cache, tables, ints([200]), ints([0, 1]), max_new=1, scale=-0.2)
+    torch.testing.assert_close(turned, plain, rtol=2 ** -7, atol=1e-3)  # the same scores: one store's rounding
+    q[0, 1, 5], q[0, 2, 6] = math.nan, math.inf
+    out, lse = ops.kv8_attention(q, cache, tables, ints([200]), ints([0, 1]), max_new=1, return_lse=True)
+    assert torch.isnan(out[0, 1:3]).all() and torch.isnan(lse[0, 1:3]).all()
+    assert torch.isfinite(out[0, [0, 3]]).all() and torch.isfinite(lse[0, [0, 3]]).all()
+
+
+@pytest.mark.parametrize("dim,page,tokens", [(256, 128, 300), (128, 256, 700), (80, 16, 50)])
+def test_append_of_groups_larger_than_the_registers_hold(ops, pkg, dim, page, tokens):
+    """Through the C entry too, whose dim may be any multiple of 16."""
+    from gemma4_omni_b200 import _lib
+    g = gen(dim)
+    pages = -(-tokens // page)
+    kc, vc = (torch.zeros(pages, 2, page, dim, dtype=I8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros(pages, 2, device="cuda") for _ in range(2))
+    k, v = (torch.randn(tokens, 2, dim, generator=g, device="cuda") for _ in range(2))
+    slots = torch.arange(tokens, device="cuda")
+    _lib.check("lb_op_kv8_append", _lib.load().lb_op_kv8_append(
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _lib.LB_F32, tokens, 2, dim, slots.data_ptr(),
+        kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, page, None, torch.cuda.current_stream().cuda_stream))
+    for codes, scale, x in ((kc, ks, k), (vc, vs, v)):
+        got = (codes.double() * scale.double()[..., None, None]).transpose(1, 2).reshape(-1, 2, dim)[:tokens]
+        step = scale.double().repeat_interleave(page, 0)[:tokens, :, None]
+        assert ((got - x.double()).abs() <= 0.5 * step * (1 + 1e-4)).all()
+        top = torch.stack([x[p * page:(p + 1) * page].double().abs().amax((0, 2)) for p in range(pages)]) / 127
+        torch.testing.assert_close(scale.double(), top, rtol=2.0 ** -22, atol=0)
