@@ -25,14 +25,22 @@
 // combine_kernel adds the parts up in the order of the keys, so results do not
 // depend on which CTA finishes first.
 //
-// Warp roles: 0 loads (TMA boxes of 64 keys, or of the largest power of two that divides a
-// page), 1 issues the MMAs of the scores, 14 those of the outputs (a thread that waits on a
-// barrier before each tile's MMAs loses some 500 cycles to it, so the two do not share one),
-// 3 splits the next task's q into digits while the present one runs, 2-5 and 6-9 turn scores
-// into digits of p (a thread a key: tensor memory's lanes), 8 queries at a time (more of them unrolled
-// outgrow the instruction cache: 16 took 6.9 thousand cycles a tile, 8 take 2.5), 10-13 add up the
-// outputs (a thread a column).  K and V lie in one ring of units of 128 keys, K freed by its
-// scores, V by its outputs; scores, digits, outputs and q have two buffers each.
+// Warp roles: 0 loads (TMA boxes of 64 keys, or of the largest power of two that divides a page; the page
+// tables of the batch of tiles after the next and the scales of the next are under way meanwhile), 1
+// issues the MMAs of the scores, 2 those of the outputs (a thread that waits on a barrier before
+// each tile's MMAs loses some 500 cycles to it, so the two do not share one), 3 splits the next task's
+// q into digits while the present one runs, 4-7 and 8-11 turn scores into digits of p (a thread a key: tensor
+// memory's lanes), 12-15 add up the outputs (a thread a column).  K and V lie in one ring of units
+// of 128 keys, K freed by its scores, V by its outputs.
+//
+// Six roles in sixteen warps share one instruction cache, and its misses bound the kernel before anything else
+// did: loops are kept rolled, a score warpgroup takes 8 queries at a time (16 unrolled took 6.9 thousand
+// cycles a tile, 8 take 2.5), waits are a few instructions.  Measured: 64 answers over 0.5 million keys with 8 kv
+// heads of 128 in 203 us (1.02 GB at 5.0 TB/s, 78 % of the copy rate; bound by the load warp and the rows'
+// raggedness), ticks of 1024 sessions with a window of 1024 keys and 16 query rows of 256 columns in 130 us (3.6
+// TB/s; bound by the score warps' chain), one answer over 16384 keys in 22 us (the chain of set-up, one
+// tile and the join), chunks of 128 to 512 tokens in 870 us (104 TFLOP/s; bound by the score warps'
+// instructions, some 25 a query and key).  Four score warpgroups instead of two were slower (answers 289 us).
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 #include "kernels.h"

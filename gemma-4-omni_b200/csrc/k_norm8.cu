@@ -6,9 +6,11 @@
 // The bytes bound it: 7 an element in 16 bits (x, r, the stored h, the code).  So a row is
 // read once and stays in registers between its three uses, T threads a row with
 // C pieces of 8 columns each.  With many rows C is 2 to 4: 16384 x 2048 bf16 with a scale for
-// 128 columns takes 46.6 us (128 threads a row; 78 % of the copy rate), against 56.9 with a warp a row
-// (8 pieces a lane: 16 warps an SM by registers), 50.1 with 64 and 49.4 with 256 threads.  With few rows
-// a piece a thread, since then the latency of one row is all there is.  Rows that are not
+// 128 columns takes 44.3 us with 128 threads a row (5.3 TB/s, 83 % of the copy rate; when measured against
+// one another, 46.6 us against 56.9 with a warp a row, whose 8 pieces a lane leave 16 warps an SM,
+// 50.1 with 64 and 49.4 with 256 threads).  What is left is instructions: 74 % of the issue slots.
+// With few rows a piece a thread, since then the latency of one row is all there is (2 x 1536: 2.1 us
+// inside a graph).  Rows that are not
 // 16-byte aligned, odd widths and groups that are no power of two of pieces take the plain kernel at the end.
 #include <cuda_fp8.h>
 
@@ -22,7 +24,7 @@ struct NormArgs {
   const void *x, *res, *w;
   long long x_ld, r_ld;
   int dtype, w_f32, rows, dim, group, e4m3;
-  float eps;
+  float eps, inv_dim, inv_top;
   uint8_t* codes;
   float* scales;
   void* hidden;
@@ -83,16 +85,18 @@ __device__ __forceinline__ uint8_t code_of(float q, bool e4m3) {
   return static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(fminf(fmaxf(q, -127.0f), 127.0f))));
 }
 
-// The codes of 8 columns, by one multiplication with the inverse (its rounding moves a code only where
-// y / s is within 2^-22 of halfway).  Below 2^-100 both take a power of two first, so that the inverse is finite.
-__device__ __forceinline__ uint2 codes_of(float (&y)[8], float s, bool e4m3) {
-  if (!(s > 0.0f)) return make_uint2(0, 0);  // all zero, or a NaN: the scale says so
-  if (s < 0x1p-100f) {
-    s *= 0x1p80f;
+// The codes of 8 columns whose group's largest value is m, by one multiplication with top / m (its
+// rounding moves a code only where y / s is within 2^-21 of halfway).  Far from 1 both take a power of two
+// first, so that the quotient stays inside the range of the fast division.
+__device__ __forceinline__ uint2 codes_of(float (&y)[8], float m, bool e4m3) {
+  if (!(m > 0.0f)) return make_uint2(0, 0);  // all zero, or a NaN: the scale says so
+  if (m < 0x1p-90f || m > 0x1p90f) {
+    const float k = m < 1.0f ? 0x1p80f : 0x1p-80f;
+    m *= k;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= 0x1p80f;
+    for (int i = 0; i < 8; ++i) y[i] *= k;
   }
-  const float inv = 1.0f / s;
+  const float inv = __fdividef(e4m3 ? 448.0f : 127.0f, m);
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] *= inv;
   uint32_t w[4];
@@ -156,8 +160,7 @@ __global__ void __launch_bounds__(kT < 256 ? 256 : kT) norm_rows_kernel(const No
 #pragma unroll
     for (int k = 0; k < kWarpsRow; ++k) sum += part[warp / kWarpsRow * kWarpsRow + k];
   }
-  const float r = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
-  const float top = a.e4m3 ? 448.0f : 127.0f;
+  const float r = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
   uint32_t m[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -185,9 +188,9 @@ __global__ void __launch_bounds__(kT < 256 ? 256 : kT) norm_rows_kernel(const No
     for (int c = 0; c < C; ++c) {
       const int i = in_row + c * kT;
       if (live && i < pieces) {
-        const float s = __uint_as_float(m[c]) / top;
-        if ((i & (width - 1)) == 0) a.scales[row * (pieces >> width_log) + (i >> width_log)] = s;
-        *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], s, a.e4m3);
+        const float most = __uint_as_float(m[c]);
+        if ((i & (width - 1)) == 0) a.scales[row * (pieces >> width_log) + (i >> width_log)] = most * a.inv_top;
+        *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], most, a.e4m3);
       }
     }
     return;
@@ -203,12 +206,11 @@ __global__ void __launch_bounds__(kT < 256 ? 256 : kT) norm_rows_kernel(const No
 #pragma unroll
     for (int k = 0; k < kWarpsRow; ++k) most = max(most, __float_as_uint(part[warp / kWarpsRow * kWarpsRow + k]));
   }
-  const float s = __uint_as_float(most) / top;
-  if (live && in_row == 0) a.scales[row] = s;
+  if (live && in_row == 0) a.scales[row] = __uint_as_float(most) * a.inv_top;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = in_row + c * kT;
-    if (live && i < pieces) *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], s, a.e4m3);
+    if (live && i < pieces) *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], __uint_as_float(most), a.e4m3);
   }
 }
 
@@ -283,7 +285,8 @@ extern "C" int lb_op_rms_norm8(const void* x, int64_t x_ld, const void* residual
       (out_dtype != LB_E4M3 && out_dtype != LB_I8))
     return LB_ERR_INVALID_ARGUMENT;
   const NormArgs a{x, residual, weight, x_ld, residual_ld, dtype, weight_dtype == LB_F32, rows, dim, group,
-                   out_dtype == LB_E4M3, eps, static_cast<uint8_t*>(codes), scales, hidden};
+                   out_dtype == LB_E4M3, eps, 1.0f / static_cast<float>(dim), out_dtype == LB_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f,
+                   static_cast<uint8_t*>(codes), scales, hidden};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t size = dtype == LB_F32 ? 4 : 2;
   const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
