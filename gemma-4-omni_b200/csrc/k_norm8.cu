@@ -6,7 +6,7 @@
 // The bytes bound it: 7 an element in 16 bits (x, r, the stored h, the code).  So a row is
 // read once and stays in registers between its three uses, T threads a row with
 // C pieces of 8 columns each.  With many rows C is 2 to 4: 16384 x 2048 bf16 with a scale for
-// 128 columns takes 44.3 us with 128 threads a row (5.3 TB/s, 83 % of the copy rate; when measured against
+// 128 columns takes 44.7 us with 128 threads a row (5.3 TB/s, 82 % of the copy rate; when measured against
 // one another, 46.6 us against 56.9 with a warp a row, whose 8 pieces a lane leave 16 warps an SM,
 // 50.1 with 64 and 49.4 with 256 threads).  What is left is instructions: 74 % of the issue slots.
 // With few rows a piece a thread, since then the latency of one row is all there is (2 x 1536: 2.1 us
@@ -23,22 +23,24 @@ namespace {
 struct NormArgs {
   const void *x, *res, *w;
   long long x_ld, r_ld;
-  int dtype, w_f32, rows, dim, group, e4m3;
+  int w_f32, rows, dim, group, e4m3;
   float eps, inv_dim, inv_top;
   uint8_t* codes;
   float* scales;
   void* hidden;
 };
 
-__device__ __forceinline__ float load_as_float(const void* p, int dtype, long long i) {
-  if (dtype == LB_F32) return static_cast<const float*>(p)[i];
-  if (dtype == LB_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
+template <typename T>
+__device__ __forceinline__ float load_as_float(const T* p) {
+  if constexpr (__is_same(T, float)) return *p;
+  else if constexpr (__is_same(T, __half)) return __half2float(*p);
+  else return __bfloat162float(*p);
 }
-__device__ __forceinline__ void store_from_float(void* p, int dtype, long long i, float v) {
-  if (dtype == LB_F32) static_cast<float*>(p)[i] = v;
-  else if (dtype == LB_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else static_cast<__half*>(p)[i] = __float2half_rn(v);
+template <typename T>
+__device__ __forceinline__ void store_from_float(T* p, float v) {
+  if constexpr (__is_same(T, float)) *p = v;
+  else if constexpr (__is_same(T, __half)) *p = __float2half_rn(v);
+  else *p = __float2bfloat16_rn(v);
 }
 
 // 8 columns
@@ -214,40 +216,94 @@ __global__ void __launch_bounds__(kT < 256 ? 256 : kT) norm_rows_kernel(const No
   }
 }
 
-// Any width, alignment and group: a CTA a row, the row in shared memory.
-constexpr int kThreads = 256;
-__global__ void __launch_bounds__(kThreads) norm_any_kernel(const NormArgs a) {
+// Any width, alignment and group: kT threads a row (a warp where rows are narrow and many), the row in
+// shared memory, a value a load.
+template <typename T, int kT>
+__global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs a) {
+  constexpr int kRowsBlock = 256 / kT;
   extern __shared__ float row_smem[];
-  __shared__ float part[kThreads / 32];
-  const long long row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = a.dim;
+  __shared__ float part[8];
+  const int in_row = threadIdx.x % kT, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.dim;
+  const long long row = static_cast<long long>(blockIdx.x) * kRowsBlock + threadIdx.x / kT;
+  if (kT == 32 && row >= a.rows) return;  // (one row a CTA: every row is there)
+  float* held = row_smem + threadIdx.x / kT * dim;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+  const T* res = a.res ? static_cast<const T*>(a.res) + row * a.r_ld : nullptr;
+  T* hidden = a.hidden ? static_cast<T*>(a.hidden) + row * dim : nullptr;
   float sum = 0.0f;
-  for (int i = tid; i < dim; i += kThreads) {
-    float h = load_as_float(a.x, a.dtype, row * a.x_ld + i);
-    if (a.res) h += load_as_float(a.res, a.dtype, row * a.r_ld + i);
-    if (a.hidden) store_from_float(a.hidden, a.dtype, row * dim + i, h);
-    row_smem[i] = h;
+#pragma unroll 4
+  for (int i = in_row; i < dim; i += kT) {
+    float h = load_as_float<T>(x + i);
+    if (res) h += load_as_float<T>(res + i);
+    if (hidden) store_from_float<T>(hidden + i, h);
+    held[i] = h;
     sum = fmaf(h, h, sum);
   }
   sum = warp_sum(sum);
-  if (lane == 0) part[warp] = sum;
-  __syncthreads();
-  sum = 0.0f;
-  for (int i = 0; i < kThreads / 32; ++i) sum += part[i];
-  const float r = rsqrtf(sum / static_cast<float>(dim) + a.eps);
-  for (int i = tid; i < dim; i += kThreads) row_smem[i] = row_smem[i] * r * load_as_float(a.w, a.w_f32 ? LB_F32 : a.dtype, i);
-  __syncthreads();
-  const int width = a.group ? a.group : dim, n_groups = dim / width;
-  const float top = a.e4m3 ? 448.0f : 127.0f;
-  for (int g = a.group ? warp : 0; g < n_groups; g += a.group ? kThreads / 32 : 1) {
-    // a warp a group; for one scale a row every warp finds the row's maximum
-    uint32_t m = 0u;
-    for (int i = lane; i < width; i += 32) m = max(m, size_of(row_smem[g * width + i]));
-    const float s = __uint_as_float(__reduce_max_sync(0xffffffffu, m)) / top;
-    if (lane == 0 && (a.group || warp == 0)) a.scales[row * n_groups + g] = s;
-    for (int i = a.group ? lane : tid; i < width; i += a.group ? 32 : kThreads)
-      a.codes[row * dim + g * width + i] = s > 0.0f ? code_of(row_smem[g * width + i] / s, a.e4m3) : uint8_t(0);
+  if constexpr (kT > 32) {
+    if (lane == 0) part[warp] = sum;
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += part[i];
+    __syncthreads();  // the sums have been read
   }
+  const float r = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
+  uint32_t most = 0;
+#pragma unroll 4
+  for (int i = in_row; i < dim; i += kT) {  // (a thread's own values)
+    const float y = held[i] * r * (a.w_f32 ? static_cast<const float*>(a.w)[i] : load_as_float<T>(static_cast<const T*>(a.w) + i));
+    held[i] = y;
+    most = max(most, size_of(y));
+  }
+  const auto write = [&](int from, int width, uint32_t m, int first, int step) {
+    const float top = __uint_as_float(m);
+    const bool plain = top > 0x1p-90f && top < 0x1p90f;
+    const float s = top * a.inv_top, inv = plain ? __fdividef(a.e4m3 ? 448.0f : 127.0f, top) : 0.0f;
+#pragma unroll 4
+    for (int i = first; i < width; i += step) {
+      const float y = held[from + i];
+      a.codes[row * dim + from + i] = plain ? code_of(y * inv, a.e4m3) : s > 0.0f ? code_of(y / s, a.e4m3) : uint8_t(0);
+    }
+    return s;
+  };
+  if (a.group == 0) {
+    most = __reduce_max_sync(0xffffffffu, most);
+    if constexpr (kT > 32) {
+      if (lane == 0) part[warp] = __uint_as_float(most);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(part[i]));
+    }
+    const float s = write(0, dim, most, in_row, kT);
+    if (in_row == 0) a.scales[row] = s;
+    return;
+  }
+  if constexpr (kT > 32) __syncthreads();
+  else __syncwarp();
+  const int n_groups = dim / a.group;
+  for (int g = in_row / 32; g < n_groups; g += kT / 32) {  // a warp a group
+    uint32_t m = 0;
+    for (int i = lane; i < a.group; i += 32) m = max(m, size_of(held[g * a.group + i]));
+    const float s = write(g * a.group, a.group, __reduce_max_sync(0xffffffffu, m), lane, 32);
+    if (lane == 0) a.scales[row * n_groups + g] = s;
+  }
+}
+template <typename T>
+cudaError_t launch_any(const NormArgs& a, cudaStream_t s) {
+  if (a.rows >= 148 * 8 && a.dim <= 1024) {
+    norm_any_kernel<T, 32><<<(a.rows + 7) / 8, 256, 8 * sizeof(float) * a.dim, s>>>(a);
+    return cudaGetLastError();
+  }
+  const size_t smem = sizeof(float) * a.dim;
+  if (smem > 40 * 1024) {
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(norm_any_kernel<T, 256>),
+                                      16384 * static_cast<int>(sizeof(float)));
+    if (e != cudaSuccess) return e;
+  }
+  norm_any_kernel<T, 256><<<a.rows, 256, smem, s>>>(a);
+  return cudaGetLastError();
 }
 
 template <typename T, int kT, int C>
@@ -284,7 +340,7 @@ extern "C" int lb_op_rms_norm8(const void* x, int64_t x_ld, const void* residual
   if ((dtype != LB_F32 && dtype != LB_BF16 && dtype != LB_F16) || (weight_dtype != LB_F32 && weight_dtype != dtype) ||
       (out_dtype != LB_E4M3 && out_dtype != LB_I8))
     return LB_ERR_INVALID_ARGUMENT;
-  const NormArgs a{x, residual, weight, x_ld, residual_ld, dtype, weight_dtype == LB_F32, rows, dim, group,
+  const NormArgs a{x, residual, weight, x_ld, residual_ld, weight_dtype == LB_F32, rows, dim, group,
                    out_dtype == LB_E4M3, eps, 1.0f / static_cast<float>(dim), out_dtype == LB_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f,
                    static_cast<uint8_t*>(codes), scales, hidden};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -295,17 +351,9 @@ extern "C" int lb_op_rms_norm8(const void* x, int64_t x_ld, const void* residual
                    reinterpret_cast<uintptr_t>(codes) % 8 == 0 && x_ld * size % 16 == 0 && residual_ld * size % 16 == 0 &&
                    (group == 0 || (group % 8 == 0 && width <= 32 && (width & (width - 1)) == 0));
   cudaError_t e;
-  if (vec) {
-    e = dtype == LB_F32 ? launch<float>(a, s) : dtype == LB_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
-  } else {
-    const size_t smem = sizeof(float) * dim;
-    e = smem > 40 * 1024 ? cudaFuncSetAttribute(norm_any_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                16384 * static_cast<int>(sizeof(float)))
-                         : cudaSuccess;
-    if (e == cudaSuccess) {
-      norm_any_kernel<<<rows, kThreads, smem, s>>>(a);
-      e = cudaGetLastError();
-    }
-  }
+  if (vec) e = dtype == LB_F32 ? launch<float>(a, s) : dtype == LB_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
+  else
+    e = dtype == LB_F32 ? launch_any<float>(a, s)
+                        : dtype == LB_BF16 ? launch_any<__nv_bfloat16>(a, s) : launch_any<__half>(a, s);
   return e == cudaSuccess ? LB_OK : LB_ERR_CUDA;
 }

@@ -20,6 +20,7 @@ There is no CPU path.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -127,7 +128,7 @@ class PageDirectory:
         # one allocation: the 64-bit slots, then the 32-bit arrays
         mp = self.max_pages
         words = 2 * max_tokens, n * mp, max_tokens, max_tokens, n, n + 1, 1
-        buf = torch.empty(sum(words), dtype=torch.int32, device=dev)
+        buf = self.lengths.new_empty(sum(words))
         slots, tables, positions, rows, kv_len, cu, status = buf.split(words)
         p_slots = buf.data_ptr()
         p_tables = p_slots + 8 * max_tokens
@@ -216,6 +217,11 @@ class Kv8Cache:
         return int(self.status_word.item())
 
 
+@functools.lru_cache(maxsize=None)
+def _workspace(dim: int, heads: int, kv_heads: int, max_new: int) -> int:
+    return _lib.load().lb_kv8_attention_workspace(dim, heads, kv_heads, max_new)
+
+
 def kv8_attention(q: torch.Tensor, cache: Kv8Cache, row_tables: torch.Tensor, kv_len: torch.Tensor,
                   cu_tokens: torch.Tensor, *, max_new: int, scale: float | None = None, window: int = 0,
                   softcap: float = 0.0, out: torch.Tensor | None = None, return_lse: bool = False):
@@ -244,13 +250,13 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, row_tables: torch.Tensor, kv
     if window < 0 or softcap < 0.0 or max_new < 1:
         raise ValueError("window and softcap must not be negative, max_new must be positive")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = q.new_empty(q.shape)
     else:
         _need(out, "out", q.dtype, (t, heads, dim), dev)
-    lse = torch.empty((t, heads), dtype=torch.float32, device=dev) if return_lse else None
+    lse = cache.k_scale.new_empty((t, heads)) if return_lse else None
     if t:
         kc, vc, ks, vs = cache._where
-        space = torch.empty(_lib.load().lb_kv8_attention_workspace(dim, heads, cache.kv_heads, max_new), dtype=torch.uint8, device=dev)
+        space = cache.k_codes.new_empty(_workspace(dim, heads, cache.kv_heads, max_new))
         _call(dev, "lb_op_kv8_attention", q.data_ptr(), q.stride(0), q.stride(1), DTYPE_CODES[q.dtype], t, n, heads,
               cache.kv_heads, dim, kc, vc, ks, vs, cache.pages, cache.page_tokens, row_tables.data_ptr(), max_pages,
               kv_len.data_ptr(), cu_tokens.data_ptr(), max_new, dim ** -0.5 if scale is None else scale, window, softcap,
@@ -281,8 +287,10 @@ def rms_norm8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor |
                                  or (x.numel() and residual.stride(1) != 1)):
         raise ValueError("residual must be like x")
     codes = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
-    scales = torch.empty((rows, dim // group if group else 1), dtype=torch.float32, device=dev)
-    hidden = x if residual is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+    n_groups = dim // group if group else 1
+    scales = (weight.new_empty((rows, n_groups)) if weight.dtype == torch.float32
+              else torch.empty((rows, n_groups), dtype=torch.float32, device=dev))
+    hidden = x if residual is None else x.new_empty(x.shape)
     if rows:
         _call(dev, "lb_op_rms_norm8", x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(),
               0 if residual is None else residual.stride(0), DTYPE_CODES[x.dtype], weight.data_ptr(),

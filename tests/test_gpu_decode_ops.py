@@ -590,3 +590,21 @@ def test_append_of_groups_larger_than_the_registers_hold(ops, pkg, dim, page, to
         assert ((got - x.double()).abs() <= 0.5 * step * (1 + 1e-4)).all()
         top = torch.stack([x[p * page:(p + 1) * page].double().abs().amax((0, 2)) for p in range(pages)]) / 127
         torch.testing.assert_close(scale.double(), top, rtol=2.0 ** -22, atol=0)
+
+
+@pytest.mark.parametrize("rows,dim,group", [(1500, 100, 0), (1184, 999, 27), (1300, 1020, 12), (1200, 1027, 0), (5, 14001, 0), (1191, 320, 40)])
+def test_norm_of_odd_widths_in_many_rows(ops, rows, dim, group):
+    g = gen(rows + dim)
+    for dtype in (BF16, F32):
+        x, res = (torch.randn(rows, dim, generator=g, device="cuda").to(dtype) for _ in range(2))
+        x[1] = 0.0
+        res[1] = 0.0
+        w = 1 + 0.3 * torch.randn(dim, generator=g, device="cuda")
+        codes, scales, hidden = ops.rms_norm8(x, w, residual=res, group=group, dtype=I8)
+        h, y = decode_ref.rms_norm(x, res, w, eps=1e-6)
+        assert ((hidden.double() - h).abs() <= HALF_ULP[dtype] * (1 + 1e-3) * h.abs() + 1e-9).all()
+        y = y.view(rows, -1, group or dim)
+        want = y.abs().amax(2) / 127
+        torch.testing.assert_close(scales.double(), want, rtol=4e-6, atol=1e-44)
+        got = codes.double().view(y.shape) * scales.double()[..., None]
+        assert ((got - y).abs() <= 0.5 * want[..., None] * (1 + 1e-3) + 1e-5 * y.abs()).all()
