@@ -102,7 +102,6 @@ class PageDirectory:
         self.tables, self.lengths, self.used = tables, lengths, used
         self.pages, self.page_tokens = int(pages), int(page_tokens)
         self._released = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._where = (tables.data_ptr(), lengths.data_ptr(), used.data_ptr())
 
     @classmethod
     def create(cls, *, sessions: int, max_pages: int, pages: int, page_tokens: int,
@@ -137,8 +136,8 @@ class PageDirectory:
         p_len = p_rows + 4 * max_tokens
         p_cu = p_len + 4 * n
         _call(dev, "lb_plan_pages", n, sessions.data_ptr(), new_tokens.data_ptr(), self.sessions, mp, self.pages,
-              self.page_tokens, self._where[0], self._where[1], self._where[2], max_tokens, p_tables, p_len, p_cu,
-              p_slots, p_pos, p_rows, p_cu + 4 * n + 4)
+              self.page_tokens, self.tables.data_ptr(), self.lengths.data_ptr(), self.used.data_ptr(), max_tokens,
+              p_tables, p_len, p_cu, p_slots, p_pos, p_rows, p_cu + 4 * n + 4)
         return PagePlan(sessions, tables.view(n, mp), kv_len, cu, slots.view(torch.int64), positions, rows, status)
 
     def commit(self, plan: PagePlan) -> None:
@@ -184,7 +183,6 @@ class Kv8Cache:
             _need(t, name, torch.float32, (self.pages, self.kv_heads), self.device)
         self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
         self.status_word = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._where = (k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
 
     @classmethod
     def create(cls, *, pages: int, kv_heads: int, page_tokens: int, dim: int,
@@ -192,6 +190,9 @@ class Kv8Cache:
         shape = (pages, kv_heads, page_tokens, dim)
         return cls(torch.zeros(shape, dtype=torch.int8, device=device), torch.zeros(shape, dtype=torch.int8, device=device),
                    torch.zeros(shape[:2], device=device), torch.zeros(shape[:2], device=device))
+
+    def _pointers(self) -> tuple[int, int, int, int]:
+        return self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Writes k, v [tokens, kv_heads, dim] to ``slots`` int64 [tokens] (negative: skipped).
@@ -207,7 +208,7 @@ class Kv8Cache:
         _need(slots, "slots", torch.int64, (n,), self.device)
         if n == 0:
             return
-        kc, vc, ks, vs = self._where
+        kc, vc, ks, vs = self._pointers()
         _call(self.device, "lb_op_kv8_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
               v.stride(1), DTYPE_CODES[k.dtype], n, self.kv_heads, self.dim, slots.data_ptr(), kc, vc, ks, vs,
               self.pages, self.page_tokens, self.status_word.data_ptr())
@@ -255,7 +256,7 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, row_tables: torch.Tensor, kv
         _need(out, "out", q.dtype, (t, heads, dim), dev)
     lse = cache.k_scale.new_empty((t, heads)) if return_lse else None
     if t:
-        kc, vc, ks, vs = cache._where
+        kc, vc, ks, vs = cache._pointers()
         space = cache.k_codes.new_empty(_workspace(dim, heads, cache.kv_heads, max_new))
         _call(dev, "lb_op_kv8_attention", q.data_ptr(), q.stride(0), q.stride(1), DTYPE_CODES[q.dtype], t, n, heads,
               cache.kv_heads, dim, kc, vc, ks, vs, cache.pages, cache.page_tokens, row_tables.data_ptr(), max_pages,
