@@ -11,9 +11,9 @@
 // subtraction leaves n - 8 exactly; x is stored in the pairs' order, so neither side is
 // shuffled.  8-bit x is exact in fp16.  A group's sum is held in 32 bits and takes its
 // scale there.  mma.sync runs at 0.5 m16n8k16 a cycle and SM, and the stream of 16 rows needs 0.36, so the
-// tensor pipe is not what binds (27 % busy): the shifts and masks that widen the codes are (11 instructions
-// for 8 codes in bf16, 9 in fp16, at half rate).  16 x 2048 x 131072 in groups of 64 takes 61.5 us, 2.4 TB/s; one
-// row 55.
+// tensor pipe is not what binds (27 % busy): instructions are, some 450 a stage and warp, nearly half of them on
+// the half-rate integer pipe (50 % busy; the widening alone is 11 for 8 codes in bf16, 9 in fp16).  16 x 2048 x
+// 131072 in groups of 64 takes 61.5 us, 2.4 TB/s (fp16 3 us less, one row 9 us less).
 //
 // K is split among the warps of a CTA (and summed in shared memory) as far as one wave of CTAs goes: 2 x
 // 1536 x 6144 takes 6.8 us inside a graph.  Larger products run 16 warps an SM that walk over the tiles (8
