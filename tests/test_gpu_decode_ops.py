@@ -608,3 +608,23 @@ def test_norm_of_odd_widths_in_many_rows(ops, rows, dim, group):
         torch.testing.assert_close(scales.double(), want, rtol=4e-6, atol=1e-44)
         got = codes.double().view(y.shape) * scales.double()[..., None]
         assert ((got - y).abs() <= 0.5 * want[..., None] * (1 + 1e-3) + 1e-5 * y.abs()).all()
+
+
+def test_exchanged_tensors_of_directory_and_cache_are_followed(ops):
+    pages = ops.PageDirectory.create(sessions=2, max_pages=4, pages=8, page_tokens=16)
+    cache = ops.Kv8Cache.create(pages=8, kv_heads=1, page_tokens=16, dim=64)
+    old = (pages.tables, pages.lengths, pages.used, cache.k_codes, cache.k_scale)
+    before = [t.clone() for t in old]
+    pages.tables, pages.lengths, pages.used = (t.clone() for t in old[:3])
+    cache.k_codes, cache.k_scale = old[3].clone(), old[4].clone()
+    pages.lengths[1] = 5
+    pages.tables[1, 0] = 3
+    pages.used[0] = 1 << 3
+    ids = torch.tensor([1], dtype=torch.int32, device="cuda")
+    plan = pages.plan(ids, torch.full_like(ids, 2), max_tokens=2)
+    assert plan.status() == 0 and plan.kv_len.tolist() == [7] and plan.slots.tolist() == [3 * 16 + 5, 3 * 16 + 6]
+    k = torch.ones(2, 1, 64, device="cuda")
+    cache.append(k, k, plan.slots)
+    pages.commit(plan)
+    assert cache.k_codes[3, 0, 5:7].eq(127).all() and pages.lengths.tolist() == [0, 7]
+    assert all(torch.equal(a, b) for a, b in zip(old, before))
