@@ -7,9 +7,11 @@
 // cache (tcgen05 kind::i8): no code is ever widened.  q and p are split into signed
 // 8-bit digits instead, which become neighbouring columns of one MMA:
 //   q * 2^e = 65536 q2 + 256 q1 + q0   (e brings the row's maximum to 2^21: 22 bits and a sign)
-//   p * sv / max sv * 63 * 2^16 = 65536 p2 + 256 p1 + p0   (per tile, relative to the tile's largest
-//                                            score: an error of 2^-23 of the tile's largest term)
+//   p * sv * c = 65536 p2 + 256 p1 + p0   (c, of each tile and query, brings the largest p * sv among the
+//                  keys that the query sees to 63 * 2^16: an error of 2^-23 of that largest p * sv a key)
 //   S^T[key, (digit, query)] = K . Q^T,   O^T[column, (digit, query)] = V^T . P^T
+// c takes the largest p * sv, not the largest p times the largest sv: the pages of a tile may have scales far
+// apart, and the key with the weight the smallest.  Pages that a query does not see do not count for it.
 // The products are exact in 32-bit integers, and the digits' sums are joined in 32-bit
 // floating point.  The fixed point of p is one of 128 keys: a tile's outputs leave
 // the tensor memory each time and are added up in registers with the tile's factor.
@@ -157,6 +159,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // Waits for a phase.  Bounded by the number of polls: try_wait sleeps in hardware, for up to the 20 us
 // that it is given, so the limit is at most 2.6 s.  Kept short, because all roles
 // together are bound by the instructions they issue.
@@ -182,7 +189,11 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, wait_one(bar, parity));
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) { return (a > b || isnan(a)) ? a : b; }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 // the largest of the warp's values, a NaN if there is one
 __device__ __forceinline__ float warp_top(float x) {
   float y;
@@ -317,7 +328,9 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------ the kernel
-template <typename T, int D, int R>
+// kHalves: boxes of 16 keys, so that a score warp's two halves have a scale of V each (a kernel of its own: the few
+// instructions more in the hot loop cost the others 3 to 7 %)
+template <typename T, int D, int R, bool kHalves>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a, const __grid_constant__ CUtensorMap k_map,
                                                              const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D, R>;
@@ -335,14 +348,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   __shared__ uint32_t tmem_slot;
   __shared__ long long pre[kThreads + 1];
   __shared__ long long warp_total[kThreads / 32];
-  __shared__ float g_ks[kInfo][kBoxes], g_vs[kInfo][kBoxes], g_top[kInfo];
+  // by box: the scales of K, those of V over the tile's unit (a power of two; kept over kFixed); bits of the boxes
+  // that are there, and from bit 8 on of those whose scale of V is not finite
+  __shared__ float g_ks[kInfo][kBoxes], g_vs[kInfo][kBoxes], g_unit[kInfo];
   __shared__ unsigned g_there[kInfo];
   __shared__ __align__(16) float fac_s[2][R];    // a query: its factor to log2 scores, and the keys that it sees
   __shared__ int last_s[2][R], first_s[2][R];
-  __shared__ float tops_s[kScorers][2][4][kQueries];  // a turn's largest scores, by warp
+  __shared__ __align__(16) float2 tops_s[kScorers][2][4][kQueries];  // a turn's largest scores by warp, and p * sv over theirs
   __shared__ __align__(16) float top_s[4 * kScorers][kQueries], beta_s[4 * kScorers][kQueries];
-  __shared__ __align__(16) float factor_s[4 * kScorers][kQueries];
-  __shared__ float mx_ring[kRing][R], v_ring[kRing];  // a tile's largest scores and largest V scale
+  __shared__ __align__(16) float factor_s[4 * kScorers][kQueries], up_s[4 * kScorers][kQueries];
+  __shared__ float mx_ring[kRing][R], down_ring[kRing][R];  // a tile's largest scores, and 1 / c
   __shared__ __align__(16) float out_f[4][R];
   __shared__ float l_part[4 * kScorers][kQueries], m_ref[kScorers][kQueries];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -520,9 +535,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       const int tiles = min(batch, b0.n - b0.tile);
       const uint64_t policy = tasks[b0.task % kTasks].q_tiles > 1 ? again : once;  // other query tiles read the same keys
       const unsigned there = __ballot_sync(0xffffffffu, w0.at >= 0);
-      float v_top = fabsf(w0.vs);
+      // the tile's unit: its largest finite scale of V, less the fraction (its inverse is a normal number)
+      int v_unit = __float_as_int(w0.vs) & 0x7f800000;
+      if (v_unit == 0x7f800000) v_unit = 0;
 #pragma unroll 1
-      for (int o = 1; o < nb; o <<= 1) v_top = max_nan(v_top, __shfl_xor_sync(0xffffffffu, v_top, o));
+      for (int o = 1; o < nb; o <<= 1) v_unit = max(v_unit, __shfl_xor_sync(0xffffffffu, v_unit, o));
+      v_unit = min(max(v_unit, 0x00800000), 0x7e800000);
+      float v_own = w0.vs * __int_as_float(0x7f000000 - v_unit);
+      const bool v_bad = !(fabsf(v_own) < INFINITY);
+      if (v_bad) v_own = 0.0f;  // (a key that does not count has digits of 0 all the same)
+      const unsigned bad = __ballot_sync(0xffffffffu, v_bad), all = (1u << nb) - 1u;
+      const unsigned boxes = own_tile < batch ? (there >> (own_tile * nb) & all) | (bad >> (own_tile * nb) & all) << 8 : 0u;
 #pragma unroll 1
       for (int j = 0; ok && j < tiles; ++j, ++i) {
         const int info = i % kInfo;
@@ -534,10 +557,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
           if (!ok) break;
           if (side == 0 && own) {
             g_ks[info][k] = w0.ks;
-            g_vs[info][k] = w0.vs;
+            g_vs[info][k] = v_own;
             if (k == 0) {
-              g_there[info] = mask;
-              g_top[info] = v_top;
+              g_there[info] = boxes;
+              g_unit[info] = __int_as_float(v_unit) * (1.0f / kFixed);
             }
           }
           __syncwarp();
@@ -737,6 +760,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
     float* own_top = top_s[warp - kFirstScorer];
     float* own_beta = beta_s[warp - kFirstScorer];
     float* own_fac = factor_s[warp - kFirstScorer];
+    float* own_up = up_s[warp - kFirstScorer];
+    const unsigned all_boxes = (1u << (kTile >> a.box_log)) - 1u;
     int i = 0, turn = 0;
     while (ok && next()) {
       const Task& t = tasks[task % kTasks];
@@ -749,7 +774,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       for (int q = 0; q < C; ++q) l[q] = 0.0f;
       float ref = -INFINITY;  // lane q: the reference maximum of query q (the four warps keep the same)
       // (a capped score has its factor already)
-      if (lane < C) own_fac[lane] = a.softcap > 0.0f ? 1.0f : fac_s[qb][c0 + lane];
+      const float fac = a.softcap > 0.0f ? 1.0f : fac_s[qb][c0 + lane % C];
+      const float fac_up = fac * (1.0f + 0x1p-22f), fac_down = fac * (1.0f - 0x1p-22f);
+      if (lane < C) own_fac[lane] = fac;
       __syncwarp();
 #pragma unroll 1
       for (int tile = 0; ok && tile < n_tiles; ++tile, ++i) {
@@ -759,11 +786,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         if (!ok) break;
         tc_fence_after();
         const int grp = key_row >> a.box_log;
-        const float ks = g_ks[info][grp], vs = g_vs[info][grp], v_top = g_top[info];
-        const bool there = (g_there[info] >> grp) & 1u;
+        const float ks = g_ks[info][grp], vs = g_vs[info][grp], unit = g_unit[info];
+        const float v0 = fabsf(g_vs[info][wq * 32 >> a.box_log]), v1 = fabsf(g_vs[info][(wq * 32 + 16) >> a.box_log]);  // of the warp's halves
+        const unsigned boxes = g_there[info];
+        const bool there = (boxes >> grp) & 1u;
         const int key0 = first_key + tile * kTile, key = key0 + key_row;
-        const bool masked = key0 + kTile > plain_stop || key0 < plain_start || __any_sync(0xffffffffu, !there);
-        const float to_fixed = v_top > 0.0f ? __fdividef(vs, v_top) * kFixed : 0.0f;
+        const bool masked = key0 + kTile > plain_stop || key0 < plain_start || boxes != all_boxes;
         unsigned char* p = p_digits + buf * S::kPBytes;
         float x[C];
         {
@@ -786,23 +814,50 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
 #pragma unroll
           for (int q = 0; q < C; ++q)
             if (!there || key > last_s[qb][c0 + q] || key < first_s[qb][c0 + q]) x[q] = -INFINITY;
+            else if (boxes >> 8 >> grp & 1u) x[q] = NAN;  // a scale of V that is no number: so is the query's output
         }
         // the turn's largest score of each query, still without its (positive) factor: warp, then the four warps
-        float mx = -INFINITY;
+        float mx = -INFINITY, my = -INFINITY;
+        if constexpr (kHalves) {
 #pragma unroll
-        for (int q = 0; q < C; ++q) {
-          const float m = warp_top(x[q]);
-          if (lane == q) mx = m;
+          for (int q = 0; q < C; ++q) {
+            const float m0 = warp_top(lane < 16 ? x[q] : -INFINITY), m1 = warp_top(lane < 16 ? -INFINITY : x[q]);
+            if (lane == q) {
+              mx = m0;
+              my = m1;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < C; ++q) {
+            const float m = warp_top(x[q]);
+            if (lane == q) mx = m;
+          }
         }
-        if (lane < C) tops_s[side][turn & 1][wq][lane] = mx;
+        if (lane < C) {
+          // rounded up, so that no exponential below passes 1 however large the scores are
+          mx = fmaxf(mx * fac_up, mx * fac_down);
+          float pv = v0;
+          if constexpr (kHalves) {
+            my = fmaxf(my * fac_up, my * fac_down);
+            const float most = max_nan(mx, my);
+            pv = fmaxf(exp2_fast(mx - most) * v0, exp2_fast(my - most) * v1);
+            mx = most;
+          }
+          tops_s[side][turn & 1][wq][lane] = make_float2(mx, pv);
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&tops[side]);
         ok = wait_warp(&tops[side], turn & 1);
         if (!ok) break;
         float alpha = 1.0f;
         if (lane < C) {
-          const float* w0 = tops_s[side][turn & 1][0];
-          mx = max_nan(max_nan(w0[lane], w0[C + lane]), max_nan(w0[2 * C + lane], w0[3 * C + lane])) * own_fac[lane];
+          const float2* tw = &tops_s[side][turn & 1][0][lane];
+          const float2 t0 = tw[0], t1 = tw[C], t2 = tw[2 * C], t3 = tw[3 * C];
+          mx = max_nan(max_nan(t0.x, t1.x), max_nan(t2.x, t3.x));
+          // the largest p * sv (a maximum drops the NaN of no key at all, and a NaN score is a NaN in mx)
+          const float pv = fmaxf(fmaxf(exp2_fast(t0.x - mx) * t0.y, exp2_fast(t1.x - mx) * t1.y),
+                                 fmaxf(exp2_fast(t2.x - mx) * t2.y, exp2_fast(t3.x - mx) * t3.y));
           if (ref == -INFINITY) {
             ref = mx;
           } else if (mx > ref + kSlack) {
@@ -811,9 +866,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
           }
           own_top[lane] = mx == -INFINITY ? 0.0f : mx;
           own_beta[lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref);
-          if (wq == 0) mx_ring[i % kRing][c0 + lane] = mx;
+          // Over the unit, so powers of two are exact: pages that the query does not see change no bit.  Not below
+          // 2^-100 of it, where c * sv would not stay finite.
+          const float top_pv = fmaxf(pv, 0x1p-100f);
+          own_up[lane] = rcp_fast(top_pv) * kFixed;
+          if (wq == 0) {
+            mx_ring[i % kRing][c0 + lane] = mx;
+            down_ring[i % kRing][c0 + lane] = top_pv * unit;
+          }
         }
-        if (wq == 0 && lane == 0 && c0 == 0) v_ring[i % kRing] = v_top;
         const bool moved = __any_sync(0xffffffffu, alpha != 1.0f);
         __syncwarp();
         if (moved) {
@@ -824,9 +885,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         for (int q = 0; q < C; ++q) {
           const float e = exp2_fast(fmaf(x[q], own_fac[q], -own_top[q]));
           l[q] = fmaf(e, own_beta[q], l[q]);
-          // v = rint(e * to_fixed) by a sum with 1.5 * 2^23.  With 128 added to each of the two lower
+          // v = rint(e * sv * c) by a sum with 1.5 * 2^23.  With 128 added to each of the two lower
           // digits' places, the bytes of v are its signed digits, the lower two with the sign bit turned over.
-          const uint32_t v = __float_as_uint(fmaf(e, to_fixed, 12582912.0f)) - 0x4B400000u;
+          const uint32_t v = __float_as_uint(fmaf(e, vs * own_up[q], 12582912.0f)) - 0x4B400000u;
           const uint32_t digits = (v + 0x8080u) ^ 0x8080u;
           unsigned char* to = p + swizzled<128>(q * kTile + key_row) + c0 * kTile;  // (c0 is a multiple of 8 rows)
           to[0] = static_cast<unsigned char>(digits >> 16);
@@ -893,7 +954,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
             alpha = exp2_fast(ref - mx);
             ref = mx;
           }
-          factor[lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref) * v_ring[i % kRing] * (1.0f / kFixed);
+          factor[lane] = mx == -INFINITY ? 0.0f : exp2_fast(mx - ref) * down_ring[i % kRing][lane];
         }
         __syncwarp();
         if (__any_sync(0xffffffffu, alpha != 1.0f)) {
@@ -1052,16 +1113,21 @@ __global__ void __launch_bounds__(512) combine_kernel(const AttendArgs a) {
 // and the threads' work are not spent on padding; at most what two score warpgroups' turns hold.
 int rows_of(int max_new, int group) { return static_cast<long long>(max_new) * group <= 8 ? 8 : 16; }
 
-template <typename T, int D, int R>
+template <typename T, int D, int R, bool kHalves>
 cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
   using S = Shape<D, R>;
+  const auto kernel = attend_kernel<T, D, R, kHalves>;
   static std::atomic<unsigned long long> done{0};
-  cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(attend_kernel<T, D, R>), S::kSmem);
+  cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), S::kSmem);
   if (e != cudaSuccess) return e;
-  attend_kernel<T, D, R><<<kSms, kThreads, S::kSmem, s>>>(a, k_map, v_map);
+  kernel<<<kSms, kThreads, S::kSmem, s>>>(a, k_map, v_map);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_kernel(true, combine_kernel<T, D, R>, dim3(kSms, R), dim3(512), 0, s, a);
+}
+template <typename T, int D, int R>
+cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
+  return a.box == 16 ? launch<T, D, R, true>(a, k_map, v_map, s) : launch<T, D, R, false>(a, k_map, v_map, s);
 }
 template <typename T, int D>
 cudaError_t launch(const AttendArgs& a, int rows, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {

@@ -1,0 +1,183 @@
+"""The text-decoder operators where their inputs' ranges and contracts end.
+
+Attention's bound, from what the kernel holds (all relative to one query):
+- q is rounded to 2^-22 of its row's largest value, the sums of products are joined in 32 bits:
+  a score is off by dx <= 2^-22 * scale * max|q| * sum |k| + 2^-21 * scale * sum |q||k|
+  + 2^-21 (1 + |score|) (the exponential's argument and its approximation);
+- p * sv is rounded to a step of 1 / (63 * 2^16) of the largest p * sv among the tile's keys that the query
+  sees: half a step times sum |code| of the tile's keys;
+- factors, the sum of p and the division: 2^-20 of sum p|v|;
+- the output's half ulp (and its smallest step).
+"""
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+from oracle import decode_ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32, E4M3, I8 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn, torch.int8
+HALF_ULP = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: 2.0 ** -24}
+SMALLEST = {BF16: 2.0 ** -133, F16: 2.0 ** -25}
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    from gemma4_omni_b200 import decode_ops
+    return decode_ops
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def make_cache(ops, g, lens, page, heads, dim):
+    """Random codes and scales on shuffled pages; the row tables."""
+    rng = random.Random(page + dim)
+    order = list(range(sum(-(-n // page) for n in lens) + 2))
+    cache = ops.Kv8Cache.create(pages=len(order), kv_heads=heads, page_tokens=page, dim=dim)
+    rng.shuffle(order)
+    width = max(1, max(-(-n // page) for n in lens))
+    tables = [[order.pop() for _ in range(-(-n // page))] for n in lens]
+    for side in (cache.k_codes, cache.v_codes):
+        side.copy_(torch.randint(-127, 128, side.shape, generator=g, device="cuda"))
+    for side in (cache.k_scale, cache.v_scale):
+        side.copy_((0.5 + torch.rand(side.shape, generator=g, device="cuda")) * 3.0 / 127)
+    return cache, ints([t + [-1] * (width - len(t)) for t in tables])
+
+
+def check(ops, cache, tables, q, lens, cu, *, max_new, scale=None, window=0, softcap=0.0):
+    """Every output against 64 bits within the bound at the top of this file; returns (out, lse)."""
+    dim, page = cache.dim, cache.page_tokens
+    out, lse = ops.kv8_attention(q, cache, tables, ints(lens), ints(cu), max_new=max_new, scale=scale, window=window,
+                                 softcap=softcap, return_lse=True)
+    scale = dim ** -0.5 if scale is None else scale
+    box = 64 if page % 64 == 0 else 32 if page % 32 == 0 else 16
+    kvh, group = cache.kv_heads, q.shape[1] // cache.kv_heads
+    for r, n in enumerate(lens):
+        a, b = cu[r], cu[r + 1]
+        held = tables[r, : -(-n // page)].long()
+
+        def rows(x):
+            return x[held].double().transpose(0, 1).reshape(kvh, -1, dim)[:, :n]
+
+        def each(x):
+            return x[held].double().t().repeat_interleave(page, 1)[:, :n]
+        kc, vc, ks, vs = rows(cache.k_codes), rows(cache.v_codes), each(cache.k_scale), each(cache.v_scale)
+        low = max(0, n - (b - a) + 1 - window) // box * box if window else 0
+        for i in range(a, b):
+            pos = n - (b - a) + i - a
+            first = max(0, pos - window + 1) if window else 0
+            if pos < first:
+                assert not out[i].any() and (lse[i] == -math.inf).all()
+                continue
+            see = slice(first, pos + 1)
+            k, v, c = kc[:, see] * ks[:, see, None], vc[:, see] * vs[:, see, None], vc[:, see].abs()
+            qi = q[i].double().view(kvh, group, dim)
+            x = scale * torch.einsum("hgd,hkd->hgk", qi, k)
+            dx = 2.0 ** -22 * abs(scale) * qi.abs().amax(2)[..., None] * k.abs().sum(2)[:, None] + 2.0 ** -21 * (
+                abs(scale) * torch.einsum("hgd,hkd->hgk", qi.abs(), k.abs()) + 1)
+            if softcap:
+                x = softcap * torch.tanh(x / softcap)
+            dx = (dx + 2.0 ** -21 * x.abs()).amax(2)
+            want = torch.logsumexp(x, 2)
+            p = torch.exp(x - want[..., None])
+            ref = torch.einsum("hgk,hkd->hgd", p, v)
+            spread = torch.einsum("hgk,hkd->hgd", p, v.abs())
+            steps = torch.zeros_like(ref)
+            tile = (torch.arange(first, pos + 1, device="cuda") - low) // 128
+            for t in tile.unique().tolist():
+                at = tile == t
+                top = (p[..., at] * vs[:, None, see][..., at].abs()).amax(2)
+                steps += top[..., None] * c[:, at].sum(1)[:, None] * (0.5 / (63 * 2 ** 16))
+            bound = HALF_ULP[q.dtype] * ref.abs() + (2 * dx[..., None] + 2.0 ** -20) * spread + 1.01 * steps + SMALLEST[q.dtype]
+            far = ((out[i].double().view(ref.shape) - ref).abs() / bound).max().item()
+            assert far <= 1.0, (r, i, far)
+            assert ((lse[i].double().view(want.shape) - want).abs() <= dx + 2.0 ** -20 * (1 + want.abs())).all()
+    assert cache.status() == 0
+    return out, lse
+
+
+# ------------------------------------------------------------------ attention: V scales far apart
+def split_scores(cache, tables, light):
+    """K codes such that q = 1 scores the keys of the `light` table columns 60 binary orders below the others."""
+    dim, page = cache.dim, cache.page_tokens
+    cache.k_codes.fill_(40)
+    cache.k_codes[tables[0, light].long()] = -40
+    cache.k_codes[:, :, :, 0] = torch.randint(-127, 128, cache.k_codes.shape[:3], device="cuda", generator=gen(1))
+    cache.k_scale.fill_(1 / 40)
+    return 60 * math.log(2) / (2 * (dim - 1))  # the score's scale
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("ratio", [1e2, 1e4, 1e5, 1e8, 2.0 ** 24, 2.0 ** 60])
+@pytest.mark.parametrize("dim,heads,page,first_light", [(64, 1, 64, True), (128, 8, 32, False), (256, 16, 16, True), (64, 2, 48, False),
+                                                        (128, 16, 128, True)])
+def test_small_v_scales_with_all_the_weight(ops, dtype, ratio, dim, heads, page, first_light):
+    g = gen(7)
+    pages = max(2, 128 // page)
+    n = pages * page
+    cache, tables = make_cache(ops, g, [n], page, 1, dim)
+    half = pages // 2
+    light = list(range(half)) if first_light else list(range(half, pages))
+    scale = split_scores(cache, tables, light)
+    cache.v_scale[tables[0, light].long()] *= ratio
+    if dtype is F16:
+        cache.v_scale /= max(1.0, ratio / 1e4)  # (the large values stay inside the type)
+    q = torch.ones(1, heads, dim, device="cuda").to(dtype)
+    q[0, heads // 2:] *= -1.0  # these see the large scales
+    check(ops, cache, tables, q, [n], [0, 1], max_new=1, scale=scale)
+
+
+@pytest.mark.parametrize("page,heads", [(16, 1), (16, 8), (32, 4), (64, 8), (128, 2)])
+def test_a_token_does_not_depend_on_the_scale_of_a_page_that_it_does_not_see(ops, page, heads):
+    g = gen(page)
+    n = page + 1  # the first of two tokens ends a page, the second begins one
+    cache, tables = make_cache(ops, g, [n, n], page, 1, 128)
+    q = torch.randn(4, heads, 128, generator=g, device="cuda").to(BF16)
+    plain, _ = check(ops, cache, tables, q, [n, n], [0, 2, 4], max_new=2)
+    for large in (1e3, 1e6, 1e25):  # (up to 2^100 times the others)
+        cache.v_scale[tables[0, 1]] = large
+        out, _ = check(ops, cache, tables, q, [n, n], [0, 2, 4], max_new=2)
+        assert torch.equal(out[0], plain[0]) and torch.equal(out[2:], plain[2:])
+    # a scale that is no number: as a page that was never written holds it
+    cache.v_scale[tables[0, 1]] = math.nan
+    out = ops.kv8_attention(q, cache, tables, ints([n, n]), ints([0, 2, 4]), max_new=2)
+    assert torch.equal(out[0], plain[0]) and torch.equal(out[2:], plain[2:]) and torch.isnan(out[1]).all()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_window_over_pages_of_very_different_scales(ops, page):
+    g = gen(page + 1)
+    lens, new = [900, 300, 128], [2, 1, 40]
+    cache, tables = make_cache(ops, g, lens, page, 2, 64)
+    exps = torch.randint(-12, 13, cache.v_scale.shape, generator=g, device="cuda").float()
+    cache.v_scale *= torch.exp2(exps)
+    q = torch.randn(43, 8, 64, generator=g, device="cuda").to(F16) * 3.0
+    for window in (0, 17, 100):
+        check(ops, cache, tables, q, lens, [0, 2, 3, 43], max_new=40, window=window)
+        check(ops, cache, tables, q[:, :2], lens, [0, 2, 3, 43], max_new=2, window=window)
+
+
+def test_zero_scales_among_others(ops):
+    g = gen(3)
+    cache, tables = make_cache(ops, g, [256], 32, 1, 128)
+    q = torch.randn(1, 8, 128, generator=g, device="cuda").to(F16)
+    cache.v_scale[tables[0, ::2].long()] = 0.0
+    check(ops, cache, tables, q, [256], [0, 1], max_new=1)
+    cache.v_scale[tables[0, 1::2].long()] = 1e-38
+    check(ops, cache, tables, q, [256], [0, 1], max_new=1)
+    cache.v_scale.zero_()
+    out, _ = check(ops, cache, tables, q, [256], [0, 1], max_new=1)
+    assert not out.any()
