@@ -159,6 +159,38 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+struct Scores {
+  float v[kQueries];
+};
+// cap * tanh(s / cap), inv = 1 / cap, for a warp together.  Near zero (u = s / cap, w = u * u below kSmall) s times the
+// series of tanh(u) / u, whose first term left out is below 2^-26; elsewhere 1 - 2 / (1 + e^2u).  An error of some
+// 2^-20 of the result for every cap.  The second form is not in line: most scores are small beside their cap.
+constexpr float kSmall = 0.0625f;
+__device__ __forceinline__ float tanh_series(float w) {
+  return fmaf(w, fmaf(w, fmaf(w, fmaf(w, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+}
+__device__ __noinline__ Scores capped_far(Scores s, float cap, float inv) {
+#pragma unroll
+  for (int q = 0; q < kQueries; ++q) {
+    const float u = s.v[q] * inv, w = u * u;
+    s.v[q] = w < kSmall ? s.v[q] * tanh_series(w) : cap - __fdividef(2.0f, 1.0f + exp2_fast(u * (2.0f * kLog2e))) * cap;
+  }
+  return s;
+}
+__device__ __forceinline__ Scores capped(Scores s, float cap, float inv) {
+  float w[kQueries];
+  bool near = true;
+#pragma unroll
+  for (int q = 0; q < kQueries; ++q) {
+    w[q] = s.v[q] * inv;
+    w[q] *= w[q];
+    near = near && w[q] < kSmall;
+  }
+  if (!__all_sync(0xffffffffu, near)) return capped_far(s, cap, inv);
+#pragma unroll
+  for (int q = 0; q < kQueries; ++q) s.v[q] *= tanh_series(w[q]);
+  return s;
+}
 __device__ __forceinline__ float rcp_fast(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -328,9 +360,10 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------ the kernel
-// kHalves: boxes of 16 keys, so that a score warp's two halves have a scale of V each (a kernel of its own: the few
-// instructions more in the hot loop cost the others 3 to 7 %)
-template <typename T, int D, int R, bool kHalves>
+// kHalves: boxes of 16 keys, so that a score warp's two halves have a scale of V each.  kCapped: scores have a soft cap.
+// Kernels of their own, for the loops' instructions: with both in every kernel windowed ticks took 162 us instead of
+// 149, answers 235 instead of 215 (in graphs).
+template <typename T, int D, int R, bool kHalves, bool kCapped>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a, const __grid_constant__ CUtensorMap k_map,
                                                              const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D, R>;
@@ -718,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         const float up1 = copysignf(__int_as_float((127 + e1) << 23), a.scale), up2 = __int_as_float((127 + e2) << 23);
         if (lane == 0) {
           // positive (a negative scale turns the digits over) and not zero, so that masked scores stay at -inf
-          const float down = __int_as_float((127 - e1) << 23) * (fabsf(a.scale) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e)) *
+          const float down = __int_as_float((127 - e1) << 23) * (fabsf(a.scale) * kLog2e) *
                              __int_as_float((127 - e2) << 23);
           fac_s[buf][qi] = !fine ? NAN : down < 0x1p-126f ? 0x1p-126f : down;
           last_s[buf][qi] = min(qi < t.rows ? pos : 0x7fffffff, t.stop - 1);
@@ -762,6 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
     float* own_fac = factor_s[warp - kFirstScorer];
     float* own_up = up_s[warp - kFirstScorer];
     const unsigned all_boxes = (1u << (kTile >> a.box_log)) - 1u;
+    const float cap = fminf(a.softcap * kLog2e, 0x1p127f), cap_inv = fminf(kLn2 / a.softcap, 0x1p127f);  // of log2 scores
     int i = 0, turn = 0;
     while (ok && next()) {
       const Task& t = tasks[task % kTasks];
@@ -774,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       for (int q = 0; q < C; ++q) l[q] = 0.0f;
       float ref = -INFINITY;  // lane q: the reference maximum of query q (the four warps keep the same)
       // (a capped score has its factor already)
-      const float fac = a.softcap > 0.0f ? 1.0f : fac_s[qb][c0 + lane % C];
+      const float fac = kCapped ? 1.0f : fac_s[qb][c0 + lane % C];
       const float fac_up = fac * (1.0f + 0x1p-22f), fac_down = fac * (1.0f - 0x1p-22f);
       if (lane < C) own_fac[lane] = fac;
       __syncwarp();
@@ -793,35 +827,35 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         const int key0 = first_key + tile * kTile, key = key0 + key_row;
         const bool masked = key0 + kTile > plain_stop || key0 < plain_start || boxes != all_boxes;
         unsigned char* p = p_digits + buf * S::kPBytes;
-        float x[C];
+        Scores x;
         {
           int d2[C], d1[C], dd[C];
           const uint32_t at = tmem + buf * S::kS + lane_at + c0;
           tmem_ld3<C>(at, at + R, at + 2 * R, d2, d1, dd);
 #pragma unroll
           for (int c = 0; c < C; ++c)
-            x[c] = fmaf(__int2float_rn(d2[c]), 65536.0f, __int2float_rn(d1[c] * 256 + dd[c])) * ks;
+            x.v[c] = fmaf(__int2float_rn(d2[c]), 65536.0f, __int2float_rn(d1[c] * 256 + dd[c])) * ks;
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_empty[buf]);
-        if (a.softcap > 0.0f) {
+        if constexpr (kCapped) {
 #pragma unroll
-          for (int q = 0; q < C; ++q)  // tanh(u) = 1 - 2 / (1 + e^2u)
-            x[q] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + exp2_fast(x[q] * fac_s[qb][c0 + q] * (2.0f * kLog2e))));
+          for (int q = 0; q < C; ++q) x.v[q] *= fac_s[qb][c0 + q];
+          x = capped(x, cap, cap_inv);
         }
         if (masked) {
 #pragma unroll
           for (int q = 0; q < C; ++q)
-            if (!there || key > last_s[qb][c0 + q] || key < first_s[qb][c0 + q]) x[q] = -INFINITY;
-            else if (boxes >> 8 >> grp & 1u) x[q] = NAN;  // a scale of V that is no number: so is the query's output
+            if (!there || key > last_s[qb][c0 + q] || key < first_s[qb][c0 + q]) x.v[q] = -INFINITY;
+            else if (boxes >> 8 >> grp & 1u) x.v[q] = NAN;  // a scale of V that is no number: so is the query's output
         }
         // the turn's largest score of each query, still without its (positive) factor: warp, then the four warps
         float mx = -INFINITY, my = -INFINITY;
         if constexpr (kHalves) {
 #pragma unroll
           for (int q = 0; q < C; ++q) {
-            const float m0 = warp_top(lane < 16 ? x[q] : -INFINITY), m1 = warp_top(lane < 16 ? -INFINITY : x[q]);
+            const float m0 = warp_top(lane < 16 ? x.v[q] : -INFINITY), m1 = warp_top(lane < 16 ? -INFINITY : x.v[q]);
             if (lane == q) {
               mx = m0;
               my = m1;
@@ -830,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         } else {
 #pragma unroll
           for (int q = 0; q < C; ++q) {
-            const float m = warp_top(x[q]);
+            const float m = warp_top(x.v[q]);
             if (lane == q) mx = m;
           }
         }
@@ -883,7 +917,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         }
 #pragma unroll
         for (int q = 0; q < C; ++q) {
-          const float e = exp2_fast(fmaf(x[q], own_fac[q], -own_top[q]));
+          const float e = exp2_fast(fmaf(x.v[q], own_fac[q], -own_top[q]));
           l[q] = fmaf(e, own_beta[q], l[q]);
           // v = rint(e * sv * c) by a sum with 1.5 * 2^23.  With 128 added to each of the two lower
           // digits' places, the bytes of v are its signed digits, the lower two with the sign bit turned over.
@@ -1113,10 +1147,10 @@ __global__ void __launch_bounds__(512) combine_kernel(const AttendArgs a) {
 // and the threads' work are not spent on padding; at most what two score warpgroups' turns hold.
 int rows_of(int max_new, int group) { return static_cast<long long>(max_new) * group <= 8 ? 8 : 16; }
 
-template <typename T, int D, int R, bool kHalves>
+template <typename T, int D, int R, bool kHalves, bool kCapped>
 cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
   using S = Shape<D, R>;
-  const auto kernel = attend_kernel<T, D, R, kHalves>;
+  const auto kernel = attend_kernel<T, D, R, kHalves, kCapped>;
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), S::kSmem);
   if (e != cudaSuccess) return e;
@@ -1124,6 +1158,11 @@ cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensor
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_kernel(true, combine_kernel<T, D, R>, dim3(kSms, R), dim3(512), 0, s, a);
+}
+template <typename T, int D, int R, bool kHalves>
+cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
+  if (a.softcap > 0.0f) return launch<T, D, R, kHalves, true>(a, k_map, v_map, s);
+  return launch<T, D, R, kHalves, false>(a, k_map, v_map, s);
 }
 template <typename T, int D, int R>
 cudaError_t launch(const AttendArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t s) {
@@ -1163,7 +1202,7 @@ extern "C" int lb_op_kv8_attention(const void* q, int64_t q_token_stride, int64_
   using namespace lb;
   if (!q || !k_codes || !v_codes || !k_scale || !v_scale || !row_tables || !kv_len || !cu_tokens || !out ||
       !workspace || n_tokens < 1 || n_rows < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || n_pages < 1 ||
-      max_pages < 1 || max_new < 1 || window < 0 || !(softcap >= 0.0f))
+      max_pages < 1 || max_new < 1 || window < 0 || !(softcap >= 0.0f && softcap < INFINITY))
     return LB_ERR_INVALID_ARGUMENT;
   if ((q_dtype != LB_BF16 && q_dtype != LB_F16) || bad_dim(dim) || page_tokens < 16 || page_tokens > 256 ||
       page_tokens % 16 != 0 || static_cast<long long>(max_pages) * page_tokens > 0x7fffffffll - 2 * kTile)

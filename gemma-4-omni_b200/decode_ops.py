@@ -248,8 +248,8 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, row_tables: torch.Tensor, kv
     _need(row_tables, "row_tables", torch.int32, (n, max_pages), dev)
     _need(kv_len, "kv_len", torch.int32, (n,), dev)
     _need(cu_tokens, "cu_tokens", torch.int32, (n + 1,), dev)
-    if window < 0 or softcap < 0.0 or max_new < 1:
-        raise ValueError("window and softcap must not be negative, max_new must be positive")
+    if window < 0 or not 0.0 <= softcap < float("inf") or max_new < 1:
+        raise ValueError("window and softcap must not be negative, softcap finite, max_new positive")
     if out is None:
         out = q.new_empty(q.shape)
     else:

@@ -470,7 +470,7 @@ int lb_op_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_strid
  * token i is at position kv_len - new + i and sees the keys j <= position, with
  * window > 0 only those with j > position - window.  q [n_tokens][heads][dim]
  * (LB_BF16 or LB_F16, strides in elements), heads a multiple of kv_heads; scores
- * are scale * q.k, with softcap > 0 softcap * tanh(score / softcap).  out
+ * are scale * q.k, with softcap > 0 (finite) softcap * tanh(score / softcap).  out
  * [n_tokens][heads][dim] of q's type, contiguous; lse f32 [n_tokens][heads] (natural
  * log-sum-exp) or NULL.  A token that sees no key, and one in no row, has out 0 and
  * lse -inf.  dim 64, 128 or 256; page_tokens a multiple of 16, at most 256.  A page id

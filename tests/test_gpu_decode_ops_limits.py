@@ -6,6 +6,7 @@ Attention's bound, from what the kernel holds (all relative to one query):
   + 2^-21 (1 + |score|) (the exponential's argument and its approximation);
 - p * sv is rounded to a step of 1 / (63 * 2^16) of the largest p * sv among the tile's keys that the query
   sees: half a step times sum |code| of the tile's keys;
+- a capped score is off by 2^-19 of itself beside that;
 - factors, the sum of p and the division: 2^-20 of sum p|v|;
 - the output's half ulp (and its smallest step).
 """
@@ -90,7 +91,7 @@ def check(ops, cache, tables, q, lens, cu, *, max_new, scale=None, window=0, sof
                 abs(scale) * torch.einsum("hgd,hkd->hgk", qi.abs(), k.abs()) + 1)
             if softcap:
                 x = softcap * torch.tanh(x / softcap)
-            dx = (dx + 2.0 ** -21 * x.abs()).amax(2)
+            dx = (dx + (2.0 ** -19 + 2.0 ** -21 if softcap else 2.0 ** -21) * x.abs()).amax(2)
             want = torch.logsumexp(x, 2)
             p = torch.exp(x - want[..., None])
             ref = torch.einsum("hgk,hkd->hgd", p, v)
@@ -181,3 +182,22 @@ def test_zero_scales_among_others(ops):
     cache.v_scale.zero_()
     out, _ = check(ops, cache, tables, q, [256], [0, 1], max_new=1)
     assert not out.any()
+
+
+# ------------------------------------------------------------------ attention: soft caps of any size
+@pytest.mark.parametrize("softcap", [1e-3, 0.5, 7.0, 1e3, 1e4, 1e6, 1e9, 1e20, 3e38])
+@pytest.mark.parametrize("dim,heads,page", [(64, 4, 32), (256, 16, 16)])
+def test_softcap_of_any_size(ops, softcap, dim, heads, page):
+    g = gen(9)
+    cache, tables = make_cache(ops, g, [300], page, 1, dim)
+    q = torch.randn(1, heads, dim, generator=g, device="cuda").to(F16)
+    q *= torch.logspace(-3, 1, heads, device="cuda").to(F16)[:, None]  # scores small and large beside the smaller caps
+    check(ops, cache, tables, q, [300], [0, 1], max_new=1, softcap=softcap)
+
+
+def test_softcaps_that_are_no_cap_are_refused(ops):
+    cache, tables = make_cache(ops, gen(1), [16], 16, 1, 64)
+    q = torch.zeros(1, 1, 64, device="cuda").to(BF16)
+    for softcap in (-1.0, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            ops.kv8_attention(q, cache, tables, ints([16]), ints([0, 1]), max_new=1, softcap=softcap)
