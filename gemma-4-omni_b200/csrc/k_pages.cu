@@ -198,6 +198,32 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
   }
 }
 
+// Does the plan still fit the directory?  One warp a row, before anything is written: the session must hold the tokens
+// and pages that it held when the plan was made, and the pages it would get must still be free.  (Another launch
+// than the commit's, so that no row is installed unless all fit.)
+__global__ void check_kernel(int n, const int* sessions, int n_sessions, int max_pages, int n_pages, int P,
+                             const int* row_tables, const int* kv_len, const int* cu_tokens, const int* tables,
+                             const int* lengths, const unsigned* used, int* status) {
+  const int r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (r >= n) return;
+  const int s = sessions[r];
+  bool stale = s < 0 || s >= n_sessions;
+  if (!stale) {
+    const long long held = lengths[s], now = kv_len[r], room = static_cast<long long>(max_pages) * P;
+    stale = held < 0 || now < held || now > room || (cu_tokens && now - held != static_cast<long long>(cu_tokens[r + 1]) - cu_tokens[r]);
+    if (!stale) {
+      const int p0 = static_cast<int>((held + P - 1) / P), p1 = static_cast<int>((now + P - 1) / P);
+      for (int c = lane; c < p1; c += 32) {
+        const int page = row_tables[static_cast<long long>(r) * max_pages + c];
+        stale = stale || (c < p0 ? page != tables[static_cast<long long>(s) * max_pages + c]
+                                 : page < 0 || page >= n_pages || (used[page >> 5] >> (page & 31) & 1u));
+      }
+    }
+  }
+  // (a refused plan has its reason there already, and is all the same not installed)
+  if (__any_sync(0xffffffffu, stale) && lane == 0 && *static_cast<volatile int*>(status) == 0) atomicOr(status, LB_DEV_STALE_COMMIT);
+}
+
 // One warp a row: the pages past the held ones become the session's.
 __global__ void commit_kernel(int n, const int* sessions, int n_sessions, int max_pages, int n_pages, int P,
                               const int* row_tables, const int* kv_len, const int* status, int* tables,
@@ -274,17 +300,27 @@ int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int
   return cudaGetLastError() == cudaSuccess ? LB_OK : LB_ERR_CUDA;
 }
 
-int lb_commit_pages(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,
-                    const int32_t* row_tables, const int32_t* kv_len, const int32_t* status, int32_t* tables,
-                    int32_t* lengths, int32_t* used, void* stream) {
+int lb_commit_step(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,
+                   const int32_t* row_tables, const int32_t* kv_len, const int32_t* cu_tokens, int32_t* status,
+                   int32_t* tables, int32_t* lengths, int32_t* used, void* stream) {
   using namespace lb;
   if (bad_shape(n, n_sessions, max_pages, n_pages, page_tokens) || !sessions || !row_tables || !kv_len || !status ||
       !tables || !lengths || !used)
     return LB_ERR_INVALID_ARGUMENT;
+  unsigned* bits = reinterpret_cast<unsigned*>(used);
+  check_kernel<<<(n + 7) / 8, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      n, sessions, n_sessions, max_pages, n_pages, page_tokens, row_tables, kv_len, cu_tokens, tables, lengths, bits, status);
+  if (cudaGetLastError() != cudaSuccess) return LB_ERR_CUDA;
   commit_kernel<<<(n + 7) / 8, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      n, sessions, n_sessions, max_pages, n_pages, page_tokens, row_tables, kv_len, status, tables, lengths,
-      reinterpret_cast<unsigned*>(used));
+      n, sessions, n_sessions, max_pages, n_pages, page_tokens, row_tables, kv_len, status, tables, lengths, bits);
   return cudaGetLastError() == cudaSuccess ? LB_OK : LB_ERR_CUDA;
+}
+
+int lb_commit_pages(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,
+                    const int32_t* row_tables, const int32_t* kv_len, int32_t* status, int32_t* tables,
+                    int32_t* lengths, int32_t* used, void* stream) {
+  return lb_commit_step(n, sessions, n_sessions, max_pages, n_pages, page_tokens, row_tables, kv_len, nullptr, status,
+                        tables, lengths, used, stream);
 }
 
 int lb_release_pages(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,

@@ -76,7 +76,7 @@ class PagePlan:
     status_word: torch.Tensor  # int32 [1]
 
     def status(self) -> int:
-        """LB_DEV_* bits of a refused plan, 0 of a good one (synchronises)."""
+        """LB_DEV_* bits of a refused plan or of a commit that came too late, 0 of a good one (synchronises)."""
         return int(self.status_word.item())
 
 
@@ -141,12 +141,14 @@ class PageDirectory:
         return PagePlan(sessions, tables.view(n, mp), kv_len, cu, slots.view(torch.int64), positions, rows, status)
 
     def commit(self, plan: PagePlan) -> None:
-        """Installs a plan made from the directory as it is now (a refused plan changes nothing)."""
+        """Installs a plan.  One that was refused, or that no longer fits the directory (another plan
+        was committed or a session released since), changes nothing; the latter gets
+        LB_DEV_STALE_COMMIT in its ``status``."""
         n = plan.sessions.numel()
         _need(plan.row_tables, "row_tables", torch.int32, (n, self.max_pages), self.device)
-        _call(self.device, "lb_commit_pages", n, plan.sessions.data_ptr(), self.sessions, self.max_pages, self.pages,
-              self.page_tokens, plan.row_tables.data_ptr(), plan.kv_len.data_ptr(), plan.status_word.data_ptr(),
-              self.tables.data_ptr(), self.lengths.data_ptr(), self.used.data_ptr())
+        _call(self.device, "lb_commit_step", n, plan.sessions.data_ptr(), self.sessions, self.max_pages, self.pages,
+              self.page_tokens, plan.row_tables.data_ptr(), plan.kv_len.data_ptr(), plan.cu_tokens.data_ptr(),
+              plan.status_word.data_ptr(), self.tables.data_ptr(), self.lengths.data_ptr(), self.used.data_ptr())
 
     def release(self, sessions: torch.Tensor) -> None:
         """Gives the pages of these distinct sessions back."""

@@ -439,9 +439,17 @@ int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int
                   const int32_t* used, int max_tokens, int32_t* row_tables, int32_t* kv_len,
                   int32_t* cu_tokens, int64_t* slots, int32_t* positions, int32_t* token_rows,
                   int32_t* status, void* stream);
-/* Installs a plan whose *status is 0: the rows' new pages, lengths and used bits. */
+/* Installs a plan whose *status is 0: the rows' new pages, lengths and used bits.  A
+ * plan that no longer fits the directory is not installed and gets LB_DEV_STALE_COMMIT
+ * in *status: a session's tokens or pages are not those that it had when the plan was
+ * made, or a page that it would get is taken. */
+int lb_commit_step(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,
+                   const int32_t* row_tables, const int32_t* kv_len, const int32_t* cu_tokens, int32_t* status,
+                   int32_t* tables, int32_t* lengths, int32_t* used, void* stream);
+/* The same without cu_tokens: a session that gained tokens within a page since the plan was
+ * made is then not noticed. */
 int lb_commit_pages(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,
-                    const int32_t* row_tables, const int32_t* kv_len, const int32_t* status, int32_t* tables,
+                    const int32_t* row_tables, const int32_t* kv_len, int32_t* status, int32_t* tables,
                     int32_t* lengths, int32_t* used, void* stream);
 /* Gives the pages of n distinct sessions back; a session out of range sets
  * LB_DEV_BAD_HANDLE in *status and is skipped. */

@@ -201,3 +201,67 @@ def test_softcaps_that_are_no_cap_are_refused(ops):
     for softcap in (-1.0, math.inf, math.nan):
         with pytest.raises(ValueError):
             ops.kv8_attention(q, cache, tables, ints([16]), ints([0, 1]), max_new=1, softcap=softcap)
+
+
+# ------------------------------------------------------------------ plans that no longer fit
+def state(d):
+    return [t.tolist() for t in (d.tables, d.lengths, d.used)]
+
+
+def test_a_plan_that_no_longer_fits_is_not_committed(ops, pkg):
+    from gemma4_omni_b200 import _lib
+    stale = _lib.DEV_STALE_COMMIT
+
+    def directory():
+        d = ops.PageDirectory.create(sessions=4, max_pages=3, pages=8, page_tokens=16)
+        d.commit(d.plan(ints([0, 1]), ints([5, 20]), max_tokens=25))
+        assert d.lengths.tolist() == [5, 20, 0, 0]
+        return d
+
+    def late(d, plan):
+        """The plan is refused and changes nothing."""
+        before = state(d)
+        d.commit(plan)
+        assert plan.status() == stale and state(d) == before
+        d.commit(plan)
+        assert plan.status() == stale and state(d) == before
+
+    d = directory()  # two plans give the same free pages to different sessions
+    a, b = (d.plan(ints([s, 3 - s]), ints([17, 0]), max_tokens=17) for s in (2, 3))
+    d.commit(a)
+    assert a.status() == 0 and d.lengths.tolist() == [5, 20, 17, 0]
+    late(d, b)
+    d = directory()  # two plans for the same tokens of a session, inside a page
+    a, b = (d.plan(ints([0]), ints([1]), max_tokens=1) for _ in range(2))
+    d.commit(a)
+    late(d, b)
+    late(d, a)  # and one that was committed before
+    d = directory()  # a release in between
+    a = d.plan(ints([1]), ints([2]), max_tokens=2)
+    d.release(ints([1]))
+    late(d, a)
+    d = directory()  # a release, and the same number of tokens in other pages
+    a = d.plan(ints([1]), ints([2]), max_tokens=2)
+    d.release(ints([0, 1]))
+    d.commit(d.plan(ints([1]), ints([20]), max_tokens=20))
+    late(d, a)
+    d = directory()  # one row of many
+    a = d.plan(ints([2, 0, 3]), ints([40, 3, 1]), max_tokens=44)
+    d.commit(d.plan(ints([0]), ints([1]), max_tokens=1))
+    late(d, a)
+    d = directory()  # other sessions' tokens within their pages do not matter, nor do rows without tokens
+    a = d.plan(ints([2, 1]), ints([3, 0]), max_tokens=3)
+    d.commit(d.plan(ints([0]), ints([1]), max_tokens=1))
+    d.commit(a)
+    assert a.status() == 0 and d.lengths.tolist() == [6, 20, 3, 0]
+
+
+def test_a_late_commit_through_the_entry_without_token_counts(ops, pkg):
+    from gemma4_omni_b200 import _lib
+    d = ops.PageDirectory.create(sessions=2, max_pages=3, pages=8, page_tokens=16)
+    a, b = (d.plan(ints([s]), ints([17]), max_tokens=17) for s in (0, 1))
+    for plan, want, lengths in ((a, 0, [17, 0]), (b, _lib.DEV_STALE_COMMIT, [17, 0])):
+        _lib.check("lb_commit_pages", _lib.load().lb_commit_pages(
+            1, plan.sessions.data_ptr(), 2, 3, 8, 16, plan.row_tables.data_ptr(), plan.kv_len.data_ptr(), plan.status_word.data_ptr(),
+            d.tables.data_ptr(), d.lengths.data_ptr(), d.used.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        assert plan.status() == want and d.lengths.tolist() == lengths
