@@ -122,6 +122,7 @@ SIGNATURES: dict[str, tuple] = {
     "lb_snapshot_ready_rows": (I, [I, P, P, P, P, P, P, P, I64, P, P, P, P, P]),
     "lb_order_ready_heads": (I, [I, P, P, P, I64, I64, I, P, P, P, P]),
     "lb_plan_pages": (I, [I, P, P, I, I, I, I, P, P, P, I, P, P, P, P, P, P, P, P]),
+    "lb_plan_step": (I, [I, P, P, I, I, I, I, P, P, P, I, P, P, P, P, P, P, P, P, P]),
     "lb_commit_step": (I, [I, P, I, I, I, I, P, P, P, P, P, P, P, P]),
     "lb_commit_pages": (I, [I, P, I, I, I, I, P, P, P, P, P, P, P]),
     "lb_release_pages": (I, [I, P, I, I, I, I, P, P, P, P, P]),

@@ -58,6 +58,7 @@ struct PlanArgs {
   const unsigned* used;
   int *row_tables, *kv_len, *cu_tokens, *positions, *token_rows, *status;
   long long* slots;
+  int* planned;  // a copy of the sessions, or null
 };
 
 __device__ __forceinline__ unsigned free_bits(const PlanArgs& a, int word) {
@@ -164,7 +165,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
   const long long first = static_cast<long long>(blockIdx.x) * kPlanThreads + tid;
   for (long long i = first; i <= a.n; i += stride) {
     a.cu_tokens[i] = status ? 0 : cu[i];
-    if (i < a.n) a.kv_len[i] = status ? 0 : before[i] + (cu[i + 1] - cu[i]);
+    if (i < a.n) {
+      a.kv_len[i] = status ? 0 : before[i] + (cu[i + 1] - cu[i]);
+      if (a.planned) a.planned[i] = a.sessions[i];
+    }
   }
   for (long long i = first; i < static_cast<long long>(a.n) * a.max_pages; i += stride) {
     const int r = static_cast<int>(i / a.max_pages), c = static_cast<int>(i - static_cast<long long>(r) * a.max_pages);
@@ -273,11 +277,11 @@ bool bad_shape(int n, int n_sessions, int max_pages, int n_pages, int page_token
 
 extern "C" {
 
-int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int n_sessions, int max_pages,
-                  int n_pages, int page_tokens, const int32_t* tables, const int32_t* lengths,
-                  const int32_t* used, int max_tokens, int32_t* row_tables, int32_t* kv_len,
-                  int32_t* cu_tokens, int64_t* slots, int32_t* positions, int32_t* token_rows,
-                  int32_t* status, void* stream) {
+int lb_plan_step(int n, const int32_t* sessions, const int32_t* new_tokens, int n_sessions, int max_pages,
+                 int n_pages, int page_tokens, const int32_t* tables, const int32_t* lengths,
+                 const int32_t* used, int max_tokens, int32_t* row_tables, int32_t* kv_len,
+                 int32_t* cu_tokens, int64_t* slots, int32_t* positions, int32_t* token_rows,
+                 int32_t* planned_sessions, int32_t* status, void* stream) {
   using namespace lb;
   if (bad_shape(n, n_sessions, max_pages, n_pages, page_tokens) || n > kMaxPlanRows || max_tokens < 1 || max_tokens > kMaxPlanTokens)
     return LB_ERR_INVALID_ARGUMENT;
@@ -286,7 +290,7 @@ int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int
     return LB_ERR_INVALID_ARGUMENT;
   PlanArgs a{n, n_sessions, max_pages, n_pages, page_tokens, max_tokens, sessions, new_tokens, tables, lengths,
              reinterpret_cast<const unsigned*>(used), row_tables, kv_len, cu_tokens, positions, token_rows, status,
-             reinterpret_cast<long long*>(slots)};
+             reinterpret_cast<long long*>(slots), planned_sessions};
   const size_t smem = sizeof(int) * (3 * static_cast<size_t>(n) + 1 + kPlanThreads + (n_sessions + 31) / 32);
   constexpr size_t kMost = sizeof(int) * (3 * kMaxPlanRows + 1 + kPlanThreads + kMaxPlanSessions / 32);
   static std::atomic<unsigned long long> done{0};
@@ -298,6 +302,15 @@ int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int
   const int grid = static_cast<int>(values / 4096 < 1 ? 1 : values / 4096 > 148 ? 148 : values / 4096);
   plan_kernel<<<grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
   return cudaGetLastError() == cudaSuccess ? LB_OK : LB_ERR_CUDA;
+}
+
+int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int n_sessions, int max_pages,
+                  int n_pages, int page_tokens, const int32_t* tables, const int32_t* lengths,
+                  const int32_t* used, int max_tokens, int32_t* row_tables, int32_t* kv_len,
+                  int32_t* cu_tokens, int64_t* slots, int32_t* positions, int32_t* token_rows,
+                  int32_t* status, void* stream) {
+  return lb_plan_step(n, sessions, new_tokens, n_sessions, max_pages, n_pages, page_tokens, tables, lengths, used,
+                      max_tokens, row_tables, kv_len, cu_tokens, slots, positions, token_rows, nullptr, status, stream);
 }
 
 int lb_commit_step(int n, const int32_t* sessions, int n_sessions, int max_pages, int n_pages, int page_tokens,

@@ -66,7 +66,7 @@ def _cuda(device: torch.device, what: str) -> torch.device:
 @dataclass
 class PagePlan:
     """One step's pages: what ``Kv8Cache.append`` and ``kv8_attention`` read."""
-    sessions: torch.Tensor    # int32 [n]
+    sessions: torch.Tensor    # int32 [n], the plan's own copy
     row_tables: torch.Tensor  # int32 [n, max_pages], -1 past a row's last page
     kv_len: torch.Tensor      # int32 [n], tokens of the session after the step
     cu_tokens: torch.Tensor   # int32 [n + 1]
@@ -126,19 +126,20 @@ class PageDirectory:
         _need(new_tokens, "new_tokens", torch.int32, (n,), dev)
         # one allocation: the 64-bit slots, then the 32-bit arrays
         mp = self.max_pages
-        words = 2 * max_tokens, n * mp, max_tokens, max_tokens, n, n + 1, 1
+        words = 2 * max_tokens, n * mp, max_tokens, max_tokens, n, n + 1, n, 1
         buf = self.lengths.new_empty(sum(words))
-        slots, tables, positions, rows, kv_len, cu, status = buf.split(words)
+        slots, tables, positions, rows, kv_len, cu, planned, status = buf.split(words)
         p_slots = buf.data_ptr()
         p_tables = p_slots + 8 * max_tokens
         p_pos = p_tables + 4 * n * mp
         p_rows = p_pos + 4 * max_tokens
         p_len = p_rows + 4 * max_tokens
         p_cu = p_len + 4 * n
-        _call(dev, "lb_plan_pages", n, sessions.data_ptr(), new_tokens.data_ptr(), self.sessions, mp, self.pages,
+        p_planned = p_cu + 4 * n + 4
+        _call(dev, "lb_plan_step", n, sessions.data_ptr(), new_tokens.data_ptr(), self.sessions, mp, self.pages,
               self.page_tokens, self.tables.data_ptr(), self.lengths.data_ptr(), self.used.data_ptr(), max_tokens,
-              p_tables, p_len, p_cu, p_slots, p_pos, p_rows, p_cu + 4 * n + 4)
-        return PagePlan(sessions, tables.view(n, mp), kv_len, cu, slots.view(torch.int64), positions, rows, status)
+              p_tables, p_len, p_cu, p_slots, p_pos, p_rows, p_planned, p_planned + 4 * n)
+        return PagePlan(planned, tables.view(n, mp), kv_len, cu, slots.view(torch.int64), positions, rows, status)
 
     def commit(self, plan: PagePlan) -> None:
         """Installs a plan.  One that was refused, or that no longer fits the directory (another plan

@@ -439,6 +439,13 @@ int lb_plan_pages(int n, const int32_t* sessions, const int32_t* new_tokens, int
                   const int32_t* used, int max_tokens, int32_t* row_tables, int32_t* kv_len,
                   int32_t* cu_tokens, int64_t* slots, int32_t* positions, int32_t* token_rows,
                   int32_t* status, void* stream);
+/* The same, and planned_sessions int32 [n] (may be NULL) gets a copy of sessions, for a
+ * commit that comes after the caller has filled its buffer anew. */
+int lb_plan_step(int n, const int32_t* sessions, const int32_t* new_tokens, int n_sessions, int max_pages,
+                 int n_pages, int page_tokens, const int32_t* tables, const int32_t* lengths,
+                 const int32_t* used, int max_tokens, int32_t* row_tables, int32_t* kv_len,
+                 int32_t* cu_tokens, int64_t* slots, int32_t* positions, int32_t* token_rows,
+                 int32_t* planned_sessions, int32_t* status, void* stream);
 /* Installs a plan whose *status is 0: the rows' new pages, lengths and used bits.  A
  * plan that no longer fits the directory is not installed and gets LB_DEV_STALE_COMMIT
  * in *status: a session's tokens or pages are not those that it had when the plan was

@@ -265,3 +265,14 @@ def test_a_late_commit_through_the_entry_without_token_counts(ops, pkg):
             1, plan.sessions.data_ptr(), 2, 3, 8, 16, plan.row_tables.data_ptr(), plan.kv_len.data_ptr(), plan.status_word.data_ptr(),
             d.tables.data_ptr(), d.lengths.data_ptr(), d.used.data_ptr(), torch.cuda.current_stream().cuda_stream))
         assert plan.status() == want and d.lengths.tolist() == lengths
+
+
+def test_a_plan_keeps_its_sessions_when_the_callers_buffer_is_filled_anew(ops):
+    d = ops.PageDirectory.create(sessions=4, max_pages=3, pages=8, page_tokens=16)
+    ids = ints([2, 0])
+    plan = d.plan(ids, ints([5, 17]), max_tokens=22)
+    ids.copy_(ints([1, 3]))
+    assert plan.sessions.tolist() == [2, 0]
+    d.commit(plan)
+    assert plan.status() == 0 and d.lengths.tolist() == [17, 0, 5, 0]
+    assert d.tables.tolist() == [[1, 2, -1], [-1] * 3, [0, -1, -1], [-1] * 3]
