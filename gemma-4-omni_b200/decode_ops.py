@@ -52,9 +52,26 @@ def _call(device: torch.device, name: str, *args) -> None:
 
 
 def _need(t: torch.Tensor, name: str, dtype, shape: tuple, device: torch.device) -> None:
-    """Refuses a tensor that is not contiguous, of this type and shape, on this device."""
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+    """Refuses what is not a contiguous tensor of this type and shape on this device."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}")
+
+
+def _exchangeable(name: str, dtype: torch.dtype, shape, align: int = 1) -> property:
+    """An attribute that holds a tensor.  It may be exchanged for another one of the same type, ``shape(owner)``
+    and device, whose address the next call takes; anything else is refused when it is set."""
+    slot = "_t_" + name
+
+    def get(self) -> torch.Tensor:
+        return getattr(self, slot)
+
+    def put(self, t: torch.Tensor) -> None:
+        _need(t, name, dtype, shape(self), self.device)
+        if t.data_ptr() % align:
+            raise ValueError(f"{name} must be {align}-byte aligned")
+        setattr(self, slot, t)
+
+    return property(get, put)
 
 
 def _cuda(device: torch.device, what: str) -> torch.device:
@@ -84,6 +101,10 @@ class PageDirectory:
     """The pages of every session: ``tables`` int32 [sessions, max_pages], ``lengths``
     int32 [sessions], ``used`` int32 words with one bit per page."""
 
+    tables = _exchangeable("tables", torch.int32, lambda d: (d.sessions, d.max_pages))
+    lengths = _exchangeable("lengths", torch.int32, lambda d: (d.sessions,))
+    used = _exchangeable("used", torch.int32, lambda d: (-(-d.pages // 32),))
+
     def __init__(self, tables: torch.Tensor, lengths: torch.Tensor, used: torch.Tensor, *, pages: int,
                  page_tokens: int):
         self.device = _cuda(tables.device, "PageDirectory")
@@ -96,11 +117,8 @@ class PageDirectory:
         self.sessions, self.max_pages = (int(v) for v in tables.shape)
         if self.max_pages * page_tokens >= 2 ** 31:
             raise ValueError("a session holds fewer than 2^31 tokens")
-        _need(tables, "tables", torch.int32, (self.sessions, self.max_pages), self.device)
-        _need(lengths, "lengths", torch.int32, (self.sessions,), self.device)
-        _need(used, "used", torch.int32, (-(-pages // 32),), self.device)
-        self.tables, self.lengths, self.used = tables, lengths, used
         self.pages, self.page_tokens = int(pages), int(page_tokens)
+        self.tables, self.lengths, self.used = tables, lengths, used
         self._released = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     @classmethod
@@ -127,7 +145,7 @@ class PageDirectory:
         # one allocation: the 64-bit slots, then the 32-bit arrays
         mp = self.max_pages
         words = 2 * max_tokens, n * mp, max_tokens, max_tokens, n, n + 1, n, 1
-        buf = self.lengths.new_empty(sum(words))
+        buf = self._t_lengths.new_empty(sum(words))
         slots, tables, positions, rows, kv_len, cu, planned, status = buf.split(words)
         p_slots = buf.data_ptr()
         p_tables = p_slots + 8 * max_tokens
@@ -137,7 +155,7 @@ class PageDirectory:
         p_cu = p_len + 4 * n
         p_planned = p_cu + 4 * n + 4
         _call(dev, "lb_plan_step", n, sessions.data_ptr(), new_tokens.data_ptr(), self.sessions, mp, self.pages,
-              self.page_tokens, self.tables.data_ptr(), self.lengths.data_ptr(), self.used.data_ptr(), max_tokens,
+              self.page_tokens, self._t_tables.data_ptr(), self._t_lengths.data_ptr(), self._t_used.data_ptr(), max_tokens,
               p_tables, p_len, p_cu, p_slots, p_pos, p_rows, p_planned, p_planned + 4 * n)
         return PagePlan(planned, tables.view(n, mp), kv_len, cu, slots.view(torch.int64), positions, rows, status)
 
@@ -146,10 +164,12 @@ class PageDirectory:
         was committed or a session released since), changes nothing; the latter gets
         LB_DEV_STALE_COMMIT in its ``status``."""
         n = plan.sessions.numel()
-        _need(plan.row_tables, "row_tables", torch.int32, (n, self.max_pages), self.device)
+        for name, shape in (("sessions", (n,)), ("row_tables", (n, self.max_pages)), ("kv_len", (n,)), ("cu_tokens", (n + 1,)),
+                            ("status_word", (1,))):
+            _need(getattr(plan, name), name, torch.int32, shape, self.device)
         _call(self.device, "lb_commit_step", n, plan.sessions.data_ptr(), self.sessions, self.max_pages, self.pages,
               self.page_tokens, plan.row_tables.data_ptr(), plan.kv_len.data_ptr(), plan.cu_tokens.data_ptr(),
-              plan.status_word.data_ptr(), self.tables.data_ptr(), self.lengths.data_ptr(), self.used.data_ptr())
+              plan.status_word.data_ptr(), self._t_tables.data_ptr(), self._t_lengths.data_ptr(), self._t_used.data_ptr())
 
     def release(self, sessions: torch.Tensor) -> None:
         """Gives the pages of these distinct sessions back."""
@@ -157,7 +177,7 @@ class PageDirectory:
         _need(sessions, "sessions", torch.int32, (n,), self.device)
         if n:
             _call(self.device, "lb_release_pages", n, sessions.data_ptr(), self.sessions, self.max_pages, self.pages,
-                  self.page_tokens, self.tables.data_ptr(), self.lengths.data_ptr(), self.used.data_ptr(),
+                  self.page_tokens, self._t_tables.data_ptr(), self._t_lengths.data_ptr(), self._t_used.data_ptr(),
                   self._released.data_ptr())
 
     def status(self) -> int:
@@ -169,6 +189,12 @@ class Kv8Cache:
     """Keys and values as int8 codes [pages, kv_heads, page_tokens, dim] with one f32
     scale per page and head [pages, kv_heads]: value = code * scale."""
 
+    k_codes = _exchangeable("k_codes", torch.int8, lambda c: (c.pages, c.kv_heads, c.page_tokens, c.dim), 16)
+    v_codes = _exchangeable("v_codes", torch.int8, lambda c: (c.pages, c.kv_heads, c.page_tokens, c.dim), 16)
+    k_scale = _exchangeable("k_scale", torch.float32, lambda c: (c.pages, c.kv_heads))
+    v_scale = _exchangeable("v_scale", torch.float32, lambda c: (c.pages, c.kv_heads))
+    status_word = _exchangeable("status_word", torch.int32, lambda c: (1,))
+
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         self.device = _cuda(k_codes.device, "Kv8Cache")
         if k_codes.dim() != 4 or 0 in k_codes.shape:
@@ -178,12 +204,6 @@ class Kv8Cache:
             raise ValueError(f"page_tokens must be a multiple of 16, at most {PAGE_TOKENS_MAX}")
         if self.dim not in HEAD_DIMS:
             raise ValueError(f"dim must be one of {HEAD_DIMS}")
-        for name, t in (("k_codes", k_codes), ("v_codes", v_codes)):
-            _need(t, name, torch.int8, (self.pages, self.kv_heads, self.page_tokens, self.dim), self.device)
-            if t.data_ptr() % 16:
-                raise ValueError(f"{name} must be 16-byte aligned")
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need(t, name, torch.float32, (self.pages, self.kv_heads), self.device)
         self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
         self.status_word = torch.zeros(1, dtype=torch.int32, device=self.device)
 
@@ -195,7 +215,9 @@ class Kv8Cache:
                    torch.zeros(shape[:2], device=device), torch.zeros(shape[:2], device=device))
 
     def _pointers(self) -> tuple[int, int, int, int]:
-        return self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
+        # (past the properties, which cost as much as the addresses)
+        return (self._t_k_codes.data_ptr(), self._t_v_codes.data_ptr(), self._t_k_scale.data_ptr(),
+                self._t_v_scale.data_ptr())
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Writes k, v [tokens, kv_heads, dim] to ``slots`` int64 [tokens] (negative: skipped).
@@ -214,7 +236,7 @@ class Kv8Cache:
         kc, vc, ks, vs = self._pointers()
         _call(self.device, "lb_op_kv8_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
               v.stride(1), DTYPE_CODES[k.dtype], n, self.kv_heads, self.dim, slots.data_ptr(), kc, vc, ks, vs,
-              self.pages, self.page_tokens, self.status_word.data_ptr())
+              self.pages, self.page_tokens, self._t_status_word.data_ptr())
 
     def status(self) -> int:
         """LB_DEV_* bits seen by appends and attention so far (synchronises)."""
@@ -257,14 +279,14 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, row_tables: torch.Tensor, kv
         out = q.new_empty(q.shape)
     else:
         _need(out, "out", q.dtype, (t, heads, dim), dev)
-    lse = cache.k_scale.new_empty((t, heads)) if return_lse else None
+    lse = cache._t_k_scale.new_empty((t, heads)) if return_lse else None
     if t:
         kc, vc, ks, vs = cache._pointers()
-        space = cache.k_codes.new_empty(_workspace(dim, heads, cache.kv_heads, max_new))
+        space = cache._t_k_codes.new_empty(_workspace(dim, heads, cache.kv_heads, max_new))
         _call(dev, "lb_op_kv8_attention", q.data_ptr(), q.stride(0), q.stride(1), DTYPE_CODES[q.dtype], t, n, heads,
               cache.kv_heads, dim, kc, vc, ks, vs, cache.pages, cache.page_tokens, row_tables.data_ptr(), max_pages,
               kv_len.data_ptr(), cu_tokens.data_ptr(), max_new, dim ** -0.5 if scale is None else scale, window, softcap,
-              out.data_ptr(), lse.data_ptr() if return_lse else None, cache.status_word.data_ptr(),
+              out.data_ptr(), lse.data_ptr() if return_lse else None, cache._t_status_word.data_ptr(),
               space.data_ptr())
     return (out, lse) if return_lse else out
 
@@ -307,6 +329,9 @@ class Int4Weight:
     """A [out, k] matrix of 4-bit codes: uint8 [out, k / 2] (low four bits: even k),
     f16 scales [out, k / group]; weight = (code - 8) * scale."""
 
+    codes = _exchangeable("codes", torch.uint8, lambda w: (w.out_features, w.k // 2), 16)
+    scales = _exchangeable("scales", torch.float16, lambda w: (w.out_features, w.k // w.group))
+
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         self.device = _cuda(codes.device, "Int4Weight")
         if codes.dim() != 2 or scales.dim() != 2 or 0 in codes.shape or 0 in scales.shape:
@@ -315,10 +340,6 @@ class Int4Weight:
         self.group = self.k // int(scales.shape[1])
         if self.group not in (32, 64, 128) or self.group * int(scales.shape[1]) != self.k:
             raise ValueError("groups must have 32, 64 or 128 columns")
-        _need(codes, "codes", torch.uint8, (self.out_features, self.k // 2), self.device)
-        _need(scales, "scales", torch.float16, (self.out_features, self.k // self.group), self.device)
-        if codes.data_ptr() % 16:
-            raise ValueError("codes must be 16-byte aligned")
         self.codes, self.scales = codes, scales
 
     @classmethod
@@ -371,7 +392,7 @@ def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | No
         raise ValueError(f"out must be [{rows}, {weight.out_features}] on {dev}, its rows contiguous")
     if rows:
         _call(dev, "lb_op_w4_matvec", x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype],
-              None if x_scale is None else x_scale.data_ptr(), group, rows, weight.codes.data_ptr(),
-              weight.scales.data_ptr(), weight.group, weight.out_features, weight.k, out.data_ptr(), out.stride(0),
+              None if x_scale is None else x_scale.data_ptr(), group, rows, weight._t_codes.data_ptr(),
+              weight._t_scales.data_ptr(), weight.group, weight.out_features, weight.k, out.data_ptr(), out.stride(0),
               DTYPE_CODES[out.dtype])
     return out

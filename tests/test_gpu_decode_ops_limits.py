@@ -276,3 +276,36 @@ def test_a_plan_keeps_its_sessions_when_the_callers_buffer_is_filled_anew(ops):
     d.commit(plan)
     assert plan.status() == 0 and d.lengths.tolist() == [17, 0, 5, 0]
     assert d.tables.tolist() == [[1, 2, -1], [-1] * 3, [0, -1, -1], [-1] * 3]
+
+
+# ------------------------------------------------------------------ tensors that are exchanged
+def test_tensors_that_do_not_fit_are_refused_when_they_are_set(ops):
+    d = ops.PageDirectory.create(sessions=4, max_pages=3, pages=40, page_tokens=16)
+    cache = ops.Kv8Cache.create(pages=4, kv_heads=2, page_tokens=16, dim=64)
+    weight = ops.Int4Weight.quantize(torch.randn(8, 256, generator=gen(1), device="cuda"))
+    for owner, names in ((d, ("tables", "lengths", "used")), (weight, ("codes", "scales")),
+                         (cache, ("k_codes", "v_codes", "k_scale", "v_scale", "status_word"))):
+        for name in names:
+            held = getattr(owner, name)
+            twice = torch.cat([held, held], -1)
+            # (a single element has no stride)
+            for bad in (held[:-1].clone(), twice[..., ::2] if held.numel() > 1 else twice, held.to(torch.int64), held.cpu(), twice, None,
+                        torch.zeros(held.numel() + 1, dtype=held.dtype, device="cuda")[1:].view(held.shape) if name.endswith("codes") else held[:0]):
+                with pytest.raises(ValueError):
+                    setattr(owner, name, bad)
+                assert getattr(owner, name) is held
+            other = held.clone()
+            setattr(owner, name, other)
+            assert getattr(owner, name) is other
+
+
+def test_commit_refuses_plans_whose_tensors_do_not_fit(ops):
+    d = ops.PageDirectory.create(sessions=4, max_pages=3, pages=8, page_tokens=16)
+    for name in ("sessions", "row_tables", "kv_len", "cu_tokens", "status_word"):
+        plan = d.plan(ints([0, 1]), ints([5, 20]), max_tokens=25)
+        held = getattr(plan, name)
+        for bad in (held[:-1].clone(), held.long(), held.cpu()):
+            setattr(plan, name, bad)
+            with pytest.raises(ValueError):
+                d.commit(plan)
+    assert d.lengths.tolist() == [0] * 4
