@@ -34,6 +34,7 @@ DEV_INGRESS_OVERFLOW = 1 << 6
 DEV_PAGES_EXHAUSTED = 1 << 7
 DEV_BAD_PAGE = 1 << 8
 DEV_NONFINITE = 1 << 9
+DEV_SPLIT_PAGE = 1 << 10
 INGRESS_JOIN, INGRESS_LEAVE, INGRESS_PAUSE, INGRESS_RESUME = 0, 1, 2, 3
 
 

@@ -14,7 +14,8 @@
 // side): with a warp a group the prompt took 69 us, its values filling the registers of 16 warps an SM.  The
 // CTAs look for the first tokens of groups in windows of the batch, so nothing
 // but the slots has to be known: a token begins a group unless the token before
-// it in the batch has the slot before it in the same page.  A group of up to 512 pieces of 8
+// it in the batch has the slot before it in the same page.  Where the last token before it that is not skipped is of
+// the same page all the same, two groups would read and write that page at once: the later one is refused.  A group of up to 512 pieces of 8
 // values stays in registers between its maximum and its codes; larger ones are read again.
 #include <cstring>
 
@@ -125,6 +126,8 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const AppendArgs a)
   const unsigned on1 = __ballot_sync(0xffffffffu, slot1 > 0 && slot1 == prev1 + 1 && page_of(slot1, P) * P != slot1);
   const unsigned long long follows = on0 | static_cast<unsigned long long>(on1) << 32;
   const bool first = lane < a.window && slot0 >= 0 && !(on0 >> lane & 1u);
+  // first tokens after one that is skipped or of the same page
+  const unsigned look = __ballot_sync(0xffffffffu, first && t0 + lane > 0 && (prev0 < 0 || (prev0 >= page0 * P && prev0 - page0 * P < P)));
   const T* src = static_cast<const T*>(side ? a.src[1] : a.src[0]) + head * (side ? a.head_stride[1] : a.head_stride[0]);
   const long long ts = side ? a.token_stride[1] : a.token_stride[0];
   // every warp finds the same groups
@@ -136,6 +139,23 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const AppendArgs a)
     if (page >= a.n_pages) {
       if (tid == 0 && a.status) atomicOr(a.status, static_cast<int>(LB_DEV_BAD_PAGE));
       continue;
+    }
+    if (look >> at & 1u) {  // the last token before it that is not skipped
+      bool split = false;
+#pragma unroll 1
+      for (long long j = t - 1; j >= 0; j -= 32) {
+        const long long s = slot_at(j - lane);
+        const unsigned there = __ballot_sync(0xffffffffu, s >= 0);
+        if (there) {
+          const long long last = __shfl_sync(0xffffffffu, s, __ffs(there) - 1);
+          split = last >= page * P && last - page * P < P;
+          break;
+        }
+      }
+      if (split) {
+        if (tid == 0 && a.status) atomicOr(a.status, static_cast<int>(LB_DEV_SPLIT_PAGE));
+        continue;
+      }
     }
     int run = __ffsll(static_cast<long long>(~(follows >> at >> 1)));  // the token and those that follow
     while (at + run >= 64 && off + run < P) {  // past the 64 tokens (pages of more than 32)

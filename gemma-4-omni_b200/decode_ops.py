@@ -223,7 +223,8 @@ class Kv8Cache:
         """Writes k, v [tokens, kv_heads, dim] to ``slots`` int64 [tokens] (negative: skipped).
 
         The tokens of one page follow one another in order, as a ``PagePlan`` has
-        them.  A page's scale only grows; the codes it held are rounded to the new scale."""
+        them, with no skipped one between: those after a gap are not written and set
+        LB_DEV_SPLIT_PAGE in ``status``.  A page's scale only grows; the codes it held are rounded to the new scale."""
         n = slots.numel()
         if k.dtype not in FLOAT_INPUTS or v.dtype != k.dtype:
             raise ValueError("k and v must both be float32, bfloat16 or float16")

@@ -51,7 +51,8 @@ enum lb_device_status_bits {
   LB_DEV_INGRESS_OVERFLOW = 1 << 6, /* a frame found its session's ingress ring full (refused) */
   LB_DEV_PAGES_EXHAUSTED = 1 << 7,  /* a page plan asks for more pages than are free, or a row for more than its table holds */
   LB_DEV_BAD_PAGE = 1 << 8,         /* a page or slot outside the cache (skipped) */
-  LB_DEV_NONFINITE = 1 << 9         /* a key or value that was written is infinite or NaN */
+  LB_DEV_NONFINITE = 1 << 9,        /* a key or value that was written is infinite or NaN */
+  LB_DEV_SPLIT_PAGE = 1 << 10       /* tokens of one page with a gap, a skipped token or a step back between them (the later ones are skipped) */
 };
 
 /* Session events of the GPU ingress (lb_ingress_events_async). */
@@ -466,7 +467,9 @@ int lb_release_pages(int n, const int32_t* sessions, int n_sessions, int max_pag
 /* Writes n_tokens keys and values into the 8-bit cache: k_codes / v_codes int8
  * [n_pages][kv_heads][page_tokens][dim], k_scale / v_scale f32 [n_pages][kv_heads]
  * (value = code * scale).  slots int64 [n_tokens] as lb_plan_pages writes them
- * (negative: skipped); the tokens of one page follow one another, in order.  A
+ * (negative: skipped); the tokens of one page follow one another, in order and without
+ * a skipped one between them: the ones after a gap are not written and set LB_DEV_SPLIT_PAGE.
+ * (Tokens of one page with another page's between them: the page's contents are of no account.)  A
  * page's scale is the running max |x| / 127 over its tokens: where new tokens
  * raise it, the codes before them are rounded again to the new scale; a token at
  * offset 0 begins the page afresh.  k, v: [n_tokens][kv_heads][dim] of dtype (LB_F32,

@@ -309,3 +309,35 @@ def test_commit_refuses_plans_whose_tensors_do_not_fit(ops):
             with pytest.raises(ValueError):
                 d.commit(plan)
     assert d.lengths.tolist() == [0] * 4
+
+
+# ------------------------------------------------------------------ append: a page met twice
+@pytest.mark.parametrize("heads,pad", [(1, 0), (8, 300), (1, 4000)])
+@pytest.mark.parametrize("slots,good", [
+    ([16, -1, 17, 32, 33], [0, 3, 4]),              # a skipped token inside a page
+    ([16, 17, 19, 20, 5], [0, 1, 4]),               # a gap
+    ([18, 17, 33, 34], [0, 2, 3]),                  # a step back
+    ([20, 20, 40], [0, 2]),                         # a slot twice
+    ([15, 16, 17, -7, 31, -1, -2, 32], [0, 1, 2, 7]),  # pages that end and begin beside them
+    ([-1] * 70 + [16] + [-1] * 70 + [17, 48], [70, 142]),  # skipped tokens past the window that a CTA looks at
+])
+def test_the_tokens_of_a_page_after_a_gap_are_refused(ops, pkg, slots, good, heads, pad):
+    from gemma4_omni_b200 import _lib
+    slots = [-1] * pad + slots
+    good = [pad + i for i in good]
+    cache = ops.Kv8Cache.create(pages=4, kv_heads=heads, page_tokens=16, dim=64)
+    want = ops.Kv8Cache.create(pages=4, kv_heads=heads, page_tokens=16, dim=64)
+    for c in (cache, want):  # what the pages held
+        for t in (c.k_codes, c.v_codes):
+            t.copy_(torch.randint(-127, 128, t.shape, generator=gen(2), device="cuda"))
+        c.k_scale.fill_(0.001)
+        c.v_scale.fill_(0.01)
+    x = torch.randn(len(slots), heads, 64, generator=gen(1), device="cuda")
+    cache.append(x, -x, torch.tensor(slots, device="cuda"))
+    kept = torch.full((len(slots),), -1, device="cuda")
+    kept[good] = torch.tensor(slots, device="cuda")[good]
+    want.append(x, -x, kept)
+    assert cache.status() == (_lib.DEV_SPLIT_PAGE if len(good) < sum(s >= 0 for s in slots) else 0)
+    if want.status() == 0:
+        for name in ("k_codes", "v_codes", "k_scale", "v_scale"):
+            assert torch.equal(getattr(cache, name), getattr(want, name)), name
