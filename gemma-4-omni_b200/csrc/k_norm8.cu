@@ -87,20 +87,31 @@ __device__ __forceinline__ uint8_t code_of(float q, bool e4m3) {
   return static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(fminf(fmaxf(q, -127.0f), 127.0f))));
 }
 
-// The codes of 8 columns whose group's largest value is m, by one multiplication with top / m (its
-// rounding moves a code only where y / s is within 2^-21 of halfway).  Far from 1 both take a power of two
-// first, so that the quotient stays inside the range of the fast division.
-__device__ __forceinline__ uint2 codes_of(float (&y)[8], float m, bool e4m3) {
-  if (!(m > 0.0f)) return make_uint2(0, 0);  // all zero, or a NaN: the scale says so
-  if (m < 0x1p-90f || m > 0x1p90f) {
-    const float k = m < 1.0f ? 0x1p80f : 0x1p-80f;
-    m *= k;
+// y / s with inv close to 1 / s: the product, then what it leaves of y (one fused multiply-add, exact) divided
+// the same way (Markstein's correction of a quotient, 1990).  Ties of the codes are those of the quotient.
+__device__ __forceinline__ float quotient(float y, float s, float inv) {
+  const float q = y * inv;
+  return fmaf(fmaf(-q, s, y), inv, q);
+}
+__device__ __forceinline__ float near_inverse(float s) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s));
+  return y;
+}
+
+// The codes of 8 columns whose group's scale is s: round(y / s).  Far from 1 both take a power of two
+// first, so that nothing leaves the range of normal numbers.
+__device__ __forceinline__ uint2 codes_of(float (&y)[8], float s, bool e4m3) {
+  if (!(s > 0.0f)) return make_uint2(0, 0);  // all zero, or a NaN: the scale says so
+  if (s < 0x1p-90f || s > 0x1p90f) {
+    const float k = s < 1.0f ? 0x1p80f : 0x1p-80f;
+    s *= k;
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] *= k;
   }
-  const float inv = __fdividef(e4m3 ? 448.0f : 127.0f, m);
+  const float inv = near_inverse(s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] *= inv;
+  for (int i = 0; i < 8; ++i) y[i] = quotient(y[i], s, inv);
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -190,9 +201,9 @@ __global__ void __launch_bounds__(kT < 256 ? 256 : kT) norm_rows_kernel(const No
     for (int c = 0; c < C; ++c) {
       const int i = in_row + c * kT;
       if (live && i < pieces) {
-        const float most = __uint_as_float(m[c]);
-        if ((i & (width - 1)) == 0) a.scales[row * (pieces >> width_log) + (i >> width_log)] = most * a.inv_top;
-        *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], most, a.e4m3);
+        const float s = __uint_as_float(m[c]) * a.inv_top;
+        if ((i & (width - 1)) == 0) a.scales[row * (pieces >> width_log) + (i >> width_log)] = s;
+        *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], s, a.e4m3);
       }
     }
     return;
@@ -208,11 +219,12 @@ __global__ void __launch_bounds__(kT < 256 ? 256 : kT) norm_rows_kernel(const No
 #pragma unroll
     for (int k = 0; k < kWarpsRow; ++k) most = max(most, __float_as_uint(part[warp / kWarpsRow * kWarpsRow + k]));
   }
-  if (live && in_row == 0) a.scales[row] = __uint_as_float(most) * a.inv_top;
+  const float s = __uint_as_float(most) * a.inv_top;
+  if (live && in_row == 0) a.scales[row] = s;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = in_row + c * kT;
-    if (live && i < pieces) *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], __uint_as_float(most), a.e4m3);
+    if (live && i < pieces) *reinterpret_cast<uint2*>(a.codes + row * a.dim + i * 8) = codes_of(h[c], s, a.e4m3);
   }
 }
 
@@ -257,13 +269,13 @@ __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs a) {
     most = max(most, size_of(y));
   }
   const auto write = [&](int from, int width, uint32_t m, int first, int step) {
-    const float top = __uint_as_float(m);
-    const bool plain = top > 0x1p-90f && top < 0x1p90f;
-    const float s = top * a.inv_top, inv = plain ? __fdividef(a.e4m3 ? 448.0f : 127.0f, top) : 0.0f;
+    const float s = __uint_as_float(m) * a.inv_top;
+    const bool plain = s > 0x1p-90f && s < 0x1p90f;
+    const float inv = plain ? near_inverse(s) : 0.0f;
 #pragma unroll 4
     for (int i = first; i < width; i += step) {
       const float y = held[from + i];
-      a.codes[row * dim + from + i] = plain ? code_of(y * inv, a.e4m3) : s > 0.0f ? code_of(y / s, a.e4m3) : uint8_t(0);
+      a.codes[row * dim + from + i] = plain ? code_of(quotient(y, s, inv), a.e4m3) : s > 0.0f ? code_of(y / s, a.e4m3) : uint8_t(0);
     }
     return s;
   };

@@ -341,3 +341,31 @@ def test_the_tokens_of_a_page_after_a_gap_are_refused(ops, pkg, slots, good, hea
     if want.status() == 0:
         for name in ("k_codes", "v_codes", "k_scale", "v_scale"):
             assert torch.equal(getattr(cache, name), getattr(want, name)), name
+
+
+# ------------------------------------------------------------------ norm: codes are those of the quotient
+def quotient_codes(w, scale, out):
+    """round(w / scale) by IEEE division in 32 bits, to nearest even."""
+    q = torch.div(w, scale.expand_as(w))
+    return q.round().clamp(-127, 127).to(I8) if out is I8 else q.clamp(-448, 448).to(E4M3)
+
+
+@pytest.mark.parametrize("out", [E4M3, I8])
+@pytest.mark.parametrize("dim,group,offset", [(4096, 0, 0), (2048, 128, 0), (256, 8, 0), (1024, 0, 1), (2048, 64, 3)])
+@pytest.mark.parametrize("rows", [1, 1200])
+def test_codes_are_the_rounded_quotient(ops, out, dim, group, offset, rows):
+    """Rows of ones have the norm 1, so that y is the weight itself, exactly; many quotients lie halfway."""
+    g = gen(dim + group)
+    top = 448 if out is E4M3 else 127
+    x = torch.ones(rows, dim + offset, device="cuda")[:, offset:]
+    whole = torch.randint(-top, top + 1, (dim,), generator=g, device="cuda").float()
+    for k, w in enumerate((whole + 0.5 * torch.randint(0, 2, (dim,), generator=g, device="cuda"), whole * 3.0, whole * 2.0 ** -100,
+                           torch.randn(dim, generator=g, device="cuda").to(BF16).float(), torch.randn(dim, generator=g, device="cuda") * 1e3,
+                           torch.randn(dim, generator=g, device="cuda") * 1e30)):
+        if k in (0, 1, 2):
+            w[::max(8, group or dim)] = top * (1.0, 6.0, 2.0 ** -100)[k]  # the scale is 1, 6 or 2^-100 in every group
+        codes, scales, _ = ops.rms_norm8(x, w, eps=0.0, group=group, dtype=out)
+        s = scales.repeat_interleave(group or dim, 1)
+        want = quotient_codes(w.expand(rows, dim), s, out)
+        assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)), k
+        torch.testing.assert_close(scales[0].double(), w.double().abs().view(-1, group or dim).amax(1) / top, rtol=2.0 ** -22, atol=0)
