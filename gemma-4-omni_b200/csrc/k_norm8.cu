@@ -102,7 +102,7 @@ __device__ __forceinline__ float near_inverse(float s) {
 // The codes of 8 columns whose group's scale is s: round(y / s).  Far from 1 both take a power of two
 // first, so that nothing leaves the range of normal numbers.
 __device__ __forceinline__ uint2 codes_of(float (&y)[8], float s, bool e4m3) {
-  if (!(s > 0.0f)) return make_uint2(0, 0);  // all zero, or a NaN: the scale says so
+  if (!(s > 0.0f && s < INFINITY)) return make_uint2(0, 0);  // all zero, or a value that is not finite: the scale says so
   if (s < 0x1p-90f || s > 0x1p90f) {
     const float k = s < 1.0f ? 0x1p80f : 0x1p-80f;
     s *= k;
@@ -270,12 +270,12 @@ __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs a) {
   }
   const auto write = [&](int from, int width, uint32_t m, int first, int step) {
     const float s = __uint_as_float(m) * a.inv_top;
-    const bool plain = s > 0x1p-90f && s < 0x1p90f;
+    const bool plain = s > 0x1p-90f && s < 0x1p90f, some = s > 0.0f && s < INFINITY;
     const float inv = plain ? near_inverse(s) : 0.0f;
 #pragma unroll 4
     for (int i = first; i < width; i += step) {
       const float y = held[from + i];
-      a.codes[row * dim + from + i] = plain ? code_of(quotient(y, s, inv), a.e4m3) : s > 0.0f ? code_of(y / s, a.e4m3) : uint8_t(0);
+      a.codes[row * dim + from + i] = plain ? code_of(quotient(y, s, inv), a.e4m3) : some ? code_of(y / s, a.e4m3) : uint8_t(0);
     }
     return s;
   };

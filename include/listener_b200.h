@@ -512,7 +512,7 @@ int64_t lb_kv8_attention_workspace(int dim, int heads, int kv_heads, int max_new
  * dtype; residual may be NULL (h = x), hidden may be NULL (h is not stored), else
  * [rows][dim].  codes [rows][dim], the quotient y / scale rounded to nearest even; scales f32
  * [rows][dim / group].  A group whose y is all zero has scale 0 and codes 0; one that holds a NaN
- * has scale NaN and codes 0.
+ * or an infinite value has that as its scale, and codes 0.
  * dim <= 16384. */
 int lb_op_rms_norm8(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int dtype,
                     const void* weight, int weight_dtype, int rows, int dim, float eps, int group, int out_dtype,

@@ -369,3 +369,14 @@ def test_codes_are_the_rounded_quotient(ops, out, dim, group, offset, rows):
         want = quotient_codes(w.expand(rows, dim), s, out)
         assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)), k
         torch.testing.assert_close(scales[0].double(), w.double().abs().view(-1, group or dim).amax(1) / top, rtol=2.0 ** -22, atol=0)
+
+
+@pytest.mark.parametrize("out", [E4M3, I8])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_a_group_with_an_infinite_value_has_codes_of_zero(ops, out, offset):
+    x = torch.ones(2, 256 + offset, device="cuda")[:, offset:]
+    w = torch.ones(256, device="cuda")
+    w[3], w[200] = math.inf, -2.0
+    codes, scales, _ = ops.rms_norm8(x, w, eps=0.0, group=128, dtype=out)
+    assert torch.isinf(scales[:, 0]).all() and not codes[:, :128].view(torch.uint8).any()
+    assert torch.equal(codes[:, 128:].view(torch.uint8), quotient_codes(w[128:].expand(2, 128), scales[:, 1:].expand(2, 128), out).view(torch.uint8))
