@@ -6,7 +6,8 @@
 // Both products run on the tensor cores in whole numbers, on the codes as they lie in the
 // cache (tcgen05 kind::i8): no code is ever widened.  q and p are split into signed
 // 8-bit digits instead, which become neighbouring columns of one MMA:
-//   q * 2^e = 65536 q2 + 256 q1 + q0   (e brings the row's maximum to 2^21: 22 bits and a sign)
+//   q * 2^e = 2^24 q3 + 65536 q2 + 256 q1 + q0   (e brings the row's maximum to 2^29: 30 bits and a sign, so that
+//                  16-bit values keep all their bits down to 2^-19 (fp16) or 2^-22 (bf16) of the largest)
 //   p * sv * c = 65536 p2 + 256 p1 + p0   (c, of each tile and query, brings the largest p * sv among the
 //                  keys that the query sees to 63 * 2^16: an error of 2^-23 of that largest p * sv a key)
 //   S^T[key, (digit, query)] = K . Q^T,   O^T[column, (digit, query)] = V^T . P^T
@@ -91,8 +92,8 @@ struct Shape {
   static constexpr int kRow = D < 128 ? D : 128;            // bytes of a shared-memory row: the swizzle's span
   static constexpr int kHalfBytes = kTile * kRow;
   static constexpr int kSide = kTile * D;                   // K (or V) of a tile
-  static constexpr int kN1 = R == 8 ? 32 : 3 * R;           // score columns: three digits (8 rows: and 8 of padding)
-  static constexpr int kN2 = kN1;                           // output columns: three digits
+  static constexpr int kN1 = 4 * R;                         // score columns: four digits
+  static constexpr int kN2 = R == 8 ? 32 : 3 * R;           // output columns: three digits (8 rows: and 8 that nobody reads)
   static constexpr int kS = (kN1 + 31) / 32 * 32;           // tensor-memory columns of a score buffer
   static constexpr int kBuffers = 4 * kS + 2 * kHalves * kN2 <= 512 ? 4 : 2;  // of scores and of digits of p
   static constexpr int kColumns = kBuffers * kS + 2 * kHalves * kN2;
@@ -101,7 +102,7 @@ struct Shape {
   static constexpr int kQBytes = (kHalves * kN1 * kRow + 1023) / 1024 * 1024;
   static constexpr int kPBytes = kN2 * kTile;
   static constexpr int kFixedBytes = 2 * kQBytes + kBuffers * kPBytes + 1024;
-  static constexpr int kRoom = (213 * 1024 - kFixedBytes) / kSide;  // (up to 14 KB are declared beside it)
+  static constexpr int kRoom = (219 * 1024 - kFixedBytes) / kSide;  // (up to 8 KB are declared beside it)
   static constexpr int kUnits = kRoom < kInfo ? kRoom : kInfo;  // (a tile's scales outlive its units)
   static constexpr int kSmem = kFixedBytes + kUnits * kSide;
   static constexpr int kTurns = R / kQueries;             // of the score warpgroups, a tile
@@ -138,7 +139,7 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t off) {
   return off ^ (((off >> 7) & (kRow == 128 ? 7u : 3u)) << 4);
 }
 
-// three loads of C columns each and their wait in one statement: the
+// three (or four) loads of C columns each and their wait in one statement: the
 // registers are not valid, and must not be touched, before the wait
 template <int C>
 __device__ __forceinline__ void tmem_ld3(uint32_t a0, uint32_t a1, uint32_t a2, int (&x)[C], int (&y)[C], int (&z)[C]);
@@ -152,6 +153,18 @@ __device__ __forceinline__ void tmem_ld3<8>(uint32_t a0, uint32_t a1, uint32_t a
       "tcgen05.wait::ld.sync.aligned;"
       : LB_R8(x), LB_R8(y), LB_R8(z)
       : "r"(a0), "r"(a1), "r"(a2)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, int (&x)[8], int (&y)[8],
+                                         int (&z)[8], int (&w)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%33];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16,%17,%18,%19,%20,%21,%22,%23}, [%34];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24,%25,%26,%27,%28,%29,%30,%31}, [%35];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : LB_R8(x), LB_R8(y), LB_R8(z), LB_R8(w)
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3)
       : "memory");
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -379,8 +392,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   __shared__ uint64_t task_full[kTasks], task_empty[kTasks];
   __shared__ Task tasks[kTasks];
   __shared__ uint32_t tmem_slot;
-  __shared__ long long pre[kThreads + 1];
-  __shared__ long long warp_total[kThreads / 32];
+  __shared__ long long warp_total[kThreads / 32], line_length;
+  // the prefix sums, which only the loading warp reads, and before it announces a task: p comes after that
+  static_assert((kThreads + 1) * sizeof(long long) <= S::kBuffers * S::kPBytes, "room");
+  long long* pre = reinterpret_cast<long long*>(p_digits);
   // by box: the scales of K, those of V over the tile's unit (a power of two; kept over kFixed); bits of the boxes
   // that are there, and from bit 8 on of those whose scale of V is not finite
   __shared__ float g_ks[kInfo][kBoxes], g_vs[kInfo][kBoxes], g_unit[kInfo];
@@ -438,14 +453,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   for (int r = tid * each; r < min(a.n_rows, (tid + 1) * each); ++r) mine += row_work(a, row_of<R>(a, r));
   long long sum = warp_prefix(mine);
   if (lane == 31) warp_total[warp] = sum;
-  if constexpr (R == 8) {  // rows of padding: zero once
-    for (int i = tid; i < 2 * S::kHalves * 8 * S::kRow / 4; i += kThreads) {
-      const int buf = i / (S::kHalves * 8 * S::kRow / 4), j = i - buf * (S::kHalves * 8 * S::kRow / 4);
-      const int h = j / (8 * S::kRow / 4), o = j - h * (8 * S::kRow / 4);
-      reinterpret_cast<uint32_t*>(q_digits + buf * S::kQBytes + h * S::kN1 * S::kRow + 24 * S::kRow)[o] = 0u;
-    }
-    fence_proxy_async_smem();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -453,6 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   for (int w = 0; w < warp; ++w) sum += warp_total[w];
   pre[tid + 1] = sum;
   if (tid == 0) pre[0] = 0;
+  if (tid == kThreads - 1) line_length = sum;
   // tokens of no row
   if (first_token != 0 || last_token != a.n_tokens) {
     const long long pieces = static_cast<long long>(a.heads) * D / 8;
@@ -467,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   __syncthreads();
   const uint32_t tmem = tmem_slot;
   const uint32_t tmem_o = tmem + S::kBuffers * S::kS;
-  const long long W = pre[kThreads];
+  const long long W = line_length;
   const long long n_ctas = min(static_cast<long long>(gridDim.x), W);
   const long long b = blockIdx.x;
   bool ok = b < n_ctas;
@@ -745,8 +753,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         for (int e = 0; e < kE; ++e) size = max(size, __float_as_uint(to_f<T>(raw.v[e])) & 0x7fffffffu);
         const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, size));
         const bool fine = top < INFINITY;
-        // 2^ex brings the maximum to [2^21, 2^22); in two factors, each inside the floating range
-        const int ex = fine && top > 0.0f ? 21 + 127 - max(1, __float_as_int(top) >> 23) : 0;
+        // 2^ex brings the maximum to [2^29, 2^30); in two factors, each inside the floating range
+        const int ex = fine && top > 0.0f ? 29 + 127 - max(1, __float_as_int(top) >> 23) : 0;
         const int e1 = ex / 2, e2 = ex - e1;
         const float up1 = copysignf(__int_as_float((127 + e1) << 23), a.scale), up2 = __int_as_float((127 + e2) << 23);
         if (lane == 0) {
@@ -761,16 +769,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
           left = G;
           ++pos;
         }
-        uint32_t w[3][kE / 4 > 0 ? kE / 4 : 1] = {};
+        uint32_t w[4][kE / 4 > 0 ? kE / 4 : 1] = {};
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const int v = fine ? __float2int_rn(to_f<T>(raw.v[e]) * up1 * up2) : 0;
-          const uint32_t d = (v + 0x8080) ^ 0x8080;  // bytes 0, 1, 2 (see the digits of p below)
+          const uint32_t d = (v + 0x808080) ^ 0x808080;  // its bytes (see the digits of p below)
 #pragma unroll
-          for (int c = 0; c < 3; ++c) w[c][e / 4] |= ((d >> (16 - 8 * c)) & 0xffu) << (8 * (e & 3));
+          for (int c = 0; c < 4; ++c) w[c][e / 4] |= ((d >> (24 - 8 * c)) & 0xffu) << (8 * (e & 3));
         }
 #pragma unroll
-        for (int c = 0; c < 3; ++c) {
+        for (int c = 0; c < 4; ++c) {
           unsigned char* to = digits + swizzled<S::kRow>((c * R + qi) * S::kRow + col);
           if constexpr (kE == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[c][0], w[c][1]);
           else if constexpr (kE == 4) *reinterpret_cast<uint32_t*>(to) = w[c][0];
@@ -829,12 +837,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
         unsigned char* p = p_digits + buf * S::kPBytes;
         Scores x;
         {
-          int d2[C], d1[C], dd[C];
+          int d3[C], d2[C], d1[C], d0[C];
           const uint32_t at = tmem + buf * S::kS + lane_at + c0;
-          tmem_ld3<C>(at, at + R, at + 2 * R, d2, d1, dd);
+          tmem_ld4(at, at + R, at + 2 * R, at + 3 * R, d3, d2, d1, d0);
 #pragma unroll
-          for (int c = 0; c < C; ++c)
-            x.v[c] = fmaf(__int2float_rn(d2[c]), 65536.0f, __int2float_rn(d1[c] * 256 + dd[c])) * ks;
+          for (int c = 0; c < C; ++c)  // (a digit's sum is below 2^22)
+            x.v[c] = fmaf(__int2float_rn(d3[c] * 256 + d2[c]), 65536.0f, __int2float_rn(d1[c] * 256 + d0[c])) * ks;
         }
         tc_fence_before();
         __syncwarp();

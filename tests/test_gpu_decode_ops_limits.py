@@ -1,8 +1,8 @@
 """The text-decoder operators where their inputs' ranges and contracts end.
 
 Attention's bound, from what the kernel holds (all relative to one query):
-- q is rounded to 2^-22 of its row's largest value, the sums of products are joined in 32 bits:
-  a score is off by dx <= 2^-22 * scale * max|q| * sum |k| + 2^-21 * scale * sum |q||k|
+- q is rounded to 2^-30 of its row's largest value, the sums of products are joined in 32 bits:
+  a score is off by dx <= 2^-30 * scale * max|q| * sum |k| + 2^-21 * scale * sum |q||k|
   + 2^-21 (1 + |score|) (the exponential's argument and its approximation);
 - p * sv is rounded to a step of 1 / (63 * 2^16) of the largest p * sv among the tile's keys that the query
   sees: half a step times sum |code| of the tile's keys;
@@ -87,7 +87,7 @@ def check(ops, cache, tables, q, lens, cu, *, max_new, scale=None, window=0, sof
             k, v, c = kc[:, see] * ks[:, see, None], vc[:, see] * vs[:, see, None], vc[:, see].abs()
             qi = q[i].double().view(kvh, group, dim)
             x = scale * torch.einsum("hgd,hkd->hgk", qi, k)
-            dx = 2.0 ** -22 * abs(scale) * qi.abs().amax(2)[..., None] * k.abs().sum(2)[:, None] + 2.0 ** -21 * (
+            dx = 2.0 ** -30 * abs(scale) * qi.abs().amax(2)[..., None] * k.abs().sum(2)[:, None] + 2.0 ** -21 * (
                 abs(scale) * torch.einsum("hgd,hkd->hgk", qi.abs(), k.abs()) + 1)
             if softcap:
                 x = softcap * torch.tanh(x / softcap)
@@ -182,6 +182,23 @@ def test_zero_scales_among_others(ops):
     cache.v_scale.zero_()
     out, _ = check(ops, cache, tables, q, [256], [0, 1], max_new=1)
     assert not out.any()
+
+
+# ------------------------------------------------------------------ attention: q far apart in its row
+@pytest.mark.parametrize("ratio", [2.0 ** 10, 2.0 ** 14, 2.0 ** 18, 2.0 ** 21])
+@pytest.mark.parametrize("dim,heads,page", [(64, 8, 64), (128, 16, 32), (256, 16, 16)])
+def test_a_channel_that_is_large_in_q_and_zero_in_the_keys(ops, ratio, dim, heads, page):
+    g = gen(5)
+    cache, tables = make_cache(ops, g, [260], page, 1, dim)
+    cache.k_codes[..., 7] = 0
+    q = torch.randn(2, heads, dim, generator=g, device="cuda").clamp(-3, 3)
+    q[:, ::2, 7] = ratio
+    q[:, 1::2, 7] = -ratio
+    out, _ = check(ops, cache, tables, q.to(BF16), [260], [0, 2], max_new=2)
+    q[..., 7] = 0.0
+    plain, _ = check(ops, cache, tables, q.to(BF16), [260], [0, 2], max_new=2)
+    if ratio <= 2.0 ** 18:  # q's steps (ratio * 2^-29) are far below its elements' own: the same scores, but for single roundings
+        assert (out.double() - plain.double()).norm() <= 2.0 ** -9 * plain.double().norm()
 
 
 # ------------------------------------------------------------------ attention: soft caps of any size
