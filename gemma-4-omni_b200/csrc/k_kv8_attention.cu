@@ -877,11 +877,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
           }
         }
         if (lane < C) {
-          // rounded up, so that no exponential below passes 1 however large the scores are
-          mx = fmaxf(mx * fac_up, mx * fac_down);
+          // rounded up, so that no exponential below passes 1 however large the scores are (-inf, no key, also stays
+          // where the factor is NaN)
+          mx = mx == -INFINITY ? mx : fmaxf(mx * fac_up, mx * fac_down);
           float pv = v0;
           if constexpr (kHalves) {
-            my = fmaxf(my * fac_up, my * fac_down);
+            my = my == -INFINITY ? my : fmaxf(my * fac_up, my * fac_down);
             const float most = max_nan(mx, my);
             pv = fmaxf(exp2_fast(mx - most) * v0, exp2_fast(my - most) * v1);
             mx = most;
@@ -956,6 +957,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
       }
       float sum_q = l[0] + __shfl_xor_sync(0xffffffffu, l[0], 2);
       sum_q += __shfl_xor_sync(0xffffffffu, sum_q, 1);
+      // a query that saw no key has no sum, though its own values be NaN
+      if (__shfl_sync(0xffffffffu, ref, lane / 4) == -INFINITY) sum_q = 0.0f;
       if ((lane & 3) == 0) l_part[warp - kFirstScorer][lane / 4] = sum_q;
       if (wq == 0 && lane < C) m_ref[side][lane] = ref;
       __syncwarp();

@@ -397,3 +397,16 @@ def test_a_group_with_an_infinite_value_has_codes_of_zero(ops, out, offset):
     codes, scales, _ = ops.rms_norm8(x, w, eps=0.0, group=128, dtype=out)
     assert torch.isinf(scales[:, 0]).all() and not codes[:, :128].view(torch.uint8).any()
     assert torch.equal(codes[:, 128:].view(torch.uint8), quotient_codes(w[128:].expand(2, 128), scales[:, 1:].expand(2, 128), out).view(torch.uint8))
+
+
+# ------------------------------------------------------------------ attention: rows that see nothing, windows, tokens
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_a_token_that_sees_no_key_gets_zeros_whatever_its_query_holds(ops, page, softcap):
+    cache, tables = make_cache(ops, gen(1), [40, 1, 300], page, 1, 64)
+    q = torch.full((8, 4, 64), math.nan, device="cuda").to(BF16)
+    q[4], q[6] = 1.0, math.inf
+    # rows: one without keys, one with more tokens than keys, one whose last token is the only one with numbers
+    out, lse = ops.kv8_attention(q, cache, tables, ints([0, 2, 300]), ints([0, 1, 5, 8]), max_new=4, softcap=softcap, return_lse=True)
+    assert not out[:3].any() and (lse[:3] == -math.inf).all()
+    assert torch.isnan(out[3]).all() and torch.isfinite(out[4]).all() and torch.isnan(out[5:]).all()
