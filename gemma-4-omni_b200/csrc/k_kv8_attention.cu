@@ -270,7 +270,7 @@ __device__ __forceinline__ Row row_of(const AttendArgs& a, int r) {
   w.len = a.kv_len[r];
   if (w.count == 0) return w;
   const int stop = min(max(w.len, 0), a.max_pages * a.page_tokens);
-  if (a.window) w.low = max(0, min(w.len - w.count + 1 - a.window, stop)) & ~(a.box - 1);
+  if (a.window) w.low = static_cast<int>(max(0ll, min(static_cast<long long>(w.len) - w.count + 1 - a.window, static_cast<long long>(stop)))) & ~(a.box - 1);
   w.tiles = max(1, (stop - w.low + kTile - 1) / kTile);
   w.q_tiles = (w.count * (a.heads / a.kv_heads) + R - 1) / R;
   return w;
@@ -367,7 +367,7 @@ struct Walk {
     t.pos_low = w.len - w.count + t.qt * R / G;
     t.pos_high = w.len - w.count + (t.qt * R + t.rows - 1) / G;
     t.stop = min(min(max(w.len, 0), a.max_pages * a.page_tokens), t.pos_high + 1);
-    t.start = a.window ? max(w.low, t.pos_low + 1 - a.window) : 0;
+    t.start = a.window ? static_cast<int>(max(static_cast<long long>(w.low), static_cast<long long>(t.pos_low) + 1 - a.window)) : 0;
     return true;
   }
 };

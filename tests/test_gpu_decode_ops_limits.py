@@ -410,3 +410,24 @@ def test_a_token_that_sees_no_key_gets_zeros_whatever_its_query_holds(ops, page,
     out, lse = ops.kv8_attention(q, cache, tables, ints([0, 2, 300]), ints([0, 1, 5, 8]), max_new=4, softcap=softcap, return_lse=True)
     assert not out[:3].any() and (lse[:3] == -math.inf).all()
     assert torch.isnan(out[3]).all() and torch.isfinite(out[4]).all() and torch.isnan(out[5:]).all()
+
+
+@pytest.mark.parametrize("window", [300, 2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5])
+@pytest.mark.parametrize("lens,new", [([300, 20], [3, 1]), ([3, 5], [7, 130])])
+def test_windows_wider_than_all_keys_hide_none(ops, window, lens, new):
+    g = gen(4)
+    cache, tables = make_cache(ops, g, [max(n, m) for n, m in zip(lens, new)], 32, 1, 64)
+    q = torch.randn(sum(new), 2, 64, generator=g, device="cuda").to(F16)
+    kv_len, cu = ints(lens), ints([0, new[0], sum(new)])
+    want = ops.kv8_attention(q, cache, tables, kv_len, cu, max_new=max(new), return_lse=True)
+    got = ops.kv8_attention(q, cache, tables, kv_len, cu, max_new=max(new), window=window, return_lse=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_hint_past_32_bits(ops):
+    g = gen(4)
+    cache, tables = make_cache(ops, g, [50], 32, 1, 64)
+    q = torch.randn(20, 1, 64, generator=g, device="cuda").to(F16)
+    want = ops.kv8_attention(q, cache, tables, ints([50]), ints([0, 20]), max_new=20)
+    for hint in (2 ** 31, 2 ** 32, 2 ** 40):
+        assert torch.equal(ops.kv8_attention(q, cache, tables, ints([50]), ints([0, 20]), max_new=hint), want)
