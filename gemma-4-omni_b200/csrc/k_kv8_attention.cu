@@ -260,17 +260,19 @@ __device__ __forceinline__ uint16_t to_bits(float v) {
 // What a row of the batch asks for.
 struct Row {
   int begin, count, len, low, tiles, q_tiles;
+  int pos0;  // position of its first token
 };
 template <int R>
 __device__ __forceinline__ Row row_of(const AttendArgs& a, int r) {
-  Row w{0, 0, 0, 0, 0, 0};
+  Row w{0, 0, 0, 0, 0, 0, 0};
   if (r >= a.n_rows) return w;
   w.begin = min(max(a.cu_tokens[r], 0), a.n_tokens);
   w.count = min(max(a.cu_tokens[r + 1], w.begin), a.n_tokens) - w.begin;
   w.len = a.kv_len[r];
+  w.pos0 = w.len - (max(a.cu_tokens[r + 1], w.begin) - w.begin);  // (also where q ends before the row does)
   if (w.count == 0) return w;
   const int stop = min(max(w.len, 0), a.max_pages * a.page_tokens);
-  if (a.window) w.low = static_cast<int>(max(0ll, min(static_cast<long long>(w.len) - w.count + 1 - a.window, static_cast<long long>(stop)))) & ~(a.box - 1);
+  if (a.window) w.low = static_cast<int>(max(0ll, min(static_cast<long long>(w.pos0) + 1 - a.window, static_cast<long long>(stop)))) & ~(a.box - 1);
   w.tiles = max(1, (stop - w.low + kTile - 1) / kTile);
   w.q_tiles = (w.count * (a.heads / a.kv_heads) + R - 1) / R;
   return w;
@@ -344,6 +346,7 @@ struct Walk {
       w.low = __shfl_sync(0xffffffffu, held.low, at);
       w.tiles = __shfl_sync(0xffffffffu, held.tiles, at);
       w.q_tiles = __shfl_sync(0xffffffffu, held.q_tiles, at);
+      w.pos0 = __shfl_sync(0xffffffffu, held.pos0, at);
       const int length = w.tiles + kTaskCost;
       const long long y = x - (base + __shfl_sync(0xffffffffu, upto, at) - row_work(a, w));
       const int task = static_cast<int>(y / length);
@@ -364,8 +367,8 @@ struct Walk {
     t.begin = w.begin;
     t.q_tiles = w.q_tiles;
     t.rows = min(R, w.count * G - t.qt * R);
-    t.pos_low = w.len - w.count + t.qt * R / G;
-    t.pos_high = w.len - w.count + (t.qt * R + t.rows - 1) / G;
+    t.pos_low = w.pos0 + t.qt * R / G;
+    t.pos_high = w.pos0 + (t.qt * R + t.rows - 1) / G;
     t.stop = min(min(max(w.len, 0), a.max_pages * a.page_tokens), t.pos_high + 1);
     t.start = a.window ? static_cast<int>(max(static_cast<long long>(w.low), static_cast<long long>(t.pos_low) + 1 - a.window)) : 0;
     return true;

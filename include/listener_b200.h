@@ -485,7 +485,7 @@ int lb_op_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_strid
 
 /* Attention of the step's tokens over that cache.  Row r holds the tokens
  * [cu_tokens[r], cu_tokens[r+1]), the last of the kv_len[r] tokens of its session:
- * token i is at position kv_len - new + i and sees the keys j <= position, with
+ * token i is at position kv_len - new + i (also where q ends before the row's last token) and sees the keys j <= position, with
  * window > 0 only those with j > position - window.  q [n_tokens][heads][dim]
  * (LB_BF16 or LB_F16, strides in elements), heads a multiple of kv_heads; scores
  * are scale * q.k, with softcap > 0 (finite) softcap * tanh(score / softcap).  out

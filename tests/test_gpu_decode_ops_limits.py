@@ -431,3 +431,16 @@ def test_a_hint_past_32_bits(ops):
     want = ops.kv8_attention(q, cache, tables, ints([50]), ints([0, 20]), max_new=20)
     for hint in (2 ** 31, 2 ** 32, 2 ** 40):
         assert torch.equal(ops.kv8_attention(q, cache, tables, ints([50]), ints([0, 20]), max_new=hint), want)
+
+
+@pytest.mark.parametrize("window", [0, 20])
+def test_q_may_end_before_the_last_rows_tokens_do(ops, window):
+    """A step's first tokens alone: each stays at its own position."""
+    g = gen(6)
+    cache, tables = make_cache(ops, g, [90, 130], 32, 1, 64)
+    q = torch.randn(40, 4, 64, generator=g, device="cuda").to(F16)
+    lens, cu = [90, 130], [0, 10, 40]
+    whole, _ = check(ops, cache, tables, q, lens, cu, max_new=30, window=window)
+    for t in (1, 9, 10, 11, 39):
+        part = ops.kv8_attention(q[:t], cache, tables, ints(lens), ints(cu), max_new=30, window=window)
+        torch.testing.assert_close(part, whole[:t], rtol=2.0 ** -10, atol=1e-5)
