@@ -58,6 +58,16 @@ def _need(t: torch.Tensor, name: str, dtype, shape: tuple, device: torch.device)
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}")
 
 
+def _row_step(t: torch.Tensor) -> int:
+    """Elements between the rows of a 2-D tensor (of a single row: its width, whatever stride it has); 0 where
+    a row's elements are not neighbours or rows overlap."""
+    rows, cols = t.shape
+    if cols > 1 and rows and t.stride(1) != 1:
+        return 0
+    step = t.stride(0) if rows > 1 else cols
+    return step if step >= cols else 0
+
+
 def _exchangeable(name: str, dtype: torch.dtype, shape, align: int = 1) -> property:
     """An attribute that holds a tensor.  It may be exchanged for another one of the same type, ``shape(owner)``
     and device, whose address the next call takes; anything else is refused when it is set."""
@@ -300,8 +310,11 @@ def rms_norm8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor |
     hidden = x + residual in x's type (x itself without a residual); codes * scales =
     hidden / rms(hidden) * weight.  ``dtype``: float8_e4m3fn or int8; ``group``: columns
     that share a scale, 0 for one scale a row."""
-    if x.dim() != 2 or x.dtype not in FLOAT_INPUTS or (x.numel() and x.stride(1) != 1):
-        raise ValueError("x must be a float32, bfloat16 or float16 [rows, dim] tensor, its rows contiguous")
+    if x.dim() != 2 or x.dtype not in FLOAT_INPUTS:
+        raise ValueError("x must be a float32, bfloat16 or float16 [rows, dim] tensor")
+    x_step = _row_step(x)
+    if not x_step and x.numel():
+        raise ValueError("x's rows must be contiguous and apart")
     dev = _cuda(x.device, "rms_norm8")
     rows, dim = x.shape
     if not 0 < dim <= 16384 or group < 0 or (group and dim % group):
@@ -311,17 +324,21 @@ def rms_norm8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor |
     if weight.dtype not in (torch.float32, x.dtype):
         raise ValueError("weight must be float32 or of x's type")
     _need(weight, "weight", weight.dtype, (dim,), dev)
-    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape or residual.device != dev
-                                 or (x.numel() and residual.stride(1) != 1)):
-        raise ValueError("residual must be like x")
+    r_step = 0
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape or residual.device != dev:
+            raise ValueError("residual must be like x")
+        r_step = _row_step(residual)
+        if not r_step and rows:
+            raise ValueError("residual's rows must be contiguous and apart")
     codes = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
     n_groups = dim // group if group else 1
     scales = (weight.new_empty((rows, n_groups)) if weight.dtype == torch.float32
               else torch.empty((rows, n_groups), dtype=torch.float32, device=dev))
     hidden = x if residual is None else x.new_empty(x.shape)
     if rows:
-        _call(dev, "lb_op_rms_norm8", x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(),
-              0 if residual is None else residual.stride(0), DTYPE_CODES[x.dtype], weight.data_ptr(),
+        _call(dev, "lb_op_rms_norm8", x.data_ptr(), x_step, None if residual is None else residual.data_ptr(),
+              r_step, DTYPE_CODES[x.dtype], weight.data_ptr(),
               DTYPE_CODES[weight.dtype], rows, dim, eps, group, DTYPE_CODES[dtype], codes.data_ptr(), scales.data_ptr(),
               None if residual is None else hidden.data_ptr())
     return codes, scales, hidden
@@ -370,9 +387,11 @@ def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | No
     [rows, groups] as ``rms_norm8`` returns them (one group a row, or groups of a
     multiple of 128 columns).  ``out_dtype`` defaults to x's type, bfloat16 for 8-bit x."""
     dev = weight.device
-    if x.dim() != 2 or x.shape[1] != weight.k or x.device != dev or (x.numel() and x.stride(1) != 1):
-        raise ValueError(f"x must be [rows, {weight.k}] on {dev}, its rows contiguous")
-    rows, group = int(x.shape[0]), 0
+    if x.dim() != 2 or x.shape[1] != weight.k or x.device != dev:
+        raise ValueError(f"x must be [rows, {weight.k}] on {dev}")
+    rows, group, x_step = int(x.shape[0]), 0, _row_step(x)
+    if not x_step and rows:
+        raise ValueError("x's rows must be contiguous and apart")
     if x.dtype in (torch.int8, torch.float8_e4m3fn):
         if x_scale is None or x_scale.dim() != 2 or x_scale.shape[1] < 1 or weight.k % x_scale.shape[1]:
             raise ValueError("8-bit x needs x_scale [rows, groups]")
@@ -389,12 +408,16 @@ def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | No
         if out_dtype not in FLOAT_INPUTS:
             raise ValueError("out_dtype must be float32, bfloat16 or float16")
         out = torch.empty((rows, weight.out_features), dtype=out_dtype, device=dev)
-    elif out.dtype not in FLOAT_INPUTS or out.shape != (rows, weight.out_features) or out.device != dev or (
-            out.numel() and out.stride(1) != 1):
-        raise ValueError(f"out must be [{rows}, {weight.out_features}] on {dev}, its rows contiguous")
+        out_step = weight.out_features
+    else:
+        if out.dtype not in FLOAT_INPUTS or out.shape != (rows, weight.out_features) or out.device != dev:
+            raise ValueError(f"out must be [{rows}, {weight.out_features}] on {dev}")
+        out_step = _row_step(out)
+        if not out_step and rows:
+            raise ValueError("out's rows must be contiguous and apart")
     if rows:
-        _call(dev, "lb_op_w4_matvec", x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype],
+        _call(dev, "lb_op_w4_matvec", x.data_ptr(), x_step, DTYPE_CODES[x.dtype],
               None if x_scale is None else x_scale.data_ptr(), group, rows, weight._t_codes.data_ptr(),
-              weight._t_scales.data_ptr(), weight.group, weight.out_features, weight.k, out.data_ptr(), out.stride(0),
+              weight._t_scales.data_ptr(), weight.group, weight.out_features, weight.k, out.data_ptr(), out_step,
               DTYPE_CODES[out.dtype])
     return out

@@ -444,3 +444,37 @@ def test_q_may_end_before_the_last_rows_tokens_do(ops, window):
     for t in (1, 9, 10, 11, 39):
         part = ops.kv8_attention(q[:t], cache, tables, ints(lens), ints(cu), max_new=30, window=window)
         torch.testing.assert_close(part, whole[:t], rtol=2.0 ** -10, atol=1e-5)
+
+
+# ------------------------------------------------------------------ shapes and strides of the wrappers
+def test_single_rows_and_columns_of_any_stride(ops):
+    """What torch calls a row's stride does not matter where there is one row, nor a column's where there is one."""
+    g = gen(3)
+    w = ops.Int4Weight.quantize(torch.randn(8, 128, generator=g, device="cuda"))
+    col = torch.randn(128, 1, generator=g, device="cuda").to(BF16)
+    x, ones = col.t(), torch.ones(128, device="cuda")  # [1, 128] with strides (1, 1)
+    assert x.stride() == (1, 1)
+    plain = x.clone(memory_format=torch.contiguous_format).view(1, 128)
+    for a, b in zip(ops.rms_norm8(x, ones, residual=x), ops.rms_norm8(plain.reshape(1, 128), ones, residual=plain)):
+        assert torch.equal(a.view(-1).float(), b.view(-1).float())
+    out = torch.zeros(8, 1, device="cuda").t()
+    ops.w4_matvec(x, w, out=out)
+    assert torch.equal(out, ops.w4_matvec(torch.empty(1, 128, device="cuda", dtype=BF16).copy_(x), w, out_dtype=F32))
+    narrow = torch.randn(5, 3, generator=g, device="cuda")[:, 1:2]  # [5, 1] with strides (3, 1)
+    for a, b in zip(ops.rms_norm8(narrow, ones[:1]), ops.rms_norm8(narrow.contiguous(), ones[:1])):
+        assert torch.equal(a.float(), b.float())
+    turned = torch.randn(1, 5, generator=g, device="cuda").t()[:, :1].as_strided((5, 1), (1, 7))
+    for a, b in zip(ops.rms_norm8(turned, ones[:1]), ops.rms_norm8(turned.clone(memory_format=torch.contiguous_format), ones[:1])):
+        assert torch.equal(a.float(), b.float())
+
+
+def test_rows_that_overlap_are_refused(ops):
+    w = ops.Int4Weight.quantize(torch.zeros(8, 128, device="cuda"))
+    ones = torch.ones(128, device="cuda")
+    one = torch.zeros(1, 128, device="cuda")
+    for f in (lambda: ops.rms_norm8(one.expand(3, 128), ones),
+              lambda: ops.rms_norm8(torch.zeros(3, 128, device="cuda"), ones, residual=one.expand(3, 128)),
+              lambda: ops.w4_matvec(one.to(BF16).expand(3, 128), w),
+              lambda: ops.w4_matvec(torch.zeros(3, 128, device="cuda").to(BF16), w, out=torch.zeros(1, 8, device="cuda").expand(3, 8))):
+        with pytest.raises(ValueError):
+            f()
