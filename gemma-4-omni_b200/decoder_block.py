@@ -83,13 +83,13 @@ class DecoderBlock:
         c = self.cfg
         t = hidden.shape[0]
         x, xs, _ = ops.rms_norm8(hidden, self.w["norm1"], eps=c.rms_eps)
-        q, k, v = ops.w4_matvec(x, self.w["qkv"], x_scale=xs).view(t, -1, c.head_dim).split(
+        q, k, v = ops.w4_matvec(x, self.w["qkv"], x_scale=xs).view(t, c.heads + 2 * c.kv_heads, c.head_dim).split(
             (c.heads, c.kv_heads, c.kv_heads), 1)
         at = plan.positions[:t]
         cache.append(rotary(k, at, c.rope_base), v, plan.slots[:t])
         y = ops.kv8_attention(rotary(q, at, c.rope_base), cache, plan.row_tables, plan.kv_len, plan.cu_tokens, max_new=max_new,
                               window=c.window, softcap=c.softcap)
-        y = ops.w4_matvec(y.view(t, -1), self.w["out"])
+        y = ops.w4_matvec(y.view(t, c.heads * c.head_dim), self.w["out"])
         x, xs, h = ops.rms_norm8(y, self.w["norm2"], residual=hidden, eps=c.rms_eps)
         gate, up = ops.w4_matvec(x, self.w["gate_up"], x_scale=xs).split(c.ffn, 1)
         return h + ops.w4_matvec(torch.nn.functional.silu(gate) * up, self.w["down"])

@@ -478,3 +478,16 @@ def test_rows_that_overlap_are_refused(ops):
               lambda: ops.w4_matvec(torch.zeros(3, 128, device="cuda").to(BF16), w, out=torch.zeros(1, 8, device="cuda").expand(3, 8))):
         with pytest.raises(ValueError):
             f()
+
+
+def test_a_step_of_the_block_without_tokens(pkg):
+    """A tick in which no session has anything new."""
+    from gemma4_omni_b200.decode_ops import PageDirectory
+    from gemma4_omni_b200.decoder_block import DecoderBlock, DecoderConfig
+    block = DecoderBlock.synthetic(DecoderConfig(hidden=256, heads=4, kv_heads=2, head_dim=64, ffn=512), seed=1)
+    pages = PageDirectory.create(sessions=2, max_pages=2, pages=4, page_tokens=16)
+    cache = block.new_cache(4, 16)
+    plan = pages.plan(ints([0, 1]), ints([0, 0]), max_tokens=1)
+    y = block.step(torch.zeros(0, 256, dtype=BF16, device="cuda"), plan, cache, max_new=1)
+    pages.commit(plan)
+    assert y.shape == (0, 256) and plan.status() == 0 and pages.lengths.tolist() == [0, 0]
