@@ -453,7 +453,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const AttendArgs a,
   const int each = (a.n_rows + kThreads - 1) / kThreads;
   long long mine = 0;
 #pragma unroll 2
-  for (int r = tid * each; r < min(a.n_rows, (tid + 1) * each); ++r) mine += row_work(a, row_of<R>(a, r));
+  for (int r = tid * each; r < min(a.n_rows, (tid + 1) * each); ++r) {
+    const Row w = row_of<R>(a, r);
+    mine += row_work(a, w);
+    // keys past the row's table are not seen: said once
+    if (blockIdx.x == 0 && w.count > 0 && w.len > a.max_pages * P && a.status) atomicOr(a.status, static_cast<int>(LB_DEV_BAD_PAGE));
+  }
   long long sum = warp_prefix(mine);
   if (lane == 31) warp_total[warp] = sum;
   tc_fence_before();

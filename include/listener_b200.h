@@ -492,7 +492,8 @@ int lb_op_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_strid
  * [n_tokens][heads][dim] of q's type, contiguous; lse f32 [n_tokens][heads] (natural
  * log-sum-exp) or NULL.  A token that sees no key, and one in no row, has out 0 and
  * lse -inf.  dim 64, 128 or 256; page_tokens a multiple of 16, at most 256.  A page id
- * out of range counts as unseen keys and sets LB_DEV_BAD_PAGE in *status (may be NULL).
+ * out of range counts as unseen keys, as do keys past a row's table, and sets LB_DEV_BAD_PAGE in
+ * *status (may be NULL).
  * max_new: the most tokens of a row, on which the split of the work goes (rows with
  * more are right, but slower).  workspace: lb_kv8_attention_workspace bytes. */
 int lb_op_kv8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_dtype, int n_tokens,

@@ -491,3 +491,17 @@ def test_a_step_of_the_block_without_tokens(pkg):
     y = block.step(torch.zeros(0, 256, dtype=BF16, device="cuda"), plan, cache, max_new=1)
     pages.commit(plan)
     assert y.shape == (0, 256) and plan.status() == 0 and pages.lengths.tolist() == [0, 0]
+
+
+def test_keys_past_a_rows_table_are_said_to_be_missing(ops, pkg):
+    from gemma4_omni_b200 import _lib
+    g = gen(8)
+    cache, tables = make_cache(ops, g, [64, 10], 16, 1, 64)
+    q = torch.randn(2, 2, 64, generator=g, device="cuda").to(F16)
+    ops.kv8_attention(q, cache, tables, ints([64, 10]), ints([0, 1, 2]), max_new=1)
+    assert cache.status() == 0
+    ops.kv8_attention(q, cache, tables, ints([65, 10]), ints([0, 1, 2]), max_new=1)
+    assert cache.status() == _lib.DEV_BAD_PAGE
+    cache.status_word.zero_()
+    ops.kv8_attention(q, cache, tables, ints([65, 10]), ints([0, 0, 1]), max_new=1)  # a row without tokens reads nothing
+    assert cache.status() == 0
