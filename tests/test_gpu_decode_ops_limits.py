@@ -505,3 +505,80 @@ def test_keys_past_a_rows_table_are_said_to_be_missing(ops, pkg):
     cache.status_word.zero_()
     ops.kv8_attention(q, cache, tables, ints([65, 10]), ints([0, 0, 1]), max_new=1)  # a row without tokens reads nothing
     assert cache.status() == 0
+
+
+# ------------------------------------------------------------------ bounds that a lost digit or column would pass
+SHAPES = [  # dim, kv heads, group, page, lens, new, window, softcap
+    (64, 1, 1, 16, [1], [1], 0, 0.0),
+    (128, 1, 1, 64, [0, 1, 2, 15, 16, 17], [1, 1, 2, 1, 0, 1], 0, 0.0),
+    (256, 1, 8, 64, [700, 64, 63, 65, 2, 1], [2, 2, 1, 2, 2, 1], 0, 0.0),
+    (128, 8, 4, 32, [1000, 33, 257], [1, 1, 1], 0, 0.0),
+    (64, 2, 3, 48, [500, 47, 49, 97], [1, 2, 3, 1], 0, 50.0),
+    (128, 2, 16, 16, [300, 20], [3, 2], 17, 0.0),
+    (256, 2, 1, 128, [3000, 5], [1, 1], 1000, 30.0),
+    (64, 4, 2, 256, [515, 260, 100], [130, 1, 100], 0, 0.0),
+    (128, 1, 2, 16, [3, 0, 5], [7, 4, 9], 0, 0.0),
+    (128, 1, 8, 64, [9000], [1], 0, 0.0),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_attention_is_as_close_as_its_digits_say(ops, dtype, shape):
+    dim, kvh, group, page, lens, new, window, softcap = SHAPES[shape]
+    g = gen(shape)
+    cache, tables = make_cache(ops, g, [max(n, 1) for n in lens], page, kvh, dim)
+    q = torch.randn(sum(new), kvh * group, dim, generator=g, device="cuda").to(dtype)
+    check(ops, cache, tables, q, lens, [sum(new[:i]) for i in range(len(new) + 1)], max_new=max(new), window=window, softcap=softcap)
+
+
+@pytest.mark.parametrize("heads,page", [(1, 16), (8, 64), (16, 32)])
+def test_values_that_cancel_show_the_digits_of_p(ops, heads, page):
+    """Values of +-127 by turns: the outputs are small beside sum p|v|, so that p's low digits stand above their rounding."""
+    g = gen(heads)
+    cache, tables = make_cache(ops, g, [4096], page, 1, 64)
+    cache.v_codes[:, :, ::2] = 127
+    cache.v_codes[:, :, 1::2] = -127
+    cache.v_scale.fill_(1 / 127)
+    q = 0.1 * torch.randn(1, heads, 64, generator=g, device="cuda").to(F16)
+    check(ops, cache, tables, q, [4096], [0, 1], max_new=1)
+
+
+@pytest.mark.parametrize("kind", [BF16, F16, E4M3, I8])
+@pytest.mark.parametrize("out,k,group", [(33, 96, 32), (70, 1536, 128), (257, 320, 64), (32, 6144, 128), (5000, 256, 64), (40, 8192, 32)])
+def test_w4_every_column_counts_with_its_own_weight(ops, kind, out, k, group):
+    """Rows with a single one in them: the products are the weights, exactly."""
+    g = gen(out + k)
+    codes = torch.randint(0, 256, (out, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (0.01 * (0.1 + torch.rand(out, k // group, generator=g, device="cuda"))).to(F16)
+    weight = ops.Int4Weight(codes, scales)
+    want = weight.dequantize()
+    n = min(k, 512)
+    at = torch.randperm(k, generator=g, device="cuda")[:n] if k > 512 else torch.arange(k, device="cuda")
+    x = torch.zeros(n, k, device="cuda")
+    x[torch.arange(n, device="cuda"), at] = 1.0
+    xs = torch.ones(n, 1, device="cuda") if kind in (E4M3, I8) else None
+    for rows in (n, 16, 3):
+        y = ops.w4_matvec(x[:rows].to(kind), weight, x_scale=None if xs is None else xs[:rows], out_dtype=F32)
+        assert torch.equal(y, want[:, at[:rows]].t())
+
+
+@pytest.mark.parametrize("kind", [BF16, F16, I8])
+@pytest.mark.parametrize("rows,out,k,group", [(1, 2048, 1536, 128), (2, 100, 512, 64), (9, 33, 2048, 32), (16, 4097, 256, 64), (37, 70, 8192, 128),
+                                              (1, 515, 16384, 128), (16, 160, 6144, 128)])
+def test_w4_sums_are_within_their_roundings(ops, kind, rows, out, k, group):
+    """Products are exact; each of a group's k / 16 additions on the tensor cores is good to 2^-21 of the sum of absolute
+    values so far, the groups' sums are added in 32 bits.  One column left out would be 1 / k of the sum."""
+    g = gen(rows + k)
+    codes = torch.randint(0, 256, (out, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (0.01 * (0.1 + torch.rand(out, k // group, generator=g, device="cuda"))).to(F16)
+    weight = ops.Int4Weight(codes, scales)
+    x, xs = torch.randn(rows, k, generator=g, device="cuda"), None
+    if kind is I8:
+        x, xs, _ = ops.rms_norm8(x, torch.ones(k, device="cuda"), dtype=I8)
+    else:
+        x = x.to(kind)
+    y = ops.w4_matvec(x, weight, x_scale=xs, out_dtype=F32)
+    ref, spread = decode_ref.w4_product(x, xs, codes, scales)
+    bound = ((group // 16 + 2) * 2.0 ** -21 + (k // group + 18) * 2.0 ** -24) * spread + 1e-30
+    assert ((y.double() - ref).abs() <= bound).all()
