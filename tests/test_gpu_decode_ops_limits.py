@@ -544,6 +544,22 @@ def test_values_that_cancel_show_the_digits_of_p(ops, heads, page):
     check(ops, cache, tables, q, [4096], [0, 1], max_new=1)
 
 
+@pytest.mark.parametrize("page", [16, 64])
+def test_two_keys_that_cancel_show_the_last_digit_of_p(ops, page):
+    """A weight of about 1 on a value of 1 against one of about 1 / 127 on -127: p without its last digit would be off by up
+    to 2^-15 * 127, a hundred times the bound."""
+    cache, tables = make_cache(ops, gen(1), [2], page, 1, 64)
+    cache.k_codes.zero_()
+    at = int(tables[0, 0])
+    cache.k_codes[at, 0, 1, 0] = 100
+    cache.k_scale.fill_(0.01)
+    cache.v_codes[at, 0, 0], cache.v_codes[at, 0, 1] = 1, -127
+    cache.v_scale.fill_(1 / 127)
+    q = torch.zeros(1, 16, 64, device="cuda")
+    q[0, :, 0] = -38.75 + torch.arange(16, device="cuda") / 32.0
+    check(ops, cache, tables, q.to(F16), [2], [0, 1], max_new=1)
+
+
 @pytest.mark.parametrize("kind", [BF16, F16, E4M3, I8])
 @pytest.mark.parametrize("out,k,group", [(33, 96, 32), (70, 1536, 128), (257, 320, 64), (32, 6144, 128), (5000, 256, 64), (40, 8192, 32)])
 def test_w4_every_column_counts_with_its_own_weight(ops, kind, out, k, group):
