@@ -14,7 +14,7 @@
 // c takes the largest p * sv, not the largest p times the largest sv: the pages of a tile may have scales far
 // apart, and the key with the weight the smallest.  Pages that a query does not see do not count for it.
 // The products are exact in 32-bit integers, and the digits' sums are joined in 32-bit
-// floating point.  The fixed point of p is one of 128 keys: a tile's outputs leave
+// floating point (up to 2^45 before they take the scale of K, so that one stays in range below 2^80).  The fixed point of p is one of 128 keys: a tile's outputs leave
 // the tensor memory each time and are added up in registers with the tile's factor.
 //
 // A task is R query rows of one (row, kv head): the tokens of the row times the
@@ -39,11 +39,11 @@
 // Six roles in sixteen warps share one instruction cache, and its misses bound the kernel before anything else
 // did: loops are kept rolled, a score warpgroup takes 8 queries at a time (16 unrolled took 6.9 thousand
 // cycles a tile, 8 take 2.5), waits are a few instructions.  Measured: 64 answers over 0.5 million keys with 8 kv
-// heads of 128 in 203 us (1.02 GB at 5.0 TB/s, 78 % of the copy rate; bound by the load warp and the rows'
-// raggedness), ticks of 1024 sessions with a window of 1024 keys and 16 query rows of 256 columns in 130 us (3.6
+// heads of 128 in 207 to 215 us (1.02 GB at 4.8 TB/s, 75 % of the copy rate; bound by the load warp and the rows'
+// raggedness), ticks of 1024 sessions with a window of 1024 keys and 16 query rows of 256 columns in 131 us (3.5
 // TB/s; bound by the score warps' chain), one answer over 16384 keys in 22 us (the chain of set-up, one
-// tile and the join), chunks of 128 to 512 tokens in 870 us (104 TFLOP/s; bound by the score warps'
-// instructions, some 25 a query and key).  Four score warpgroups instead of two were slower (answers 289 us).
+// tile and the join), chunks of 128 to 512 tokens with a soft cap in 900 us (101 TFLOP/s; bound by the score warps'
+// instructions, some 27 a query and key).  Four score warpgroups instead of two were slower (answers 289 us).
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 #include "kernels.h"

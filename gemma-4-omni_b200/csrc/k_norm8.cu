@@ -6,12 +6,13 @@
 // The bytes bound it: 7 an element in 16 bits (x, r, the stored h, the code).  So a row is
 // read once and stays in registers between its three uses, T threads a row with
 // C pieces of 8 columns each.  With many rows C is 2 to 4: 16384 x 2048 bf16 with a scale for
-// 128 columns takes 44.7 us with 128 threads a row (5.3 TB/s, 82 % of the copy rate; when measured against
+// 128 columns takes 45 to 47 us with 128 threads a row (5.1 TB/s, 79 % of the copy rate; when measured against
 // one another, 46.6 us against 56.9 with a warp a row, whose 8 pieces a lane leave 16 warps an SM,
-// 50.1 with 64 and 49.4 with 256 threads).  What is left is instructions: 74 % of the issue slots.
+// 50.1 with 64 and 49.4 with 256 threads).  What is left is instructions: 72 % of the issue slots (int8 codes: 2 us more).
 // With few rows a piece a thread, since then the latency of one row is all there is (2 x 1536: 2.1 us
 // inside a graph).  Rows that are not
-// 16-byte aligned, odd widths and groups that are no power of two of pieces take the plain kernel at the end.
+// 16-byte aligned, odd widths and groups that are no power of two of pieces take the plain kernel at the end
+// (16384 x 2047: 140 us, groups of 41 in 2050: 200 us).
 #include <cuda_fp8.h>
 
 #include "../../include/listener_b200.h"
