@@ -334,6 +334,10 @@ struct Walk {
       while (after == 0) {
         base += __shfl_sync(0xffffffffu, upto, 31);
         win += 32;
+        if (win >= a.n_rows) {  // (only where the lengths changed under the call: its outputs are lost, but it ends)
+          t.n = 0;
+          return false;
+        }
         held = row_of<R>(a, win + (threadIdx.x & 31));
         upto = warp_prefix(row_work(a, held));
         after = __ballot_sync(0xffffffffu, base + upto > x);
@@ -358,7 +362,7 @@ struct Walk {
       t.n = max(0, to - kTaskCost) - t.tile0;
       x += to - from;
       // the CTA whose share holds the task's last tile
-      t.last_cta = static_cast<int>(((x + (length - to)) * n_ctas - 1) / line);
+      t.last_cta = static_cast<int>(min(((x + (length - to)) * n_ctas - 1) / line, n_ctas - 1));
     } while (t.n == 0);
     t.from_start = t.tile0 == 0;
     t.to_end = t.tile0 + t.n == w.tiles;
