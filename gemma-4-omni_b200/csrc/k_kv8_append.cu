@@ -16,8 +16,8 @@
 // CTAs look for the first tokens of groups in windows of the batch, so nothing
 // but the slots has to be known: a token begins a group unless the token before
 // it in the batch has the slot before it in the same page.  Where the last token before it that is not skipped is of
-// the same page all the same, two groups would read and write that page at once: the later one is refused.  A group of up to 512 pieces of 8
-// values stays in registers between its maximum and its codes; larger ones are read again.
+// the same page all the same, two groups would read and write that page at once: the later one is refused.  A
+// group of up to 512 pieces of 8 values stays in registers between its maximum and its codes; larger ones are read again.
 #include <cstring>
 
 #include "../../include/listener_b200.h"

@@ -14,8 +14,9 @@
 // c takes the largest p * sv, not the largest p times the largest sv: the pages of a tile may have scales far
 // apart, and the key with the weight the smallest.  Pages that a query does not see do not count for it.
 // The products are exact in 32-bit integers, and the digits' sums are joined in 32-bit
-// floating point (up to 2^45 before they take the scale of K, so that one stays in range below 2^80).  The fixed point of p is one of 128 keys: a tile's outputs leave
-// the tensor memory each time and are added up in registers with the tile's factor.
+// floating point (up to 2^45 before they take the scale of K, so that one stays in range below 2^80).  The
+// fixed point of p is one of 128 keys: a tile's outputs leave the tensor memory each time and are added up in
+// registers with the tile's factor.
 //
 // A task is R query rows of one (row, kv head): the tokens of the row times the
 // query heads that share the kv head, so the cache is read once for all of them.
@@ -272,7 +273,10 @@ __device__ __forceinline__ Row row_of(const AttendArgs& a, int r) {
   w.pos0 = w.len - (max(a.cu_tokens[r + 1], w.begin) - w.begin);  // (also where q ends before the row does)
   if (w.count == 0) return w;
   const int stop = min(max(w.len, 0), a.max_pages * a.page_tokens);
-  if (a.window) w.low = static_cast<int>(max(0ll, min(static_cast<long long>(w.pos0) + 1 - a.window, static_cast<long long>(stop)))) & ~(a.box - 1);
+  if (a.window) {
+    const long long low = min(static_cast<long long>(w.pos0) + 1 - a.window, static_cast<long long>(stop));
+    w.low = static_cast<int>(max(0ll, low)) & ~(a.box - 1);
+  }
   w.tiles = max(1, (stop - w.low + kTile - 1) / kTile);
   w.q_tiles = (w.count * (a.heads / a.kv_heads) + R - 1) / R;
   return w;

@@ -6,16 +6,16 @@
 // 128 k, 2 KB of codes and the groups' scales) that runs on from one tile of outputs
 // to the next, and no barrier of the block in the main loop.  x lies in shared memory
 // (16 bits, loaded once a CTA).  The codes become the A fragments of mma.sync in
-// registers by the published conversion under an exponent (Kim, Henry, Fahim and Awadalla, 2022): a word of 8
-// codes masks into four pairs (k, k + 4) by shifts and one
-// logic operation each, as 1024 + n (fp16) or 128 + n (bf16), from which one
-// subtraction leaves n - 8 exactly; x is stored in the pairs' order, so neither side is
-// shuffled.  8-bit x is exact in fp16.  A group's sum is held in 32 bits and takes its
+// registers by the published conversion under an exponent (Kim, Henry, Fahim and Awadalla,
+// 2022): a word of 8 codes masks into four pairs (k, k + 4) by shifts and one logic operation
+// each, as 1024 + n (fp16) or 128 + n (bf16), from which one subtraction leaves n - 8
+// exactly; x is stored in the pairs' order, so neither side is shuffled.  8-bit x is exact in fp16.  A group's sum is held in 32 bits and takes its
 // scale there.  mma.sync runs at 0.5 m16n8k16 a cycle and SM, and the stream of 16 rows needs 0.36, so the
 // tensor pipe is not what binds (27 % busy): instructions are, some 450 a stage and warp, nearly half of them on
 // the half-rate integer pipe (50 % busy; the widening alone is 11 for 8 codes in bf16, 9 in fp16).  16 x 2048 x
-// 131072 in groups of 64 takes 61.5 us, 2.4 TB/s (fp16 3 us less, one row 9 us less).  Whole tiles are dealt out, so the last pass leaves SMs idle: of
-// that product's 148 CTAs 40 make one pass where 108 make two; 16 x 1536 x 12288 has 96 CTAs.
+// 131072 in groups of 64 takes 61.5 us, 2.4 TB/s (fp16 3 us less, one row 9 us less).  Whole tiles are dealt out,
+// so the last pass leaves SMs idle: of that product's 148 CTAs 40 make one pass where 108 make two; 16 x 1536 x
+// 12288 has 96 CTAs.
 //
 // More rows than 16 (8 where k is above some 4600) read and widen the whole matrix again for every 16: 128, 512 and 2048
 // rows of 1536 x 12288 take 47, 117 and 426 us, the last against 46 for its operations.

@@ -297,7 +297,8 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, row_tables: torch.Tensor, kv
         space = cache._t_k_codes.new_empty(_workspace(dim, heads, cache.kv_heads, min(max_new, INT32_MAX)))
         _call(dev, "lb_op_kv8_attention", q.data_ptr(), q.stride(0), q.stride(1), DTYPE_CODES[q.dtype], t, n, heads,
               cache.kv_heads, dim, kc, vc, ks, vs, cache.pages, cache.page_tokens, row_tables.data_ptr(), max_pages,
-              kv_len.data_ptr(), cu_tokens.data_ptr(), min(max_new, INT32_MAX), dim ** -0.5 if scale is None else scale, min(window, INT32_MAX), softcap,
+              kv_len.data_ptr(), cu_tokens.data_ptr(), min(max_new, INT32_MAX),
+              dim ** -0.5 if scale is None else scale, min(window, INT32_MAX), softcap,
               out.data_ptr(), lse.data_ptr() if return_lse else None, cache._t_status_word.data_ptr(),
               space.data_ptr())
     return (out, lse) if return_lse else out

@@ -512,7 +512,7 @@ int64_t lb_kv8_attention_workspace(int dim, int heads, int kv_heads, int max_new
  * LB_BF16, LB_F16), x_ld / residual_ld elements between rows; weight LB_F32 or
  * dtype; residual may be NULL (h = x), hidden may be NULL (h is not stored), else
  * [rows][dim].  codes [rows][dim], the quotient y / scale rounded to nearest even; scales f32
- * [rows][dim / group].  A group whose y is all zero has scale 0 and codes 0; one that holds a NaN
+ * [rows][dim / group], max |y| / top to an ulp.  A group whose y is all zero has scale 0 and codes 0; one that holds a NaN
  * or an infinite value has that as its scale, and codes 0.
  * dim <= 16384. */
 int lb_op_rms_norm8(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int dtype,
