@@ -1,0 +1,298 @@
+// Norms of queries and keys for each head, with the position rotation in the same pass:
+//   y = x / sqrt(mean(x^2) + eps) * w        (over the dim values of one head)
+//   (a, b) -> (a cos t - b sin t, b cos t + a sin t),   t = position * frequency_i
+// for the first `rotary` values of a head, paired as halves (i, i + rotary / 2) or neighbours (2 i, 2 i + 1).
+//
+// Angles are exact up to their last rounding at any position: a frequency is a 64-bit fraction of a turn, its
+// product with the position modulo 2^64 is the fraction of a turn that is left, and no bit of it is lost before the
+// quadrant is taken off.  sin and cos of what is left (at most pi / 4) are their Taylor series up to x^9 and x^10
+// (first terms left out: 2e-9 and 2e-10).
+//
+// The pass is bound by its bytes: a value is read once, kept in registers through sum, norm and
+// rotation (all in 32 bits) and rounded once.  A warp takes a token, turns its angles into sines
+// once and walks over the token's heads; a head of dim values takes dim / 8 lanes, each with four neighbours
+// and the four that they are paired with.  Where tokens are few, a token's heads are dealt out to several warps.
+#include "../../include/listener_b200.h"
+#include "common.cuh"
+
+namespace lb {
+namespace {
+
+constexpr int kWarps = 4;     // of a CTA
+constexpr int kMaxDim = 1024;
+
+struct HeadsSide {
+  const void* x;
+  void* out;
+  const void* weight;  // or null
+  long long token, head, out_token, out_head;  // strides
+  int heads;
+};
+struct HeadsArgs {
+  HeadsSide q, k;
+  const void* positions;
+  const unsigned long long* turns;
+  int n_tokens, dim, rotary, neighbours, positions64, weight_f32, norm, slices;
+  float eps;
+};
+
+template <typename T>
+__device__ __forceinline__ float as_float(T v) {
+  if constexpr (__is_same(T, float)) return v;
+  else if constexpr (__is_same(T, __half)) return __half2float(v);
+  else return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_float(float v) {
+  if constexpr (__is_same(T, float)) return v;
+  else if constexpr (__is_same(T, __half)) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T v[4];
+};
+
+__device__ __forceinline__ void sin_cos(unsigned long long turns, float& s, float& c) {
+  const unsigned h = static_cast<unsigned>(turns >> 32);       // 2^-32 turns
+  const unsigned quadrant = (h + (1u << 29)) >> 30;            // (wraps to 0 with the turn)
+  const int left = static_cast<int>(h - (quadrant << 30));     // at most an eighth of a turn either way
+  const float x = static_cast<float>(left) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  const float z = x * x;
+  const float sx = fmaf(x * z, fmaf(z, fmaf(z, fmaf(z, 1.0f / 362880.0f, -1.0f / 5040.0f), 1.0f / 120.0f), -1.0f / 6.0f), x);
+  const float cx = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.0f / 3628800.0f, 1.0f / 40320.0f), -1.0f / 720.0f), 1.0f / 24.0f), -0.5f), 1.0f);
+  const bool swap = quadrant & 1u;
+  s = swap ? cx : sx;
+  c = swap ? sx : cx;
+  if (quadrant & 2u) s = -s;
+  if ((quadrant + 1u) & 2u) c = -c;
+}
+__device__ __forceinline__ unsigned long long position_of(const HeadsArgs& a, int token) {
+  return a.positions64 ? static_cast<unsigned long long>(static_cast<const long long*>(a.positions)[token])
+                       : static_cast<unsigned long long>(static_cast<long long>(static_cast<const int*>(a.positions)[token]));
+}
+template <typename T>
+__device__ __forceinline__ float weight_at(const HeadsArgs& a, const HeadsSide& s, int i) {
+  if (!s.weight) return 1.0f;
+  return a.weight_f32 ? static_cast<const float*>(s.weight)[i] : as_float(static_cast<const T*>(s.weight)[i]);
+}
+
+// The heads [first, last) of a side that this group of lanes takes, `stride` apart.
+template <typename T, int LANES>
+__device__ __forceinline__ void walk(const HeadsArgs& a, const HeadsSide& side, int token, int first, int last, int ea, int eb,
+                                     bool there, bool turned, const float (&sn)[4], const float (&cs)[4]) {
+  constexpr int kStep = 32 / LANES, kAhead = sizeof(T) == 4 ? 2 : 4;
+  float wa[4], wb[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    wa[j] = there ? weight_at<T>(a, side, ea + j) : 0.0f;
+    wb[j] = there ? weight_at<T>(a, side, eb + j) : 0.0f;
+  }
+  const T* x = static_cast<const T*>(side.x) + token * side.token;
+  T* out = static_cast<T*>(side.out) + token * side.out_token;
+  const float inv_dim = 1.0f / static_cast<float>(a.dim);
+  const int group = (threadIdx.x & 31) / LANES;
+  for (int h0 = first; h0 < last; h0 += kStep * kAhead) {
+    Four<T> ra[kAhead], rb[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int h = h0 + u * kStep + group;
+      if (there && h < last) {
+        ra[u] = *reinterpret_cast<const Four<T>*>(x + h * side.head + ea);
+        rb[u] = *reinterpret_cast<const Four<T>*>(x + h * side.head + eb);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ra[u].v[j] = rb[u].v[j] = from_float<T>(0.0f);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int h = h0 + u * kStep + group;
+      float va[4], vb[4], sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        va[j] = as_float(ra[u].v[j]);
+        vb[j] = as_float(rb[u].v[j]);
+        sum = fmaf(va[j], va[j], fmaf(vb[j], vb[j], sum));
+      }
+      if (a.norm) {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = __frsqrt_rn(fmaf(sum, inv_dim, a.eps));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          va[j] *= inv * wa[j];
+          vb[j] *= inv * wb[j];
+        }
+      }
+      if (turned) {
+        if (a.neighbours) {
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const float p = va[j], r = vb[j];
+            va[j] = fmaf(p, cs[j / 2], -va[j + 1] * sn[j / 2]);
+            va[j + 1] = fmaf(va[j + 1], cs[j / 2], p * sn[j / 2]);
+            vb[j] = fmaf(r, cs[2 + j / 2], -vb[j + 1] * sn[2 + j / 2]);
+            vb[j + 1] = fmaf(vb[j + 1], cs[2 + j / 2], r * sn[2 + j / 2]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = va[j];
+            va[j] = fmaf(p, cs[j], -vb[j] * sn[j]);
+            vb[j] = fmaf(vb[j], cs[j], p * sn[j]);
+          }
+        }
+      }
+      if (there && h < last) {
+        Four<T> oa, ob;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          oa.v[j] = from_float<T>(va[j]);
+          ob.v[j] = from_float<T>(vb[j]);
+        }
+        *reinterpret_cast<Four<T>*>(out + h * side.out_head + ea) = oa;
+        *reinterpret_cast<Four<T>*>(out + h * side.out_head + eb) = ob;
+      }
+    }
+  }
+}
+
+// LANES: lanes of a head, at least dim / 8
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kWarps * 32) heads_kernel(const HeadsArgs a) {
+  const long long warp = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (warp >= static_cast<long long>(a.n_tokens) * a.slices) return;
+  const int token = static_cast<int>(warp / a.slices), slice = static_cast<int>(warp - static_cast<long long>(token) * a.slices);
+  constexpr int kStep = 32 / LANES;
+  const int l = threadIdx.x & (LANES - 1);
+  const bool there = 8 * l < a.dim, turned = 8 * l < a.rotary;
+  int ea = 8 * l, eb = 8 * l + 4;
+  if (!a.neighbours && turned) {
+    ea = 4 * l;
+    eb = 4 * l + a.rotary / 2;
+  }
+  float sn[4] = {0.0f, 0.0f, 0.0f, 0.0f}, cs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+  if (turned) {
+    const unsigned long long p = position_of(a, token);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sin_cos(p * a.turns[4 * l + j], sn[j], cs[j]);
+  }
+  // the token's heads in one line, q's before k's, in steps of a warp's heads; this warp's part of it
+  const int q_steps = (a.q.heads + kStep - 1) / kStep, k_steps = (a.k.heads + kStep - 1) / kStep;
+  const int from = static_cast<int>(static_cast<long long>(q_steps + k_steps) * slice / a.slices);
+  const int to = static_cast<int>(static_cast<long long>(q_steps + k_steps) * (slice + 1) / a.slices);
+  if (from < q_steps)
+    walk<T, LANES>(a, a.q, token, from * kStep, min(min(to, q_steps) * kStep, a.q.heads), ea, eb, there, turned, sn, cs);
+  if (to > q_steps)
+    walk<T, LANES>(a, a.k, token, (max(from, q_steps) - q_steps) * kStep, min((to - q_steps) * kStep, a.k.heads), ea, eb, there,
+                   turned, sn, cs);
+}
+
+// Any even dim and rotary, any alignment: a warp a head, read twice, value by value.
+template <typename T>
+__global__ void __launch_bounds__(kWarps * 32) heads_any_kernel(const HeadsArgs a) {
+  const long long warp = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int all = a.q.heads + a.k.heads;
+  if (warp >= static_cast<long long>(a.n_tokens) * all) return;
+  const int token = static_cast<int>(warp / all), lane = threadIdx.x & 31;
+  int h = static_cast<int>(warp - static_cast<long long>(token) * all);
+  const bool is_k = h >= a.q.heads;
+  const HeadsSide& side = is_k ? a.k : a.q;
+  if (is_k) h -= a.q.heads;
+  const T* x = static_cast<const T*>(side.x) + token * side.token + h * side.head;
+  T* out = static_cast<T*>(side.out) + token * side.out_token + h * side.out_head;
+  float inv = 1.0f;
+  if (a.norm) {
+    float sum = 0.0f;
+    for (int i = lane; i < a.dim; i += 32) {
+      const float v = as_float(x[i]);
+      sum = fmaf(v, v, sum);
+    }
+    inv = __frsqrt_rn(fmaf(warp_sum(sum), 1.0f / static_cast<float>(a.dim), a.eps));
+  }
+  const unsigned long long p = position_of(a, token);
+  const int half = a.rotary / 2;
+  // a lane reads both values of a pair before it writes them, so that out may be x
+  for (int i = lane; i < half; i += 32) {
+    const int ia = a.neighbours ? 2 * i : i, ib = a.neighbours ? 2 * i + 1 : i + half;
+    float s, c, va = as_float(x[ia]), vb = as_float(x[ib]);
+    sin_cos(p * a.turns[i], s, c);
+    if (a.norm) {
+      va *= inv * weight_at<T>(a, side, ia);
+      vb *= inv * weight_at<T>(a, side, ib);
+    }
+    out[ia] = from_float<T>(fmaf(va, c, -vb * s));
+    out[ib] = from_float<T>(fmaf(vb, c, va * s));
+  }
+  for (int i = a.rotary + lane; i < a.dim; i += 32) {
+    const float v = as_float(x[i]);
+    out[i] = from_float<T>(a.norm ? v * (inv * weight_at<T>(a, side, i)) : v);
+  }
+}
+
+bool aligned(const HeadsSide& s, int n_tokens, int unit, int size) {
+  if (s.heads == 0) return true;
+  const uintptr_t bytes = static_cast<uintptr_t>(unit) * size;
+  const auto whole = [&](long long stride, int n) { return n == 1 || stride % unit == 0; };
+  return reinterpret_cast<uintptr_t>(s.x) % bytes == 0 && reinterpret_cast<uintptr_t>(s.out) % bytes == 0 &&
+         whole(s.token, n_tokens) && whole(s.out_token, n_tokens) && whole(s.head, s.heads) && whole(s.out_head, s.heads);
+}
+
+template <typename T>
+cudaError_t launch(HeadsArgs a, cudaStream_t s) {
+  const bool fast = a.dim % 8 == 0 && a.dim <= 256 && a.rotary % 8 == 0 && aligned(a.q, a.n_tokens, 4, sizeof(T)) &&
+                    aligned(a.k, a.n_tokens, 4, sizeof(T));
+  if (!fast) {
+    const long long warps = static_cast<long long>(a.n_tokens) * (a.q.heads + a.k.heads);
+    heads_any_kernel<T><<<static_cast<unsigned>((warps + kWarps - 1) / kWarps), kWarps * 32, 0, s>>>(a);
+    return cudaGetLastError();
+  }
+  const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32, step = 32 / lanes;
+  const int steps = (a.q.heads + step - 1) / step + (a.k.heads + step - 1) / step;
+  // as many warps as the GPU holds at 16 an SM, if the heads go that far
+  const long long want = (148ll * 16 + a.n_tokens - 1) / a.n_tokens;
+  a.slices = static_cast<int>(want < steps ? want : steps);
+  const long long warps = static_cast<long long>(a.n_tokens) * a.slices;
+  const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
+  if (lanes == 8) heads_kernel<T, 8><<<grid, kWarps * 32, 0, s>>>(a);
+  else if (lanes == 16) heads_kernel<T, 16><<<grid, kWarps * 32, 0, s>>>(a);
+  else heads_kernel<T, 32><<<grid, kWarps * 32, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace lb
+
+extern "C" int lb_op_head_norm_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int heads, const void* k,
+                                      int64_t k_token_stride, int64_t k_head_stride, int kv_heads, int dtype, int n_tokens,
+                                      int dim, const void* positions, int positions64, const uint64_t* turns, int rotary,
+                                      int neighbours, const void* q_weight, const void* k_weight, int weight_dtype, int norm,
+                                      float eps, void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                                      void* k_out, int64_t k_out_token_stride, int64_t k_out_head_stride, void* stream) {
+  using namespace lb;
+  if (!q || !q_out || n_tokens < 1 || heads < 1 || kv_heads < 0 || (kv_heads > 0 && (!k || !k_out))) return LB_ERR_INVALID_ARGUMENT;
+  if (dim < 2 || dim > kMaxDim || dim % 2 != 0 || rotary < 0 || rotary > dim || rotary % 2 != 0 || !(eps >= 0.0f))
+    return LB_ERR_INVALID_ARGUMENT;
+  if (!positions || (rotary > 0 && !turns)) return LB_ERR_INVALID_ARGUMENT;
+  if (dtype != LB_F32 && dtype != LB_BF16 && dtype != LB_F16) return LB_ERR_INVALID_ARGUMENT;
+  if (weight_dtype != LB_F32 && weight_dtype != dtype) return LB_ERR_INVALID_ARGUMENT;
+  if (heads > 65536 || kv_heads > 65536 || static_cast<long long>(n_tokens) * (heads + kv_heads) > (1ll << 32))
+    return LB_ERR_CAPACITY;
+  HeadsArgs a{};
+  a.q = {q, q_out, q_weight, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride, heads};
+  a.k = {k, k_out, k_weight, k_token_stride, k_head_stride, k_out_token_stride, k_out_head_stride, kv_heads};
+  a.positions = positions;
+  a.turns = reinterpret_cast<const unsigned long long*>(turns);
+  a.n_tokens = n_tokens;
+  a.dim = dim;
+  a.rotary = rotary;
+  a.neighbours = neighbours != 0;
+  a.positions64 = positions64 != 0;
+  a.weight_f32 = weight_dtype == LB_F32;
+  a.norm = norm != 0;
+  a.eps = eps;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == LB_F32 ? launch<float>(a, s) : dtype == LB_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
+  return e == cudaSuccess ? LB_OK : LB_ERR_CUDA;
+}

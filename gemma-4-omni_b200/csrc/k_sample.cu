@@ -1,0 +1,639 @@
+// The next token from the logits x of a row: temperature T, top-k, top-p and min-p, with a given random number u.
+//
+//   m_i = rint(2^45 exp((x_i - max x) / T))          a token's mass, a whole number
+//   top-k: the first k by (x down, index up)
+//   top-p: of those, each whose predecessors' masses sum to less than ceil(p * their total)
+//   min-p: m_i >= ceil(p_min * 2^45)
+//   token: the first by index with (sum of the kept masses up to it) > floor(u * their total)
+//
+// Masses are whole numbers, so that sums of them are the same in any order: no result depends on
+// which thread comes first.  They are computed in 64-bit floating point (to some 2^-52): a row has 10^5 borders between tokens,
+// and u falls between two roundings of one of them the more rarely the finer they are.  2^45 * 2^18 tokens stay below 2^63.
+//
+// The logits are read once.  A cluster of CTAs takes a row, each CTA holds its part of it in shared
+// memory.  Nothing is sorted but the few hundred tokens around a cut: counts and masses by bins of the distance
+// to the maximum (64 to a unit of T, shared-memory atomics on whole numbers; a mass in three limbs of 16 bits), added up over
+// the cluster, say in which bin a cut lies.  If at most 512 tokens lie in and above it, as with the usual settings, one CTA gathers
+// and sorts them and finishes alone.  Otherwise the bin's tokens are sorted, or divided again where they are many; one value that
+// they all have is cut by index.
+#include <cooperative_groups.h>
+
+#include "../../include/listener_b200.h"
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace lb {
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kList = kThreads;       // tokens that are sorted
+constexpr int kMaxCluster = 8;
+constexpr int kMaxVocab = 1 << 18;
+constexpr int kMaxPart = kMaxVocab / kMaxCluster;  // tokens of a CTA
+constexpr int kTop = 45;              // log2 of the largest mass
+constexpr unsigned long long kNone = ~0ull;
+
+typedef unsigned long long u64;
+
+struct SampleArgs {
+  const void* logits;
+  long long row_stride;
+  const void* uniform;
+  const float *temperature, *top_p, *min_p;  // by row, or null: the values below
+  const int* top_k;
+  float temperature1, top_p1, min_p1;
+  int top_k1, rows, vocab, part, uniform64;
+  long long* tokens;
+  float* logprobs;
+};
+
+struct Result {  // of one division into bins
+  u64 above;         // weight before the bin
+  int bin, count, before;  // tokens in it and before it
+};
+
+struct Shared {
+  double power[64];             // 2^(j / 64)
+  unsigned hist[4][kBins];      // counts; masses in limbs of 16 bits
+  u64 list[kList];
+  u64 mass[kList];
+  u64 scan[kWarps], scan2[kWarps];
+  // written by the other CTAs
+  float top[kMaxCluster];
+  u64 slice_mass[2][kMaxCluster];
+  unsigned slice_count[2][kMaxCluster];
+  Result result[2];
+  unsigned low[kMaxCluster], high[kMaxCluster];
+  unsigned tie_count[2][kMaxCluster];
+  u64 part_mass[kMaxCluster];
+  int cut_index;
+  float cut_value;
+  unsigned listed;
+  int at;
+};
+
+template <typename T>
+__device__ __forceinline__ float logit(T v) {  // a NaN is never drawn
+  float f;
+  if constexpr (__is_same(T, float)) f = v;
+  else if constexpr (__is_same(T, __half)) f = __half2float(v);
+  else f = __bfloat162float(v);
+  return f == f ? f : -INFINITY;
+}
+// whole numbers in the order of the values (both zeros are one value)
+__device__ __forceinline__ unsigned ordered(float x) {
+  const unsigned b = __float_as_uint(x + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(unsigned u) {
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+
+// exp by a table of 64 powers of two and a Taylor series: |f ln 2| <= 0.0055, first term left out below 4e-17
+struct Masses {
+  double top, scale;  // the maximum, log2(e) / T
+  float top_f;
+  const double* power;
+  __device__ __forceinline__ u64 operator()(float x) const {
+    if (x == top_f) return 1ull << kTop;
+    const double y = (static_cast<double>(x) - top) * scale;
+    if (!(y > -47.0)) return 0;
+    const double magic = 105553116266496.0;  // 1.5 * 2^46: the sum's last bit is 2^-6
+    const double t = y + magic;
+    const int n = __double2loint(t);         // 64 y, rounded
+    const double f = (y - (t - magic)) * 0.69314718055994530942;
+    double p = fma(f, fma(f, fma(f, fma(f, fma(f, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
+    const double w = power[n & 63];
+    p *= __hiloint2double(__double2hiint(w) + (((n >> 6) + kTop) << 20), __double2loint(w));
+    return static_cast<u64>(__double_as_longlong(p + 4503599627370496.0)) & 0xfffffffffffffull;  // rint: below 2^51
+  }
+};
+
+struct Cut {  // kept: what comes up to this token in the order (value down, index up)
+  float value;
+  int index;
+  __device__ __forceinline__ bool keeps(float x, int i) const { return x > value || (x == value && i <= index); }
+};
+
+__device__ __forceinline__ u64 warp_inclusive(u64 v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+// by the whole CTA; total: of all threads
+__device__ __forceinline__ u64 block_inclusive(u64 v, u64* scan, u64& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_inclusive(v);
+  __syncthreads();
+  if (lane == 31) scan[warp] = v;
+  __syncthreads();
+  u64 before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  return v + before;
+}
+// 512 values, one a thread, rising
+__device__ __forceinline__ u64 block_sort(u64 v, u64* room) {
+  const int t = threadIdx.x;
+#pragma unroll 1
+  for (int size = 2; size <= kList; size <<= 1) {
+#pragma unroll 1
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      u64 other;
+      if (step >= 32) {
+        __syncthreads();
+        room[t] = v;
+        __syncthreads();
+        other = room[t ^ step];
+      } else {
+        other = __shfl_xor_sync(0xffffffffu, v, step);
+      }
+      const bool low = ((t & step) == 0) == ((t & size) == 0);
+      v = low ? (v < other ? v : other) : (v < other ? other : v);
+    }
+  }
+  return v;
+}
+
+__device__ __forceinline__ u64 share_of(double p, u64 total) {  // ceil(p * total), at least 1
+  const double x = ceil(p * static_cast<double>(total));
+  return x >= 1.0 ? static_cast<u64>(x) : 1;
+}
+__device__ __forceinline__ u64 target_of(double u, u64 total) {  // floor(u * total), below the total
+  const double x = floor(u * static_cast<double>(total));
+  const u64 t = x > 0.0 ? static_cast<u64>(x) : 0;
+  return t < total ? t : total - 1;
+}
+
+// What all threads of a row's CTAs know.
+struct Row {
+  int row, n, first, k;      // this CTA's tokens: n from `first` on
+  const float* x;            // in shared memory
+  double u, top_p;
+  u64 min_mass;
+  float bin_scale;
+  Masses mass;
+  __device__ __forceinline__ int bin(float v) const {  // (a difference of two infinities is bin 0)
+    return min(kBins - 1, __float2int_rz((mass.top_f - v) * bin_scale));
+  }
+};
+
+__device__ __forceinline__ void emit(const SampleArgs& a, const Row& r, int token, u64 mass, u64 total) {
+  a.tokens[r.row] = token;
+  if (a.logprobs) a.logprobs[r.row] = static_cast<float>(log(static_cast<double>(mass) / static_cast<double>(total)));
+}
+
+// One CTA has in s.list all tokens that can be drawn (n, in any order): the rest of the work.  k: of them the first k
+// count; limit: the mass up to which top-p keeps, 0 where it is to be taken from their own sum.
+__device__ __noinline__ void finish_list(const SampleArgs& a, const Row& r, Shared& s, int n, int k, u64 limit) {
+  const int t = threadIdx.x;
+  const u64 key = block_sort(t < n ? s.list[t] : kNone, s.mass);
+  const float x = from_ordered(~static_cast<unsigned>(key >> 32));
+  const int index = static_cast<int>(static_cast<unsigned>(key));
+  u64 m = t < n && t < k ? r.mass(x) : 0, total;
+  const u64 upto = block_inclusive(m, s.scan, total);
+  if (r.top_p < 1.0) {
+    if (limit == 0) limit = share_of(r.top_p, total);
+    if (upto - m >= limit) m = 0;
+  }
+  if (m < r.min_mass) m = 0;
+  __syncthreads();  // (the sort's room is free)
+  s.mass[t] = m;
+  const u64 by_index = block_sort(m ? static_cast<u64>(index) << 32 | t : kNone, s.list);
+  const u64 mine = by_index == kNone ? 0 : s.mass[by_index & (kList - 1)];
+  const u64 to = block_inclusive(mine, s.scan, total);
+  const u64 target = target_of(r.u, total);
+  if (mine && target >= to - mine && target < to) emit(a, r, static_cast<int>(by_index >> 32), mine, total);
+}
+
+// Where the cut of the first k tokens (kMass false) or of a share of the masses (true) lies among the tokens that `kept` keeps.
+// Returns true where the row is done (the leading CTA had all that could be drawn in its list).
+template <bool kMass>
+__device__ __noinline__ bool select(const SampleArgs& a, const Row& r, Shared& s, cg::cluster_group& cluster, Cut& kept) {
+  const int t = threadIdx.x, rank = cluster.block_rank(), ctas = cluster.num_blocks();
+  const int slice = kBins / ctas, each = (slice + kThreads - 1) / kThreads;  // bins of a CTA and of a thread (at most 4)
+  u64 limit = kMass ? 0 : r.k, above = 0;
+  int before = 0;
+  unsigned lo = 0, hi = 0;
+  int shift = 0;
+  // (each division leaves one value, or 2048 times fewer: five are never reached)
+  for (int level = 0; level < 5; ++level) {
+    const int turn = level & 1;
+    // ---- tokens and masses by bins
+    for (int i = t; i < (kMass ? 4 : 1) * kBins; i += kThreads) (&s.hist[0][0])[i] = 0;
+    if (t == 0) s.listed = 0;
+    __syncthreads();
+    const auto bin_of = [&](float x, int i) -> int {  // or -1
+      if (!(x > -INFINITY) || !kept.keeps(x, r.first + i)) return -1;
+      if (level == 0) return r.bin(x);
+      const unsigned o = ordered(x);
+      return o < lo || o > hi ? -1 : static_cast<int>((hi - o) >> shift);
+    };
+    for (int i = t; i < r.n; i += kThreads) {
+      const float x = r.x[i];
+      const int b = bin_of(x, i);
+      if (b < 0) continue;
+      atomicAdd(&s.hist[0][b], 1u);
+      if constexpr (kMass) {
+        const u64 m = r.mass(x);
+        const unsigned m0 = m & 0xffff, m1 = (m >> 16) & 0xffff, m2 = static_cast<unsigned>(m >> 32);
+        if (m0) atomicAdd(&s.hist[1][b], m0);
+        if (m1) atomicAdd(&s.hist[2][b], m1);
+        if (m2) atomicAdd(&s.hist[3][b], m2);
+      }
+    }
+    cluster.sync();
+    // ---- each CTA adds up a slice of the bins over the cluster
+    u64 bin_mass[4];
+    unsigned bin_count[4];
+    u64 my_mass = 0;
+    unsigned my_count = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bin_mass[j] = 0;
+      bin_count[j] = 0;
+      if (j < each && t * each + j < slice) {
+        const int b = rank * slice + t * each + j;
+        for (int c = 0; c < ctas; ++c) {
+          const unsigned* h = cluster.map_shared_rank(&s.hist[0][0], c);
+          bin_count[j] += h[b];
+          if constexpr (kMass)
+            bin_mass[j] += h[kBins + b] + (static_cast<u64>(h[2 * kBins + b]) << 16) + (static_cast<u64>(h[3 * kBins + b]) << 32);
+        }
+        my_mass += bin_mass[j];
+        my_count += bin_count[j];
+      }
+    }
+    u64 slice_count, slice_mass = 0, upto_mass = 0;
+    const u64 upto_count = block_inclusive(my_count, s.scan, slice_count);
+    if constexpr (kMass) upto_mass = block_inclusive(my_mass, s.scan2, slice_mass);
+    if (t < ctas) {
+      *cluster.map_shared_rank(&s.slice_count[turn][rank], t) = static_cast<unsigned>(slice_count);
+      *cluster.map_shared_rank(&s.slice_mass[turn][rank], t) = slice_mass;
+    }
+    cluster.sync();
+    u64 base_mass = 0, all_mass = 0;
+    unsigned base_count = 0, all_count = 0;
+    for (int c = 0; c < ctas; ++c) {
+      if (c < rank) {
+        base_mass += s.slice_mass[turn][c];
+        base_count += s.slice_count[turn][c];
+      }
+      all_mass += s.slice_mass[turn][c];
+      all_count += s.slice_count[turn][c];
+    }
+    if (level == 0) {
+      if constexpr (kMass) limit = share_of(r.top_p, all_mass);
+      else if (limit > all_count) return false;  // no more than k tokens: all are kept
+    }
+    // ---- the bin that holds the cut: one thread of one CTA finds it
+    {
+      u64 w = above + (kMass ? base_mass + upto_mass - my_mass : base_count + upto_count - my_count);
+      unsigned n = before + base_count + static_cast<unsigned>(upto_count) - my_count;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u64 mine = kMass ? bin_mass[j] : bin_count[j];
+        if (w < limit && limit <= w + mine) {
+          const Result found{w, rank * slice + t * each + j, static_cast<int>(bin_count[j]), static_cast<int>(n)};
+          for (int c = 0; c < ctas; ++c) *cluster.map_shared_rank(&s.result[turn], c) = found;
+        }
+        w += mine;
+        n += bin_count[j];
+      }
+    }
+    cluster.sync();
+    const Result found = s.result[turn];
+    above = found.above;
+    before = found.before;
+    const bool all = found.before + found.count <= kList;  // everything down to the cut fits the list
+    if (all || found.count <= kList) {
+      Shared& lead = *cluster.map_shared_rank(&s, 0);
+      const unsigned bin_top = hi - (static_cast<unsigned>(found.bin) << shift), span = (1u << shift) - 1;
+      const unsigned bin_low = bin_top - lo > span ? bin_top - span : lo;
+      const int lane = t & 31;
+      for (int i0 = t - lane; i0 < r.n; i0 += kThreads) {
+        const int i = i0 + lane;
+        bool take = false;
+        float x = 0.0f;
+        if (i < r.n) {
+          x = r.x[i];
+          if (all && level > 0) {  // also what was above the first division's bin
+            take = x > -INFINITY && kept.keeps(x, r.first + i) && ordered(x) >= bin_low;
+          } else {
+            const int b = bin_of(x, i);
+            take = b >= 0 && (all ? b <= found.bin : b == found.bin);
+          }
+        }
+        const unsigned who = __ballot_sync(0xffffffffu, take);
+        if (!who) continue;
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(&lead.listed, __popc(who));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+        if (take && at < kList) lead.list[at] = static_cast<u64>(~ordered(x)) << 32 | static_cast<unsigned>(r.first + i);
+      }
+      cluster.sync();
+      if (all) {
+        if (rank == 0) finish_list(a, r, s, found.before + found.count, kMass ? kList : r.k, limit * kMass);
+        return true;
+      }
+      if (rank == 0) {
+        const u64 key = block_sort(t < found.count ? s.list[t] : kNone, s.mass);
+        const float x = from_ordered(~static_cast<unsigned>(key >> 32));
+        const u64 w = t < found.count ? (kMass ? r.mass(x) : 1) : 0;
+        u64 total;
+        const u64 to = above + block_inclusive(w, s.scan, total);
+        if (to - w < limit && limit <= to) {
+          for (int c = 0; c < ctas; ++c) {
+            *cluster.map_shared_rank(&s.cut_value, c) = x;
+            *cluster.map_shared_rank(&s.cut_index, c) = static_cast<int>(static_cast<unsigned>(key));
+          }
+        }
+      }
+      cluster.sync();
+      kept = {s.cut_value, s.cut_index};
+      return false;
+    }
+    // ---- too many: the bin's values are the next division's range
+    bool single;
+    if (level == 0) {
+      unsigned least = 0xffffffffu, most = 0;
+      for (int i = t; i < r.n; i += kThreads) {
+        const float x = r.x[i];
+        if (bin_of(x, i) == found.bin) {
+          least = min(least, ordered(x));
+          most = max(most, ordered(x));
+        }
+      }
+      least = __reduce_min_sync(0xffffffffu, least);
+      most = __reduce_max_sync(0xffffffffu, most);
+      __syncthreads();
+      if ((t & 31) == 0) s.scan[t >> 5] = static_cast<u64>(most) << 32 | least;
+      __syncthreads();
+      if (t < ctas) {
+        for (int w = 0; w < kWarps; ++w) {
+          least = min(least, static_cast<unsigned>(s.scan[w]));
+          most = max(most, static_cast<unsigned>(s.scan[w] >> 32));
+        }
+        *cluster.map_shared_rank(&s.low[rank], t) = least;
+        *cluster.map_shared_rank(&s.high[rank], t) = most;
+      }
+      cluster.sync();
+      lo = s.low[0];
+      hi = s.high[0];
+      for (int c = 1; c < ctas; ++c) {
+        lo = min(lo, s.low[c]);
+        hi = max(hi, s.high[c]);
+      }
+      single = lo == hi;
+    } else {
+      single = shift == 0;
+      hi -= static_cast<unsigned>(found.bin) << shift;
+      lo = hi - lo >= 1u << shift ? hi - ((1u << shift) - 1) : lo;
+    }
+    if (!single) {
+      for (shift = 0; (hi - lo) >> shift >= kBins;) ++shift;
+      continue;
+    }
+    // ---- one value: so many of its tokens, the lowest indexes first
+    const float x = from_ordered(lo);
+    const u64 w = kMass ? r.mass(x) : 1;
+    const unsigned want = static_cast<unsigned>((limit - above + w - 1) / w);
+    unsigned ties = 0;
+    const int seg = ((a.part + kWarps - 1) / kWarps + 31) / 32 * 32, lane = t & 31, warp = t >> 5;
+    const int from = min(r.n, warp * seg), to = min(r.n, from + seg);
+    for (int i = from + lane; i < to; i += 32) ties += r.x[i] == x && kept.keeps(x, r.first + i);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    u64 cta_ties;
+    const u64 upto = block_inclusive(lane == 31 ? ties : 0, s.scan, cta_ties);
+    if (t < ctas) *cluster.map_shared_rank(&s.tie_count[turn][rank], t) = static_cast<unsigned>(cta_ties);
+    cluster.sync();
+    unsigned seen = 0;
+    for (int c = 0; c < rank; ++c) seen += s.tie_count[turn][c];
+    seen += __shfl_sync(0xffffffffu, static_cast<unsigned>(upto), 31) - ties;  // before this warp
+    if (seen < want && want <= seen + ties) {
+      for (int i0 = from; i0 < to; i0 += 32) {
+        const int i = i0 + lane;
+        const bool tie = i < to && r.x[i] == x && kept.keeps(x, r.first + i);
+        const unsigned who = __ballot_sync(0xffffffffu, tie);
+        if (tie && seen + __popc(who & ((2u << lane) - 1)) == want) {
+          for (int c = 0; c < ctas; ++c) *cluster.map_shared_rank(&s.cut_index, c) = r.first + i;
+        }
+        seen += __popc(who);
+      }
+    }
+    cluster.sync();
+    kept = {x, s.cut_index};
+    return false;
+  }
+  return false;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
+  __shared__ Shared s;
+  extern __shared__ __align__(16) float x_raw[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int rank = cluster.block_rank(), ctas = cluster.num_blocks();
+  Row r;
+  r.row = blockIdx.x / ctas;
+  r.first = min(a.vocab, rank * a.part);
+  r.n = min(a.vocab, r.first + a.part) - r.first;
+
+  // ---- this CTA's logits as floats; the aligned part by 16 bytes
+  constexpr int kVec = 16 / sizeof(T);
+  const T* src = static_cast<const T*>(a.logits) + r.row * a.row_stride + r.first;
+  const int head = min(r.n, static_cast<int>((16 - reinterpret_cast<uintptr_t>(src) % 16) % 16 / sizeof(T)));
+  const int vecs = (r.n - head) / kVec, pad = (kVec - head) % kVec;
+  float* x = x_raw + pad;
+  r.x = x;
+  float top = -INFINITY;
+  const uint4* body = reinterpret_cast<const uint4*>(src + head);
+  constexpr int kAhead = 4;
+  for (int v0 = t; v0 < vecs; v0 += kThreads * kAhead) {
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (v0 + j * kThreads < vecs) raw[j] = __ldcs(body + v0 + j * kThreads);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int v = v0 + j * kThreads;
+      if (v >= vecs) break;
+      const T* part = reinterpret_cast<const T*>(&raw[j]);
+#pragma unroll
+      for (int e = 0; e < kVec; e += 4) {
+        const float4 f = make_float4(logit(part[e]), logit(part[e + 1]), logit(part[e + 2]), logit(part[e + 3]));
+        top = fmaxf(top, fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)));
+        *reinterpret_cast<float4*>(x + head + v * kVec + e) = f;
+      }
+    }
+  }
+  const int rest = r.n - head - vecs * kVec;
+  if (t < head + rest) {
+    const int i = t < head ? t : head + vecs * kVec + (t - head);
+    x[i] = logit(src[i]);
+    top = fmaxf(top, x[i]);
+  }
+  if (t < 64) s.power[t] = exp2(static_cast<double>(t) / 64.0);
+
+  // ---- the row's settings and its maximum
+  const float heat = a.temperature ? a.temperature[r.row] : a.temperature1;
+  const float p = a.top_p ? a.top_p[r.row] : a.top_p1, least = a.min_p ? a.min_p[r.row] : a.min_p1;
+  r.k = a.top_k ? a.top_k[r.row] : a.top_k1;
+  if (r.k <= 0 || r.k > a.vocab) r.k = a.vocab;
+  r.top_p = p < 1.0f ? static_cast<double>(p) : 1.0;
+  r.min_mass = least > 0.0f ? static_cast<u64>(ceil(static_cast<double>(fminf(least, 1.0f)) * static_cast<double>(1ull << kTop))) : 0;
+  r.u = a.uniform64 ? static_cast<const double*>(a.uniform)[r.row] : static_cast<double>(static_cast<const float*>(a.uniform)[r.row]);
+  const bool greedy = !(heat > 0.0f);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s.scan[warp] = __float_as_uint(top);
+  __syncthreads();
+  if (t < ctas) {
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, __uint_as_float(static_cast<unsigned>(s.scan[w])));
+    *cluster.map_shared_rank(&s.top[rank], t) = top;
+  }
+  cluster.sync();
+  top = s.top[0];
+  for (int c = 1; c < ctas; ++c) top = fmaxf(top, s.top[c]);
+  r.mass = {static_cast<double>(top), 1.4426950408889634074 / static_cast<double>(heat), top, s.power};
+  r.bin_scale = fminf(64.0f / heat, 1e30f);
+
+  if (top == -INFINITY) {  // nothing to draw from
+    if (rank == 0 && t == 0) {
+      a.tokens[r.row] = -1;
+      if (a.logprobs) a.logprobs[r.row] = -INFINITY;
+    }
+    return;
+  }
+  if (greedy) {  // the lowest index of the maximum
+    unsigned at = 0xffffffffu;
+    for (int i = t; i < r.n; i += kThreads)
+      if (x[i] == top) at = min(at, static_cast<unsigned>(r.first + i));
+    at = __reduce_min_sync(0xffffffffu, at);
+    __syncthreads();
+    if (lane == 0) s.scan[warp] = at;
+    __syncthreads();
+    if (t == 0) {
+      for (int w = 0; w < kWarps; ++w) at = min(at, static_cast<unsigned>(s.scan[w]));
+      *cluster.map_shared_rank(&s.low[rank], 0) = at;
+    }
+    cluster.sync();
+    if (rank == 0 && t == 0) {
+      for (int c = 0; c < ctas; ++c) at = min(at, s.low[c]);
+      a.tokens[r.row] = at;
+      if (a.logprobs) a.logprobs[r.row] = 0.0f;
+    }
+    return;
+  }
+  if (a.vocab <= kList) {  // (one CTA)
+    const bool there = t < r.n && x[t] > -INFINITY;
+    s.list[t] = there ? static_cast<u64>(~ordered(x[t])) << 32 | static_cast<unsigned>(t) : kNone;
+    finish_list(a, r, s, kList, r.k, 0);  // (what cannot be drawn sorts behind the rest and has no mass)
+    return;
+  }
+  Cut kept{-INFINITY, 0x7fffffff};
+  if (r.k < a.vocab && select<false>(a, r, s, cluster, kept)) return;
+  if (r.top_p < 1.0 && select<true>(a, r, s, cluster, kept)) return;
+
+  // ---- the kept masses in the order of the indexes: by warps, by CTAs, and the part with the target once more
+  const int seg = ((a.part + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const auto kept_mass = [&](int i) -> u64 {
+    const float v = x[i];
+    if (!kept.keeps(v, r.first + i)) return 0;
+    const u64 m = r.mass(v);
+    return m >= r.min_mass ? m : 0;
+  };
+  const auto warp_mass = [&](int from, int to) {
+    u64 sum = 0;
+    for (int i = from + lane; i < to; i += 32) sum += kept_mass(i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+  };
+  u64 mine = warp_mass(min(r.n, warp * seg), min(r.n, (warp + 1) * seg)), cta_mass;
+  u64 upto = __shfl_sync(0xffffffffu, block_inclusive(lane == 31 ? mine : 0, s.scan, cta_mass), 31);
+  if (t < ctas) *cluster.map_shared_rank(&s.part_mass[rank], t) = cta_mass;
+  cluster.sync();
+  u64 base = 0, total = 0;
+  for (int c = 0; c < ctas; ++c) {
+    if (c < rank) base += s.part_mass[c];
+    total += s.part_mass[c];
+  }
+  const u64 target = target_of(r.u, total);
+  if (target < base || target >= base + cta_mass) return;
+  if (base + upto - mine <= target && target < base + upto && lane == 0) {
+    s.at = warp * seg;
+    s.mass[0] = base + upto - mine;
+  }
+  __syncthreads();
+  const int start = s.at, sub = (seg / kWarps + 31) / 32 * 32;
+  base = s.mass[0];
+  const int from = min(r.n, min(start + seg, start + warp * sub)), to = min(r.n, min(start + seg, start + (warp + 1) * sub));
+  mine = warp_mass(from, to);
+  upto = base + __shfl_sync(0xffffffffu, block_inclusive(lane == 31 ? mine : 0, s.scan, cta_mass), 31);
+  if (upto - mine <= target && target < upto) {
+    u64 done = upto - mine;
+    for (int i0 = from; i0 < to; i0 += 32) {
+      const u64 m = i0 + lane < to ? kept_mass(i0 + lane) : 0;
+      const u64 sum = done + warp_inclusive(m);
+      if (m && sum - m <= target && target < sum) emit(a, r, r.first + i0 + lane, m, total);
+      done = __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch(SampleArgs a, int ctas, cudaStream_t s) {
+  const auto kernel = sample_kernel<T>;
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), (kMaxPart + 8) * 4);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = static_cast<unsigned>(a.rows) * ctas;
+  cfg.blockDim = kThreads;
+  cfg.dynamicSmemBytes = (a.part + 8) * sizeof(float);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, a);
+  return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
+}  // namespace
+}  // namespace lb
+
+extern "C" int lb_op_sample(const void* logits, int64_t row_stride, int dtype, int rows, int vocab, const void* uniform,
+                            int uniform64, const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
+                            const float* top_p, float top_p1, const float* min_p, float min_p1, int64_t* tokens,
+                            float* logprobs, void* stream) {
+  using namespace lb;
+  if (!logits || !uniform || !tokens || rows < 1 || vocab < 1 || row_stride < vocab) return LB_ERR_INVALID_ARGUMENT;
+  if (dtype != LB_F32 && dtype != LB_BF16 && dtype != LB_F16) return LB_ERR_INVALID_ARGUMENT;
+  if (!temperature && !(temperature1 >= 0.0f && temperature1 <= 3.4e38f)) return LB_ERR_INVALID_ARGUMENT;
+  if ((!top_p && !(top_p1 >= 0.0f)) || (!min_p && !(min_p1 >= 0.0f && min_p1 <= 1.0f))) return LB_ERR_INVALID_ARGUMENT;
+  if (vocab > kMaxVocab || rows > (1 << 24)) return LB_ERR_CAPACITY;
+  // 16384 tokens a CTA, 32768 beyond 131072
+  int ctas = 1;
+  while (ctas < kMaxCluster && (vocab + ctas - 1) / ctas > 16384) ctas *= 2;
+  const int part = ((vocab + ctas - 1) / ctas + 7) / 8 * 8;
+  SampleArgs a{logits, row_stride, uniform, temperature, top_p, min_p, top_k, temperature1, top_p1, min_p1, top_k1, rows, vocab,
+               part, uniform64 != 0, reinterpret_cast<long long*>(tokens), logprobs};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == LB_F32 ? launch<float>(a, ctas, s) : dtype == LB_BF16 ? launch<__nv_bfloat16>(a, ctas, s)
+                                                                                     : launch<__half>(a, ctas, s);
+  return e == cudaSuccess ? LB_OK : LB_ERR_CUDA;
+}

@@ -13,6 +13,8 @@ Here the caches of all sessions share one pool of pages:
   ``append`` writes the planned tokens, ``kv8_attention`` reads them.
 - ``rms_norm8``: residual addition + RMS norm with an 8-bit output and scales.
 - ``Int4Weight`` / ``w4_matvec``: products with 4-bit weights and group scales.
+- ``Rotary`` / ``head_norm_rotary``: norms of queries and keys for each head, with the position rotation.
+- ``sample_tokens``: the next tokens from logits and given random numbers.
 
 Every call is enqueued on torch's current stream of the tensors' device and can be
 captured into a CUDA graph; none synchronises except the ``status`` reads.
@@ -20,7 +22,9 @@ There is no CPU path.
 """
 from __future__ import annotations
 
+import decimal
 import functools
+import math
 from dataclasses import dataclass
 
 import torch
@@ -36,6 +40,8 @@ MAX_PLAN_ROWS = 8192
 MAX_SESSIONS = 262144
 MAX_PLAN_TOKENS = 1 << 26
 INT32_MAX = (1 << 31) - 1
+MAX_HEAD_DIM = 1024
+MAX_VOCAB = 262144
 
 
 def _call(device: torch.device, name: str, *args) -> None:
@@ -66,6 +72,13 @@ def _row_step(t: torch.Tensor) -> int:
         return 0
     step = t.stride(0) if rows > 1 else cols
     return step if step >= cols else 0
+
+
+def _spread(t: torch.Tensor) -> bool:
+    """Whether the values of a 3-D tensor lie apart: heads within tokens, or tokens within heads."""
+    (n, heads, dim), (a, b, _) = t.shape, t.stride()
+    a, b = a if n > 1 else heads * dim * max(b, 1), b if heads > 1 else dim
+    return (b >= dim and a >= (heads - 1) * b + dim) or (n > 1 and a >= dim and b >= (n - 1) * a + dim)
 
 
 def _exchangeable(name: str, dtype: torch.dtype, shape, align: int = 1) -> property:
@@ -422,3 +435,165 @@ def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | No
               weight._t_scales.data_ptr(), weight.group, weight.out_features, weight.k, out.data_ptr(), out_step,
               DTYPE_CODES[out.dtype])
     return out
+
+
+_PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510")
+
+
+@functools.lru_cache(maxsize=64)
+def _turns(rotary_dim: int, base: float) -> tuple[float, ...]:
+    """The frequencies base ** (-2 i / rotary_dim), in turns a position, as signed 64-bit fractions of a turn."""
+    with decimal.localcontext() as c:
+        c.prec = 50
+        return tuple(_fraction(decimal.Decimal(base) ** (decimal.Decimal(-2 * i) / rotary_dim)) for i in range(rotary_dim // 2))
+
+
+def _fraction(radians: decimal.Decimal) -> int:
+    """radians / (2 pi) modulo 1 as a whole number of 2^-64, in the range of int64."""
+    with decimal.localcontext() as c:
+        c.prec = 400  # the whole turns of any double, and 64 bits behind the point
+        v = int((radians / (2 * _PI) * 2 ** 64).to_integral_value(decimal.ROUND_HALF_EVEN)) % 2 ** 64
+    return v - 2 ** 64 if v >= 2 ** 63 else v
+
+
+class Rotary:
+    """The frequencies of a position rotation of heads of ``dim`` values.
+
+    ``turns`` int64 [rotary_dim / 2]: frequencies in turns a position, as 64-bit fractions, so that the angle of any
+    position is exact.  ``pairs``: "halves" pairs value i with i + rotary_dim / 2, "neighbours" 2 i with 2 i + 1;
+    values from rotary_dim on are not rotated."""
+
+    turns = _exchangeable("turns", torch.int64, lambda r: (r.rotary_dim // 2,), 8)
+
+    def __init__(self, turns: torch.Tensor, dim: int, *, pairs: str = "halves"):
+        self.device = _cuda(turns.device, "Rotary")
+        if turns.dim() != 1 or turns.shape[0] < 1:
+            raise ValueError("turns must be [rotary_dim / 2]")
+        self.dim, self.rotary_dim = int(dim), 2 * int(turns.shape[0])
+        if self.dim % 2 or not self.rotary_dim <= self.dim <= MAX_HEAD_DIM:
+            raise ValueError(f"dim must be even, at most {MAX_HEAD_DIM}, and no less than rotary_dim")
+        if pairs not in ("halves", "neighbours"):
+            raise ValueError('pairs are "halves" or "neighbours"')
+        self.pairs = pairs
+        self.turns = turns
+
+    @classmethod
+    def create(cls, dim: int, *, rotary_dim: int | None = None, base: float = 10_000.0, pairs: str = "halves",
+               device: torch.device | str = "cuda") -> "Rotary":
+        """Frequencies base ** (-2 i / rotary_dim) radians a position."""
+        rotary_dim = dim if rotary_dim is None else rotary_dim
+        if rotary_dim < 2 or rotary_dim % 2 or not 0.0 < base < math.inf:
+            raise ValueError("rotary_dim must be even and positive, base positive")
+        return cls(torch.tensor(_turns(rotary_dim, float(base)), dtype=torch.int64, device=device), dim, pairs=pairs)
+
+    @classmethod
+    def from_frequencies(cls, frequencies, dim: int, *, pairs: str = "halves", device: torch.device | str = "cuda") -> "Rotary":
+        """Given frequencies (a sequence of floats or a tensor), in radians a position."""
+        values = [float(f) for f in frequencies]
+        if not all(math.isfinite(f) for f in values):
+            raise ValueError("frequencies must be finite")
+        return cls(torch.tensor([_fraction(decimal.Decimal(f)) for f in values], dtype=torch.int64, device=device), dim, pairs=pairs)
+
+
+def head_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary, *,
+                     q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                     norm: bool = True, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Norms of queries and keys for each head, and their rotation by ``positions``, in one pass: (q, k).
+
+    q [tokens, heads, dim], k [tokens, kv_heads, dim] (or None) of one type, such as views of one product's output; positions
+    int32 or int64 [tokens], as a ``PagePlan`` has them.  With ``norm`` each head's values become x / sqrt(mean(x^2) + eps) *
+    weight (weights f32 or of q's type, None: 1).  ``q_out`` / ``k_out`` may be q and k themselves."""
+    dev = rotary.device
+    if q.dim() != 3 or q.dtype not in FLOAT_INPUTS:
+        raise ValueError("q must be a float32, bfloat16 or float16 [tokens, heads, dim] tensor")
+    t, heads, dim = q.shape
+    if dim != rotary.dim or heads < 1:
+        raise ValueError(f"heads have {rotary.dim} values")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError("positions must be int32 or int64")
+    _need(positions, "positions", positions.dtype, (t,), dev)
+    sides = [("q", q, q_out, q_weight)]
+    if k is not None:
+        if k.dim() != 3 or k.dtype != q.dtype or k.shape[0] != t or k.shape[2] != dim:
+            raise ValueError("k must be like q but for its number of heads")
+        sides.append(("k", k, k_out, k_weight))
+    elif k_out is not None or k_weight is not None:
+        raise ValueError("k_out and k_weight come with k")
+    weight_dtype = torch.float32
+    for name, x, out, weight in sides:
+        if x.device != dev or (x.numel() and x.stride(2) != 1):
+            raise ValueError(f"{name} must be on {dev}, its rows contiguous")
+        if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != dev
+                                or (out.numel() and (out.stride(2) != 1 or not _spread(out)))):
+            raise ValueError(f"{name}_out must be like {name}, its rows contiguous and apart")
+        if out is not None and out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and t:
+            raise ValueError(f"{name}_out must have {name}'s strides where it is {name}")
+        if weight is not None:
+            if not norm:
+                raise ValueError("weights belong to the norm")
+            if weight.dtype not in (torch.float32, q.dtype):
+                raise ValueError("weights must be float32 or of q's type")
+            _need(weight, f"{name}_weight", weight.dtype, (dim,), dev)
+            weight_dtype = weight.dtype
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("weights must be of one type")
+    if not 0.0 <= eps < math.inf:
+        raise ValueError("eps must not be negative")
+    if q_out is None:
+        q_out = q.new_empty(q.shape)
+    if k is not None and k_out is None:
+        k_out = k.new_empty(k.shape)
+    if t:
+        if k is None:
+            k_args = out_args = (None, 0, 0)
+            kv_heads = 0
+        else:
+            k_args, out_args = (k.data_ptr(), k.stride(0), k.stride(1)), (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
+            kv_heads = k.shape[1]
+        _call(dev, "lb_op_head_norm_rotary", q.data_ptr(), q.stride(0), q.stride(1), heads, *k_args, kv_heads, DTYPE_CODES[q.dtype],
+              t, dim, positions.data_ptr(), positions.dtype == torch.int64, rotary._t_turns.data_ptr(), rotary.rotary_dim,
+              rotary.pairs == "neighbours", None if q_weight is None else q_weight.data_ptr(),
+              None if k_weight is None else k_weight.data_ptr(), DTYPE_CODES[weight_dtype], norm, eps,
+              q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *out_args)
+    return q_out, k_out
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  return_logprobs: bool = False):
+    """Draws a token a row from ``logits`` [rows, vocab] with the given random numbers ``uniform`` [rows] in [0, 1).
+
+    ``temperature`` (0: the likeliest token), ``top_k`` (0: all), ``top_p`` (1: all) and ``min_p`` (0: all) are numbers, or tensors
+    with one for each row (float32; top_k int32).  top_k keeps the first tokens by falling logit (the lower index first),
+    top_p of those the first whose probabilities reach top_p, min_p those of at least min_p times the largest
+    probability; the token is the first by index at which the sum of what is kept exceeds ``uniform`` times its total.
+    Masses are whole numbers of 2^-45 of the largest, so that a result depends on no order of summation.
+    Returns int64 [rows] (-1 where a row has nothing to draw: all -inf or NaN), with ``return_logprobs`` also
+    float32 [rows], the logarithm of the token's part in what was kept."""
+    if logits.dim() != 2 or logits.dtype not in FLOAT_INPUTS:
+        raise ValueError("logits must be a float32, bfloat16 or float16 [rows, vocab] tensor")
+    dev = _cuda(logits.device, "sample_tokens")
+    rows, vocab = logits.shape
+    if not 0 < vocab <= MAX_VOCAB:
+        raise ValueError(f"a row has between 1 and {MAX_VOCAB} logits")
+    step = _row_step(logits)
+    if not step and rows:
+        raise ValueError("the rows of logits must be contiguous and apart")
+    if uniform.dtype not in (torch.float32, torch.float64):
+        raise ValueError("uniform must be float32 or float64")
+    _need(uniform, "uniform", uniform.dtype, (rows,), dev)
+    settings = []
+    for name, value, dtype, low, high in (("temperature", temperature, torch.float32, 0.0, 3e38), ("top_k", top_k, torch.int32, 0, math.inf),
+                                          ("top_p", top_p, torch.float32, 0.0, math.inf), ("min_p", min_p, torch.float32, 0.0, 1.0)):
+        if isinstance(value, torch.Tensor):
+            _need(value, name, dtype, (rows,), dev)
+            settings += [value.data_ptr(), 0]
+        else:
+            if not low <= value <= high:
+                raise ValueError(f"{name} must be between {low} and {high}")
+            settings += [None, min(value, vocab) if dtype == torch.int32 else value]
+    tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if return_logprobs else None
+    if rows:
+        _call(dev, "lb_op_sample", logits.data_ptr(), step, DTYPE_CODES[logits.dtype], rows, vocab, uniform.data_ptr(),
+              uniform.dtype == torch.float64, *settings, tokens.data_ptr(), logprobs.data_ptr() if return_logprobs else None)
+    return (tokens, logprobs) if return_logprobs else tokens

@@ -530,6 +530,41 @@ int lb_op_w4_matvec(const void* x, int64_t x_ld, int x_dtype, const float* x_sca
                     const void* codes, const void* w_scale, int group, int out_features, int k, void* out,
                     int64_t ld_out, int out_dtype, void* stream);
 
+/* Norms of queries and keys for each head and the position rotation, in one pass.  For every
+ * token and head of q [n_tokens][heads][dim] and k [n_tokens][kv_heads][dim] (kv_heads 0: no k):
+ *   y = x / sqrt(mean(x^2) + eps) * weight   (norm 0: y = x; weight NULL: 1),
+ * and of the first `rotary` values the pairs (i, i + rotary / 2), or with neighbours != 0
+ * (2 i, 2 i + 1), become (a cos t - b sin t, b cos t + a sin t) with t = 2 pi * frac(position *
+ * turns[i] / 2^64): turns uint64 [rotary / 2] is the frequency in turns a position, as a
+ * 64-bit fraction.  positions int32 [n_tokens] (positions64 != 0: int64), of any sign.  q, k and the
+ * outputs of dtype (LB_F32, LB_BF16, LB_F16), strides in elements, the last dimension contiguous; an output may
+ * be its input (with the same strides).  Weights [dim] of weight_dtype: LB_F32 or dtype.  All
+ * in 32 bits, rounded once.  dim even, at most 1024, rotary even. */
+int lb_op_head_norm_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int heads, const void* k,
+                           int64_t k_token_stride, int64_t k_head_stride, int kv_heads, int dtype, int n_tokens,
+                           int dim, const void* positions, int positions64, const uint64_t* turns, int rotary,
+                           int neighbours, const void* q_weight, const void* k_weight, int weight_dtype, int norm,
+                           float eps, void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                           void* k_out, int64_t k_out_token_stride, int64_t k_out_head_stride, void* stream);
+
+/* Draws a token a row from logits [rows][vocab] (LB_F32, LB_BF16, LB_F16; row_stride elements between rows)
+ * with the given random numbers: uniform f32 [rows] (uniform64 != 0: f64) in [0, 1).
+ *   mass_i = rint(2^45 * exp((x_i - max x) / temperature)), a whole number (in 64 bits)
+ *   top_k > 0:  the first top_k tokens by (x down, index up) stay
+ *   top_p < 1:  of those, in that order, each stays whose predecessors' masses sum to less than
+ *               ceil(top_p * the sum of all of them) (at least the first)
+ *   min_p > 0:  of those, each with mass >= ceil(min_p * 2^45) stays
+ *   the token: the first by index whose masses up to it exceed floor(uniform * their sum)
+ * temperature 0: the lowest index of the maximum.  Settings by row (f32 / int32 [rows]), or the value after
+ * each pointer where it is NULL; values of rows that are out of range count as 0 (temperature), none (top_k, top_p)
+ * or the nearer end (min_p, uniform).  A NaN counts as -infinity, which is never drawn; infinities share the draw alone.  tokens int64
+ * [rows], -1 for a row with nothing to draw; logprobs f32 [rows] (or NULL): log of the token's part in what stayed
+ * (greedy 0, nothing to draw -infinity).  vocab at most 262144. */
+int lb_op_sample(const void* logits, int64_t row_stride, int dtype, int rows, int vocab, const void* uniform,
+                 int uniform64, const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
+                 const float* top_p, float top_p1, const float* min_p, float min_p1, int64_t* tokens,
+                 float* logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

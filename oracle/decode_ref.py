@@ -88,3 +88,46 @@ def w4_product(x, x_scale, codes, scales):
     if x_scale is not None:
         x = x * x_scale.double().repeat_interleave(k // x_scale.shape[1], 1)
     return x @ w.t(), x.abs() @ w.abs().t()
+
+
+def head_norm_rotary(x, weight, positions, frequencies, *, rotary, pairs, eps, norm=True):
+    """x [tokens, heads, dim] normed by head and rotated; frequencies: radians a position, as Python floats."""
+    y = x.double()
+    if norm:
+        y = y / torch.sqrt((y * y).mean(2, keepdim=True) + eps)
+        y = y if weight is None else y * weight.double()
+    angle = torch.tensor([[math.remainder(p * f, 2 * math.pi) for f in frequencies] for p in positions.tolist()],
+                         dtype=torch.float64, device=x.device).view(-1, 1, rotary // 2)
+    a, b = (y[..., : rotary // 2], y[..., rotary // 2:rotary]) if pairs == "halves" else (y[..., 0:rotary:2], y[..., 1:rotary:2])
+    turned = a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()
+    turned = torch.cat(turned, 2) if pairs == "halves" else torch.stack(turned, 3).flatten(2)
+    return torch.cat([turned, y[..., rotary:]], 2)
+
+
+def sample(logits, u, *, temperature, top_k=0, top_p=1.0, min_p=0.0):
+    """(token, logprob) of one row of logits, over Python numbers."""
+    x = [v if v == v else -math.inf for v in logits.double().tolist()]
+    order = sorted((i for i in range(len(x)) if x[i] > -math.inf), key=lambda i: (-x[i], i))
+    if not order:
+        return -1, -math.inf
+    if temperature == 0.0:
+        return order[0], 0.0
+    top = x[order[0]]
+    mass = {i: 1 << 45 if x[i] == top else round(2.0 ** 45 * math.exp((x[i] - top) / temperature)) for i in order}
+    if top_k > 0:
+        order = order[:top_k]
+    if top_p < 1.0:
+        limit, before, kept = max(1, math.ceil(top_p * float(sum(mass[i] for i in order)))), 0, []
+        for i in order:
+            if before >= limit:
+                break
+            kept.append(i)
+            before += mass[i]
+        order = kept
+    order = sorted(i for i in order if mass[i] >= math.ceil(min_p * 2.0 ** 45) and mass[i] > 0)
+    total = sum(mass[i] for i in order)
+    target, upto = min(total - 1, math.floor(u * float(total))), 0
+    for i in order:
+        upto += mass[i]
+        if upto > target:
+            return i, math.log(mass[i] / total)

@@ -1,0 +1,54 @@
+"""The entries between a block's products and at its end refuse bad arguments before they touch a GPU."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+P = 1 << 20  # a 16-byte aligned address that no call reads
+
+
+@pytest.fixture(scope="module")
+def lib(pkg):
+    from gemma4_omni_b200 import _lib, build
+    build.build_library()
+    return _lib.load()
+
+
+@pytest.mark.parametrize("name,good,changes", [
+    ("lb_op_head_norm_rotary",
+     [P, 512, 64, 8, P, 128, 64, 2, 1, 1, 64, P, 0, P, 64, 0, P, P, 0, 1, 1e-6, P, 512, 64, P, 128, 64, None],
+     [(0, None), (3, 0), (4, None), (7, -1), (8, 2), (9, 0), (10, 0), (10, 63), (10, 1026), (11, None), (13, None), (14, 66), (14, 31),
+      (18, 2), (20, -1.0), (20, math.nan), (21, None), (24, None)]),
+    ("lb_op_sample", [P, 100, 1, 2, 100, P, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None, None],
+     [(0, None), (1, 99), (2, 2), (2, 7), (3, 0), (4, 0), (5, None), (8, -1.0), (8, math.nan), (8, math.inf), (12, -0.5), (12, math.nan),
+      (14, -0.1), (14, 1.5), (14, math.nan), (15, None)]),
+])
+def test_refusals(lib, name, good, changes):
+    for at, value in changes:
+        args = list(good)
+        args[at] = value
+        assert getattr(lib, name)(*args) == -1, (at, value)
+
+
+def test_capacity(lib):
+    assert lib.lb_op_sample(P, 300000, 1, 2, 262145, P, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None, None) == -4
+
+
+def test_turns_are_the_frequencies(pkg):
+    """base ** (-2 i / dim) radians as 64-bit fractions of a turn, to 2^-52 of a radian as doubles have them."""
+    from gemma4_omni_b200 import decode_ops as ops
+    for dim, base in ((64, 10000.0), (256, 1000000.0), (2, 10.0)):
+        turns = ops._turns(dim, base)
+        assert len(turns) == dim // 2
+        for i, t in enumerate(turns):
+            assert abs(t / 2.0 ** 64 * 2 * math.pi - base ** (-2.0 * i / dim)) <= 2.0 ** -51
+
+
+def test_wrappers_have_no_cpu_path(pkg):
+    import torch
+    from gemma4_omni_b200 import decode_ops as ops
+    with pytest.raises(ValueError):
+        ops.Rotary.create(64, device="cpu")
+    with pytest.raises(ValueError):
+        ops.sample_tokens(torch.zeros(2, 64), torch.zeros(2))
