@@ -132,6 +132,7 @@ SIGNATURES: dict[str, tuple] = {
     "lb_kv8_attention_workspace": (I64, [I, I, I, I]),
     "lb_op_rms_norm8": (I, [P, I64, P, I64, I, P, I, I, I, F, I, I, P, P, P, P]),
     "lb_op_head_norm_rotary": (I, [P, I64, I64, I, P, I64, I64, I, I, I, I, P, I, P, I, I, P, P, I, I, F, P, I64, I64, P, I64, I64, P]),
+    "lb_op_w4_gated": (I, [P, I64, I, P, I, I, P, P, I, I, I, I, P, I64, I, P, P]),
     "lb_op_sample": (I, [P, I64, I, I, I, P, I, P, F, P, I, P, F, P, F, P, P, P]),
     "lb_op_w4_matvec": (I, [P, I64, I, P, I, I, P, P, I, I, I, P, I64, I, P]),
 }

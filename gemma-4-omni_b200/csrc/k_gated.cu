@@ -1,0 +1,682 @@
+// The first half of a gated feed-forward block with 4-bit weights, in one kernel:
+//   out[t][o] = act(g) * u,  g = sum_k x[t][k] W[o][k],  u = sum_k x[t][k] W[f + o][k],  W = (n - 8) * s[row][k / group]
+//
+// Both products run on tcgen05 from one token to thousands, with the outputs as the rows of the MMA (128 gate rows and
+// the 128 up rows that belong to them) and the tokens as its columns.  The weights are never rounded: the
+// MMAs take the whole numbers n - 8, exact in each operand type (bf16 or fp16 for x of that type, e4m3 and int8 for 8-bit x, which
+// goes to the tensor cores as it lies), and the sum of each group leaves the tensor memory and takes its scale in 32
+// bits, where an output's lane makes the scale a register.
+//
+// Widened codes never see shared memory: a warpgroup reads the codes that TMA brought, widens them in registers
+// (x 128 k: some 12 instructions for 8 codes, 5 to int8) and stores them to the tensor memory, from where the MMAs take them
+// as their A operand.  Shared memory then only has to feed x to the MMAs.
+//
+// Warpgroups: 0 loads (warp 0: TMA; warp 2: x's scales of a group) and issues the MMAs (warp 1); 1 widens; 2 and 3 add up, half
+// of the tokens each, and finish the tile.  A unit is one side's (gate or up) product over one group: while the one
+// side's sums are taken out of the tensor memory the other side's MMAs run.
+//
+// Few tokens: the tiles of outputs are fewer than the SMs, so K is dealt out to the CTAs of a cluster, whose partial
+// sums meet in shared memory (read over the cluster, in the order of the CTAs).
+#include "../../include/listener_b200.h"
+#include "common.cuh"
+#include "kernels.h"
+
+namespace lb {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kBlockO = 128;                   // outputs of a tile
+constexpr int kBlockK = 128;                   // k of a stage
+constexpr int kSideBytes = kBlockO * kBlockK / 2;
+constexpr int kCodeBytes = 2 * kSideBytes;     // gate and up
+constexpr int kABuffers = 4, kAColumn = 256, kAWidth = 64;  // widened codes in the tensor memory
+constexpr int kScaleRing = 4;
+constexpr int kMaxSplit = 8;
+constexpr int kSms = 148;
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum XKind { kXBf16, kXF16, kXE4m3, kXI8 };
+
+struct GatedArgs {
+  const float* x_scale;       // or null
+  const __half* w_scale;      // [2 f][k / group]
+  void* out;
+  long long ld_out;
+  int* status;
+  int x_group, m, f, k, group, out_dtype, gelu;
+  int o_tiles, t_tiles, k_blocks;  // blocks of kBlockK
+};
+
+template <int X, int NT>
+struct Shape {
+  static constexpr bool kWide = X == kXBf16 || X == kXF16;    // 16-bit operands
+  static constexpr int kXBytes = NT * kBlockK * (kWide ? 2 : 1);
+  static constexpr int kStage = kCodeBytes + kXBytes;
+  static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
+  static constexpr int kPartial = 2 * NT * kBlockO * 4;       // a CTA's sums, in the stages' place
+  static constexpr int kSmem = kStages * kStage + 1024;
+  static_assert(kPartial <= kStages * kStage, "room");
+  static constexpr int kD = NT == 128 ? 2 : 4;                // accumulators in the tensor memory
+  static constexpr int kCols = NT / 2;                        // tokens of an adding warpgroup
+  static constexpr int kSteps = kWide ? 16 : 32;              // k of an MMA
+  static_assert(kD * NT <= kAColumn, "tensor memory");
+};
+
+// D(tmem) (+)= A(tmem) * B(smem)^T
+template <int X>
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+#define LB_TS(kind)                                                     \
+  asm volatile(                                                         \
+      "{\n\t.reg .pred p;\n\t"                                          \
+      "setp.ne.b32 p, %4, 0;\n\t"                                       \
+      "tcgen05.mma.cta_group::1.kind::" kind " [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) \
+      : "memory")
+  if constexpr (X == kXBf16 || X == kXF16) LB_TS("f16");
+  else if constexpr (X == kXE4m3) LB_TS("f8f6f4");
+  else LB_TS("i8");
+#undef LB_TS
+}
+template <int X>
+__host__ __device__ constexpr uint32_t idesc_of(int m, int n) {
+  const uint32_t shape = static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
+  return X == kXBf16 ? shape | 1u << 4 | 1u << 7 | 1u << 10   // f32 sums, bf16
+         : X == kXI8 ? shape | 2u << 4 | 1u << 7 | 1u << 10   // s32 sums, s8
+                     : shape | 1u << 4;                        // f32 sums; format 0: f16, e4m3
+}
+
+// 32 lanes x 32 columns, a lane's 32 values from its registers
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 16 columns and their wait in one statement
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at)
+      : "memory");
+}
+
+// Waits for a phase, with a limit of some 2.6 s (try_wait sleeps for up to the 20 us that it is given).
+constexpr int kPolls = 1 << 17;
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_u32(bar);
+#pragma unroll 1
+  for (int n = 0; n < kPolls; ++n) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(at), "r"(parity), "r"(20000u)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_one(bar, parity));
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float peer_load(uint32_t at, uint32_t rank) {
+  float v;
+  uint32_t peer;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer) : "memory");
+  return v;
+}
+
+template <typename H>
+__device__ __forceinline__ uint32_t bits_of(H v) { return *reinterpret_cast<const uint32_t*>(&v); }
+
+// 8 codes n (lowest bits first) as n - 8 in the operand's type and in their order.
+// bf16, fp16: two codes under the exponent of 128 or 1024, where they count in ones, less 136 or 1032 (fp16: the odd
+// codes as they lie, in sixteens, come down by the product).
+__device__ __forceinline__ void widen(uint32_t w, uint32_t* r, std::integral_constant<int, kXBf16>) {
+  const __nv_bfloat162 bias = __floats2bfloat162_rn(136.0f, 136.0f);
+  const uint32_t odd = w >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = (__byte_perm(w, odd, 0x0400 + 0x0101 * i) & 0x000f000fu) | 0x43004300u;
+    r[i] = bits_of(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair), bias));
+  }
+}
+__device__ __forceinline__ void widen(uint32_t w, uint32_t* r, std::integral_constant<int, kXF16>) {
+  const __half2 factor = __floats2half2_rn(1.0f, 0.0625f), bias = __floats2half2_rn(-1032.0f, -72.0f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = (__byte_perm(w, 0, 0x0101 * i) & 0x00f0000fu) | 0x64006400u;
+    r[i] = bits_of(__hfma2(*reinterpret_cast<const __half2*>(&pair), factor, bias));
+  }
+}
+// e4m3: below 16 the bits count in steps of 2^-9 (a sign and four bits), so a code becomes the sign and the size of n - 8
+// and the scale 2^9 larger.  A byte permute looks a code's lower three bits up in a table of eight, and where the fourth
+// is set gives the looked-up byte's sign instead: 0 in these tables.
+__device__ __forceinline__ uint32_t look_up(uint32_t low, uint32_t high, uint32_t w) {  // (__byte_perm has no sign mode)
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(low), "r"(high), "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t signed4(uint32_t w) {
+  const uint32_t below = look_up(0x05060708u, 0x01020304u, w);            // n < 8: 8 - n
+  const uint32_t above = look_up(0x03020100u, 0x07060504u, w ^ 0x8888u);  // n >= 8: n - 8
+  const uint32_t sign = look_up(0x7f7f7f7fu, 0x7f7f7f7fu, w);             // n < 8: 0x7f
+  return below | above | ((sign << 1) & 0x80808080u);
+}
+__device__ __forceinline__ void widen(uint32_t w, uint32_t* r, std::integral_constant<int, kXE4m3>) {
+  r[0] = signed4(w);
+  r[1] = signed4(w >> 16);
+}
+// int8: 16 (n - 8), a code with its top bit turned as the byte's upper half
+__device__ __forceinline__ void widen(uint32_t w, uint32_t* r, std::integral_constant<int, kXI8>) {
+  const uint32_t odd = (w & 0xf0f0f0f0u) ^ 0x80808080u, even = ((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+  r[0] = __byte_perm(even, odd, 0x5140);
+  r[1] = __byte_perm(even, odd, 0x7362);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// g / (1 + exp(-z)): silu with z = g, gelu's tanh form with z = 2 sqrt(2 / pi) (g + 0.044715 g^3), as
+// (1 + tanh(a)) / 2 = 1 / (1 + exp(-2 a)).  The exponent's rounding comes back by its remainder, so that the result is good
+// to some 2^-21 of itself for any g.
+__device__ __forceinline__ float activated(float g, bool gelu) {
+  float z = g;
+  if (gelu) z = 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
+  const float y = -kLog2e * z, rest = fmaf(-kLog2e, z, -y) - z * 1.925963033500e-8f;  // log2(e) = kLog2e + 1.926e-8
+  const float e = exp2_fast(y);
+  return g * rcp_fast(1.0f + (fabsf(y) < 126.0f ? fmaf(e, rest * 0.6931471805599453f, e) : e));
+}
+
+template <int X, int NT>
+__global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, const __grid_constant__ CUtensorMap w_map,
+                                                            const __grid_constant__ CUtensorMap x_map) {
+  using S = Shape<X, NT>;
+  extern __shared__ unsigned char gated_raw[];
+  unsigned char* smem = gated_raw + ((1024 - (smem_u32(gated_raw) & 1023)) & 1023);
+  unsigned char* x_stages = smem;                             // [stage][half of k][token][128 bytes], swizzled
+  unsigned char* c_stages = smem + S::kStages * S::kXBytes;   // [stage][side][row][64 bytes], swizzled
+  __shared__ uint64_t c_full[S::kStages], c_empty[S::kStages], x_full[S::kStages], x_empty[S::kStages];
+  __shared__ uint64_t a_full[kABuffers], a_empty[kABuffers], d_full[S::kD], d_empty[S::kD];
+  __shared__ uint64_t s_full[kScaleRing], s_empty[kScaleRing];
+  __shared__ __align__(16) float xs_s[kScaleRing][NT];
+  __shared__ uint32_t tmem_slot;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t splits;
+  asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(splits));
+  const int split = static_cast<int>(cluster_rank());
+  if (tid == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&c_full[i], 1);
+      mbar_init(&c_empty[i], 4);
+      mbar_init(&x_full[i], 1);
+      mbar_init(&x_empty[i], 1);
+    }
+    for (int i = 0; i < kABuffers; ++i) {
+      mbar_init(&a_full[i], 4);
+      mbar_init(&a_empty[i], 1);
+    }
+    for (int i = 0; i < S::kD; ++i) {
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 8);
+    }
+    for (int i = 0; i < kScaleRing; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 8);
+    }
+    fence_barrier_init();
+    tma_prefetch_desc(&w_map);
+    tma_prefetch_desc(&x_map);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  // this CTA's blocks of K and its tiles (one, where K is dealt out)
+  const int kb0 = a.k_blocks * split / static_cast<int>(splits), kb1 = a.k_blocks * (split + 1) / static_cast<int>(splits);
+  const int first = blockIdx.x / splits, step = gridDim.x / splits, tiles = a.o_tiles * a.t_tiles;
+  const int subs = kBlockK / a.group;  // groups of a block
+  const bool grouped = a.x_group != 0;
+  bool ok = true;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 0 && lane == 0) {
+      // ---------------- loads
+      int st = 0;
+      uint32_t ph = 0;
+      int held = 0;  // stages that were requested
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        const int o0 = tile % a.o_tiles * kBlockO, t0 = tile / a.o_tiles * NT;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = wait_one(&c_empty[st], ph ^ 1);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&c_full[st], kCodeBytes);
+          unsigned char* c = c_stages + st * kCodeBytes;
+          asm volatile(
+              "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(c)),
+              "l"(reinterpret_cast<uint64_t>(&w_map)), "r"(smem_u32(&c_full[st])), "r"(kb * (kBlockK / 2)), "r"(o0)
+              : "memory");
+          asm volatile(
+              "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+                  smem_u32(c + kSideBytes)),
+              "l"(reinterpret_cast<uint64_t>(&w_map)), "r"(smem_u32(&c_full[st])), "r"(kb * (kBlockK / 2)), "r"(a.f + o0)
+              : "memory");
+          ok = wait_one(&x_empty[st], ph ^ 1);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&x_full[st], S::kXBytes);
+          unsigned char* x = x_stages + st * S::kXBytes;
+#pragma unroll
+          for (int h = 0; h < (S::kWide ? 2 : 1); ++h)
+            asm volatile(
+                "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+                    smem_u32(x + h * NT * 128)),
+                "l"(reinterpret_cast<uint64_t>(&x_map)), "r"(smem_u32(&x_full[st])), "r"(kb * kBlockK + 64 * h), "r"(t0)
+                : "memory");
+          ++held;
+          if (++st == S::kStages) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      if (!ok) {  // the copies in flight, before the CTA may end: every stage's last request
+        for (int i = 0; i < S::kStages && i < held; ++i) {
+          st = st == 0 ? S::kStages - 1 : st - 1;
+          if (st == S::kStages - 1) ph ^= 1;
+          wait_one(&c_full[st], ph);
+          wait_one(&x_full[st], ph);
+        }
+      }
+    } else if (warp == 1 && lane == 0) {
+      // ---------------- MMAs
+      int st = 0, ab = 0, db = 0;
+      uint32_t ph = 0, aph = 0, dph = 0;
+      constexpr uint32_t idesc = idesc_of<X>(kBlockO, NT);
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          ok = wait_one(&x_full[st], ph);
+          const uint32_t x = smem_u32(x_stages + st * S::kXBytes);
+          for (int side = 0; side < 2 && ok; ++side) {
+            ok = wait_one(&a_full[ab], aph);
+            const uint32_t wide = tmem + kAColumn + ab * kAWidth;
+            for (int sub = 0; sub < subs && ok; ++sub) {
+              ok = wait_one(&d_empty[db], dph ^ 1);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t d = tmem + db * NT;
+              const int per = a.group / S::kSteps;  // MMAs of the group
+#pragma unroll 1
+              for (int i = 0; i < per; ++i) {
+                const int j = sub * per + i;  // of the block: 32 bytes of a row of x, 8 columns of the codes
+                const uint32_t at = S::kWide ? x + (j >> 2) * (NT * 128) + (j & 3) * 32 : x + j * 32;
+                umma_ts<X>(d, wide + j * 8, smem_desc_k128(at), idesc, i > 0);
+              }
+              umma_commit(&d_full[db]);
+              if (++db == S::kD) {
+                db = 0;
+                dph ^= 1;
+              }
+            }
+            if (!ok) break;
+            umma_commit(&a_empty[ab]);
+            if (++ab == kABuffers) {
+              ab = 0;
+              aph ^= 1;
+            }
+          }
+          if (!ok) break;
+          umma_commit(&x_empty[st]);
+          if (++st == S::kStages) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    } else if (warp == 2 && grouped) {
+      // ---------------- x's scales of a block's group
+      int ring = 0;
+      uint32_t ph = 0;
+      const int groups = a.k / a.x_group;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        const int t0 = tile / a.o_tiles * NT;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          float v[NT / 32];
+          const int g = kb * kBlockK / a.x_group;
+#pragma unroll
+          for (int i = 0; i < NT / 32; ++i) {
+            const int t = t0 + 32 * i + lane;
+            v[i] = t < a.m ? a.x_scale[static_cast<long long>(t) * groups + g] : 0.0f;
+          }
+          ok = wait_warp(&s_empty[ring], ph ^ 1);
+          if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < NT / 32; ++i) xs_s[ring][32 * i + lane] = v[i];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_full[ring]);
+          if (++ring == kScaleRing) {
+            ring = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    // ---------------- codes -> operands
+    int st = 0, ab = 0;
+    uint32_t ph = 0, aph = 0;
+    const int row = 32 * (warp & 3) + lane;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes, in the address's upper half
+    for (int tile = first; tile < tiles && ok; tile += step) {
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        ok = wait_warp(&c_full[st], ph);
+        const unsigned char* c = c_stages + st * kCodeBytes + row * 64;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+          uint4 raw[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4*>(c + side * kSideBytes + ((i ^ ((row >> 1) & 3)) << 4));
+          if (side == 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c_empty[st]);
+          }
+          ok = ok && wait_warp(&a_empty[ab], aph ^ 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t wide = tmem + lanes + kAColumn + ab * kAWidth;
+          using Kind = std::integral_constant<int, X>;
+          if constexpr (S::kWide) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t r[32];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                widen(raw[2 * h + i].x, r + 16 * i, Kind{});
+                widen(raw[2 * h + i].y, r + 16 * i + 4, Kind{});
+                widen(raw[2 * h + i].z, r + 16 * i + 8, Kind{});
+                widen(raw[2 * h + i].w, r + 16 * i + 12, Kind{});
+              }
+              tmem_st32(wide + 32 * h, r);
+            }
+          } else {
+            uint32_t r[32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              widen(raw[i].x, r + 8 * i, Kind{});
+              widen(raw[i].y, r + 8 * i + 2, Kind{});
+              widen(raw[i].z, r + 8 * i + 4, Kind{});
+              widen(raw[i].w, r + 8 * i + 6, Kind{});
+            }
+            tmem_st32(wide, r);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&a_full[ab]);
+          if (++ab == kABuffers) {
+            ab = 0;
+            aph ^= 1;
+          }
+        }
+        if (++st == S::kStages) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---------------- sums and results
+    const int half = (warp - 8) >> 2, row = 32 * (warp & 3) + lane;
+    const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * S::kCols;
+    const int groups = a.k / a.group;
+    int db = 0, ring = 0;
+    uint32_t dph = 0, rph = 0;
+    constexpr float kUnit = X == kXE4m3 ? 512.0f : X == kXI8 ? 0.0625f : 1.0f;  // of the widened codes
+    for (int tile = first; tile < tiles && ok; tile += step) {
+      const int o = tile % a.o_tiles * kBlockO + row, t0 = tile / a.o_tiles * NT + half * S::kCols;
+      const bool there = o < a.f;
+      const __half* scale[2] = {a.w_scale + static_cast<long long>(there ? o : 0) * groups,
+                                a.w_scale + static_cast<long long>(there ? a.f + o : 0) * groups};
+      float acc[2][S::kCols];
+#pragma unroll
+      for (int j = 0; j < S::kCols; ++j) acc[0][j] = acc[1][j] = 0.0f;
+      // a block's scales (up to four halves a side), one block ahead
+      const auto scales_of = [&](int side, int kb) {
+        uint2 v = make_uint2(0, 0);
+        uint16_t h[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < subs && there && kb < kb1 && kb * subs + i < groups) h[i] = __half_as_ushort(scale[side][kb * subs + i]);
+        v.x = h[0] | static_cast<uint32_t>(h[1]) << 16;
+        v.y = h[2] | static_cast<uint32_t>(h[3]) << 16;
+        return v;
+      };
+      uint2 next[2] = {scales_of(0, kb0), scales_of(1, kb0)};
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        uint2 now[2] = {next[0], next[1]};
+#pragma unroll
+        for (int side = 0; side < 2; ++side) next[side] = scales_of(side, kb + 1);
+        if (grouped) ok = wait_warp(&s_full[ring], rph);
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+#pragma unroll 1
+          for (int sub = 0; sub < subs; ++sub) {
+            const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(now[side].x))) * kUnit;
+            now[side].x = now[side].x >> 16 | now[side].y << 16;
+            now[side].y >>= 16;
+            ok = ok && wait_warp(&d_full[db], dph);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int j0 = 0; j0 < S::kCols; j0 += 16) {
+              uint32_t d[16];
+              tmem_ld16(from + db * NT + j0, d);
+              if (j0 + 16 == S::kCols) {  // the sums are in registers
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_empty[db]);
+              }
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                float v = __uint_as_float(d[j]);
+                if constexpr (X == kXI8) v = __uint_as_float(0x4b400000u + d[j]) - 12582912.0f;  // below 2^22
+                if constexpr (!S::kWide) {
+                  if (grouped) v *= xs_s[ring][half * S::kCols + j0 + j];
+                }
+                acc[side][j0 + j] = fmaf(v, s, acc[side][j0 + j]);
+              }
+            }
+            if (++db == S::kD) {
+              db = 0;
+              dph ^= 1;
+            }
+          }
+        }
+        if (grouped) {
+          __syncwarp();
+          if (lane == 0 && ok) mbar_arrive(&s_empty[ring]);
+          if (++ring == kScaleRing) {
+            ring = 0;
+            rph ^= 1;
+          }
+        }
+      }
+      if (!ok) break;
+      const auto finish = [&](int t, float g, float u) {
+        if (!there || t >= a.m) return;
+        if (!S::kWide && !grouped) {
+          const float xs = a.x_scale[t];
+          g *= xs;
+          u *= xs;
+        }
+        const float v = activated(g, a.gelu) * u;
+        const long long at = t * a.ld_out + o;
+        if (a.out_dtype == LB_F32) static_cast<float*>(a.out)[at] = v;
+        else if (a.out_dtype == LB_BF16) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+        else static_cast<__half*>(a.out)[at] = __float2half_rn(v);
+      };
+      if (splits == 1) {
+#pragma unroll
+        for (int j = 0; j < S::kCols; ++j) finish(t0 + j, acc[0][j], acc[1][j]);
+      } else {
+        // every stage was read (this CTA's last sums have come), so the partial sums may take their place
+        float* mine = reinterpret_cast<float*>(smem) + row;
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+          for (int j = 0; j < S::kCols; ++j) mine[(side * NT + half * S::kCols + j) * kBlockO] = acc[side][j];
+      }
+    }
+  }
+  if (!ok && a.status) atomicOr(a.status, static_cast<int>(kStatusWaitTimeout));
+  __syncwarp();
+  if (splits > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 8) {  // a CTA finishes every splits-th token
+      const int row = 32 * (warp & 3) + lane, o = first % a.o_tiles * kBlockO + row, t0 = first / a.o_tiles * NT;
+      const uint32_t at = smem_u32(smem) + row * 4;
+      for (int j = split + static_cast<int>(splits) * ((warp - 8) >> 2); j < NT && t0 + j < a.m; j += 2 * static_cast<int>(splits)) {
+        float g = 0.0f, u = 0.0f;
+        for (uint32_t r = 0; r < splits; ++r) {
+          g += peer_load(at + j * kBlockO * 4, r);
+          u += peer_load(at + (NT + j) * kBlockO * 4, r);
+        }
+        if (o < a.f) {
+          const int t = t0 + j;
+          if (!S::kWide && !grouped) {
+            g *= a.x_scale[t];
+            u *= a.x_scale[t];
+          }
+          const float v = activated(g, a.gelu) * u;
+          const long long to = t * a.ld_out + o;
+          if (a.out_dtype == LB_F32) static_cast<float*>(a.out)[to] = v;
+          else if (a.out_dtype == LB_BF16) static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(v);
+          else static_cast<__half*>(a.out)[to] = __float2half_rn(v);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int X, int NT>
+cudaError_t launch(const GatedArgs& a, int splits, const CUtensorMap& w_map, const CUtensorMap& x_map, cudaStream_t s) {
+  using S = Shape<X, NT>;
+  const auto kernel = gated_kernel<X, NT>;
+  static std::atomic<unsigned long long> done{0};
+  static std::atomic<int> registers{0};
+  cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), S::kSmem);
+  if (e != cudaSuccess) return e;
+  if (registers.load(std::memory_order_relaxed) == 0) {
+    // the warpgroups' shares of the registers add up to 128 a thread: what the block has to be launched with
+    cudaFuncAttributes f;
+    if ((e = cudaFuncGetAttributes(&f, reinterpret_cast<const void*>(kernel))) != cudaSuccess) return e;
+    registers.store(f.numRegs, std::memory_order_relaxed);
+  }
+  if (registers.load(std::memory_order_relaxed) != 128) return cudaErrorInvalidConfiguration;
+  const int tiles = a.o_tiles * a.t_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = static_cast<unsigned>(splits > 1 ? tiles * splits : tiles < kSms ? tiles : kSms);
+  cfg.blockDim = kThreads;
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(splits), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, a, w_map, x_map);
+  return e == cudaSuccess ? cudaGetLastError() : e;
+}
+template <int X>
+cudaError_t launch(const GatedArgs& a, int nt, int splits, const CUtensorMap& w_map, const CUtensorMap& x_map, cudaStream_t s) {
+  if (nt == 32) return launch<X, 32>(a, splits, w_map, x_map, s);
+  if (nt == 64) return launch<X, 64>(a, splits, w_map, x_map, s);
+  return launch<X, 128>(a, splits, w_map, x_map, s);
+}
+
+}  // namespace
+}  // namespace lb
+
+extern "C" int lb_op_w4_gated(const void* x, int64_t x_ld, int x_dtype, const float* x_scale, int x_group, int m,
+                              const void* codes, const void* w_scale, int group, int ffn, int k, int activation, void* out,
+                              int64_t ld_out, int out_dtype, int32_t* status, void* stream) {
+  using namespace lb;
+  if (!x || !codes || !w_scale || !out || m < 1 || ffn < 1 || k < 1 || x_ld < k || ld_out < ffn || activation < 0 || activation > 1)
+    return LB_ERR_INVALID_ARGUMENT;
+  if ((group != 32 && group != 64 && group != 128) || k % group != 0) return LB_ERR_INVALID_ARGUMENT;
+  const bool eight = x_dtype == LB_E4M3 || x_dtype == LB_I8;
+  if ((!eight && x_dtype != LB_BF16 && x_dtype != LB_F16) || eight != (x_scale != nullptr)) return LB_ERR_INVALID_ARGUMENT;
+  if (x_group < 0 || (x_group && (!eight || x_group % 128 != 0 || k % x_group != 0))) return LB_ERR_INVALID_ARGUMENT;
+  if (out_dtype != LB_F32 && out_dtype != LB_BF16 && out_dtype != LB_F16) return LB_ERR_INVALID_ARGUMENT;
+  const int64_t size = eight ? 1 : 2;
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(x) % 16 != 0 || (m > 1 && x_ld * size % 16 != 0))
+    return LB_ERR_INVALID_ARGUMENT;
+  if (ffn > (1 << 24) || m > (1 << 24) || x_ld > (1ll << 36)) return LB_ERR_CAPACITY;
+  GatedArgs a{x_scale, static_cast<const __half*>(w_scale), out, ld_out, status, x_group == k ? 0 : x_group, m, ffn, k, group, out_dtype,
+              activation, 0, 0, 0};
+  const int nt = m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  a.o_tiles = (ffn + kBlockO - 1) / kBlockO;
+  a.t_tiles = (m + nt - 1) / nt;
+  a.k_blocks = (k + kBlockK - 1) / kBlockK;
+  const long long tiles = static_cast<long long>(a.o_tiles) * a.t_tiles;
+  if (tiles > 0x3fffffffll) return LB_ERR_CAPACITY;
+  int splits = static_cast<int>(tiles >= kSms ? 1 : kSms / tiles);
+  if (splits > kMaxSplit) splits = kMaxSplit;
+  if (splits > a.k_blocks) splits = a.k_blocks;
+  CUtensorMap w_map, x_map;
+  const int64_t x_row = m > 1 ? x_ld * size : (static_cast<int64_t>(k) * size + 15) / 16 * 16;
+  if (make_tensor_map_u8(&w_map, codes, k / 2, 2ull * ffn, 64, kBlockO) != 0 ||
+      make_tensor_map_2d(&x_map, x, static_cast<int>(size), k, m, x_row, eight ? 128 : 64, nt, true, x_dtype == LB_F16) != 0)
+    return LB_ERR_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (x_dtype == LB_BF16) e = launch<kXBf16>(a, nt, splits, w_map, x_map, s);
+  else if (x_dtype == LB_F16) e = launch<kXF16>(a, nt, splits, w_map, x_map, s);
+  else if (x_dtype == LB_E4M3) e = launch<kXE4m3>(a, nt, splits, w_map, x_map, s);
+  else e = launch<kXI8>(a, nt, splits, w_map, x_map, s);
+  return e == cudaSuccess ? LB_OK : LB_ERR_CUDA;
+}

@@ -14,6 +14,7 @@ Here the caches of all sessions share one pool of pages:
 - ``rms_norm8``: residual addition + RMS norm with an 8-bit output and scales.
 - ``Int4Weight`` / ``w4_matvec``: products with 4-bit weights and group scales.
 - ``Rotary`` / ``head_norm_rotary``: norms of queries and keys for each head, with the position rotation.
+- ``w4_gated``: both projections of a gated feed-forward block, the activation and the product.
 - ``sample_tokens``: the next tokens from logits and given random numbers.
 
 Every call is enqueued on torch's current stream of the tensors' device and can be
@@ -364,6 +365,7 @@ class Int4Weight:
 
     codes = _exchangeable("codes", torch.uint8, lambda w: (w.out_features, w.k // 2), 16)
     scales = _exchangeable("scales", torch.float16, lambda w: (w.out_features, w.k // w.group))
+    status_word = _exchangeable("status_word", torch.int32, lambda w: (1,))
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         self.device = _cuda(codes.device, "Int4Weight")
@@ -374,6 +376,11 @@ class Int4Weight:
         if self.group not in (32, 64, 128) or self.group * int(scales.shape[1]) != self.k:
             raise ValueError("groups must have 32, 64 or 128 columns")
         self.codes, self.scales = codes, scales
+        self.status_word = torch.zeros(1, dtype=torch.int32, device=self.device)
+
+    def status(self) -> int:
+        """LB_DEV_* bits of the gated products so far (synchronises)."""
+        return int(self.status_word.item())
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, group: int = 128) -> "Int4Weight":
@@ -393,13 +400,8 @@ class Int4Weight:
         return ((both.float() - 8.0) * self.scales.float()[:, :, None]).view(self.out_features, self.k)
 
 
-def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | None = None,
-              out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """x [rows, k] times the transposed weight -> [rows, out].
-
-    x is bfloat16 / float16, or float8_e4m3fn / int8 codes with ``x_scale`` f32
-    [rows, groups] as ``rms_norm8`` returns them (one group a row, or groups of a
-    multiple of 128 columns).  ``out_dtype`` defaults to x's type, bfloat16 for 8-bit x."""
+def _product_input(x: torch.Tensor, weight: Int4Weight, x_scale: torch.Tensor | None) -> tuple[int, int, int]:
+    """(rows, columns of a group of x_scale or 0, elements between rows) of a product's x."""
     dev = weight.device
     if x.dim() != 2 or x.shape[1] != weight.k or x.device != dev:
         raise ValueError(f"x must be [rows, {weight.k}] on {dev}")
@@ -417,6 +419,18 @@ def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | No
             raise ValueError("groups of x must have a multiple of 128 columns")
     elif x.dtype not in (torch.bfloat16, torch.float16) or x_scale is not None:
         raise ValueError("x must be bfloat16 or float16 without x_scale, or float8_e4m3fn / int8 with it")
+    return rows, group, x_step
+
+
+def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | None = None,
+              out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x [rows, k] times the transposed weight -> [rows, out].
+
+    x is bfloat16 / float16, or float8_e4m3fn / int8 codes with ``x_scale`` f32
+    [rows, groups] as ``rms_norm8`` returns them (one group a row, or groups of a
+    multiple of 128 columns).  ``out_dtype`` defaults to x's type, bfloat16 for 8-bit x."""
+    dev = weight.device
+    rows, group, x_step = _product_input(x, weight, x_scale)
     if out is None:
         out_dtype = out_dtype or (x.dtype if x_scale is None else torch.bfloat16)
         if out_dtype not in FLOAT_INPUTS:
@@ -434,6 +448,45 @@ def w4_matvec(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | No
               None if x_scale is None else x_scale.data_ptr(), group, rows, weight._t_codes.data_ptr(),
               weight._t_scales.data_ptr(), weight.group, weight.out_features, weight.k, out.data_ptr(), out_step,
               DTYPE_CODES[out.dtype])
+    return out
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def w4_gated(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | None = None, activation: str = "silu",
+             out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The first half of a gated feed-forward block: act(x gate^T) * (x up^T) -> [rows, ffn], in one kernel.
+
+    ``weight`` [2 * ffn, k] has the gate's rows, then those of up.  x and ``x_scale`` as in ``w4_matvec``, from one row
+    to thousands; both products, the activation ("silu", or "gelu" in its tanh form) and the product are in 32
+    bits, rounded once.  ``out_dtype`` defaults to x's type, bfloat16 for 8-bit x."""
+    dev = weight.device
+    rows, group, x_step = _product_input(x, weight, x_scale)
+    if weight.out_features % 2:
+        raise ValueError("weight must have as many rows for the gate as for up")
+    ffn = weight.out_features // 2
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
+    if out is None:
+        out_dtype = out_dtype or (x.dtype if x_scale is None else torch.bfloat16)
+        if out_dtype not in FLOAT_INPUTS:
+            raise ValueError("out_dtype must be float32, bfloat16 or float16")
+        out = torch.empty((rows, ffn), dtype=out_dtype, device=dev)
+        out_step = ffn
+    else:
+        if out.dtype not in FLOAT_INPUTS or out.shape != (rows, ffn) or out.device != dev:
+            raise ValueError(f"out must be [{rows}, {ffn}] on {dev}")
+        out_step = _row_step(out)
+        if not out_step and rows:
+            raise ValueError("out's rows must be contiguous and apart")
+    if rows:
+        size = x.element_size()
+        if x.data_ptr() % 16 or (rows > 1 and x_step * size % 16):  # rows that TMA cannot address are laid out anew
+            x, x_step = x.new_empty(x.shape).copy_(x), weight.k
+        _call(dev, "lb_op_w4_gated", x.data_ptr(), x_step, DTYPE_CODES[x.dtype], None if x_scale is None else x_scale.data_ptr(),
+              group, rows, weight._t_codes.data_ptr(), weight._t_scales.data_ptr(), weight.group, ffn, weight.k,
+              ACTIVATIONS[activation], out.data_ptr(), out_step, DTYPE_CODES[out.dtype], weight._t_status_word.data_ptr())
     return out
 
 

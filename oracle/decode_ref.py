@@ -131,3 +131,14 @@ def sample(logits, u, *, temperature, top_k=0, top_p=1.0, min_p=0.0):
         upto += mass[i]
         if upto > target:
             return i, math.log(mass[i] / total)
+
+
+def gated(x, x_scale, codes, scales, *, activation):
+    """(out, bound on out's error for products off by e * sum |w||x| each, as a function of e)."""
+    y, reach = w4_product(x, x_scale, codes, scales)
+    g, u = y.chunk(2, 1)
+    dg, du = reach.chunk(2, 1)
+    z = g if activation == "silu" else 2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)
+    act = g * torch.sigmoid(z)
+    # neither activation is steeper than 1.13 anywhere, nor larger than its argument
+    return act * u, lambda e: e * (1.13 * dg * u.abs() + act.abs() * du + 1.13 * e * dg * du)

@@ -20,6 +20,9 @@ def lib(pkg):
      [P, 512, 64, 8, P, 128, 64, 2, 1, 1, 64, P, 0, P, 64, 0, P, P, 0, 1, 1e-6, P, 512, 64, P, 128, 64, None],
      [(0, None), (3, 0), (4, None), (7, -1), (8, 2), (9, 0), (10, 0), (10, 63), (10, 1026), (11, None), (13, None), (14, 66), (14, 31),
       (18, 2), (20, -1.0), (20, math.nan), (21, None), (24, None)]),
+    ("lb_op_w4_gated", [P, 256, 1, None, 0, 4, P, P, 64, 100, 256, 0, P, 100, 1, None, None],
+     [(0, None), (0, P + 2), (1, 255), (1, 257), (2, 0), (2, 4), (3, P), (4, 128), (5, 0), (6, None), (6, P + 8), (7, None), (8, 16), (8, 256),
+      (9, 0), (10, 0), (10, 100), (11, 2), (11, -1), (12, None), (13, 99), (14, 2), (14, 4)]),
     ("lb_op_sample", [P, 100, 1, 2, 100, P, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None, None],
      [(0, None), (1, 99), (2, 2), (2, 7), (3, 0), (4, 0), (5, None), (8, -1.0), (8, math.nan), (8, math.inf), (12, -0.5), (12, math.nan),
       (14, -0.1), (14, 1.5), (14, math.nan), (15, None)]),
