@@ -84,28 +84,36 @@ __host__ __device__ constexpr uint32_t idesc_of(int m, int n) {
                      : shape | 1u << 4;                        // f32 sums; format 0: f16, e4m3
 }
 
-// 32 lanes x 32 columns, a lane's 32 values from its registers
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
+// 32 lanes x 16 (or 8) columns, a lane's values from its registers
+__device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-      "r"(r[31])
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 16 columns and their wait in one statement
+// 16 columns; the registers hold them, and may be touched, after tmem_wait of the same array
 __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
         "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(at)
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 
 // Waits for a phase, with a limit of some 2.6 s (try_wait sleeps for up to the 20 us that it is given).
@@ -126,8 +134,37 @@ __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity) {
   }
   return false;
 }
+// the same by polls without sleep, for the one thread that the MMAs wait for
+__device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_u32(bar);
+#pragma unroll 1
+  for (int n = 0; n < (1 << 26); ++n) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(at), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, wait_one(bar, parity));
+}
+__device__ __forceinline__ bool wait_spin_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_spin(bar, parity));
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -142,6 +179,30 @@ __device__ __forceinline__ float peer_load(uint32_t at, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(rank));
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer) : "memory");
   return v;
+}
+
+// two 32-bit values an instruction
+typedef unsigned long long pair_t;
+__device__ __forceinline__ pair_t pair_of(float a, float b) {
+  pair_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void unpair(pair_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+  pair_t p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
+  return p;
+}
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+  pair_t p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+  return p;
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+  pair_t p;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+  return p;
 }
 
 template <typename H>
@@ -213,7 +274,23 @@ __device__ __forceinline__ float activated(float g, bool gelu) {
   return g * rcp_fast(1.0f + (fabsf(y) < 126.0f ? fmaf(e, rest * 0.6931471805599453f, e) : e));
 }
 
-template <int X, int NT>
+template <int X>
+__device__ __forceinline__ float result(const GatedArgs& a, bool grouped, int t, float g, float u, bool live) {
+  if constexpr (X == kXE4m3 || X == kXI8) {
+    if (!grouped) {
+      const float xs = live ? a.x_scale[t] : 0.0f;
+      g *= xs;
+      u *= xs;
+    }
+  }
+  return activated(g, a.gelu) * u;
+}
+__device__ __forceinline__ void store(unsigned char* at, float v, bool wide, bool bf16) {
+  if (wide) *reinterpret_cast<float*>(at) = v;
+  else *reinterpret_cast<uint16_t*>(at) = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+}
+
+template <int X, int NT, int SUBS>
 __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, const __grid_constant__ CUtensorMap w_map,
                                                             const __grid_constant__ CUtensorMap x_map) {
   using S = Shape<X, NT>;
@@ -227,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   __shared__ __align__(16) float xs_s[kScaleRing][NT];
   __shared__ uint32_t tmem_slot;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint32_t splits;
   asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(splits));
   const int split = static_cast<int>(cluster_rank());
@@ -266,7 +343,6 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   // this CTA's blocks of K and its tiles (one, where K is dealt out)
   const int kb0 = a.k_blocks * split / static_cast<int>(splits), kb1 = a.k_blocks * (split + 1) / static_cast<int>(splits);
   const int first = blockIdx.x / splits, step = gridDim.x / splits, tiles = a.o_tiles * a.t_tiles;
-  const int subs = kBlockK / a.group;  // groups of a block
   const bool grouped = a.x_group != 0;
   bool ok = true;
 
@@ -319,45 +395,52 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
           wait_one(&x_full[st], ph);
         }
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---------------- MMAs
       int st = 0, ab = 0, db = 0;
       uint32_t ph = 0, aph = 0, dph = 0;
       constexpr uint32_t idesc = idesc_of<X>(kBlockO, NT);
+      // the warp walks together and one lane issues: descriptors and barriers stay uniform
+      const bool leader = elect_one();
       for (int tile = first; tile < tiles && ok; tile += step) {
         for (int kb = kb0; kb < kb1 && ok; ++kb) {
-          ok = wait_one(&x_full[st], ph);
-          const uint32_t x = smem_u32(x_stages + st * S::kXBytes);
+          ok = wait_spin_warp(&x_full[st], ph);
+          const uint64_t x = smem_desc_k128(smem_u32(x_stages + st * S::kXBytes));
+#pragma unroll 1
           for (int side = 0; side < 2 && ok; ++side) {
-            ok = wait_one(&a_full[ab], aph);
+            ok = wait_spin_warp(&a_full[ab], aph);
             const uint32_t wide = tmem + kAColumn + ab * kAWidth;
-            for (int sub = 0; sub < subs && ok; ++sub) {
-              ok = wait_one(&d_empty[db], dph ^ 1);
+#pragma unroll
+            for (int sub = 0; sub < SUBS; ++sub) {
+              ok = ok && wait_spin_warp(&d_empty[db], dph ^ 1);
               if (!ok) break;
               tc_fence_after();
               const uint32_t d = tmem + db * NT;
-              const int per = a.group / S::kSteps;  // MMAs of the group
-#pragma unroll 1
-              for (int i = 0; i < per; ++i) {
-                const int j = sub * per + i;  // of the block: 32 bytes of a row of x, 8 columns of the codes
-                const uint32_t at = S::kWide ? x + (j >> 2) * (NT * 128) + (j & 3) * 32 : x + j * 32;
-                umma_ts<X>(d, wide + j * 8, smem_desc_k128(at), idesc, i > 0);
+              constexpr int kPer = kBlockK / SUBS / S::kSteps;  // MMAs of a group
+              if (leader) {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                  const int j = sub * kPer + i;  // of the block: 32 bytes of a row of x, 8 columns of the codes
+                  const int at = S::kWide ? (j >> 2) * (NT * 128) + (j & 3) * 32 : j * 32;
+                  umma_ts<X>(d, wide + j * 8, x + (at >> 4), idesc, i > 0);
+                }
+                umma_commit(&d_full[db]);
               }
-              umma_commit(&d_full[db]);
+              __syncwarp();
               if (++db == S::kD) {
                 db = 0;
                 dph ^= 1;
               }
             }
             if (!ok) break;
-            umma_commit(&a_empty[ab]);
+            if (leader) umma_commit(&a_empty[ab]);
             if (++ab == kABuffers) {
               ab = 0;
               aph ^= 1;
             }
           }
           if (!ok) break;
-          umma_commit(&x_empty[st]);
+          if (leader) umma_commit(&x_empty[st]);
           if (++st == S::kStages) {
             st = 0;
             ph ^= 1;
@@ -404,48 +487,35 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
       for (int kb = kb0; kb < kb1 && ok; ++kb) {
         ok = wait_warp(&c_full[st], ph);
         const unsigned char* c = c_stages + st * kCodeBytes + row * 64;
-#pragma unroll
+#pragma unroll 1
         for (int side = 0; side < 2; ++side) {
-          uint4 raw[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4*>(c + side * kSideBytes + ((i ^ ((row >> 1) & 3)) << 4));
-          if (side == 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&c_empty[st]);
-          }
           ok = ok && wait_warp(&a_empty[ab], aph ^ 1);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t wide = tmem + lanes + kAColumn + ab * kAWidth;
-          using Kind = std::integral_constant<int, X>;
-          if constexpr (S::kWide) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t r[32];
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                widen(raw[2 * h + i].x, r + 16 * i, Kind{});
-                widen(raw[2 * h + i].y, r + 16 * i + 4, Kind{});
-                widen(raw[2 * h + i].z, r + 16 * i + 8, Kind{});
-                widen(raw[2 * h + i].w, r + 16 * i + 12, Kind{});
-              }
-              tmem_st32(wide + 32 * h, r);
-            }
-          } else {
-            uint32_t r[32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              widen(raw[i].x, r + 8 * i, Kind{});
-              widen(raw[i].y, r + 8 * i + 2, Kind{});
-              widen(raw[i].z, r + 8 * i + 4, Kind{});
-              widen(raw[i].w, r + 8 * i + 6, Kind{});
-            }
-            tmem_st32(wide, r);
+          constexpr int kRegs = S::kWide ? 16 : 8;  // of 32 codes
+          uint32_t wide = tmem + lanes + kAColumn + ab * kAWidth;
+          uint4 raw = *reinterpret_cast<const uint4*>(c + (((row >> 1) & 3) << 4));
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            const uint4 next = *reinterpret_cast<const uint4*>(c + ((((i + 1) & 3) ^ ((row >> 1) & 3)) << 4));
+            uint32_t r[kRegs];
+            using Kind = std::integral_constant<int, X>;
+            widen(raw.x, r, Kind{});
+            widen(raw.y, r + kRegs / 4, Kind{});
+            widen(raw.z, r + kRegs / 2, Kind{});
+            widen(raw.w, r + kRegs * 3 / 4, Kind{});
+            tmem_st(wide, r);
+            wide += kRegs;
+            raw = next;
           }
+          c += kSideBytes;
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&a_full[ab]);
+          if (lane == 0) {
+            mbar_arrive(&a_full[ab]);
+            if (side == 1) mbar_arrive(&c_empty[st]);
+          }
           if (++ab == kABuffers) {
             ab = 0;
             aph ^= 1;
@@ -471,16 +541,16 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
       const bool there = o < a.f;
       const __half* scale[2] = {a.w_scale + static_cast<long long>(there ? o : 0) * groups,
                                 a.w_scale + static_cast<long long>(there ? a.f + o : 0) * groups};
-      float acc[2][S::kCols];
+      pair_t acc[2][S::kCols / 2];
 #pragma unroll
-      for (int j = 0; j < S::kCols; ++j) acc[0][j] = acc[1][j] = 0.0f;
+      for (int j = 0; j < S::kCols / 2; ++j) acc[0][j] = acc[1][j] = 0;
       // a block's scales (up to four halves a side), one block ahead
       const auto scales_of = [&](int side, int kb) {
         uint2 v = make_uint2(0, 0);
         uint16_t h[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (i < subs && there && kb < kb1 && kb * subs + i < groups) h[i] = __half_as_ushort(scale[side][kb * subs + i]);
+          if (i < SUBS && there && kb < kb1 && kb * SUBS + i < groups) h[i] = __half_as_ushort(scale[side][kb * SUBS + i]);
         v.x = h[0] | static_cast<uint32_t>(h[1]) << 16;
         v.y = h[2] | static_cast<uint32_t>(h[3]) << 16;
         return v;
@@ -493,31 +563,50 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
         if (grouped) ok = wait_warp(&s_full[ring], rph);
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-#pragma unroll 1
-          for (int sub = 0; sub < subs; ++sub) {
-            const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(now[side].x))) * kUnit;
-            now[side].x = now[side].x >> 16 | now[side].y << 16;
-            now[side].y >>= 16;
+#pragma unroll
+          for (int sub = 0; sub < SUBS; ++sub) {
+            const uint32_t h = sub & 1 ? (sub & 2 ? now[side].y : now[side].x) >> 16 : sub & 2 ? now[side].y : now[side].x;
+            const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(h))) * kUnit;
+            const pair_t s2 = pair_of(s, s);
             ok = ok && wait_warp(&d_full[db], dph);
             if (!ok) break;
             tc_fence_after();
+            const uint32_t d = from + db * NT;
+            const auto take = [&](const uint32_t(&r)[16], int j0) {
 #pragma unroll
-            for (int j0 = 0; j0 < S::kCols; j0 += 16) {
-              uint32_t d[16];
-              tmem_ld16(from + db * NT + j0, d);
-              if (j0 + 16 == S::kCols) {  // the sums are in registers
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&d_empty[db]);
-              }
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                float v = __uint_as_float(d[j]);
-                if constexpr (X == kXI8) v = __uint_as_float(0x4b400000u + d[j]) - 12582912.0f;  // below 2^22
-                if constexpr (!S::kWide) {
-                  if (grouped) v *= xs_s[ring][half * S::kCols + j0 + j];
+              for (int j = 0; j < 16; j += 2) {
+                pair_t v;
+                if constexpr (X == kXI8) {  // sums below 2^22, under the exponent of 3 * 2^22
+                  v = add2(pair_of(__uint_as_float(0x4b400000u + r[j]), __uint_as_float(0x4b400000u + r[j + 1])),
+                           pair_of(-12582912.0f, -12582912.0f));
+                } else {
+                  v = pair_of(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
                 }
-                acc[side][j0 + j] = fmaf(v, s, acc[side][j0 + j]);
+                if constexpr (!S::kWide) {
+                  if (grouped) v = mul2(v, *reinterpret_cast<const pair_t*>(&xs_s[ring][half * S::kCols + j0 + j]));
+                }
+                acc[side][(j0 + j) / 2] = fma2(v, s2, acc[side][(j0 + j) / 2]);
+              }
+            };
+            // 16 columns are under way while 16 are taken
+            uint32_t r0[16], r1[16];
+            const auto leave = [&]() {  // the sums are in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&d_empty[db]);
+            };
+            tmem_ld16(d, r0);
+#pragma unroll
+            for (int j0 = 0; j0 < S::kCols; j0 += 32) {
+              tmem_wait(r0);
+              if (j0 + 16 < S::kCols) tmem_ld16(d + j0 + 16, r1);
+              else leave();
+              take(r0, j0);
+              if (j0 + 16 < S::kCols) {
+                tmem_wait(r1);
+                if (j0 + 32 < S::kCols) tmem_ld16(d + j0 + 32, r0);
+                else leave();
+                take(r1, j0 + 16);
               }
             }
             if (++db == S::kD) {
@@ -536,29 +625,41 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
         }
       }
       if (!ok) break;
-      const auto finish = [&](int t, float g, float u) {
-        if (!there || t >= a.m) return;
-        if (!S::kWide && !grouped) {
-          const float xs = a.x_scale[t];
-          g *= xs;
-          u *= xs;
-        }
-        const float v = activated(g, a.gelu) * u;
-        const long long at = t * a.ld_out + o;
-        if (a.out_dtype == LB_F32) static_cast<float*>(a.out)[at] = v;
-        else if (a.out_dtype == LB_BF16) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
-        else static_cast<__half*>(a.out)[at] = __float2half_rn(v);
-      };
       if (splits == 1) {
+        const int live = there ? a.m - t0 : 0;  // tokens from t0 on
+        const bool wide_out = a.out_dtype == LB_F32, bf16_out = a.out_dtype == LB_BF16;
+        const long long pitch = a.ld_out * (wide_out ? 4 : 2);
+        unsigned char* at = static_cast<unsigned char*>(a.out) + t0 * pitch + static_cast<long long>(o) * (wide_out ? 4 : 2);
+        // 16 tokens a turn, the rest move up: a loop that stays in the instruction cache
+#pragma unroll 1
+        for (int j0 = 0; j0 < S::kCols; j0 += 16) {
 #pragma unroll
-        for (int j = 0; j < S::kCols; ++j) finish(t0 + j, acc[0][j], acc[1][j]);
+          for (int j = 0; j < 16; ++j) {
+            float g[2], u[2];
+            unpair(acc[0][j / 2], g[0], g[1]);
+            unpair(acc[1][j / 2], u[0], u[1]);
+            const float v = result<X>(a, grouped, t0 + j0 + j, g[j & 1], u[j & 1], j0 + j < live);
+            if (j0 + j < live) store(at, v, wide_out, bf16_out);
+            at += pitch;
+          }
+#pragma unroll
+          for (int j = 0; j + 8 < S::kCols / 2; ++j) {
+            acc[0][j] = acc[0][j + 8];
+            acc[1][j] = acc[1][j + 8];
+          }
+        }
       } else {
         // every stage was read (this CTA's last sums have come), so the partial sums may take their place
         float* mine = reinterpret_cast<float*>(smem) + row;
 #pragma unroll
         for (int side = 0; side < 2; ++side)
 #pragma unroll
-          for (int j = 0; j < S::kCols; ++j) mine[(side * NT + half * S::kCols + j) * kBlockO] = acc[side][j];
+          for (int j = 0; j < S::kCols; j += 2) {
+            float v[2];
+            unpair(acc[side][j / 2], v[0], v[1]);
+            mine[(side * NT + half * S::kCols + j) * kBlockO] = v[0];
+            mine[(side * NT + half * S::kCols + j + 1) * kBlockO] = v[1];
+          }
       }
     }
   }
@@ -577,16 +678,9 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
           u += peer_load(at + (NT + j) * kBlockO * 4, r);
         }
         if (o < a.f) {
-          const int t = t0 + j;
-          if (!S::kWide && !grouped) {
-            g *= a.x_scale[t];
-            u *= a.x_scale[t];
-          }
-          const float v = activated(g, a.gelu) * u;
-          const long long to = t * a.ld_out + o;
-          if (a.out_dtype == LB_F32) static_cast<float*>(a.out)[to] = v;
-          else if (a.out_dtype == LB_BF16) static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(v);
-          else static_cast<__half*>(a.out)[to] = __float2half_rn(v);
+          const bool wide_out = a.out_dtype == LB_F32;
+          const long long to = ((t0 + j) * a.ld_out + o) * (wide_out ? 4 : 2);
+          store(static_cast<unsigned char*>(a.out) + to, result<X>(a, grouped, t0 + j, g, u, true), wide_out, a.out_dtype == LB_BF16);
         }
       }
     }
@@ -602,10 +696,10 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   }
 }
 
-template <int X, int NT>
+template <int X, int NT, int SUBS>
 cudaError_t launch(const GatedArgs& a, int splits, const CUtensorMap& w_map, const CUtensorMap& x_map, cudaStream_t s) {
   using S = Shape<X, NT>;
-  const auto kernel = gated_kernel<X, NT>;
+  const auto kernel = gated_kernel<X, NT, SUBS>;
   static std::atomic<unsigned long long> done{0};
   static std::atomic<int> registers{0};
   cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), S::kSmem);
@@ -630,6 +724,12 @@ cudaError_t launch(const GatedArgs& a, int splits, const CUtensorMap& w_map, con
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kernel, a, w_map, x_map);
   return e == cudaSuccess ? cudaGetLastError() : e;
+}
+template <int X, int NT>
+cudaError_t launch(const GatedArgs& a, int splits, const CUtensorMap& w_map, const CUtensorMap& x_map, cudaStream_t s) {
+  if (a.group == 128) return launch<X, NT, 1>(a, splits, w_map, x_map, s);
+  if (a.group == 64) return launch<X, NT, 2>(a, splits, w_map, x_map, s);
+  return launch<X, NT, 4>(a, splits, w_map, x_map, s);
 }
 template <int X>
 cudaError_t launch(const GatedArgs& a, int nt, int splits, const CUtensorMap& w_map, const CUtensorMap& x_map, cudaStream_t s) {
