@@ -24,13 +24,14 @@
 namespace lb {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640, kFirstAdder = 12;  // warps
 constexpr int kBlockO = 128;                   // outputs of a tile
 constexpr int kBlockK = 128;                   // k of a stage
 constexpr int kSideBytes = kBlockO * kBlockK / 2;
 constexpr int kCodeBytes = 2 * kSideBytes;     // gate and up
 constexpr int kABuffers = 4, kAColumn = 256, kAWidth = 64;  // widened codes in the tensor memory
 constexpr int kScaleRing = 4;
+constexpr int kWeightRing = 8;                 // units whose weights' scales are kept: more than the buffers reach ahead
 constexpr int kMaxSplit = 8;
 constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -54,7 +55,7 @@ struct Shape {
   static constexpr int kStage = kCodeBytes + kXBytes;
   static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
   static constexpr int kPartial = 2 * NT * kBlockO * 4;       // a CTA's sums, in the stages' place
-  static constexpr int kSmem = kStages * kStage + 1024;
+  static constexpr int kSmem = kStages * kStage + 1024;       // (up to 12 KB are declared beside it)
   static_assert(kPartial <= kStages * kStage, "room");
   static constexpr int kD = NT == 128 ? 2 : 4;                // accumulators in the tensor memory
   static constexpr int kCols = NT / 2;                        // tokens of an adding warpgroup
@@ -266,25 +267,15 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // g / (1 + exp(-z)): silu with z = g, gelu's tanh form with z = 2 sqrt(2 / pi) (g + 0.044715 g^3), as
 // (1 + tanh(a)) / 2 = 1 / (1 + exp(-2 a)).  The exponent's rounding comes back by its remainder, so that the result is good
 // to some 2^-21 of itself for any g.
-__device__ __forceinline__ float activated(float g, bool gelu) {
+template <bool kGelu>
+__device__ __forceinline__ float activated(float g) {
   float z = g;
-  if (gelu) z = 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
+  if constexpr (kGelu) z = 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
   const float y = -kLog2e * z, rest = fmaf(-kLog2e, z, -y) - z * 1.925963033500e-8f;  // log2(e) = kLog2e + 1.926e-8
   const float e = exp2_fast(y);
   return g * rcp_fast(1.0f + (fabsf(y) < 126.0f ? fmaf(e, rest * 0.6931471805599453f, e) : e));
 }
 
-template <int X>
-__device__ __forceinline__ float result(const GatedArgs& a, bool grouped, int t, float g, float u, bool live) {
-  if constexpr (X == kXE4m3 || X == kXI8) {
-    if (!grouped) {
-      const float xs = live ? a.x_scale[t] : 0.0f;
-      g *= xs;
-      u *= xs;
-    }
-  }
-  return activated(g, a.gelu) * u;
-}
 __device__ __forceinline__ void store(unsigned char* at, float v, bool wide, bool bf16) {
   if (wide) *reinterpret_cast<float*>(at) = v;
   else *reinterpret_cast<uint16_t*>(at) = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
@@ -302,6 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   __shared__ uint64_t a_full[kABuffers], a_empty[kABuffers], d_full[S::kD], d_empty[S::kD];
   __shared__ uint64_t s_full[kScaleRing], s_empty[kScaleRing];
   __shared__ __align__(16) float xs_s[kScaleRing][NT];
+  __shared__ uint16_t ws_s[kWeightRing][SUBS][kBlockO];  // f16, by unit
   __shared__ uint32_t tmem_slot;
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -311,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&c_full[i], 1);
-      mbar_init(&c_empty[i], 4);
+      mbar_init(&c_empty[i], 8);
       mbar_init(&x_full[i], 1);
       mbar_init(&x_empty[i], 1);
     }
@@ -347,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   bool ok = true;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0 && lane == 0) {
       // ---------------- loads
       int st = 0;
@@ -476,51 +468,57 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
       }
     }
     __syncwarp();
-  } else if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    // ---------------- codes -> operands
-    int st = 0, ab = 0;
-    uint32_t ph = 0, aph = 0;
-    const int row = 32 * (warp & 3) + lane;
+  } else if (warp < kFirstAdder) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    // ---------------- codes -> operands, a warpgroup a side; a lane has a row, and brings the row's scales too
+    const int side = (warp - 4) >> 2, row = 32 * (warp & 3) + lane, groups = a.k / a.group;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes, in the address's upper half
+    int st = 0, unit = side;
+    uint32_t ph = 0;
     for (int tile = first; tile < tiles && ok; tile += step) {
-      for (int kb = kb0; kb < kb1 && ok; ++kb) {
-        ok = wait_warp(&c_full[st], ph);
-        const unsigned char* c = c_stages + st * kCodeBytes + row * 64;
-#pragma unroll 1
-        for (int side = 0; side < 2; ++side) {
-          ok = ok && wait_warp(&a_empty[ab], aph ^ 1);
-          if (!ok) break;
-          tc_fence_after();
-          constexpr int kRegs = S::kWide ? 16 : 8;  // of 32 codes
-          uint32_t wide = tmem + lanes + kAColumn + ab * kAWidth;
-          uint4 raw = *reinterpret_cast<const uint4*>(c + (((row >> 1) & 3) << 4));
-#pragma unroll 1
-          for (int i = 0; i < 4; ++i) {
-            const uint4 next = *reinterpret_cast<const uint4*>(c + ((((i + 1) & 3) ^ ((row >> 1) & 3)) << 4));
-            uint32_t r[kRegs];
-            using Kind = std::integral_constant<int, X>;
-            widen(raw.x, r, Kind{});
-            widen(raw.y, r + kRegs / 4, Kind{});
-            widen(raw.z, r + kRegs / 2, Kind{});
-            widen(raw.w, r + kRegs * 3 / 4, Kind{});
-            tmem_st(wide, r);
-            wide += kRegs;
-            raw = next;
-          }
-          c += kSideBytes;
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&a_full[ab]);
-            if (side == 1) mbar_arrive(&c_empty[st]);
-          }
-          if (++ab == kABuffers) {
-            ab = 0;
-            aph ^= 1;
-          }
+      const int o = tile % a.o_tiles * kBlockO + row;
+      const bool there = o < a.f;
+      const uint16_t* scale = reinterpret_cast<const uint16_t*>(a.w_scale) + static_cast<long long>(there ? side * a.f + o : 0) * groups;
+      uint16_t next[SUBS];
+      const auto fetch = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) next[i] = there && kb < kb1 && kb * SUBS + i < groups ? scale[kb * SUBS + i] : 0;
+      };
+      fetch(kb0);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int ab = unit & (kABuffers - 1);
+        // the ring's place is free: MMAs of the unit four back are over, so the adders have left all before the last two (or
+        // four) of them.  They read it after those of this unit, which come after this warp's arrival.
+        ok = wait_warp(&c_full[st], ph) && wait_warp(&a_empty[ab], (unit / kABuffers & 1) ^ 1);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) ws_s[unit & (kWeightRing - 1)][i][row] = next[i];
+        fetch(kb + 1);
+        constexpr int kRegs = S::kWide ? 16 : 8;  // of 32 codes
+        uint32_t wide = tmem + lanes + kAColumn + ab * kAWidth;
+        const unsigned char* c = c_stages + st * kCodeBytes + side * kSideBytes + row * 64;
+        uint4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4*>(c + ((i ^ ((row >> 1) & 3)) << 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t r[kRegs];
+          using Kind = std::integral_constant<int, X>;
+          widen(raw[i].x, r, Kind{});
+          widen(raw[i].y, r + kRegs / 4, Kind{});
+          widen(raw[i].z, r + kRegs / 2, Kind{});
+          widen(raw[i].w, r + kRegs * 3 / 4, Kind{});
+          tmem_st(wide + i * kRegs, r);
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&a_full[ab]);
+          mbar_arrive(&c_empty[st]);
+        }
+        unit += 2;
         if (++st == S::kStages) {
           st = 0;
           ph ^= 1;
@@ -528,51 +526,46 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ---------------- sums and results
-    const int half = (warp - 8) >> 2, row = 32 * (warp & 3) + lane;
+    const int half = (warp - kFirstAdder) >> 2, row = 32 * (warp & 3) + lane;
     const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * S::kCols;
-    const int groups = a.k / a.group;
-    int db = 0, ring = 0;
+    int db = 0, ring = 0, unit = 0;
     uint32_t dph = 0, rph = 0;
     constexpr float kUnit = X == kXE4m3 ? 512.0f : X == kXI8 ? 0.0625f : 1.0f;  // of the widened codes
     for (int tile = first; tile < tiles && ok; tile += step) {
       const int o = tile % a.o_tiles * kBlockO + row, t0 = tile / a.o_tiles * NT + half * S::kCols;
-      const bool there = o < a.f;
-      const __half* scale[2] = {a.w_scale + static_cast<long long>(there ? o : 0) * groups,
-                                a.w_scale + static_cast<long long>(there ? a.f + o : 0) * groups};
+      // 8-bit x with a scale a row: a lane keeps those of two tokens for the end
+      float row_scale[2] = {1.0f, 1.0f};
+      if (!S::kWide && !grouped) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) row_scale[i] = 32 * i + lane < S::kCols && t0 + 32 * i + lane < a.m ? a.x_scale[t0 + 32 * i + lane] : 0.0f;
+      }
       pair_t acc[2][S::kCols / 2];
 #pragma unroll
       for (int j = 0; j < S::kCols / 2; ++j) acc[0][j] = acc[1][j] = 0;
-      // a block's scales (up to four halves a side), one block ahead
-      const auto scales_of = [&](int side, int kb) {
-        uint2 v = make_uint2(0, 0);
-        uint16_t h[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < SUBS && there && kb < kb1 && kb * SUBS + i < groups) h[i] = __half_as_ushort(scale[side][kb * SUBS + i]);
-        v.x = h[0] | static_cast<uint32_t>(h[1]) << 16;
-        v.y = h[2] | static_cast<uint32_t>(h[3]) << 16;
-        return v;
-      };
-      uint2 next[2] = {scales_of(0, kb0), scales_of(1, kb0)};
       for (int kb = kb0; kb < kb1 && ok; ++kb) {
-        uint2 now[2] = {next[0], next[1]};
-#pragma unroll
-        for (int side = 0; side < 2; ++side) next[side] = scales_of(side, kb + 1);
         if (grouped) ok = wait_warp(&s_full[ring], rph);
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
 #pragma unroll
           for (int sub = 0; sub < SUBS; ++sub) {
-            const uint32_t h = sub & 1 ? (sub & 2 ? now[side].y : now[side].x) >> 16 : sub & 2 ? now[side].y : now[side].x;
-            const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(h))) * kUnit;
-            const pair_t s2 = pair_of(s, s);
             ok = ok && wait_warp(&d_full[db], dph);
             if (!ok) break;
             tc_fence_after();
+            const float s = __half2float(__ushort_as_half(ws_s[unit & (kWeightRing - 1)][sub][row])) * kUnit;
+            const pair_t s2 = pair_of(s, s);
             const uint32_t d = from + db * NT;
-            const auto take = [&](const uint32_t(&r)[16], int j0) {
+#pragma unroll
+            for (int j0 = 0; j0 < S::kCols; j0 += 16) {
+              uint32_t r[16];
+              tmem_ld16(d + j0, r);
+              tmem_wait(r);
+              if (j0 + 16 == S::kCols) {  // the sums are in registers
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_empty[db]);
+              }
 #pragma unroll
               for (int j = 0; j < 16; j += 2) {
                 pair_t v;
@@ -587,33 +580,13 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
                 }
                 acc[side][(j0 + j) / 2] = fma2(v, s2, acc[side][(j0 + j) / 2]);
               }
-            };
-            // 16 columns are under way while 16 are taken
-            uint32_t r0[16], r1[16];
-            const auto leave = [&]() {  // the sums are in registers
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&d_empty[db]);
-            };
-            tmem_ld16(d, r0);
-#pragma unroll
-            for (int j0 = 0; j0 < S::kCols; j0 += 32) {
-              tmem_wait(r0);
-              if (j0 + 16 < S::kCols) tmem_ld16(d + j0 + 16, r1);
-              else leave();
-              take(r0, j0);
-              if (j0 + 16 < S::kCols) {
-                tmem_wait(r1);
-                if (j0 + 32 < S::kCols) tmem_ld16(d + j0 + 32, r0);
-                else leave();
-                take(r1, j0 + 16);
-              }
             }
             if (++db == S::kD) {
               db = 0;
               dph ^= 1;
             }
           }
+          ++unit;
         }
         if (grouped) {
           __syncwarp();
@@ -626,22 +599,48 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
       }
       if (!ok) break;
       if (splits == 1) {
-        const int live = there ? a.m - t0 : 0;  // tokens from t0 on
-        const bool wide_out = a.out_dtype == LB_F32, bf16_out = a.out_dtype == LB_BF16;
-        const long long pitch = a.ld_out * (wide_out ? 4 : 2);
-        unsigned char* at = static_cast<unsigned char*>(a.out) + t0 * pitch + static_cast<long long>(o) * (wide_out ? 4 : 2);
+        const int live = o < a.f ? a.m - t0 : 0;  // tokens from t0 on
+        const long long pitch = a.ld_out * (a.out_dtype == LB_F32 ? 4 : 2);
+        unsigned char* at = static_cast<unsigned char*>(a.out) + t0 * pitch + static_cast<long long>(o) * (a.out_dtype == LB_F32 ? 4 : 2);
         // 16 tokens a turn, the rest move up: a loop that stays in the instruction cache
 #pragma unroll 1
         for (int j0 = 0; j0 < S::kCols; j0 += 16) {
+          float v[16];
+          const auto work = [&](auto gelu) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float g[2], u[2];
-            unpair(acc[0][j / 2], g[0], g[1]);
-            unpair(acc[1][j / 2], u[0], u[1]);
-            const float v = result<X>(a, grouped, t0 + j0 + j, g[j & 1], u[j & 1], j0 + j < live);
-            if (j0 + j < live) store(at, v, wide_out, bf16_out);
-            at += pitch;
+            for (int j = 0; j < 16; j += 2) {
+              float g[2], u[2];
+              unpair(acc[0][j / 2], g[0], g[1]);
+              unpair(acc[1][j / 2], u[0], u[1]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (!S::kWide) {
+                  const float xs = __shfl_sync(0xffffffffu, j0 & 32 ? row_scale[1] : row_scale[0], (j0 & 16) + j + e);
+                  if (!grouped) {
+                    g[e] *= xs;
+                    u[e] *= xs;
+                  }
+                }
+                v[j + e] = activated<decltype(gelu)::value>(g[e]) * u[e];
+              }
+            }
+          };
+          if (a.gelu) work(std::true_type{});
+          else work(std::false_type{});
+          if (a.out_dtype == LB_F32) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (j0 + j < live) *reinterpret_cast<float*>(at + j * pitch) = v[j];
+          } else if (a.out_dtype == LB_BF16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (j0 + j < live) *reinterpret_cast<__nv_bfloat16*>(at + j * pitch) = __float2bfloat16_rn(v[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (j0 + j < live) *reinterpret_cast<__half*>(at + j * pitch) = __float2half_rn(v[j]);
           }
+          at += 16 * pitch;
 #pragma unroll
           for (int j = 0; j + 8 < S::kCols / 2; ++j) {
             acc[0][j] = acc[0][j + 8];
@@ -668,10 +667,10 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   if (splits > 1) {
     cluster_arrive();
     cluster_wait();
-    if (warp >= 8) {  // a CTA finishes every splits-th token
+    if (warp >= kFirstAdder) {  // a CTA finishes every splits-th token
       const int row = 32 * (warp & 3) + lane, o = first % a.o_tiles * kBlockO + row, t0 = first / a.o_tiles * NT;
       const uint32_t at = smem_u32(smem) + row * 4;
-      for (int j = split + static_cast<int>(splits) * ((warp - 8) >> 2); j < NT && t0 + j < a.m; j += 2 * static_cast<int>(splits)) {
+      for (int j = split + static_cast<int>(splits) * ((warp - kFirstAdder) >> 2); j < NT && t0 + j < a.m; j += 2 * static_cast<int>(splits)) {
         float g = 0.0f, u = 0.0f;
         for (uint32_t r = 0; r < splits; ++r) {
           g += peer_load(at + j * kBlockO * 4, r);
@@ -680,7 +679,12 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
         if (o < a.f) {
           const bool wide_out = a.out_dtype == LB_F32;
           const long long to = ((t0 + j) * a.ld_out + o) * (wide_out ? 4 : 2);
-          store(static_cast<unsigned char*>(a.out) + to, result<X>(a, grouped, t0 + j, g, u, true), wide_out, a.out_dtype == LB_BF16);
+          if (!S::kWide && !grouped) {
+            g *= a.x_scale[t0 + j];
+            u *= a.x_scale[t0 + j];
+          }
+          store(static_cast<unsigned char*>(a.out) + to, (a.gelu ? activated<true>(g) : activated<false>(g)) * u, wide_out,
+                a.out_dtype == LB_BF16);
         }
       }
     }
@@ -705,12 +709,12 @@ cudaError_t launch(const GatedArgs& a, int splits, const CUtensorMap& w_map, con
   cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), S::kSmem);
   if (e != cudaSuccess) return e;
   if (registers.load(std::memory_order_relaxed) == 0) {
-    // the warpgroups' shares of the registers add up to 128 a thread: what the block has to be launched with
+    // the warpgroups' shares of the registers (40 + 2 * 48 + 2 * 168 a thread of each) have to fit what the block is launched with
     cudaFuncAttributes f;
     if ((e = cudaFuncGetAttributes(&f, reinterpret_cast<const void*>(kernel))) != cudaSuccess) return e;
     registers.store(f.numRegs, std::memory_order_relaxed);
   }
-  if (registers.load(std::memory_order_relaxed) != 128) return cudaErrorInvalidConfiguration;
+  if (registers.load(std::memory_order_relaxed) * 5 < 40 + 2 * 48 + 2 * 168) return cudaErrorInvalidConfiguration;
   const int tiles = a.o_tiles * a.t_tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = static_cast<unsigned>(splits > 1 ? tiles * splits : tiles < kSms ? tiles : kSms);
