@@ -11,8 +11,8 @@
 // (x 128 k: some 12 instructions for 8 codes, 5 to int8) and stores them to the tensor memory, from where the MMAs take them
 // as their A operand.  Shared memory then only has to feed x to the MMAs.
 //
-// Warpgroups: 0 loads (warp 0: TMA; warp 2: x's scales of a group) and issues the MMAs (warp 1); 1 widens; 2 and 3 add up, half
-// of the tokens each, and finish the tile.  A unit is one side's (gate or up) product over one group: while the one
+// Warpgroups: 0 loads (warp 0: TMA; warp 2: x's scales of a group) and issues the MMAs (warps 1 and 3, a side each); 1 and 2 widen, a
+// side each; 3 and 4 add up, half of the tokens each, and finish the tile.  A unit is one side's (gate or up) product over one group: while the one
 // side's sums are taken out of the tensor memory the other side's MMAs run.
 //
 // Few tokens: the tiles of outputs are fewer than the SMs, so K is dealt out to the CTAs of a cluster, whose partial
@@ -57,11 +57,14 @@ struct Shape {
   static constexpr int kPartial = 2 * NT * kBlockO * 4;       // a CTA's sums, in the stages' place
   static constexpr int kSmem = kStages * kStage + 1024;       // (up to 12 KB are declared beside it)
   static_assert(kPartial <= kStages * kStage, "room");
-  static constexpr int kD = NT == 128 ? 2 : 4;                // accumulators in the tensor memory
+  static constexpr int kSideD = NT == 128 ? 1 : 2, kD = 2 * kSideD;  // accumulators in the tensor memory, of a side and in all
   static constexpr int kCols = NT / 2;                        // tokens of an adding warpgroup
   static constexpr int kSteps = kWide ? 16 : 32;              // k of an MMA
   static_assert(kD * NT <= kAColumn, "tensor memory");
 };
+
+// two 32-bit values an instruction
+typedef unsigned long long pair_t;
 
 // D(tmem) (+)= A(tmem) * B(smem)^T
 template <int X>
@@ -99,59 +102,42 @@ __device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&r)[8]) {
                : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 16 columns; the registers hold them, and may be touched, after tmem_wait of the same array
-__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+// 16 columns as pairs, and their wait in one statement
+__device__ __forceinline__ void tmem_ld16(uint32_t at, pair_t (&r)[8]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      "{\n\t.reg .b32 t<16>;\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {t0,t1,t2,t3,t4,t5,t6,t7,t8,t9,t10,t11,t12,t13,t14,t15}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n\t"
+      "mov.b64 %0, {t0, t1};\n\tmov.b64 %1, {t2, t3};\n\tmov.b64 %2, {t4, t5};\n\tmov.b64 %3, {t6, t7};\n\t"
+      "mov.b64 %4, {t8, t9};\n\tmov.b64 %5, {t10, t11};\n\tmov.b64 %6, {t12, t13};\n\tmov.b64 %7, {t14, t15};\n\t}"
+      : "=l"(r[0]), "=l"(r[1]), "=l"(r[2]), "=l"(r[3]), "=l"(r[4]), "=l"(r[5]), "=l"(r[6]), "=l"(r[7])
       : "r"(at)
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-}
-
-// Waits for a phase, with a limit of some 2.6 s (try_wait sleeps for up to the 20 us that it is given).
+// Waits for a phase, with a limit of some 2.6 s (try_wait sleeps for up to the 20 us that it is given).  One look is in line.
 constexpr int kPolls = 1 << 17;
+__device__ __forceinline__ bool look(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "r"(20000u)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int n = 0; n < kPolls; ++n)
+    if (look(bar, parity)) return true;
+  return false;
+}
 __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity) {
-  const uint32_t at = smem_u32(bar);
-#pragma unroll 1
-  for (int n = 0; n < kPolls; ++n) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(at), "r"(parity), "r"(20000u)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
+  return look(smem_u32(bar), parity) || wait_on(smem_u32(bar), parity);
 }
-// the same by polls without sleep, for the one thread that the MMAs wait for
-__device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity) {
-  const uint32_t at = smem_u32(bar);
-#pragma unroll 1
-  for (int n = 0; n < (1 << 26); ++n) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(at), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
-}
+// by a whole warp: the same answer for every lane
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile(
@@ -162,10 +148,8 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, wait_one(bar, parity));
-}
-__device__ __forceinline__ bool wait_spin_warp(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, wait_spin(bar, parity));
+  if (__all_sync(0xffffffffu, look(smem_u32(bar), parity))) return true;
+  return __all_sync(0xffffffffu, wait_on(smem_u32(bar), parity));
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -182,8 +166,6 @@ __device__ __forceinline__ float peer_load(uint32_t at, uint32_t rank) {
   return v;
 }
 
-// two 32-bit values an instruction
-typedef unsigned long long pair_t;
 __device__ __forceinline__ pair_t pair_of(float a, float b) {
   pair_t p;
   asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
@@ -265,21 +247,23 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return y;
 }
 // g / (1 + exp(-z)): silu with z = g, gelu's tanh form with z = 2 sqrt(2 / pi) (g + 0.044715 g^3), as
-// (1 + tanh(a)) / 2 = 1 / (1 + exp(-2 a)).  The exponent's rounding comes back by its remainder, so that the result is good
-// to some 2^-21 of itself for any g.
-template <bool kGelu>
+// (1 + tanh(a)) / 2 = 1 / (1 + exp(-2 a)).  The rounding of the exponent z log2(e) costs |z| 2^-24 of the result, below 2^-17 where
+// it is not 0 in 16 bits; for 32-bit outputs (kFine) it comes back by its remainder, so that the result is good to some 2^-21.
+template <bool kGelu, bool kFine>
 __device__ __forceinline__ float activated(float g) {
   float z = g;
   if constexpr (kGelu) z = 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
-  const float y = -kLog2e * z, rest = fmaf(-kLog2e, z, -y) - z * 1.925963033500e-8f;  // log2(e) = kLog2e + 1.926e-8
-  const float e = exp2_fast(y);
-  return g * rcp_fast(1.0f + (fabsf(y) < 126.0f ? fmaf(e, rest * 0.6931471805599453f, e) : e));
+  const float y = -kLog2e * z;
+  float e = exp2_fast(y);
+  if constexpr (kFine) {
+    const float rest = fmaf(-kLog2e, z, -y) - z * 1.925963033500e-8f;  // log2(e) = kLog2e + 1.926e-8
+    e = fabsf(y) < 126.0f ? fmaf(e, rest * 0.6931471805599453f, e) : e;
+  }
+  return g * rcp_fast(1.0f + e);
 }
-
-__device__ __forceinline__ void store(unsigned char* at, float v, bool wide, bool bf16) {
-  if (wide) *reinterpret_cast<float*>(at) = v;
-  else *reinterpret_cast<uint16_t*>(at) = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
-}
+__device__ __forceinline__ void put(float* at, float v) { *at = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* at, float v) { *at = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half* at, float v) { *at = __float2half_rn(v); }
 
 template <int X, int NT, int SUBS>
 __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, const __grid_constant__ CUtensorMap w_map,
@@ -305,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
       mbar_init(&c_full[i], 1);
       mbar_init(&c_empty[i], 8);
       mbar_init(&x_full[i], 1);
-      mbar_init(&x_empty[i], 1);
+      mbar_init(&x_empty[i], 2);
     }
     for (int i = 0; i < kABuffers; ++i) {
       mbar_init(&a_full[i], 4);
@@ -387,52 +371,44 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
           wait_one(&x_full[st], ph);
         }
       }
-    } else if (warp == 1) {
-      // ---------------- MMAs
-      int st = 0, ab = 0, db = 0;
-      uint32_t ph = 0, aph = 0, dph = 0;
+    } else if (warp & 1) {
+      // ---------------- MMAs, a warp a side: each one's waits and commits pass while the other's MMAs run.  The warp walks together
+      // and one lane issues, so that descriptors and barriers stay uniform (a lane by itself took twice as long).
+      const int side = warp >> 1;
+      int st = 0, unit = side;
+      uint32_t ph = 0;
       constexpr uint32_t idesc = idesc_of<X>(kBlockO, NT);
-      // the warp walks together and one lane issues: descriptors and barriers stay uniform
       const bool leader = elect_one();
       for (int tile = first; tile < tiles && ok; tile += step) {
         for (int kb = kb0; kb < kb1 && ok; ++kb) {
-          ok = wait_spin_warp(&x_full[st], ph);
+          const int ab = unit & (kABuffers - 1);
+          ok = wait_warp(&x_full[st], ph) && wait_warp(&a_full[ab], unit / kABuffers & 1);
           const uint64_t x = smem_desc_k128(smem_u32(x_stages + st * S::kXBytes));
-#pragma unroll 1
-          for (int side = 0; side < 2 && ok; ++side) {
-            ok = wait_spin_warp(&a_full[ab], aph);
-            const uint32_t wide = tmem + kAColumn + ab * kAWidth;
+          const uint32_t wide = tmem + kAColumn + ab * kAWidth;
 #pragma unroll
-            for (int sub = 0; sub < SUBS; ++sub) {
-              ok = ok && wait_spin_warp(&d_empty[db], dph ^ 1);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t d = tmem + db * NT;
-              constexpr int kPer = kBlockK / SUBS / S::kSteps;  // MMAs of a group
-              if (leader) {
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                  const int j = sub * kPer + i;  // of the block: 32 bytes of a row of x, 8 columns of the codes
-                  const int at = S::kWide ? (j >> 2) * (NT * 128) + (j & 3) * 32 : j * 32;
-                  umma_ts<X>(d, wide + j * 8, x + (at >> 4), idesc, i > 0);
-                }
-                umma_commit(&d_full[db]);
-              }
-              __syncwarp();
-              if (++db == S::kD) {
-                db = 0;
-                dph ^= 1;
-              }
-            }
+          for (int sub = 0; sub < SUBS; ++sub) {
+            const int turn = unit / 2 * SUBS + sub, db = side * S::kSideD + (turn & (S::kSideD - 1));
+            ok = ok && wait_warp(&d_empty[db], (turn / S::kSideD & 1) ^ 1);
             if (!ok) break;
-            if (leader) umma_commit(&a_empty[ab]);
-            if (++ab == kABuffers) {
-              ab = 0;
-              aph ^= 1;
+            tc_fence_after();
+            const uint32_t d = tmem + db * NT;
+            constexpr int kPer = kBlockK / SUBS / S::kSteps;  // MMAs of a group
+            if (leader) {
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) {
+                const int j = sub * kPer + i;  // of the block: 32 bytes of a row of x, 8 columns of the codes
+                const int at = S::kWide ? (j >> 2) * (NT * 128) + (j & 3) * 32 : j * 32;
+                umma_ts<X>(d, wide + j * 8, x + (at >> 4), idesc, i > 0);
+              }
+              umma_commit(&d_full[db]);
+              if (sub == SUBS - 1) {
+                umma_commit(&a_empty[ab]);
+                umma_commit(&x_empty[st]);
+              }
             }
+            __syncwarp();
           }
-          if (!ok) break;
-          if (leader) umma_commit(&x_empty[st]);
+          unit += 2;
           if (++st == S::kStages) {
             st = 0;
             ph ^= 1;
@@ -530,8 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
     // ---------------- sums and results
     const int half = (warp - kFirstAdder) >> 2, row = 32 * (warp & 3) + lane;
     const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * S::kCols;
-    int db = 0, ring = 0, unit = 0;
-    uint32_t dph = 0, rph = 0;
+    int turn = 0, ring = 0, unit = 0;
+    uint32_t rph = 0;
     constexpr float kUnit = X == kXE4m3 ? 512.0f : X == kXI8 ? 0.0625f : 1.0f;  // of the widened codes
     for (int tile = first; tile < tiles && ok; tile += step) {
       const int o = tile % a.o_tiles * kBlockO + row, t0 = tile / a.o_tiles * NT + half * S::kCols;
@@ -547,47 +523,44 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
       for (int kb = kb0; kb < kb1 && ok; ++kb) {
         if (grouped) ok = wait_warp(&s_full[ring], rph);
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
+        for (int sub = 0; sub < SUBS; ++sub) {
 #pragma unroll
-          for (int sub = 0; sub < SUBS; ++sub) {
-            ok = ok && wait_warp(&d_full[db], dph);
+          for (int side = 0; side < 2; ++side) {
+            const int db = side * S::kSideD + (turn & (S::kSideD - 1));
+            ok = ok && wait_warp(&d_full[db], turn / S::kSideD & 1);
             if (!ok) break;
             tc_fence_after();
-            const float s = __half2float(__ushort_as_half(ws_s[unit & (kWeightRing - 1)][sub][row])) * kUnit;
+            const float s = __half2float(__ushort_as_half(ws_s[(unit + side) & (kWeightRing - 1)][sub][row])) * kUnit;
             const pair_t s2 = pair_of(s, s);
             const uint32_t d = from + db * NT;
 #pragma unroll
             for (int j0 = 0; j0 < S::kCols; j0 += 16) {
-              uint32_t r[16];
+              pair_t r[8];
               tmem_ld16(d + j0, r);
-              tmem_wait(r);
               if (j0 + 16 == S::kCols) {  // the sums are in registers
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&d_empty[db]);
               }
 #pragma unroll
-              for (int j = 0; j < 16; j += 2) {
-                pair_t v;
+              for (int j = 0; j < 8; ++j) {
+                pair_t v = r[j];
                 if constexpr (X == kXI8) {  // sums below 2^22, under the exponent of 3 * 2^22
-                  v = add2(pair_of(__uint_as_float(0x4b400000u + r[j]), __uint_as_float(0x4b400000u + r[j + 1])),
+                  float lo, hi;
+                  unpair(v, lo, hi);
+                  v = add2(pair_of(__uint_as_float(0x4b400000u + __float_as_uint(lo)), __uint_as_float(0x4b400000u + __float_as_uint(hi))),
                            pair_of(-12582912.0f, -12582912.0f));
-                } else {
-                  v = pair_of(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
                 }
                 if constexpr (!S::kWide) {
-                  if (grouped) v = mul2(v, *reinterpret_cast<const pair_t*>(&xs_s[ring][half * S::kCols + j0 + j]));
+                  if (grouped) v = mul2(v, *reinterpret_cast<const pair_t*>(&xs_s[ring][half * S::kCols + j0 + 2 * j]));
                 }
-                acc[side][(j0 + j) / 2] = fma2(v, s2, acc[side][(j0 + j) / 2]);
+                acc[side][j0 / 2 + j] = fma2(v, s2, acc[side][j0 / 2 + j]);
               }
             }
-            if (++db == S::kD) {
-              db = 0;
-              dph ^= 1;
-            }
           }
-          ++unit;
+          ++turn;
         }
+        unit += 2;
         if (grouped) {
           __syncwarp();
           if (lane == 0 && ok) mbar_arrive(&s_empty[ring]);
@@ -602,51 +575,50 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
         const int live = o < a.f ? a.m - t0 : 0;  // tokens from t0 on
         const long long pitch = a.ld_out * (a.out_dtype == LB_F32 ? 4 : 2);
         unsigned char* at = static_cast<unsigned char*>(a.out) + t0 * pitch + static_cast<long long>(o) * (a.out_dtype == LB_F32 ? 4 : 2);
-        // 16 tokens a turn, the rest move up: a loop that stays in the instruction cache
+        // up to 32 tokens a turn, the rest move up: a loop that stays in the instruction cache
+        constexpr int kTurn = S::kCols < 32 ? S::kCols : 32;
+        const bool whole = tile % a.o_tiles * kBlockO + kBlockO <= a.f && t0 + S::kCols <= a.m;
+        const auto turn = [&](auto gelu, auto type) {
+          using Out = decltype(type);
 #pragma unroll 1
-        for (int j0 = 0; j0 < S::kCols; j0 += 16) {
-          float v[16];
-          const auto work = [&](auto gelu) {
+          for (int j0 = 0; j0 < S::kCols; j0 += kTurn) {
+            float v[kTurn];
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {
+            for (int j = 0; j < kTurn; ++j) {
               float g[2], u[2];
               unpair(acc[0][j / 2], g[0], g[1]);
               unpair(acc[1][j / 2], u[0], u[1]);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                if (!S::kWide) {
-                  const float xs = __shfl_sync(0xffffffffu, j0 & 32 ? row_scale[1] : row_scale[0], (j0 & 16) + j + e);
-                  if (!grouped) {
-                    g[e] *= xs;
-                    u[e] *= xs;
-                  }
-                }
-                v[j + e] = activated<decltype(gelu)::value>(g[e]) * u[e];
+              float gate = g[j & 1], up = u[j & 1];
+              if (!S::kWide && !grouped) {
+                const float xs = __shfl_sync(0xffffffffu, j0 & 32 ? row_scale[1] : row_scale[0], j);
+                gate *= xs;
+                up *= xs;
               }
+              v[j] = activated<decltype(gelu)::value, sizeof(Out) == 4>(gate) * up;
             }
-          };
-          if (a.gelu) work(std::true_type{});
-          else work(std::false_type{});
-          if (a.out_dtype == LB_F32) {
+            if (whole) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j0 + j < live) *reinterpret_cast<float*>(at + j * pitch) = v[j];
-          } else if (a.out_dtype == LB_BF16) {
+              for (int j = 0; j < kTurn; ++j) put(reinterpret_cast<Out*>(at + j * pitch), v[j]);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j0 + j < live) *reinterpret_cast<__nv_bfloat16*>(at + j * pitch) = __float2bfloat16_rn(v[j]);
-          } else {
+              for (int j = 0; j < kTurn; ++j)
+                if (j0 + j < live) put(reinterpret_cast<Out*>(at + j * pitch), v[j]);
+            }
+            at += kTurn * pitch;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j0 + j < live) *reinterpret_cast<__half*>(at + j * pitch) = __float2half_rn(v[j]);
+            for (int j = 0; j + kTurn / 2 < S::kCols / 2; ++j) {
+              acc[0][j] = acc[0][j + kTurn / 2];
+              acc[1][j] = acc[1][j + kTurn / 2];
+            }
           }
-          at += 16 * pitch;
-#pragma unroll
-          for (int j = 0; j + 8 < S::kCols / 2; ++j) {
-            acc[0][j] = acc[0][j + 8];
-            acc[1][j] = acc[1][j + 8];
-          }
-        }
+        };
+        const auto typed = [&](auto gelu) {
+          if (a.out_dtype == LB_F32) turn(gelu, float{});
+          else if (a.out_dtype == LB_BF16) turn(gelu, __nv_bfloat16{});
+          else turn(gelu, __half{});
+        };
+        if (a.gelu) typed(std::true_type{});
+        else typed(std::false_type{});
       } else {
         // every stage was read (this CTA's last sums have come), so the partial sums may take their place
         float* mine = reinterpret_cast<float*>(smem) + row;
@@ -677,14 +649,15 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
           u += peer_load(at + (NT + j) * kBlockO * 4, r);
         }
         if (o < a.f) {
-          const bool wide_out = a.out_dtype == LB_F32;
-          const long long to = ((t0 + j) * a.ld_out + o) * (wide_out ? 4 : 2);
           if (!S::kWide && !grouped) {
             g *= a.x_scale[t0 + j];
             u *= a.x_scale[t0 + j];
           }
-          store(static_cast<unsigned char*>(a.out) + to, (a.gelu ? activated<true>(g) : activated<false>(g)) * u, wide_out,
-                a.out_dtype == LB_BF16);
+          const float v = (a.gelu ? activated<true, true>(g) : activated<false, true>(g)) * u;
+          const long long to = (t0 + j) * a.ld_out + o;
+          if (a.out_dtype == LB_F32) put(static_cast<float*>(a.out) + to, v);
+          else if (a.out_dtype == LB_BF16) put(static_cast<__nv_bfloat16*>(a.out) + to, v);
+          else put(static_cast<__half*>(a.out) + to, v);
         }
       }
     }
