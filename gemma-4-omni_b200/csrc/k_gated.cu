@@ -15,8 +15,8 @@
 // side each; 3 and 4 add up, half of the tokens each, and finish the tile.  A unit is one side's (gate or up) product over one group: while the one
 // side's sums are taken out of the tensor memory the other side's MMAs run.
 //
-// Few tokens: the tiles of outputs are fewer than the SMs, so K is dealt out to the CTAs of a cluster, whose partial
-// sums meet in shared memory (read over the cluster, in the order of the CTAs).
+// Few tokens: the tiles of outputs are fewer than the SMs, so K is dealt out to the CTAs of a cluster.  Each sends its partial
+// sums to the CTA that finishes the token (stores over the cluster), which adds them up in the order of K.
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 #include "kernels.h"
@@ -53,10 +53,10 @@ struct Shape {
   static constexpr bool kWide = X == kXBf16 || X == kXF16;    // 16-bit operands
   static constexpr int kXBytes = NT * kBlockK * (kWide ? 2 : 1);
   static constexpr int kStage = kCodeBytes + kXBytes;
-  static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
-  static constexpr int kPartial = 2 * NT * kBlockO * 4;       // a CTA's sums, in the stages' place
-  static constexpr int kSmem = kStages * kStage + 1024;       // (up to 12 KB are declared beside it)
-  static_assert(kPartial <= kStages * kStage, "room");
+  static constexpr int kParts = NT < 128 ? 2 * (NT + kMaxSplit) * kBlockO * 4 : 0;  // partial sums of the tokens that a CTA finishes
+  static constexpr int kRoom = 200 * 1024 - kParts;
+  static constexpr int kStages = kRoom / kStage > 8 ? 8 : kRoom / kStage;
+  static constexpr int kSmem = kStages * kStage + kParts + 1024;  // (up to 12 KB are declared beside it)
   static constexpr int kSideD = NT == 128 ? 1 : 2, kD = 2 * kSideD;  // accumulators in the tensor memory, of a side and in all
   static constexpr int kCols = NT / 2;                        // tokens of an adding warpgroup
   static constexpr int kSteps = kWide ? 16 : 32;              // k of an MMA
@@ -158,12 +158,13 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float peer_load(uint32_t at, uint32_t rank) {
-  float v;
+__device__ __forceinline__ uint32_t peer_address(uint32_t at, uint32_t rank) {
   uint32_t peer;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer) : "memory");
-  return v;
+  return peer;
+}
+__device__ __forceinline__ void peer_store(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ pair_t pair_of(float a, float b) {
@@ -191,50 +192,86 @@ __device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
 template <typename H>
 __device__ __forceinline__ uint32_t bits_of(H v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
-// 8 codes n (lowest bits first) as n - 8 in the operand's type and in their order.
-// bf16, fp16: two codes under the exponent of 128 or 1024, where they count in ones, less 136 or 1032 (fp16: the odd
-// codes as they lie, in sixteens, come down by the product).
-__device__ __forceinline__ void widen(uint32_t w, uint32_t* r, std::integral_constant<int, kXBf16>) {
-  const __nv_bfloat162 bias = __floats2bfloat162_rn(136.0f, 136.0f);
-  const uint32_t odd = w >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t pair = (__byte_perm(w, odd, 0x0400 + 0x0101 * i) & 0x000f000fu) | 0x43004300u;
-    r[i] = bits_of(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair), bias));
-  }
+// 8 codes n (lowest bits first) as n - 8 in the operand's type and in their order.  The logic runs on a pipe of half rate
+// that bounds the widening, so the constants are held in registers that the compiler cannot know (it made them anew for each use).
+__device__ __forceinline__ uint32_t held(uint32_t v) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
-__device__ __forceinline__ void widen(uint32_t w, uint32_t* r, std::integral_constant<int, kXF16>) {
-  const __half2 factor = __floats2half2_rn(1.0f, 0.0625f), bias = __floats2half2_rn(-1032.0f, -72.0f);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t pair = (__byte_perm(w, 0, 0x0101 * i) & 0x00f0000fu) | 0x64006400u;
-    r[i] = bits_of(__hfma2(*reinterpret_cast<const __half2*>(&pair), factor, bias));
-  }
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
-// e4m3: below 16 the bits count in steps of 2^-9 (a sign and four bits), so a code becomes the sign and the size of n - 8
-// and the scale 2^9 larger.  A byte permute looks a code's lower three bits up in a table of eight, and where the fourth
-// is set gives the looked-up byte's sign instead: 0 in these tables.
 __device__ __forceinline__ uint32_t look_up(uint32_t low, uint32_t high, uint32_t w) {  // (__byte_perm has no sign mode)
   uint32_t r;
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(low), "r"(high), "r"(w));
   return r;
 }
-__device__ __forceinline__ uint32_t signed4(uint32_t w) {
-  const uint32_t below = look_up(0x05060708u, 0x01020304u, w);            // n < 8: 8 - n
-  const uint32_t above = look_up(0x03020100u, 0x07060504u, w ^ 0x8888u);  // n >= 8: n - 8
-  const uint32_t sign = look_up(0x7f7f7f7fu, 0x7f7f7f7fu, w);             // n < 8: 0x7f
-  return below | above | ((sign << 1) & 0x80808080u);
-}
-__device__ __forceinline__ void widen(uint32_t w, uint32_t* r, std::integral_constant<int, kXE4m3>) {
-  r[0] = signed4(w);
-  r[1] = signed4(w >> 16);
-}
+template <int X>
+struct Widen;
+// bf16, fp16: two codes under the exponent of 128 or 1024, where they count in ones, less 136 or 1032 (fp16: the odd
+// codes as they lie, in sixteens, come down by the product).
+template <>
+struct Widen<kXBf16> {
+  uint32_t mask = held(0x000f000fu), exponent = held(0x43004300u);
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t* r) const {
+    const __nv_bfloat162 bias = __floats2bfloat162_rn(136.0f, 136.0f);
+    const uint32_t odd = w >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t pair = and_or(__byte_perm(w, odd, 0x0400 + 0x0101 * i), mask, exponent);
+      r[i] = bits_of(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair), bias));
+    }
+  }
+};
+template <>
+struct Widen<kXF16> {
+  uint32_t mask = held(0x00f0000fu), exponent = held(0x64006400u);
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t* r) const {
+    const __half2 factor = __floats2half2_rn(1.0f, 0.0625f), bias = __floats2half2_rn(-1032.0f, -72.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t pair = and_or(__byte_perm(w, w, 0x0101 * i), mask, exponent);
+      r[i] = bits_of(__hfma2(*reinterpret_cast<const __half2*>(&pair), factor, bias));
+    }
+  }
+};
+// e4m3: below 16 the bits count in steps of 2^-9 (a sign and four bits), so a code becomes the sign and the size of n - 8
+// and the scale 2^9 larger.  A byte permute looks a code's lower three bits up in a table of eight, and where the fourth
+// is set gives the looked-up byte's sign instead: 0 in these tables.
+template <>
+struct Widen<kXE4m3> {
+  uint32_t b0 = held(0x05060708u), b1 = held(0x01020304u), a0 = held(0x03020100u), a1 = held(0x07060504u), low = held(0x7f7f7f7fu),
+           top = held(0x80808080u);
+  __device__ __forceinline__ uint32_t four(uint32_t w, uint32_t turned) const {
+    const uint32_t below = look_up(b0, b1, w);       // n < 8: 8 - n
+    const uint32_t above = look_up(a0, a1, turned);  // n >= 8: n - 8
+    const uint32_t sign = look_up(low, low, w);      // n < 8: 0x7f
+    return and_or(sign + sign, top, below | above);
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t* r) const {
+    const uint32_t turned = w ^ 0x88888888u;
+    r[0] = four(w, turned);
+    r[1] = four(w >> 16, turned >> 16);
+  }
+};
 // int8: 16 (n - 8), a code with its top bit turned as the byte's upper half
-__device__ __forceinline__ void widen(uint32_t w, uint32_t* r, std::integral_constant<int, kXI8>) {
-  const uint32_t odd = (w & 0xf0f0f0f0u) ^ 0x80808080u, even = ((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
-  r[0] = __byte_perm(even, odd, 0x5140);
-  r[1] = __byte_perm(even, odd, 0x7362);
-}
+template <>
+struct Widen<kXI8> {
+  uint32_t high = held(0xf0f0f0f0u), top = held(0x80808080u);
+  __device__ __forceinline__ uint32_t upper(uint32_t w) const {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(high), "r"(top));  // (w & high) ^ top
+    return r;
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t* r) const {
+    const uint32_t odd = upper(w), even = upper(w << 4);
+    r[0] = __byte_perm(even, odd, 0x5140);
+    r[1] = __byte_perm(even, odd, 0x7362);
+  }
+};
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -273,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   unsigned char* smem = gated_raw + ((1024 - (smem_u32(gated_raw) & 1023)) & 1023);
   unsigned char* x_stages = smem;                             // [stage][half of k][token][128 bytes], swizzled
   unsigned char* c_stages = smem + S::kStages * S::kXBytes;   // [stage][side][row][64 bytes], swizzled
+  unsigned char* parts = smem + S::kStages * S::kStage;
   __shared__ uint64_t c_full[S::kStages], c_empty[S::kStages], x_full[S::kStages], x_empty[S::kStages];
   __shared__ uint64_t a_full[kABuffers], a_empty[kABuffers], d_full[S::kD], d_empty[S::kD];
   __shared__ uint64_t s_full[kScaleRing], s_empty[kScaleRing];
@@ -320,7 +358,8 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   const int kb0 = a.k_blocks * split / static_cast<int>(splits), kb1 = a.k_blocks * (split + 1) / static_cast<int>(splits);
   const int first = blockIdx.x / splits, step = gridDim.x / splits, tiles = a.o_tiles * a.t_tiles;
   const bool grouped = a.x_group != 0;
-  bool ok = true;
+  bool ok = true, joined = splits == 1 || NT == 128;
+  if (!joined) cluster_arrive();
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -448,6 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     // ---------------- codes -> operands, a warpgroup a side; a lane has a row, and brings the row's scales too
     const int side = (warp - 4) >> 2, row = 32 * (warp & 3) + lane, groups = a.k / a.group;
+    const Widen<X> widen;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes, in the address's upper half
     int st = 0, unit = side;
     uint32_t ph = 0;
@@ -480,11 +520,10 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t r[kRegs];
-          using Kind = std::integral_constant<int, X>;
-          widen(raw[i].x, r, Kind{});
-          widen(raw[i].y, r + kRegs / 4, Kind{});
-          widen(raw[i].z, r + kRegs / 2, Kind{});
-          widen(raw[i].w, r + kRegs * 3 / 4, Kind{});
+          widen(raw[i].x, r);
+          widen(raw[i].y, r + kRegs / 4);
+          widen(raw[i].z, r + kRegs / 2);
+          widen(raw[i].w, r + kRegs * 3 / 4);
           tmem_st(wide + i * kRegs, r);
         }
         tmem_wait_st();
@@ -620,50 +659,65 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
         if (a.gelu) typed(std::true_type{});
         else typed(std::false_type{});
       } else {
-        // every stage was read (this CTA's last sums have come), so the partial sums may take their place
-        float* mine = reinterpret_cast<float*>(smem) + row;
+        // token j of the tile is finished by CTA j % splits, as its token j / splits: [source][side][token][row]
+        if (!joined) {  // (the others have begun)
+          cluster_wait();
+          joined = true;
+        }
+        if constexpr (NT < 128) {
+          const int own = (NT + static_cast<int>(splits) - 1) / static_cast<int>(splits), live = min(S::kCols, a.m - t0);
+          int to = half * S::kCols % static_cast<int>(splits), i = half * S::kCols / static_cast<int>(splits);
+          const uint32_t at = smem_u32(parts) + (split * 2 * own * kBlockO + row) * 4;
 #pragma unroll
-        for (int side = 0; side < 2; ++side)
-#pragma unroll
-          for (int j = 0; j < S::kCols; j += 2) {
-            float v[2];
-            unpair(acc[side][j / 2], v[0], v[1]);
-            mine[(side * NT + half * S::kCols + j) * kBlockO] = v[0];
-            mine[(side * NT + half * S::kCols + j + 1) * kBlockO] = v[1];
+          for (int j = 0; j < S::kCols; ++j) {
+            float g[2], u[2];
+            unpair(acc[0][j / 2], g[0], g[1]);
+            unpair(acc[1][j / 2], u[0], u[1]);
+            if (j < live) {
+              const uint32_t peer = peer_address(at + i * kBlockO * 4, to);
+              peer_store(peer, g[j & 1]);
+              peer_store(peer + own * kBlockO * 4, u[j & 1]);
+            }
+            if (++to == static_cast<int>(splits)) {
+              to = 0;
+              ++i;
+            }
           }
+        }
       }
     }
   }
   if (!ok && a.status) atomicOr(a.status, static_cast<int>(kStatusWaitTimeout));
   __syncwarp();
-  if (splits > 1) {
+  if (NT < 128 && splits > 1) {
+    if (!joined) cluster_wait();
     cluster_arrive();
     cluster_wait();
-    if (warp >= kFirstAdder) {  // a CTA finishes every splits-th token
+    if (warp >= kFirstAdder) {
       const int row = 32 * (warp & 3) + lane, o = first % a.o_tiles * kBlockO + row, t0 = first / a.o_tiles * NT;
-      const uint32_t at = smem_u32(smem) + row * 4;
-      for (int j = split + static_cast<int>(splits) * ((warp - kFirstAdder) >> 2); j < NT && t0 + j < a.m; j += 2 * static_cast<int>(splits)) {
+      const int own = (NT + static_cast<int>(splits) - 1) / static_cast<int>(splits);
+      const float* part = reinterpret_cast<const float*>(parts) + row;
+      for (int i = (warp - kFirstAdder) >> 2; i < own; i += 2) {
+        const int j = split + i * static_cast<int>(splits), t = t0 + j;
+        if (j >= NT || t >= a.m) break;
         float g = 0.0f, u = 0.0f;
-        for (uint32_t r = 0; r < splits; ++r) {
-          g += peer_load(at + j * kBlockO * 4, r);
-          u += peer_load(at + (NT + j) * kBlockO * 4, r);
+        for (int r = 0; r < static_cast<int>(splits); ++r) {
+          g += part[(r * 2 * own + i) * kBlockO];
+          u += part[((r * 2 + 1) * own + i) * kBlockO];
         }
         if (o < a.f) {
           if (!S::kWide && !grouped) {
-            g *= a.x_scale[t0 + j];
-            u *= a.x_scale[t0 + j];
+            g *= a.x_scale[t];
+            u *= a.x_scale[t];
           }
           const float v = (a.gelu ? activated<true, true>(g) : activated<false, true>(g)) * u;
-          const long long to = (t0 + j) * a.ld_out + o;
+          const long long to = t * a.ld_out + o;
           if (a.out_dtype == LB_F32) put(static_cast<float*>(a.out) + to, v);
           else if (a.out_dtype == LB_BF16) put(static_cast<__nv_bfloat16*>(a.out) + to, v);
           else put(static_cast<__half*>(a.out) + to, v);
         }
       }
     }
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
   }
   tc_fence_before();
   __syncthreads();
@@ -741,7 +795,7 @@ extern "C" int lb_op_w4_gated(const void* x, int64_t x_ld, int x_dtype, const fl
   a.k_blocks = (k + kBlockK - 1) / kBlockK;
   const long long tiles = static_cast<long long>(a.o_tiles) * a.t_tiles;
   if (tiles > 0x3fffffffll) return LB_ERR_CAPACITY;
-  int splits = static_cast<int>(tiles >= kSms ? 1 : kSms / tiles);
+  int splits = static_cast<int>(tiles >= kSms || nt == 128 ? 1 : kSms / tiles);
   if (splits > kMaxSplit) splits = kMaxSplit;
   if (splits > a.k_blocks) splits = a.k_blocks;
   CUtensorMap w_map, x_map;
