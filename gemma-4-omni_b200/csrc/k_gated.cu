@@ -32,7 +32,6 @@ constexpr int kCodeBytes = 2 * kSideBytes;     // gate and up
 constexpr int kABuffers = 4, kAColumn = 256, kAWidth = 64;  // widened codes in the tensor memory
 constexpr int kScaleRing = 4;
 constexpr int kWeightRing = 8;                 // units whose weights' scales are kept: more than the buffers reach ahead
-constexpr int kMaxSplit = 8;
 constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -53,7 +52,8 @@ struct Shape {
   static constexpr bool kWide = X == kXBf16 || X == kXF16;    // 16-bit operands
   static constexpr int kXBytes = NT * kBlockK * (kWide ? 2 : 1);
   static constexpr int kStage = kCodeBytes + kXBytes;
-  static constexpr int kParts = NT < 128 ? 2 * (NT + kMaxSplit) * kBlockO * 4 : 0;  // partial sums of the tokens that a CTA finishes
+  // partial sums of the groups of four tokens that a CTA finishes, from 2, 4 or 8 CTAs
+  static constexpr int kParts = NT < 128 ? 2 * (NT / 4) * kBlockO * 16 : 0;
   static constexpr int kRoom = 200 * 1024 - kParts;
   static constexpr int kStages = kRoom / kStage > 8 ? 8 : kRoom / kStage;
   static constexpr int kSmem = kStages * kStage + kParts + 1024;  // (up to 12 KB are declared beside it)
@@ -163,8 +163,8 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t at, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(rank));
   return peer;
 }
-__device__ __forceinline__ void peer_store(uint32_t at, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+__device__ __forceinline__ void peer_store(uint32_t at, pair_t a, pair_t b) {
+  asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(at), "l"(a), "l"(b) : "memory");
 }
 
 __device__ __forceinline__ pair_t pair_of(float a, float b) {
@@ -659,26 +659,25 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
         if (a.gelu) typed(std::true_type{});
         else typed(std::false_type{});
       } else {
-        // token j of the tile is finished by CTA j % splits, as its token j / splits: [source][side][token][row]
+        // the tile's four tokens from 4 q on are finished by CTA q % splits, as its group q / splits: [source][side][group][row][4]
+        // (stores of 16 bytes: a warp's store over the cluster takes some 27 cycles whatever its width)
         if (!joined) {  // (the others have begun)
           cluster_wait();
           joined = true;
         }
         if constexpr (NT < 128) {
-          const int own = (NT + static_cast<int>(splits) - 1) / static_cast<int>(splits), live = min(S::kCols, a.m - t0);
-          int to = half * S::kCols % static_cast<int>(splits), i = half * S::kCols / static_cast<int>(splits);
-          const uint32_t at = smem_u32(parts) + (split * 2 * own * kBlockO + row) * 4;
+          const int n = static_cast<int>(splits), own = (NT / 4 + n - 1) / n, first_q = half * S::kCols / 4;
+          const int live = (min(S::kCols, a.m - t0) + 3) / 4;
+          int to = first_q % n, i = first_q / n;
+          const uint32_t at = smem_u32(parts) + (split * 2 * own * kBlockO + row) * 16;
 #pragma unroll
-          for (int j = 0; j < S::kCols; ++j) {
-            float g[2], u[2];
-            unpair(acc[0][j / 2], g[0], g[1]);
-            unpair(acc[1][j / 2], u[0], u[1]);
-            if (j < live) {
-              const uint32_t peer = peer_address(at + i * kBlockO * 4, to);
-              peer_store(peer, g[j & 1]);
-              peer_store(peer + own * kBlockO * 4, u[j & 1]);
+          for (int q = 0; q < S::kCols / 4; ++q) {
+            if (q < live) {
+              const uint32_t peer = peer_address(at + i * kBlockO * 16, to);
+              peer_store(peer, acc[0][2 * q], acc[0][2 * q + 1]);
+              peer_store(peer + own * kBlockO * 16, acc[1][2 * q], acc[1][2 * q + 1]);
             }
-            if (++to == static_cast<int>(splits)) {
+            if (++to == n) {
               to = 0;
               ++i;
             }
@@ -695,23 +694,27 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
     cluster_wait();
     if (warp >= kFirstAdder) {
       const int row = 32 * (warp & 3) + lane, o = first % a.o_tiles * kBlockO + row, t0 = first / a.o_tiles * NT;
-      const int own = (NT + static_cast<int>(splits) - 1) / static_cast<int>(splits);
-      const float* part = reinterpret_cast<const float*>(parts) + row;
+      const int n = static_cast<int>(splits), own = (NT / 4 + n - 1) / n;
+      const float4* part = reinterpret_cast<const float4*>(parts) + row;
       for (int i = (warp - kFirstAdder) >> 2; i < own; i += 2) {
-        const int j = split + i * static_cast<int>(splits), t = t0 + j;
+        const int j = 4 * (split + i * n), t = t0 + j;
         if (j >= NT || t >= a.m) break;
-        float g = 0.0f, u = 0.0f;
-        for (int r = 0; r < static_cast<int>(splits); ++r) {
-          g += part[(r * 2 * own + i) * kBlockO];
-          u += part[((r * 2 + 1) * own + i) * kBlockO];
+        float g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int r = 0; r < n; ++r) {
+          const float4 x = part[(r * 2 * own + i) * kBlockO], y = part[((r * 2 + 1) * own + i) * kBlockO];
+          g[0] += x.x, g[1] += x.y, g[2] += x.z, g[3] += x.w;
+          u[0] += y.x, u[1] += y.y, u[2] += y.z, u[3] += y.w;
         }
-        if (o < a.f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (o >= a.f || t + e >= a.m) break;
           if (!S::kWide && !grouped) {
-            g *= a.x_scale[t];
-            u *= a.x_scale[t];
+            const float xs = a.x_scale[t + e];
+            g[e] *= xs;
+            u[e] *= xs;
           }
-          const float v = (a.gelu ? activated<true, true>(g) : activated<false, true>(g)) * u;
-          const long long to = t * a.ld_out + o;
+          const float v = (a.gelu ? activated<true, true>(g[e]) : activated<false, true>(g[e])) * u[e];
+          const long long to = (t + e) * a.ld_out + o;
           if (a.out_dtype == LB_F32) put(static_cast<float*>(a.out) + to, v);
           else if (a.out_dtype == LB_BF16) put(static_cast<__nv_bfloat16*>(a.out) + to, v);
           else put(static_cast<__half*>(a.out) + to, v);
@@ -789,15 +792,26 @@ extern "C" int lb_op_w4_gated(const void* x, int64_t x_ld, int x_dtype, const fl
   if (ffn > (1 << 24) || m > (1 << 24) || x_ld > (1ll << 36)) return LB_ERR_CAPACITY;
   GatedArgs a{x_scale, static_cast<const __half*>(w_scale), out, ld_out, status, x_group == k ? 0 : x_group, m, ffn, k, group, out_dtype,
               activation, 0, 0, 0};
-  const int nt = m <= 32 ? 32 : m <= 64 ? 64 : 128;
   a.o_tiles = (ffn + kBlockO - 1) / kBlockO;
-  a.t_tiles = (m + nt - 1) / nt;
   a.k_blocks = (k + kBlockK - 1) / kBlockK;
-  const long long tiles = static_cast<long long>(a.o_tiles) * a.t_tiles;
-  if (tiles > 0x3fffffffll) return LB_ERR_CAPACITY;
-  int splits = static_cast<int>(tiles >= kSms || nt == 128 ? 1 : kSms / tiles);
-  if (splits > kMaxSplit) splits = kMaxSplit;
-  if (splits > a.k_blocks) splits = a.k_blocks;
+  // The width of a tile and the dealing out of K by an estimate of the time in tenths of a microsecond: a wave of tiles takes 4 us
+  // and for each block of K 0.67, 0.7 or 1 at 32, 64 or 128 tokens (1536 x 6144: 128 rows take 18 us as 48 tiles of 128 tokens, 14 as 96
+  // of 64; 499 rows 34 us as 192 of 128, some 43 as 384 of 64).  K is dealt out where all clusters fit the GPU at once: 2
+  // rows of 1536 x 6144 take 14 us whole, 10 in clusters of two, but 15 in clusters of three, not all of which fit.
+  int nt = 0, splits = 1;
+  long long best = 0;
+  for (const int width : {32, 64, 128}) {
+    const long long t_tiles = (m + width - 1) / width, tiles = a.o_tiles * t_tiles;
+    const int split = width == 128 ? 1 : tiles <= 16 && a.k_blocks >= 8 ? 8 : tiles <= 32 && a.k_blocks >= 4 ? 4 : tiles <= 74 && a.k_blocks >= 2 ? 2 : 1;
+    const long long time = (tiles * split + kSms - 1) / kSms * (40 + (width == 32 ? 67 : width == 64 ? 70 : 100) * ((a.k_blocks + split - 1) / split) / 10);
+    if (nt == 0 || time < best) {
+      nt = width;
+      splits = split;
+      best = time;
+    }
+  }
+  if (static_cast<long long>(a.o_tiles) * ((m + nt - 1) / nt) > 0x3fffffffll) return LB_ERR_CAPACITY;
+  a.t_tiles = (m + nt - 1) / nt;
   CUtensorMap w_map, x_map;
   const int64_t x_row = m > 1 ? x_ld * size : (static_cast<int64_t>(k) * size + 15) / 16 * 16;
   if (make_tensor_map_u8(&w_map, codes, k / 2, 2ull * ffn, 64, kBlockO) != 0 ||
