@@ -11,11 +11,13 @@
 // and u falls between two roundings of one of them the more rarely the finer they are.  2^45 * 2^18 tokens stay below 2^63.
 //
 // The logits are read once.  A cluster of CTAs takes a row, each CTA holds its part of it in shared
-// memory.  Nothing is sorted but the few hundred tokens around a cut: counts and masses by bins of the distance
-// to the maximum (64 to a unit of T, shared-memory atomics on whole numbers; a mass in three limbs of 16 bits), added up over
-// the cluster, say in which bin a cut lies.  If at most 512 tokens lie in and above it, as with the usual settings, one CTA gathers
-// and sorts them and finishes alone.  Otherwise the bin's tokens are sorted, or divided again where they are many; one value that
-// they all have is cut by index.
+// memory, each warp a part of that.  Nothing is sorted but the few hundred tokens around a cut: counts, and for top-p masses, by
+// bins of the distance to the maximum (shared-memory atomics on whole numbers; a mass in three limbs of 16 bits), added up
+// over the cluster, say in which bin a cut lies.  If at most 512 tokens lie in and above it, as with the usual settings, one CTA
+// gathers and sorts them and finishes alone.  Otherwise the bin's tokens are sorted, or divided again where they are many; one
+// value that they all have is cut by index.  What a cut leaves, each warp moves together in place, in the order of the indexes,
+// so that every later pass goes over that alone: for top-p the sum of all masses and a look at a few distances come first, and
+// only what lies above the distance behind the cut is divided into bins.
 #include <cooperative_groups.h>
 
 #include "../../include/listener_b200.h"
@@ -27,13 +29,16 @@ namespace lb {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kBins = 512;
 constexpr int kList = kThreads;       // tokens that are sorted
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxPart = kMaxVocab / kMaxCluster;  // tokens of a CTA
 constexpr int kTop = 45;              // log2 of the largest mass
 constexpr unsigned long long kNone = ~0ull;
+// Distances to the maximum, in units of T, between which a share's cut is looked for first.
+constexpr int kZones = 4;
+__host__ __device__ constexpr float zone_end(int z) { return z == 0 ? 4.0f : z == 1 ? 8.0f : z == 2 ? 11.0f : 14.0f; }
 
 typedef unsigned long long u64;
 
@@ -56,23 +61,31 @@ struct Result {  // of one division into bins
 
 struct Shared {
   double power[64];             // 2^(j / 64)
-  unsigned hist[4][kBins];      // counts; masses in limbs of 16 bits
+  union {
+    unsigned hist[4][kBins];    // counts; masses in limbs of 16 bits
+    u64 mass[kList];            // while tokens are sorted
+  };
   u64 list[kList];
-  u64 mass[kList];
   u64 scan[kWarps], scan2[kWarps];
+  unsigned zone[kWarps][kZones];
   // written by the other CTAs
   float top[kMaxCluster];
   u64 slice_mass[2][kMaxCluster];
   unsigned slice_count[2][kMaxCluster];
   Result result[2];
   unsigned low[kMaxCluster], high[kMaxCluster];
-  unsigned tie_count[2][kMaxCluster];
-  u64 part_mass[kMaxCluster];
+  unsigned tie_count[kMaxCluster];
+  u64 part_mass[kMaxCluster], zone_sum[kMaxCluster][kZones], above_mass[kMaxCluster];
+  unsigned above_count[kMaxCluster];
   int cut_index;
   float cut_value;
   unsigned listed;
   int at;
 };
+
+// (the struct, the logits, their indexes; by its symbol in every function, so that the accesses are known to be to shared memory)
+extern __shared__ __align__(16) unsigned char sample_smem[];
+#define LB_S (*reinterpret_cast<Shared*>(sample_smem))
 
 template <typename T>
 __device__ __forceinline__ float logit(T v) {  // a NaN is never drawn
@@ -95,7 +108,6 @@ __device__ __forceinline__ float from_ordered(unsigned u) {
 struct Masses {
   double top, scale;  // the maximum, log2(e) / T
   float top_f;
-  const double* power;
   __device__ __forceinline__ u64 operator()(float x) const {
     if (x == top_f) return 1ull << kTop;
     const double y = (static_cast<double>(x) - top) * scale;
@@ -105,16 +117,10 @@ struct Masses {
     const int n = __double2loint(t);         // 64 y, rounded
     const double f = (y - (t - magic)) * 0.69314718055994530942;
     double p = fma(f, fma(f, fma(f, fma(f, fma(f, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
-    const double w = power[n & 63];
+    const double w = LB_S.power[n & 63];
     p *= __hiloint2double(__double2hiint(w) + (((n >> 6) + kTop) << 20), __double2loint(w));
     return static_cast<u64>(__double_as_longlong(p + 4503599627370496.0)) & 0xfffffffffffffull;  // rint: below 2^51
   }
-};
-
-struct Cut {  // kept: what comes up to this token in the order (value down, index up)
-  float value;
-  int index;
-  __device__ __forceinline__ bool keeps(float x, int i) const { return x > value || (x == value && i <= index); }
 };
 
 __device__ __forceinline__ u64 warp_inclusive(u64 v) {
@@ -124,6 +130,11 @@ __device__ __forceinline__ u64 warp_inclusive(u64 v) {
     const u64 y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += y;
   }
+  return v;
+}
+__device__ __forceinline__ u64 warp_sum64(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 // by the whole CTA; total: of all threads
@@ -177,14 +188,61 @@ __device__ __forceinline__ u64 target_of(double u, u64 total) {  // floor(u * to
 
 // What all threads of a row's CTAs know.
 struct Row {
-  int row, n, first, k;      // this CTA's tokens: n from `first` on
-  const float* x;            // in shared memory
+  int row, first, k;         // first: the index of this CTA's first token
+  int pad, part;             // floats before its logits in shared memory; tokens of a CTA
   double u, top_p;
   u64 min_mass;
-  float bin_scale;
+  float floor;               // below it no token has min_mass
+  float inv_heat;
   Masses mass;
-  __device__ __forceinline__ int bin(float v) const {  // (a difference of two infinities is bin 0)
-    return min(kBins - 1, __float2int_rz((mass.top_f - v) * bin_scale));
+  __device__ __forceinline__ float distance(float v) const { return (mass.top_f - v) * inv_heat; }  // (NaN: of two infinities)
+  __device__ __forceinline__ float* logits() const { return reinterpret_cast<float*>(sample_smem + sizeof(Shared)) + pad; }
+  __device__ __forceinline__ uint16_t* indexes() const {
+    return reinterpret_cast<uint16_t*>(sample_smem + sizeof(Shared) + (part + 8) * sizeof(float));
+  }
+};
+
+// A warp's tokens that are left: at first all of its part of the CTA's tokens.
+struct Left {
+  int base, n;
+  bool moved;  // they have been moved together, and their indexes (less base) stand beside them
+  // body(logit, index in the CTA) for each, in order, lanes taking neighbours
+  template <typename Body>
+  __device__ __forceinline__ void each(const Row& r, Body body) const {
+    const float* x = r.logits() + base;
+    const int lane = threadIdx.x & 31;
+    if (moved) {
+      const uint16_t* at = r.indexes() + base;
+#pragma unroll 1
+      for (int j = lane; j < n; j += 32) body(x[j], base + at[j]);
+    } else {
+#pragma unroll 4
+      for (int j = lane; j < n; j += 32) body(x[j], base + j);
+    }
+  }
+  // moves those together that pred(logit, index in the CTA) picks
+  template <typename Pred>
+  __device__ __forceinline__ void keep(const Row& r, Pred pred) {
+    float* x = r.logits() + base;
+    uint16_t* at = r.indexes() + base;
+    const int lane = threadIdx.x & 31;
+    int kept = 0;
+    for (int j0 = 0; j0 < n; j0 += 32) {
+      const int j = j0 + lane;
+      const float v = j < n ? x[j] : 0.0f;
+      const int i = moved && j < n ? at[j] : j;
+      const bool take = j < n && pred(v, base + i);
+      const unsigned who = __ballot_sync(0xffffffffu, take);  // (everyone has read before anyone writes)
+      if (take) {
+        const int to = kept + __popc(who & ((1u << lane) - 1));
+        x[to] = v;
+        at[to] = static_cast<uint16_t>(i);
+      }
+      kept += __popc(who);
+      __syncwarp();
+    }
+    n = kept;
+    moved = true;
   }
 };
 
@@ -195,7 +253,8 @@ __device__ __forceinline__ void emit(const SampleArgs& a, const Row& r, int toke
 
 // One CTA has in s.list all tokens that can be drawn (n, in any order): the rest of the work.  k: of them the first k
 // count; limit: the mass up to which top-p keeps, 0 where it is to be taken from their own sum.
-__device__ __noinline__ void finish_list(const SampleArgs& a, const Row& r, Shared& s, int n, int k, u64 limit) {
+__device__ __forceinline__ void finish_list(const SampleArgs& a, const Row& r, int n, int k, u64 limit) {
+  Shared& s = LB_S;
   const int t = threadIdx.x;
   const u64 key = block_sort(t < n ? s.list[t] : kNone, s.mass);
   const float x = from_ordered(~static_cast<unsigned>(key >> 32));
@@ -216,62 +275,122 @@ __device__ __noinline__ void finish_list(const SampleArgs& a, const Row& r, Shar
   if (mine && target >= to - mine && target < to) emit(a, r, static_cast<int>(by_index >> 32), mine, total);
 }
 
-// Where the cut of the first k tokens (kMass false) or of a share of the masses (true) lies among the tokens that `kept` keeps.
-// Returns true where the row is done (the leading CTA had all that could be drawn in its list).
+// Cuts what is left to the first k tokens (kMass false), or to the first whose masses reach a share of the sum (true), in the
+// order (value down, index up).  Returns true where the leading CTA has all that can be drawn in its list, as finish_list takes it.
+struct Listed {
+  int n, k;
+  u64 limit;
+};
 template <bool kMass>
-__device__ __noinline__ bool select(const SampleArgs& a, const Row& r, Shared& s, cg::cluster_group& cluster, Cut& kept) {
-  const int t = threadIdx.x, rank = cluster.block_rank(), ctas = cluster.num_blocks();
-  const int slice = kBins / ctas, each = (slice + kThreads - 1) / kThreads;  // bins of a CTA and of a thread (at most 4)
+__device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster, Left& left, Listed& listed) {
+  Shared& s = LB_S;
+  const int t = threadIdx.x, rank = cluster.block_rank(), ctas = cluster.num_blocks(), lane = t & 31, warp = t >> 5;
+  const int slice = kBins / ctas;  // bins that a CTA adds up, at most one a thread
   u64 limit = kMass ? 0 : r.k, above = 0;
   int before = 0;
   unsigned lo = 0, hi = 0;
   int shift = 0;
-  // (each division leaves one value, or 2048 times fewer: five are never reached)
-  for (int level = 0; level < 5; ++level) {
+  // the first division: distances from zone_lo on
+  float zone_lo = 0.0f, zone_bins = 16.0f;
+  if constexpr (kMass) {
+    // the sum of all masses, and what comes of it up to some distances in 2^24 units, each token's part rounded down
+    u64 sum = 0;
+    unsigned zone[kZones];
+#pragma unroll
+    for (int z = 0; z < kZones; ++z) zone[z] = 0;
+    left.each(r, [&](float x, int) {
+      const u64 m = r.mass(x);
+      sum += m;
+      const unsigned about = static_cast<unsigned>(m >> 24);
+      const float d = r.distance(x);
+#pragma unroll
+      for (int z = 0; z < kZones; ++z) zone[z] += d >= zone_end(z) ? 0u : about;
+    });
+#pragma unroll
+    for (int z = 0; z < kZones; ++z) {  // (2^12 tokens a warp, each at most 2^21)
+      const u64 all = warp_sum64(zone[z]);
+      if (lane == 0) s.zone[warp][z] = static_cast<unsigned>(all >> 3);
+    }
+    u64 total;
+    block_inclusive(sum, s.scan, total);  // (a barrier for the zones too)
+    if (t < ctas) {
+      *cluster.map_shared_rank(&s.part_mass[rank], t) = total;
+#pragma unroll
+      for (int z = 0; z < kZones; ++z) {
+        u64 v = 0;
+        for (int w = 0; w < kWarps; ++w) v += s.zone[w][z];
+        *cluster.map_shared_rank(&s.zone_sum[rank][z], t) = v;
+      }
+    }
+    cluster.sync();
+    total = 0;
+    for (int c = 0; c < ctas; ++c) total += s.part_mass[c];
+    limit = share_of(r.top_p, total);
+    // The sums are in units of 2^27, each short of its true value by less than 2^16 of them: a unit for each of 2^18 tokens and each warp.
+    const u64 want = limit >> 27;
+    float zone_hi = INFINITY;
+#pragma unroll
+    for (int z = kZones - 1; z >= 0; --z) {
+      u64 v = 0;
+      for (int c = 0; c < ctas; ++c) v += s.zone_sum[c][z];
+      if (v > want) zone_hi = zone_end(z);
+      if (zone_lo == 0.0f && v + (1u << 16) < want) zone_lo = zone_end(z);
+    }
+    zone_bins = zone_hi < INFINITY ? kBins / (zone_hi - zone_lo) : 16.0f;
+    left.keep(r, [&](float x, int) { return !(r.distance(x) >= zone_hi); });
+  }
+  for (int level = 0; level < 6; ++level) {  // (each division leaves one value, or 512 times fewer: six are never reached)
     const int turn = level & 1;
     // ---- tokens and masses by bins
     for (int i = t; i < (kMass ? 4 : 1) * kBins; i += kThreads) (&s.hist[0][0])[i] = 0;
     if (t == 0) s.listed = 0;
     __syncthreads();
-    const auto bin_of = [&](float x, int i) -> int {  // or -1
-      if (!(x > -INFINITY) || !kept.keeps(x, r.first + i)) return -1;
-      if (level == 0) return r.bin(x);
+    const auto bin_of = [&](float x) -> int {  // -1: below, -2: above
+      if (level == 0) {
+        const float d = r.distance(x);
+        return d >= INFINITY ? -1 : d < zone_lo ? -2 : min(kBins - 1, __float2int_rz((d - zone_lo) * zone_bins));
+      }
       const unsigned o = ordered(x);
-      return o < lo || o > hi ? -1 : static_cast<int>((hi - o) >> shift);
+      return o < lo ? -1 : o > hi ? -2 : static_cast<int>((hi - o) >> shift);
     };
-    for (int i = t; i < r.n; i += kThreads) {
-      const float x = r.x[i];
-      const int b = bin_of(x, i);
-      if (b < 0) continue;
-      atomicAdd(&s.hist[0][b], 1u);
+    u64 over = 0;  // of the tokens above the zone
+    unsigned over_count = 0;
+    left.each(r, [&](float x, int) {
+      const int b = bin_of(x);
+      if (b >= 0) atomicAdd(&s.hist[0][b], 1u);
       if constexpr (kMass) {
+        if (b == -1) return;
+        if (b == -2 && level > 0) return;
         const u64 m = r.mass(x);
-        const unsigned m0 = m & 0xffff, m1 = (m >> 16) & 0xffff, m2 = static_cast<unsigned>(m >> 32);
-        if (m0) atomicAdd(&s.hist[1][b], m0);
-        if (m1) atomicAdd(&s.hist[2][b], m1);
-        if (m2) atomicAdd(&s.hist[3][b], m2);
+        if (b >= 0) {
+          const unsigned m0 = m & 0xffff, m1 = (m >> 16) & 0xffff, m2 = static_cast<unsigned>(m >> 32);
+          if (m0) atomicAdd(&s.hist[1][b], m0);
+          if (m1) atomicAdd(&s.hist[2][b], m1);
+          if (m2) atomicAdd(&s.hist[3][b], m2);
+        } else {
+          over += m;
+          ++over_count;
+        }
+      }
+    });
+    if (kMass && level == 0) {
+      u64 count;
+      block_inclusive(over, s.scan, over);
+      block_inclusive(over_count, s.scan2, count);
+      if (t < ctas) {
+        *cluster.map_shared_rank(&s.above_mass[rank], t) = over;
+        *cluster.map_shared_rank(&s.above_count[rank], t) = static_cast<unsigned>(count);
       }
     }
     cluster.sync();
     // ---- each CTA adds up a slice of the bins over the cluster
-    u64 bin_mass[4];
-    unsigned bin_count[4];
     u64 my_mass = 0;
     unsigned my_count = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bin_mass[j] = 0;
-      bin_count[j] = 0;
-      if (j < each && t * each + j < slice) {
-        const int b = rank * slice + t * each + j;
-        for (int c = 0; c < ctas; ++c) {
-          const unsigned* h = cluster.map_shared_rank(&s.hist[0][0], c);
-          bin_count[j] += h[b];
-          if constexpr (kMass)
-            bin_mass[j] += h[kBins + b] + (static_cast<u64>(h[2 * kBins + b]) << 16) + (static_cast<u64>(h[3 * kBins + b]) << 32);
-        }
-        my_mass += bin_mass[j];
-        my_count += bin_count[j];
+    if (t < slice) {
+      for (int c = 0; c < ctas; ++c) {
+        const unsigned* h = cluster.map_shared_rank(&s.hist[0][0], c) + rank * slice + t;
+        my_count += h[0];
+        if constexpr (kMass) my_mass += h[kBins] + (static_cast<u64>(h[2 * kBins]) << 16) + (static_cast<u64>(h[3 * kBins]) << 32);
       }
     }
     u64 slice_count, slice_mass = 0, upto_mass = 0;
@@ -282,33 +401,28 @@ __device__ __noinline__ bool select(const SampleArgs& a, const Row& r, Shared& s
       *cluster.map_shared_rank(&s.slice_mass[turn][rank], t) = slice_mass;
     }
     cluster.sync();
-    u64 base_mass = 0, all_mass = 0;
+    u64 base_mass = 0;
     unsigned base_count = 0, all_count = 0;
     for (int c = 0; c < ctas; ++c) {
       if (c < rank) {
         base_mass += s.slice_mass[turn][c];
         base_count += s.slice_count[turn][c];
       }
-      all_mass += s.slice_mass[turn][c];
       all_count += s.slice_count[turn][c];
+      if (kMass && level == 0) {
+        above += s.above_mass[c];
+        before += s.above_count[c];
+      }
     }
-    if (level == 0) {
-      if constexpr (kMass) limit = share_of(r.top_p, all_mass);
-      else if (limit > all_count) return false;  // no more than k tokens: all are kept
-    }
+    if (!kMass && level == 0 && limit > all_count) return false;  // no more than k tokens: all are kept
     // ---- the bin that holds the cut: one thread of one CTA finds it
     {
-      u64 w = above + (kMass ? base_mass + upto_mass - my_mass : base_count + upto_count - my_count);
-      unsigned n = before + base_count + static_cast<unsigned>(upto_count) - my_count;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u64 mine = kMass ? bin_mass[j] : bin_count[j];
-        if (w < limit && limit <= w + mine) {
-          const Result found{w, rank * slice + t * each + j, static_cast<int>(bin_count[j]), static_cast<int>(n)};
-          for (int c = 0; c < ctas; ++c) *cluster.map_shared_rank(&s.result[turn], c) = found;
-        }
-        w += mine;
-        n += bin_count[j];
+      const u64 w = above + (kMass ? base_mass + upto_mass - my_mass : base_count + upto_count - my_count);
+      const u64 mine = kMass ? my_mass : my_count;
+      if (w < limit && limit <= w + mine) {
+        const Result found{w, rank * slice + t, static_cast<int>(my_count),
+                           static_cast<int>(before + base_count + static_cast<unsigned>(upto_count) - my_count)};
+        for (int c = 0; c < ctas; ++c) *cluster.map_shared_rank(&s.result[turn], c) = found;
       }
     }
     cluster.sync();
@@ -316,123 +430,121 @@ __device__ __noinline__ bool select(const SampleArgs& a, const Row& r, Shared& s
     above = found.above;
     before = found.before;
     const bool all = found.before + found.count <= kList;  // everything down to the cut fits the list
+    const auto down_to = [&](float x) {
+      const int b = bin_of(x);
+      return b == -2 || (b >= 0 && b <= found.bin);
+    };
     if (all || found.count <= kList) {
       Shared& lead = *cluster.map_shared_rank(&s, 0);
-      const unsigned bin_top = hi - (static_cast<unsigned>(found.bin) << shift), span = (1u << shift) - 1;
-      const unsigned bin_low = bin_top - lo > span ? bin_top - span : lo;
-      const int lane = t & 31;
-      for (int i0 = t - lane; i0 < r.n; i0 += kThreads) {
-        const int i = i0 + lane;
-        bool take = false;
-        float x = 0.0f;
-        if (i < r.n) {
-          x = r.x[i];
-          if (all && level > 0) {  // also what was above the first division's bin
-            take = x > -INFINITY && kept.keeps(x, r.first + i) && ordered(x) >= bin_low;
-          } else {
-            const int b = bin_of(x, i);
-            take = b >= 0 && (all ? b <= found.bin : b == found.bin);
-          }
-        }
+      left.keep(r, [&](float x, int) { return down_to(x); });
+      const float* x = r.logits() + left.base;
+      const uint16_t* at = r.indexes() + left.base;
+      for (int j0 = 0; j0 < left.n; j0 += 32) {
+        const int j = j0 + lane;
+        const bool take = j < left.n && (all || bin_of(x[j]) == found.bin);
         const unsigned who = __ballot_sync(0xffffffffu, take);
         if (!who) continue;
-        unsigned at = 0;
-        if (lane == 0) at = atomicAdd(&lead.listed, __popc(who));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
-        if (take && at < kList) lead.list[at] = static_cast<u64>(~ordered(x)) << 32 | static_cast<unsigned>(r.first + i);
+        unsigned to = 0;
+        if (lane == 0) to = atomicAdd(&lead.listed, __popc(who));
+        to = __shfl_sync(0xffffffffu, to, 0) + __popc(who & ((1u << lane) - 1));
+        if (take && to < kList) lead.list[to] = static_cast<u64>(~ordered(x[j])) << 32 | static_cast<unsigned>(r.first + left.base + at[j]);
       }
       cluster.sync();
       if (all) {
-        if (rank == 0) finish_list(a, r, s, found.before + found.count, kMass ? kList : r.k, limit * kMass);
+        listed = {found.before + found.count, kMass ? kList : r.k, limit * kMass};
         return true;
       }
       if (rank == 0) {
         const u64 key = block_sort(t < found.count ? s.list[t] : kNone, s.mass);
-        const float x = from_ordered(~static_cast<unsigned>(key >> 32));
-        const u64 w = t < found.count ? (kMass ? r.mass(x) : 1) : 0;
+        const float v = from_ordered(~static_cast<unsigned>(key >> 32));
+        const u64 w = t < found.count ? (kMass ? r.mass(v) : 1) : 0;
         u64 total;
         const u64 to = above + block_inclusive(w, s.scan, total);
         if (to - w < limit && limit <= to) {
           for (int c = 0; c < ctas; ++c) {
-            *cluster.map_shared_rank(&s.cut_value, c) = x;
+            *cluster.map_shared_rank(&s.cut_value, c) = v;
             *cluster.map_shared_rank(&s.cut_index, c) = static_cast<int>(static_cast<unsigned>(key));
           }
         }
       }
       cluster.sync();
-      kept = {s.cut_value, s.cut_index};
-      return false;
-    }
-    // ---- too many: the bin's values are the next division's range
-    bool single;
-    if (level == 0) {
-      unsigned least = 0xffffffffu, most = 0;
-      for (int i = t; i < r.n; i += kThreads) {
-        const float x = r.x[i];
-        if (bin_of(x, i) == found.bin) {
-          least = min(least, ordered(x));
-          most = max(most, ordered(x));
+    } else {
+      // ---- too many: the bin's values are the next division's range
+      bool single;
+      if (level == 0) {
+        left.keep(r, [&](float x, int) { return down_to(x); });
+        unsigned least = 0xffffffffu, most = 0;
+        left.each(r, [&](float x, int) {
+          if (bin_of(x) == found.bin) {
+            least = min(least, ordered(x));
+            most = max(most, ordered(x));
+          }
+        });
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        __syncthreads();
+        if (lane == 0) s.scan[warp] = static_cast<u64>(most) << 32 | least;
+        __syncthreads();
+        if (t < ctas) {
+          for (int w = 0; w < kWarps; ++w) {
+            least = min(least, static_cast<unsigned>(s.scan[w]));
+            most = max(most, static_cast<unsigned>(s.scan[w] >> 32));
+          }
+          *cluster.map_shared_rank(&s.low[rank], t) = least;
+          *cluster.map_shared_rank(&s.high[rank], t) = most;
         }
+        cluster.sync();
+        lo = s.low[0];
+        hi = s.high[0];
+        for (int c = 1; c < ctas; ++c) {
+          lo = min(lo, s.low[c]);
+          hi = max(hi, s.high[c]);
+        }
+        single = lo == hi;
+      } else {
+        single = shift == 0;
+        hi -= static_cast<unsigned>(found.bin) << shift;
+        lo = hi - lo >= 1u << shift ? hi - ((1u << shift) - 1) : lo;
       }
-      least = __reduce_min_sync(0xffffffffu, least);
-      most = __reduce_max_sync(0xffffffffu, most);
-      __syncthreads();
-      if ((t & 31) == 0) s.scan[t >> 5] = static_cast<u64>(most) << 32 | least;
-      __syncthreads();
-      if (t < ctas) {
-        for (int w = 0; w < kWarps; ++w) {
-          least = min(least, static_cast<unsigned>(s.scan[w]));
-          most = max(most, static_cast<unsigned>(s.scan[w] >> 32));
+      if (!single) {
+        for (shift = 0; (hi - lo) >> shift >= kBins;) ++shift;
+        continue;
+      }
+      // ---- one value: so many of its tokens, the lowest indexes first
+      const float value = from_ordered(lo);
+      const u64 w = kMass ? r.mass(value) : 1;
+      const unsigned want = static_cast<unsigned>((limit - above + w - 1) / w);
+      unsigned ties = 0;
+      left.each(r, [&](float x, int) { ties += x == value; });
+      ties = __reduce_add_sync(0xffffffffu, ties);
+      u64 cta_ties;
+      const u64 upto = block_inclusive(lane == 31 ? ties : 0, s.scan, cta_ties);
+      if (t < ctas) *cluster.map_shared_rank(&s.tie_count[rank], t) = static_cast<unsigned>(cta_ties);
+      cluster.sync();
+      unsigned seen = 0;
+      for (int c = 0; c < rank; ++c) seen += s.tie_count[c];
+      seen += __shfl_sync(0xffffffffu, static_cast<unsigned>(upto), 31) - ties;  // before this warp
+      if (seen < want && want <= seen + ties) {
+        const float* x = r.logits() + left.base;
+        for (int j0 = 0; j0 < left.n; j0 += 32) {
+          const int j = j0 + lane;
+          const bool tie = j < left.n && x[j] == value;
+          const unsigned who = __ballot_sync(0xffffffffu, tie);
+          if (tie && seen + __popc(who & ((2u << lane) - 1)) == want) {
+            const int at = r.first + left.base + (left.moved ? r.indexes()[left.base + j] : j);
+            for (int c = 0; c < ctas; ++c) {
+              *cluster.map_shared_rank(&s.cut_value, c) = value;
+              *cluster.map_shared_rank(&s.cut_index, c) = at;
+            }
+          }
+          seen += __popc(who);
         }
-        *cluster.map_shared_rank(&s.low[rank], t) = least;
-        *cluster.map_shared_rank(&s.high[rank], t) = most;
       }
       cluster.sync();
-      lo = s.low[0];
-      hi = s.high[0];
-      for (int c = 1; c < ctas; ++c) {
-        lo = min(lo, s.low[c]);
-        hi = max(hi, s.high[c]);
-      }
-      single = lo == hi;
-    } else {
-      single = shift == 0;
-      hi -= static_cast<unsigned>(found.bin) << shift;
-      lo = hi - lo >= 1u << shift ? hi - ((1u << shift) - 1) : lo;
     }
-    if (!single) {
-      for (shift = 0; (hi - lo) >> shift >= kBins;) ++shift;
-      continue;
-    }
-    // ---- one value: so many of its tokens, the lowest indexes first
-    const float x = from_ordered(lo);
-    const u64 w = kMass ? r.mass(x) : 1;
-    const unsigned want = static_cast<unsigned>((limit - above + w - 1) / w);
-    unsigned ties = 0;
-    const int seg = ((a.part + kWarps - 1) / kWarps + 31) / 32 * 32, lane = t & 31, warp = t >> 5;
-    const int from = min(r.n, warp * seg), to = min(r.n, from + seg);
-    for (int i = from + lane; i < to; i += 32) ties += r.x[i] == x && kept.keeps(x, r.first + i);
-    ties = __reduce_add_sync(0xffffffffu, ties);
-    u64 cta_ties;
-    const u64 upto = block_inclusive(lane == 31 ? ties : 0, s.scan, cta_ties);
-    if (t < ctas) *cluster.map_shared_rank(&s.tie_count[turn][rank], t) = static_cast<unsigned>(cta_ties);
-    cluster.sync();
-    unsigned seen = 0;
-    for (int c = 0; c < rank; ++c) seen += s.tie_count[turn][c];
-    seen += __shfl_sync(0xffffffffu, static_cast<unsigned>(upto), 31) - ties;  // before this warp
-    if (seen < want && want <= seen + ties) {
-      for (int i0 = from; i0 < to; i0 += 32) {
-        const int i = i0 + lane;
-        const bool tie = i < to && r.x[i] == x && kept.keeps(x, r.first + i);
-        const unsigned who = __ballot_sync(0xffffffffu, tie);
-        if (tie && seen + __popc(who & ((2u << lane) - 1)) == want) {
-          for (int c = 0; c < ctas; ++c) *cluster.map_shared_rank(&s.cut_index, c) = r.first + i;
-        }
-        seen += __popc(who);
-      }
-    }
-    cluster.sync();
-    kept = {x, s.cut_index};
+    const float cut = s.cut_value;
+    const int cut_index = s.cut_index;
+    left.keep(r, [&](float x, int i) { return x > cut || (x == cut && r.first + i <= cut_index); });
     return false;
   }
   return false;
@@ -440,23 +552,23 @@ __device__ __noinline__ bool select(const SampleArgs& a, const Row& r, Shared& s
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
-  __shared__ Shared s;
-  extern __shared__ __align__(16) float x_raw[];
+  Shared& s = LB_S;
   cg::cluster_group cluster = cg::this_cluster();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int rank = cluster.block_rank(), ctas = cluster.num_blocks();
   Row r;
   r.row = blockIdx.x / ctas;
   r.first = min(a.vocab, rank * a.part);
-  r.n = min(a.vocab, r.first + a.part) - r.first;
+  r.part = a.part;
+  const int n = min(a.vocab, r.first + a.part) - r.first;
 
   // ---- this CTA's logits as floats; the aligned part by 16 bytes
   constexpr int kVec = 16 / sizeof(T);
   const T* src = static_cast<const T*>(a.logits) + r.row * a.row_stride + r.first;
-  const int head = min(r.n, static_cast<int>((16 - reinterpret_cast<uintptr_t>(src) % 16) % 16 / sizeof(T)));
-  const int vecs = (r.n - head) / kVec, pad = (kVec - head) % kVec;
-  float* x = x_raw + pad;
-  r.x = x;
+  const int head = min(n, static_cast<int>((16 - reinterpret_cast<uintptr_t>(src) % 16) % 16 / sizeof(T)));
+  const int vecs = (n - head) / kVec, pad = (kVec - head) % kVec;
+  r.pad = pad;
+  float* x = r.logits();
   float top = -INFINITY;
   const uint4* body = reinterpret_cast<const uint4*>(src + head);
   constexpr int kAhead = 4;
@@ -478,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       }
     }
   }
-  const int rest = r.n - head - vecs * kVec;
+  const int rest = n - head - vecs * kVec;
   if (t < head + rest) {
     const int i = t < head ? t : head + vecs * kVec + (t - head);
     x[i] = logit(src[i]);
@@ -506,8 +618,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   cluster.sync();
   top = s.top[0];
   for (int c = 1; c < ctas; ++c) top = fmaxf(top, s.top[c]);
-  r.mass = {static_cast<double>(top), 1.4426950408889634074 / static_cast<double>(heat), top, s.power};
-  r.bin_scale = fminf(64.0f / heat, 1e30f);
+  r.mass = {static_cast<double>(top), 1.4426950408889634074 / static_cast<double>(heat), top};
+  r.inv_heat = fminf(1.0f / heat, 1e30f);
+  r.floor = -INFINITY;
+  if (r.min_mass && top < INFINITY) {
+    const double reach = (kTop + 0.01 - log2(static_cast<double>(r.min_mass))) / r.mass.scale;  // a hundredth of an octave to spare
+    r.floor = __double2float_rd(static_cast<double>(top) - reach);
+  }
 
   if (top == -INFINITY) {  // nothing to draw from
     if (rank == 0 && t == 0) {
@@ -518,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   }
   if (greedy) {  // the lowest index of the maximum
     unsigned at = 0xffffffffu;
-    for (int i = t; i < r.n; i += kThreads)
+    for (int i = t; i < n; i += kThreads)
       if (x[i] == top) at = min(at, static_cast<unsigned>(r.first + i));
     at = __reduce_min_sync(0xffffffffu, at);
     __syncthreads();
@@ -536,32 +653,31 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     }
     return;
   }
-  if (a.vocab <= kList) {  // (one CTA)
-    const bool there = t < r.n && x[t] > -INFINITY;
+  const int seg = ((a.part + kWarps - 1) / kWarps + 31) / 32 * 32;
+  Left left{min(n, warp * seg), min(n, (warp + 1) * seg) - min(n, warp * seg), false};
+  Listed listed{kList, r.k, 0};
+  bool done = false;
+  if (a.vocab <= kList) {  // (one CTA; what cannot be drawn sorts behind the rest and has no mass)
+    const bool there = t < n && x[t] > -INFINITY;
     s.list[t] = there ? static_cast<u64>(~ordered(x[t])) << 32 | static_cast<unsigned>(t) : kNone;
-    finish_list(a, r, s, kList, r.k, 0);  // (what cannot be drawn sorts behind the rest and has no mass)
+    done = true;
+  }
+  if (!done && r.k < a.vocab) done = select<false>(r, cluster, left, listed);
+  if (!done && r.top_p < 1.0) done = select<true>(r, cluster, left, listed);
+  if (done) {
+    if (rank == 0) finish_list(a, r, listed.n, listed.k, listed.limit);
     return;
   }
-  Cut kept{-INFINITY, 0x7fffffff};
-  if (r.k < a.vocab && select<false>(a, r, s, cluster, kept)) return;
-  if (r.top_p < 1.0 && select<true>(a, r, s, cluster, kept)) return;
 
-  // ---- the kept masses in the order of the indexes: by warps, by CTAs, and the part with the target once more
-  const int seg = ((a.part + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const auto kept_mass = [&](int i) -> u64 {
-    const float v = x[i];
-    if (!kept.keeps(v, r.first + i)) return 0;
+  // ---- the kept masses in the order of the indexes: by warps, by CTAs, and the warp with the target once more
+  if (r.min_mass) left.keep(r, [&](float v, int) { return v >= r.floor; });
+  const auto mass_of = [&](float v) -> u64 {
     const u64 m = r.mass(v);
     return m >= r.min_mass ? m : 0;
   };
-  const auto warp_mass = [&](int from, int to) {
-    u64 sum = 0;
-    for (int i = from + lane; i < to; i += 32) sum += kept_mass(i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
-  };
-  u64 mine = warp_mass(min(r.n, warp * seg), min(r.n, (warp + 1) * seg)), cta_mass;
+  u64 mine = 0, cta_mass;
+  left.each(r, [&](float v, int) { mine += mass_of(v); });
+  mine = warp_sum64(mine);
   u64 upto = __shfl_sync(0xffffffffu, block_inclusive(lane == 31 ? mine : 0, s.scan, cta_mass), 31);
   if (t < ctas) *cluster.map_shared_rank(&s.part_mass[rank], t) = cta_mass;
   cluster.sync();
@@ -572,23 +688,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   }
   const u64 target = target_of(r.u, total);
   if (target < base || target >= base + cta_mass) return;
-  if (base + upto - mine <= target && target < base + upto && lane == 0) {
-    s.at = warp * seg;
-    s.mass[0] = base + upto - mine;
+  if (base + upto - mine <= target && target < base + upto) {  // this warp's tokens, which all warps share now
+    if (lane == 0) {
+      s.at = warp;
+      s.list[0] = base + upto - mine;
+      s.list[1] = static_cast<u64>(left.base) << 32 | static_cast<unsigned>(left.n) << 1 | (left.moved ? 1u : 0u);
+    }
   }
   __syncthreads();
-  const int start = s.at, sub = (seg / kWarps + 31) / 32 * 32;
-  base = s.mass[0];
-  const int from = min(r.n, min(start + seg, start + warp * sub)), to = min(r.n, min(start + seg, start + (warp + 1) * sub));
-  mine = warp_mass(from, to);
+  base = s.list[0];
+  const u64 where = s.list[1];
+  const int share = static_cast<int>(static_cast<unsigned>(where) >> 1), from_base = static_cast<int>(where >> 32);
+  const bool moved = where & 1;
+  const int sub = (share + kWarps * 32 - 1) / (kWarps * 32) * 32, from = min(share, warp * sub), to = min(share, from + sub);
+  mine = 0;
+  for (int j = from + lane; j < to; j += 32) mine += mass_of(x[from_base + j]);
+  mine = warp_sum64(mine);
   upto = base + __shfl_sync(0xffffffffu, block_inclusive(lane == 31 ? mine : 0, s.scan, cta_mass), 31);
   if (upto - mine <= target && target < upto) {
-    u64 done = upto - mine;
-    for (int i0 = from; i0 < to; i0 += 32) {
-      const u64 m = i0 + lane < to ? kept_mass(i0 + lane) : 0;
-      const u64 sum = done + warp_inclusive(m);
-      if (m && sum - m <= target && target < sum) emit(a, r, r.first + i0 + lane, m, total);
-      done = __shfl_sync(0xffffffffu, sum, 31);
+    u64 sum_before = upto - mine;
+    for (int j0 = from; j0 < to; j0 += 32) {
+      const int j = j0 + lane;
+      const u64 m = j < to ? mass_of(x[from_base + j]) : 0;
+      const u64 sum = sum_before + warp_inclusive(m);
+      if (m && sum - m <= target && target < sum)
+        emit(a, r, r.first + from_base + (moved ? r.indexes()[from_base + j] : j), m, total);
+      sum_before = __shfl_sync(0xffffffffu, sum, 31);
     }
   }
 }
@@ -597,12 +722,12 @@ template <typename T>
 cudaError_t launch(SampleArgs a, int ctas, cudaStream_t s) {
   const auto kernel = sample_kernel<T>;
   static std::atomic<unsigned long long> done{0};
-  cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), (kMaxPart + 8) * 4);
+  cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), static_cast<int>(sizeof(Shared)) + (kMaxPart + 8) * 6);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = static_cast<unsigned>(a.rows) * ctas;
   cfg.blockDim = kThreads;
-  cfg.dynamicSmemBytes = (a.part + 8) * sizeof(float);
+  cfg.dynamicSmemBytes = sizeof(Shared) + (a.part + 8) * (sizeof(float) + sizeof(uint16_t));
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
