@@ -29,12 +29,15 @@ namespace lb {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 512;
+constexpr int kBins = kThreads;
+constexpr int kGroups = 8, kGroupBins = kBins / kGroups;  // of bins
 constexpr int kList = kThreads;       // tokens that are sorted
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxPart = kMaxVocab / kMaxCluster;  // tokens of a CTA
 constexpr int kTop = 45;              // log2 of the largest mass
+constexpr int kPowers = 256;
+constexpr float kMaxHeat = 1e30f;     // so that 47 octaves stay inside the 32-bit numbers
 constexpr unsigned long long kNone = ~0ull;
 // Distances to the maximum, in units of T, between which a share's cut is looked for first.
 constexpr int kZones = 4;
@@ -59,8 +62,8 @@ struct Result {  // of one division into bins
   int bin, count, before;  // tokens in it and before it
 };
 
-struct Shared {
-  double power[64];             // 2^(j / 64)
+struct alignas(16) Shared {
+  double power[kPowers];        // 2^(j / kPowers)
   union {
     unsigned hist[4][kBins];    // counts; masses in limbs of 16 bits
     u64 mass[kList];            // while tokens are sorted
@@ -70,18 +73,21 @@ struct Shared {
   unsigned zone[kWarps][kZones];
   // written by the other CTAs
   float top[kMaxCluster];
-  u64 slice_mass[2][kMaxCluster];
-  unsigned slice_count[2][kMaxCluster];
-  Result result[2];
+  u64 group_mass[2][kGroups][kMaxCluster];
+  unsigned group_count[2][kGroups][kMaxCluster];
+  Result result;
+  unsigned warp_count[kWarps];
   unsigned low[kMaxCluster], high[kMaxCluster];
   unsigned tie_count[kMaxCluster];
-  u64 part_mass[kMaxCluster], zone_sum[kMaxCluster][kZones], above_mass[kMaxCluster];
-  unsigned above_count[kMaxCluster];
+  u64 part_mass[kMaxCluster], zone_sum[kZones][kMaxCluster], above_mass[kMaxCluster];
+  u64 above_count[kMaxCluster];
   int cut_index;
   float cut_value;
   unsigned listed;
   int at;
 };
+
+static_assert(sizeof(Shared) % 16 == 0, "the logits after it are stored 16 bytes at a time");
 
 // (the struct, the logits, their indexes; by its symbol in every function, so that the accesses are known to be to shared memory)
 extern __shared__ __align__(16) unsigned char sample_smem[];
@@ -104,24 +110,27 @@ __device__ __forceinline__ float from_ordered(unsigned u) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-// exp by a table of 64 powers of two and a Taylor series: |f ln 2| <= 0.0055, first term left out below 4e-17
+// 2^y by a table of 2^(j / 256) and a Taylor series in f, |f| <= 2^-9 (first term left out below 4e-17 of the result).
 struct Masses {
   double top, scale;  // the maximum, log2(e) / T
-  float top_f;
-  __device__ __forceinline__ u64 operator()(float x) const {
-    if (x == top_f) return 1ull << kTop;
-    const double y = (static_cast<double>(x) - top) * scale;
-    if (!(y > -47.0)) return 0;
-    const double magic = 105553116266496.0;  // 1.5 * 2^46: the sum's last bit is 2^-6
+  float top_f, least; // least: so far down that its mass, and all below it, is 0
+  // the mass in the low 52 bits; above them, always the same, the exponent of 2^52 (which the sum with it left there)
+  __device__ __forceinline__ u64 bits(float x) const {
+    const double y = (static_cast<double>(fmaxf(x, least)) - top) * scale;
+    const double magic = 26388279066624.0;  // 1.5 * 2^44: the sum's last bit is 2^-8
     const double t = y + magic;
-    const int n = __double2loint(t);         // 64 y, rounded
-    const double f = (y - (t - magic)) * 0.69314718055994530942;
-    double p = fma(f, fma(f, fma(f, fma(f, fma(f, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
-    const double w = LB_S.power[n & 63];
-    p *= __hiloint2double(__double2hiint(w) + (((n >> 6) + kTop) << 20), __double2loint(w));
-    return static_cast<u64>(__double_as_longlong(p + 4503599627370496.0)) & 0xfffffffffffffull;  // rint: below 2^51
+    const int n = __double2loint(t);        // 256 y, rounded
+    const double f = y - (t - magic);
+    constexpr double kLn2 = 0.69314718055994530942;
+    const double p = fma(f, fma(f, fma(f, fma(f, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0), kLn2 * kLn2 / 2.0), kLn2), 1.0);
+    const double w = LB_S.power[n & (kPowers - 1)];
+    // (the exponent goes up by whole powers of two)
+    const double v = p * __hiloint2double(__double2hiint(w) + ((n & ~(kPowers - 1)) << (20 - 8)) + (kTop << 20), __double2loint(w));
+    return static_cast<u64>(__double_as_longlong(v + 4503599627370496.0));  // rint: below 2^51
   }
+  __device__ __forceinline__ u64 operator()(float x) const { return bits(x) & 0xfffffffffffffull; }
 };
+constexpr u64 kExponent = 0x433ull << 52;  // of 2^52
 
 __device__ __forceinline__ u64 warp_inclusive(u64 v) {
   const int lane = threadIdx.x & 31;
@@ -144,14 +153,37 @@ __device__ __forceinline__ u64 block_inclusive(u64 v, u64* scan, u64& total) {
   __syncthreads();
   if (lane == 31) scan[warp] = v;
   __syncthreads();
-  u64 before = 0;
-  total = 0;
+  u64 sums = lane < kWarps ? scan[lane] : 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += scan[w];
-    total += scan[w];
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const u64 y = __shfl_up_sync(0xffffffffu, sums, o);
+    if (lane >= o) sums += y;
   }
-  return v + before;
+  total = __shfl_sync(0xffffffffu, sums, kWarps - 1);
+  const u64 before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
+  return warp ? v + before : v;
+}
+// the sum alone
+__device__ __forceinline__ u64 block_sum(u64 v, u64* scan) {
+  const int lane = threadIdx.x & 31;
+  v = warp_sum64(v);
+  __syncthreads();
+  if (lane == 0) scan[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_sum64(lane < kWarps ? scan[lane] : 0);
+}
+// over the CTAs of the cluster, one value each (by a warp): the sum, and of those before `rank`
+__device__ __forceinline__ u64 slot_sum(const u64* slot, int ctas, int rank, u64& before) {
+  const int lane = threadIdx.x & 31;
+  const u64 v = lane < ctas ? slot[lane] : 0;
+  u64 all = v, low = lane < rank ? v : 0;
+#pragma unroll
+  for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    low += __shfl_xor_sync(0xffffffffu, low, o);
+  }
+  before = __shfl_sync(0xffffffffu, low, 0);
+  return __shfl_sync(0xffffffffu, all, 0);
 }
 // 512 values, one a thread, rising
 __device__ __forceinline__ u64 block_sort(u64 v, u64* room) {
@@ -193,7 +225,7 @@ struct Row {
   double u, top_p;
   u64 min_mass;
   float floor;               // below it no token has min_mass
-  float inv_heat;
+  float heat, inv_heat;
   Masses mass;
   __device__ __forceinline__ float distance(float v) const { return (mass.top_f - v) * inv_heat; }  // (NaN: of two infinities)
   __device__ __forceinline__ float* logits() const { return reinterpret_cast<float*>(sample_smem + sizeof(Shared)) + pad; }
@@ -226,20 +258,48 @@ struct Left {
     float* x = r.logits() + base;
     uint16_t* at = r.indexes() + base;
     const int lane = threadIdx.x & 31;
+    const unsigned before = (1u << lane) - 1;
     int kept = 0;
-    for (int j0 = 0; j0 < n; j0 += 32) {
-      const int j = j0 + lane;
-      const float v = j < n ? x[j] : 0.0f;
-      const int i = moved && j < n ? at[j] : j;
-      const bool take = j < n && pred(v, base + i);
-      const unsigned who = __ballot_sync(0xffffffffu, take);  // (everyone has read before anyone writes)
-      if (take) {
-        const int to = kept + __popc(who & ((1u << lane) - 1));
-        x[to] = v;
-        at[to] = static_cast<uint16_t>(i);
+    if (moved) {
+#pragma unroll 1
+      for (int j0 = 0; j0 < n; j0 += 32) {
+        const int j = j0 + lane;
+        const float v = j < n ? x[j] : 0.0f;
+        const int i = j < n ? at[j] : 0;
+        const bool take = j < n && pred(v, base + i);
+        const unsigned who = __ballot_sync(0xffffffffu, take);  // (everyone has read before anyone writes)
+        if (take) {
+          const int to = kept + __popc(who & before);
+          x[to] = v;
+          at[to] = static_cast<uint16_t>(i);
+        }
+        kept += __popc(who);
+        __syncwarp();
       }
-      kept += __popc(who);
-      __syncwarp();
+    } else {
+      constexpr int kLooks = 4;
+#pragma unroll 1
+      for (int j0 = 0; j0 < n; j0 += 32 * kLooks) {
+        float v[kLooks];
+        unsigned who[kLooks];
+#pragma unroll
+        for (int q = 0; q < kLooks; ++q) {
+          const int j = j0 + 32 * q + lane;
+          v[q] = j < n ? x[j] : 0.0f;
+          who[q] = __ballot_sync(0xffffffffu, j < n && pred(v[q], base + j));
+        }
+#pragma unroll
+        for (int q = 0; q < kLooks; ++q) {
+          if (who[q] == 0) continue;
+          if (who[q] >> lane & 1u) {
+            const int to = kept + __popc(who[q] & before);
+            x[to] = v[q];
+            at[to] = static_cast<uint16_t>(j0 + 32 * q + lane);
+          }
+          kept += __popc(who[q]);
+        }
+        __syncwarp();
+      }
     }
     n = kept;
     moved = true;
@@ -285,59 +345,64 @@ template <bool kMass>
 __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster, Left& left, Listed& listed) {
   Shared& s = LB_S;
   const int t = threadIdx.x, rank = cluster.block_rank(), ctas = cluster.num_blocks(), lane = t & 31, warp = t >> 5;
-  const int slice = kBins / ctas;  // bins that a CTA adds up, at most one a thread
   u64 limit = kMass ? 0 : r.k, above = 0;
   int before = 0;
   unsigned lo = 0, hi = 0;
   int shift = 0;
   // the first division: distances from zone_lo on
-  float zone_lo = 0.0f, zone_bins = 16.0f;
+  float zone_lo = 0.0f, zone_top = INFINITY, zone_bins = 16.0f;
   if constexpr (kMass) {
     // the sum of all masses, and what comes of it up to some distances in 2^24 units, each token's part rounded down
     u64 sum = 0;
     unsigned zone[kZones];
 #pragma unroll
     for (int z = 0; z < kZones; ++z) zone[z] = 0;
-    left.each(r, [&](float x, int) {
-      const u64 m = r.mass(x);
-      sum += m;
-      const unsigned about = static_cast<unsigned>(m >> 24);
-      const float d = r.distance(x);
+    float end[kZones];
 #pragma unroll
-      for (int z = 0; z < kZones; ++z) zone[z] += d >= zone_end(z) ? 0u : about;
+    for (int z = 0; z < kZones; ++z) end[z] = r.mass.top_f - zone_end(z) * r.heat;
+    left.each(r, [&](float x, int) {
+      const u64 m = r.mass.bits(x);
+      sum += m;
+      const unsigned about = static_cast<unsigned>(m >> 24) & ((1u << 28) - 1);
+#pragma unroll
+      for (int z = 0; z < kZones; ++z) zone[z] += x > end[z] ? about : 0u;
     });
+    sum -= static_cast<u64>(lane < left.n ? (left.n - lane + 31) / 32 : 0) * kExponent;
 #pragma unroll
     for (int z = 0; z < kZones; ++z) {  // (2^12 tokens a warp, each at most 2^21)
       const u64 all = warp_sum64(zone[z]);
       if (lane == 0) s.zone[warp][z] = static_cast<unsigned>(all >> 3);
     }
-    u64 total;
-    block_inclusive(sum, s.scan, total);  // (a barrier for the zones too)
+    u64 total = block_sum(sum, s.scan), none;  // (a barrier for the zones too)
     if (t < ctas) {
       *cluster.map_shared_rank(&s.part_mass[rank], t) = total;
 #pragma unroll
       for (int z = 0; z < kZones; ++z) {
         u64 v = 0;
         for (int w = 0; w < kWarps; ++w) v += s.zone[w][z];
-        *cluster.map_shared_rank(&s.zone_sum[rank][z], t) = v;
+        *cluster.map_shared_rank(&s.zone_sum[z][rank], t) = v;
       }
     }
     cluster.sync();
-    total = 0;
-    for (int c = 0; c < ctas; ++c) total += s.part_mass[c];
+    total = slot_sum(s.part_mass, ctas, 0, none);
     limit = share_of(r.top_p, total);
     // The sums are in units of 2^27, each short of its true value by less than 2^16 of them: a unit for each of 2^18 tokens and each warp.
     const u64 want = limit >> 27;
-    float zone_hi = INFINITY;
+    float zone_hi = INFINITY, low = r.mass.least;
 #pragma unroll
     for (int z = kZones - 1; z >= 0; --z) {
-      u64 v = 0;
-      for (int c = 0; c < ctas; ++c) v += s.zone_sum[c][z];
-      if (v > want) zone_hi = zone_end(z);
-      if (zone_lo == 0.0f && v + (1u << 16) < want) zone_lo = zone_end(z);
+      const u64 v = slot_sum(s.zone_sum[z], ctas, 0, none);
+      if (v > want) {
+        zone_hi = zone_end(z);
+        low = end[z];
+      }
+      if (zone_lo == 0.0f && v + (1u << 16) < want) {
+        zone_lo = zone_end(z);
+        zone_top = end[z];
+      }
     }
     zone_bins = zone_hi < INFINITY ? kBins / (zone_hi - zone_lo) : 16.0f;
-    left.keep(r, [&](float x, int) { return !(r.distance(x) >= zone_hi); });
+    left.keep(r, [&](float x, int) { return x > low; });
   }
   for (int level = 0; level < 6; ++level) {  // (each division leaves one value, or 512 times fewer: six are never reached)
     const int turn = level & 1;
@@ -348,7 +413,7 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
     const auto bin_of = [&](float x) -> int {  // -1: below, -2: above
       if (level == 0) {
         const float d = r.distance(x);
-        return d >= INFINITY ? -1 : d < zone_lo ? -2 : min(kBins - 1, __float2int_rz((d - zone_lo) * zone_bins));
+        return d >= INFINITY ? -1 : x > zone_top ? -2 : max(0, min(kBins - 1, __float2int_rz((d - zone_lo) * zone_bins)));
       }
       const unsigned o = ordered(x);
       return o < lo ? -1 : o > hi ? -2 : static_cast<int>((hi - o) >> shift);
@@ -374,59 +439,107 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
       }
     });
     if (kMass && level == 0) {
-      u64 count;
-      block_inclusive(over, s.scan, over);
-      block_inclusive(over_count, s.scan2, count);
+      over = block_sum(over, s.scan);
+      const u64 count = block_sum(over_count, s.scan2);
       if (t < ctas) {
         *cluster.map_shared_rank(&s.above_mass[rank], t) = over;
-        *cluster.map_shared_rank(&s.above_count[rank], t) = static_cast<unsigned>(count);
+        *cluster.map_shared_rank(&s.above_count[rank], t) = count;
       }
     }
-    cluster.sync();
-    // ---- each CTA adds up a slice of the bins over the cluster
-    u64 my_mass = 0;
-    unsigned my_count = 0;
-    if (t < slice) {
-      for (int c = 0; c < ctas; ++c) {
-        const unsigned* h = cluster.map_shared_rank(&s.hist[0][0], c) + rank * slice + t;
-        my_count += h[0];
-        if constexpr (kMass) my_mass += h[kBins] + (static_cast<u64>(h[2 * kBins]) << 16) + (static_cast<u64>(h[3 * kBins]) << 32);
-      }
-    }
-    u64 slice_count, slice_mass = 0, upto_mass = 0;
-    const u64 upto_count = block_inclusive(my_count, s.scan, slice_count);
-    if constexpr (kMass) upto_mass = block_inclusive(my_mass, s.scan2, slice_mass);
-    if (t < ctas) {
-      *cluster.map_shared_rank(&s.slice_count[turn][rank], t) = static_cast<unsigned>(slice_count);
-      *cluster.map_shared_rank(&s.slice_mass[turn][rank], t) = slice_mass;
-    }
-    cluster.sync();
-    u64 base_mass = 0;
-    unsigned base_count = 0, all_count = 0;
-    for (int c = 0; c < ctas; ++c) {
-      if (c < rank) {
-        base_mass += s.slice_mass[turn][c];
-        base_count += s.slice_count[turn][c];
-      }
-      all_count += s.slice_count[turn][c];
-      if (kMass && level == 0) {
-        above += s.above_mass[c];
-        before += s.above_count[c];
-      }
-    }
-    if (!kMass && level == 0 && limit > all_count) return false;  // no more than k tokens: all are kept
-    // ---- the bin that holds the cut: one thread of one CTA finds it
+    __syncthreads();
+    // ---- sums of groups of bins go to every CTA
     {
-      const u64 w = above + (kMass ? base_mass + upto_mass - my_mass : base_count + upto_count - my_count);
-      const u64 mine = kMass ? my_mass : my_count;
-      if (w < limit && limit <= w + mine) {
-        const Result found{w, rank * slice + t, static_cast<int>(my_count),
-                           static_cast<int>(before + base_count + static_cast<unsigned>(upto_count) - my_count)};
-        for (int c = 0; c < ctas; ++c) *cluster.map_shared_rank(&s.result[turn], c) = found;
+      const unsigned c = __reduce_add_sync(0xffffffffu, s.hist[0][t]);
+      u64 m = 0;
+      if constexpr (kMass) m = warp_sum64(s.hist[1][t] + (static_cast<u64>(s.hist[2][t]) << 16) + (static_cast<u64>(s.hist[3][t]) << 32));
+      if (lane == 0) {
+        s.warp_count[warp] = c;
+        s.scan[warp] = m;
       }
     }
+    __syncthreads();
+    if (t < kGroups * ctas) {
+      constexpr int kEach = kWarps / kGroups;
+      const int g = t % kGroups, to = t / kGroups;
+      unsigned c = 0;
+      u64 m = 0;
+#pragma unroll
+      for (int w = 0; w < kEach; ++w) {
+        c += s.warp_count[g * kEach + w];
+        m += s.scan[g * kEach + w];
+      }
+      *cluster.map_shared_rank(&s.group_count[turn][g][rank], to) = c;
+      if constexpr (kMass) *cluster.map_shared_rank(&s.group_mass[turn][g][rank], to) = m;
+    }
     cluster.sync();
-    const Result found = s.result[turn];
+    if (kMass && level == 0) {
+      u64 none;
+      above = slot_sum(s.above_mass, ctas, 0, none);
+      before = static_cast<int>(slot_sum(s.above_count, ctas, 0, none));
+    }
+    // ---- the group that holds the cut, then its bins over the cluster: every CTA finds the bin for itself
+    if (warp < 2) {  // kGroupBins threads
+      unsigned c = 0;
+      u64 m = 0;
+      if (lane < kGroups)
+        for (int q = 0; q < ctas; ++q) {
+          c += s.group_count[turn][lane][q];
+          if constexpr (kMass) m += s.group_mass[turn][lane][q];
+        }
+      unsigned upto_c = c;
+      u64 upto_m = m;
+#pragma unroll
+      for (int o = 1; o < kGroups; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, upto_c, o);
+        const u64 z = kMass ? __shfl_up_sync(0xffffffffu, upto_m, o) : 0;
+        if (lane >= o) {
+          upto_c += y;
+          upto_m += z;
+        }
+      }
+      const u64 to = above + (kMass ? upto_m : upto_c), mine = kMass ? m : c;
+      const unsigned who = __ballot_sync(0xffffffffu, lane < kGroups && to - mine < limit && limit <= to);
+      if (who) {
+        const int g = __ffs(who) - 1;
+        u64 base = __shfl_sync(0xffffffffu, to - mine, g);
+        unsigned seen = before + __shfl_sync(0xffffffffu, upto_c - c, g);
+        // both warps add up the group's first 32 bins, the second its own after them
+        u64 bin_w[2];
+        unsigned bin_c[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          bin_c[h] = 0;
+          u64 bin_m = 0;
+          if (h <= warp)
+            for (int q = 0; q < ctas; ++q) {
+              const unsigned* p = cluster.map_shared_rank(&s.hist[0][0], q) + g * kGroupBins + 32 * h + lane;
+              bin_c[h] += p[0];
+              if constexpr (kMass) bin_m += p[kBins] + (static_cast<u64>(p[2 * kBins]) << 16) + (static_cast<u64>(p[3 * kBins]) << 32);
+            }
+          bin_w[h] = kMass ? bin_m : bin_c[h];
+        }
+        if (warp == 1) {
+          base += warp_sum64(bin_w[0]);
+          seen += __reduce_add_sync(0xffffffffu, bin_c[0]);
+        }
+        const u64 w = warp ? bin_w[1] : bin_w[0];
+        const unsigned n = warp ? bin_c[1] : bin_c[0];
+        const u64 upto = base + warp_inclusive(w);
+        unsigned upto_n = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned y = __shfl_up_sync(0xffffffffu, upto_n, o);
+          if (lane >= o) upto_n += y;
+        }
+        if (upto - w < limit && limit <= upto)
+          s.result = {upto - w, g * kGroupBins + 32 * warp + lane, static_cast<int>(n), static_cast<int>(seen + upto_n - n)};
+      } else if (warp == 0 && lane == 0) {
+        s.result = {0, -1, 0, 0};  // (counts: fewer than the limit)
+      }
+    }
+    __syncthreads();
+    const Result found = s.result;
+    if (found.bin < 0) return false;  // no more than k tokens: all are kept
     above = found.above;
     before = found.before;
     const bool all = found.before + found.count <= kList;  // everything down to the cut fits the list
@@ -439,15 +552,22 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
       left.keep(r, [&](float x, int) { return down_to(x); });
       const float* x = r.logits() + left.base;
       const uint16_t* at = r.indexes() + left.base;
-      for (int j0 = 0; j0 < left.n; j0 += 32) {
-        const int j = j0 + lane;
-        const bool take = j < left.n && (all || bin_of(x[j]) == found.bin);
-        const unsigned who = __ballot_sync(0xffffffffu, take);
-        if (!who) continue;
+      int mine = 0;
+      if (all) mine = left.n;
+      else left.each(r, [&](float v, int) { mine += bin_of(v) == found.bin; });
+      if (!all) mine = __reduce_add_sync(0xffffffffu, mine);
+      if (mine > 0) {
         unsigned to = 0;
-        if (lane == 0) to = atomicAdd(&lead.listed, __popc(who));
-        to = __shfl_sync(0xffffffffu, to, 0) + __popc(who & ((1u << lane) - 1));
-        if (take && to < kList) lead.list[to] = static_cast<u64>(~ordered(x[j])) << 32 | static_cast<unsigned>(r.first + left.base + at[j]);
+        if (lane == 0) to = atomicAdd(&lead.listed, mine);
+        to = __shfl_sync(0xffffffffu, to, 0);
+        for (int j0 = 0; j0 < left.n; j0 += 32) {
+          const int j = j0 + lane;
+          const bool take = j < left.n && (all || bin_of(x[j]) == found.bin);
+          const unsigned who = __ballot_sync(0xffffffffu, take);
+          const unsigned place = to + __popc(who & ((1u << lane) - 1));
+          if (take && place < kList) lead.list[place] = static_cast<u64>(~ordered(x[j])) << 32 | static_cast<unsigned>(r.first + left.base + at[j]);
+          to += __popc(who);
+        }
       }
       cluster.sync();
       if (all) {
@@ -502,6 +622,7 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
         }
         single = lo == hi;
       } else {
+        cluster.sync();  // (the bins have been read everywhere)
         single = shift == 0;
         hi -= static_cast<unsigned>(found.bin) << shift;
         lo = hi - lo >= 1u << shift ? hi - ((1u << shift) - 1) : lo;
@@ -596,17 +717,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     x[i] = logit(src[i]);
     top = fmaxf(top, x[i]);
   }
-  if (t < 64) s.power[t] = exp2(static_cast<double>(t) / 64.0);
+  if (t < kPowers) s.power[t] = exp2(static_cast<double>(t) / kPowers);
 
   // ---- the row's settings and its maximum
-  const float heat = a.temperature ? a.temperature[r.row] : a.temperature1;
+  const float heat = fminf(a.temperature ? a.temperature[r.row] : a.temperature1, kMaxHeat);  // (NaN: the limit)
   const float p = a.top_p ? a.top_p[r.row] : a.top_p1, least = a.min_p ? a.min_p[r.row] : a.min_p1;
   r.k = a.top_k ? a.top_k[r.row] : a.top_k1;
   if (r.k <= 0 || r.k > a.vocab) r.k = a.vocab;
   r.top_p = p < 1.0f ? static_cast<double>(p) : 1.0;
   r.min_mass = least > 0.0f ? static_cast<u64>(ceil(static_cast<double>(fminf(least, 1.0f)) * static_cast<double>(1ull << kTop))) : 0;
   r.u = a.uniform64 ? static_cast<const double*>(a.uniform)[r.row] : static_cast<double>(static_cast<const float*>(a.uniform)[r.row]);
-  const bool greedy = !(heat > 0.0f);
+  const bool greedy = !(heat > 0.0f) || (a.temperature && a.temperature[r.row] != a.temperature[r.row]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) s.scan[warp] = __float_as_uint(top);
@@ -618,14 +739,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   cluster.sync();
   top = s.top[0];
   for (int c = 1; c < ctas; ++c) top = fmaxf(top, s.top[c]);
-  r.mass = {static_cast<double>(top), 1.4426950408889634074 / static_cast<double>(heat), top};
-  r.inv_heat = fminf(1.0f / heat, 1e30f);
-  r.floor = -INFINITY;
-  if (r.min_mass && top < INFINITY) {
-    const double reach = (kTop + 0.01 - log2(static_cast<double>(r.min_mass))) / r.mass.scale;  // a hundredth of an octave to spare
-    r.floor = __double2float_rd(static_cast<double>(top) - reach);
-  }
-
   if (top == -INFINITY) {  // nothing to draw from
     if (rank == 0 && t == 0) {
       a.tokens[r.row] = -1;
@@ -653,6 +766,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     }
     return;
   }
+  if (top == INFINITY) {  // infinities share the draw alone: they become 0, the rest nothing
+    for (int i = t; i < n; i += kThreads) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+    top = 0.0f;
+    __syncthreads();
+  }
+  r.heat = heat;
+  r.inv_heat = fminf(1.0f / heat, 1e30f);
+  // (where the next number below the top has no mass any more, no larger scale is needed: exponents stay above -150)
+  const double next = static_cast<double>(top) - static_cast<double>(nextafterf(top, -INFINITY));
+  r.mass = {static_cast<double>(top), fmin(1.4426950408889634074 / static_cast<double>(heat), 47.0 / next), top, 0.0f};
+  r.mass.least = __double2float_rd(static_cast<double>(top) - 47.0 / r.mass.scale);  // 2^-47 of the top's mass is 0
+  r.floor = -INFINITY;
+  if (r.min_mass)  // a hundredth of an octave to spare
+    r.floor = __double2float_rd(static_cast<double>(top) - (kTop + 0.01 - log2(static_cast<double>(r.min_mass))) / r.mass.scale);
   const int seg = ((a.part + kWarps - 1) / kWarps + 31) / 32 * 32;
   Left left{min(n, warp * seg), min(n, (warp + 1) * seg) - min(n, warp * seg), false};
   Listed listed{kList, r.k, 0};
@@ -676,16 +803,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     return m >= r.min_mass ? m : 0;
   };
   u64 mine = 0, cta_mass;
-  left.each(r, [&](float v, int) { mine += mass_of(v); });
+  if (r.min_mass) {
+    left.each(r, [&](float v, int) { mine += mass_of(v); });
+  } else {
+    left.each(r, [&](float v, int) { mine += r.mass.bits(v); });
+    mine -= static_cast<u64>(lane < left.n ? (left.n - lane + 31) / 32 : 0) * kExponent;
+  }
   mine = warp_sum64(mine);
   u64 upto = __shfl_sync(0xffffffffu, block_inclusive(lane == 31 ? mine : 0, s.scan, cta_mass), 31);
   if (t < ctas) *cluster.map_shared_rank(&s.part_mass[rank], t) = cta_mass;
   cluster.sync();
-  u64 base = 0, total = 0;
-  for (int c = 0; c < ctas; ++c) {
-    if (c < rank) base += s.part_mass[c];
-    total += s.part_mass[c];
-  }
+  u64 base;
+  const u64 total = slot_sum(s.part_mass, ctas, rank, base);
   const u64 target = target_of(r.u, total);
   if (target < base || target >= base + cta_mass) return;
   if (base + upto - mine <= target && target < base + upto) {  // this warp's tokens, which all warps share now
@@ -748,7 +877,7 @@ extern "C" int lb_op_sample(const void* logits, int64_t row_stride, int dtype, i
   using namespace lb;
   if (!logits || !uniform || !tokens || rows < 1 || vocab < 1 || row_stride < vocab) return LB_ERR_INVALID_ARGUMENT;
   if (dtype != LB_F32 && dtype != LB_BF16 && dtype != LB_F16) return LB_ERR_INVALID_ARGUMENT;
-  if (!temperature && !(temperature1 >= 0.0f && temperature1 <= 3.4e38f)) return LB_ERR_INVALID_ARGUMENT;
+  if (!temperature && !(temperature1 >= 0.0f && temperature1 <= kMaxHeat)) return LB_ERR_INVALID_ARGUMENT;
   if ((!top_p && !(top_p1 >= 0.0f)) || (!min_p && !(min_p1 >= 0.0f && min_p1 <= 1.0f))) return LB_ERR_INVALID_ARGUMENT;
   if (vocab > kMaxVocab || rows > (1 << 24)) return LB_ERR_CAPACITY;
   // 16384 tokens a CTA, 32768 beyond 131072

@@ -635,7 +635,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
         raise ValueError("uniform must be float32 or float64")
     _need(uniform, "uniform", uniform.dtype, (rows,), dev)
     settings = []
-    for name, value, dtype, low, high in (("temperature", temperature, torch.float32, 0.0, 3e38), ("top_k", top_k, torch.int32, 0, math.inf),
+    for name, value, dtype, low, high in (("temperature", temperature, torch.float32, 0.0, 1e30), ("top_k", top_k, torch.int32, 0, math.inf),
                                           ("top_p", top_p, torch.float32, 0.0, math.inf), ("min_p", min_p, torch.float32, 0.0, 1.0)):
         if isinstance(value, torch.Tensor):
             _need(value, name, dtype, (rows,), dev)

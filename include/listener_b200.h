@@ -556,8 +556,8 @@ int lb_op_head_norm_rotary(const void* q, int64_t q_token_stride, int64_t q_head
  *   min_p > 0:  of those, each with mass >= ceil(min_p * 2^45) stays
  *   the token: the first by index whose masses up to it exceed floor(uniform * their sum)
  * temperature 0: the lowest index of the maximum.  Settings by row (f32 / int32 [rows]), or the value after
- * each pointer where it is NULL; values of rows that are out of range count as 0 (temperature), none (top_k, top_p)
- * or the nearer end (min_p, uniform).  A NaN counts as -infinity, which is never drawn; infinities share the draw alone.  tokens int64
+ * each pointer where it is NULL.  temperature is at most 1e30.  Values of rows that are out of range: a temperature that is
+ * negative or NaN counts as 0, top_k and top_p as none, others as the nearer end.  A NaN counts as -infinity, which is never drawn; infinities share the draw alone.  tokens int64
  * [rows], -1 for a row with nothing to draw; logprobs f32 [rows] (or NULL): log of the token's part in what stayed
  * (greedy 0, nothing to draw -infinity).  vocab at most 262144. */
 int lb_op_sample(const void* logits, int64_t row_stride, int dtype, int rows, int vocab, const void* uniform,
