@@ -32,11 +32,12 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = kThreads;
 constexpr int kGroups = 8, kGroupBins = kBins / kGroups;  // of bins
 constexpr int kList = kThreads;       // tokens that are sorted
+constexpr int kFew = 96;              // of them, that are ranked instead (a sort takes as long as some 100)
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxPart = kMaxVocab / kMaxCluster;  // tokens of a CTA
 constexpr int kTop = 45;              // log2 of the largest mass
-constexpr int kPowers = 256;
+constexpr int kPowers = 128;
 constexpr float kMaxHeat = 1e30f;     // so that 47 octaves stay inside the 32-bit numbers
 constexpr unsigned long long kNone = ~0ull;
 // Distances to the maximum, in units of T, between which a share's cut is looked for first.
@@ -110,22 +111,22 @@ __device__ __forceinline__ float from_ordered(unsigned u) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-// 2^y by a table of 2^(j / 256) and a Taylor series in f, |f| <= 2^-9 (first term left out below 4e-17 of the result).
+// 2^y by a table of 2^(j / 128) and a Taylor series in f, |f| <= 2^-8 (first term left out below 2^-49 of the result).
 struct Masses {
   double top, scale;  // the maximum, log2(e) / T
   float top_f, least; // least: so far down that its mass, and all below it, is 0
   // the mass in the low 52 bits; above them, always the same, the exponent of 2^52 (which the sum with it left there)
   __device__ __forceinline__ u64 bits(float x) const {
     const double y = (static_cast<double>(fmaxf(x, least)) - top) * scale;
-    const double magic = 26388279066624.0;  // 1.5 * 2^44: the sum's last bit is 2^-8
+    const double magic = 52776558133248.0;  // 1.5 * 2^45: the sum's last bit is 2^-7
     const double t = y + magic;
-    const int n = __double2loint(t);        // 256 y, rounded
+    const int n = __double2loint(t);        // 128 y, rounded
     const double f = y - (t - magic);
     constexpr double kLn2 = 0.69314718055994530942;
     const double p = fma(f, fma(f, fma(f, fma(f, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0), kLn2 * kLn2 / 2.0), kLn2), 1.0);
     const double w = LB_S.power[n & (kPowers - 1)];
     // (the exponent goes up by whole powers of two)
-    const double v = p * __hiloint2double(__double2hiint(w) + ((n & ~(kPowers - 1)) << (20 - 8)) + (kTop << 20), __double2loint(w));
+    const double v = p * __hiloint2double(__double2hiint(w) + ((n & ~(kPowers - 1)) << (20 - 7)) + (kTop << 20), __double2loint(w));
     return static_cast<u64>(__double_as_longlong(v + 4503599627370496.0));  // rint: below 2^51
   }
   __device__ __forceinline__ u64 operator()(float x) const { return bits(x) & 0xfffffffffffffull; }
@@ -227,7 +228,8 @@ struct Row {
   float floor;               // below it no token has min_mass
   float heat, inv_heat;
   Masses mass;
-  __device__ __forceinline__ float distance(float v) const { return (mass.top_f - v) * inv_heat; }  // (NaN: of two infinities)
+  // Several passes have to put a token into the same bin, so nothing here may be contracted in one place and not in another.
+  __device__ __forceinline__ float distance(float v) const { return __fmul_rn(__fsub_rn(mass.top_f, v), inv_heat); }
   __device__ __forceinline__ float* logits() const { return reinterpret_cast<float*>(sample_smem + sizeof(Shared)) + pad; }
   __device__ __forceinline__ uint16_t* indexes() const {
     return reinterpret_cast<uint16_t*>(sample_smem + sizeof(Shared) + (part + 8) * sizeof(float));
@@ -359,7 +361,7 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
     for (int z = 0; z < kZones; ++z) zone[z] = 0;
     float end[kZones];
 #pragma unroll
-    for (int z = 0; z < kZones; ++z) end[z] = r.mass.top_f - zone_end(z) * r.heat;
+    for (int z = 0; z < kZones; ++z) end[z] = __fsub_rn(r.mass.top_f, __fmul_rn(zone_end(z), r.heat));
     left.each(r, [&](float x, int) {
       const u64 m = r.mass.bits(x);
       sum += m;
@@ -413,7 +415,7 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
     const auto bin_of = [&](float x) -> int {  // -1: below, -2: above
       if (level == 0) {
         const float d = r.distance(x);
-        return d >= INFINITY ? -1 : x > zone_top ? -2 : max(0, min(kBins - 1, __float2int_rz((d - zone_lo) * zone_bins)));
+        return d >= INFINITY ? -1 : x > zone_top ? -2 : max(0, min(kBins - 1, __float2int_rz(__fmul_rn(__fsub_rn(d, zone_lo), zone_bins))));
       }
       const unsigned o = ordered(x);
       return o < lo ? -1 : o > hi ? -2 : static_cast<int>((hi - o) >> shift);
@@ -478,68 +480,91 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
       before = static_cast<int>(slot_sum(s.above_count, ctas, 0, none));
     }
     // ---- the group that holds the cut, then its bins over the cluster: every CTA finds the bin for itself
-    if (warp < 2) {  // kGroupBins threads
+    int group = -1;
+    u64 base = 0;
+    unsigned seen = 0;
+    {
+      // a lane has a group and every fourth CTA
+      const int g = lane % kGroups;
       unsigned c = 0;
       u64 m = 0;
-      if (lane < kGroups)
-        for (int q = 0; q < ctas; ++q) {
-          c += s.group_count[turn][lane][q];
-          if constexpr (kMass) m += s.group_mass[turn][lane][q];
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; q += 32 / kGroups) {
+        const int from = q + lane / kGroups;
+        if (from < ctas) {
+          c += s.group_count[turn][g][from];
+          if constexpr (kMass) m += s.group_mass[turn][g][from];
         }
+      }
+#pragma unroll
+      for (int o = kGroups; o < 32; o <<= 1) {
+        c += __shfl_xor_sync(0xffffffffu, c, o);
+        if constexpr (kMass) m += __shfl_xor_sync(0xffffffffu, m, o);
+      }
       unsigned upto_c = c;
       u64 upto_m = m;
 #pragma unroll
       for (int o = 1; o < kGroups; o <<= 1) {
-        const unsigned y = __shfl_up_sync(0xffffffffu, upto_c, o);
-        const u64 z = kMass ? __shfl_up_sync(0xffffffffu, upto_m, o) : 0;
-        if (lane >= o) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, upto_c, o, kGroups);
+        const u64 z = kMass ? __shfl_up_sync(0xffffffffu, upto_m, o, kGroups) : 0;
+        if (g >= o) {
           upto_c += y;
           upto_m += z;
         }
       }
       const u64 to = above + (kMass ? upto_m : upto_c), mine = kMass ? m : c;
       const unsigned who = __ballot_sync(0xffffffffu, lane < kGroups && to - mine < limit && limit <= to);
-      if (who) {
-        const int g = __ffs(who) - 1;
-        u64 base = __shfl_sync(0xffffffffu, to - mine, g);
-        unsigned seen = before + __shfl_sync(0xffffffffu, upto_c - c, g);
-        // both warps add up the group's first 32 bins, the second its own after them
-        u64 bin_w[2];
-        unsigned bin_c[2];
+      if (who == 0) return false;  // (counts: no more than k tokens, all are kept)
+      group = __ffs(who) - 1;
+      base = __shfl_sync(0xffffffffu, to - mine, group);
+      seen = before + __shfl_sync(0xffffffffu, upto_c - c, group);
+    }
+    if (warp == 0) {  // two bins a lane
+      static_assert(kGroupBins == 64, "two bins a lane");
+      u64 w[2] = {0, 0};
+      unsigned n[2] = {0, 0};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          bin_c[h] = 0;
-          u64 bin_m = 0;
-          if (h <= warp)
-            for (int q = 0; q < ctas; ++q) {
-              const unsigned* p = cluster.map_shared_rank(&s.hist[0][0], q) + g * kGroupBins + 32 * h + lane;
-              bin_c[h] += p[0];
-              if constexpr (kMass) bin_m += p[kBins] + (static_cast<u64>(p[2 * kBins]) << 16) + (static_cast<u64>(p[3 * kBins]) << 32);
+      for (int q0 = 0; q0 < kMaxCluster; q0 += 4) {  // four CTAs' bins are under way at once
+        uint2 v[4][kMass ? 4 : 1];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q0 + q < ctas) {
+            const uint2* p = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&s.hist[0][0], q0 + q) + group * kGroupBins) + lane;
+#pragma unroll
+            for (int l = 0; l < (kMass ? 4 : 1); ++l) v[q][l] = p[l * (kBins / 2)];
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q0 + q < ctas) {
+            n[0] += v[q][0].x;
+            n[1] += v[q][0].y;
+            if constexpr (kMass) {
+              w[0] += v[q][1].x + (static_cast<u64>(v[q][2].x) << 16) + (static_cast<u64>(v[q][3].x) << 32);
+              w[1] += v[q][1].y + (static_cast<u64>(v[q][2].y) << 16) + (static_cast<u64>(v[q][3].y) << 32);
             }
-          bin_w[h] = kMass ? bin_m : bin_c[h];
+          }
         }
-        if (warp == 1) {
-          base += warp_sum64(bin_w[0]);
-          seen += __reduce_add_sync(0xffffffffu, bin_c[0]);
-        }
-        const u64 w = warp ? bin_w[1] : bin_w[0];
-        const unsigned n = warp ? bin_c[1] : bin_c[0];
-        const u64 upto = base + warp_inclusive(w);
-        unsigned upto_n = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned y = __shfl_up_sync(0xffffffffu, upto_n, o);
-          if (lane >= o) upto_n += y;
-        }
-        if (upto - w < limit && limit <= upto)
-          s.result = {upto - w, g * kGroupBins + 32 * warp + lane, static_cast<int>(n), static_cast<int>(seen + upto_n - n)};
-      } else if (warp == 0 && lane == 0) {
-        s.result = {0, -1, 0, 0};  // (counts: fewer than the limit)
       }
+      if constexpr (!kMass) {
+        w[0] = n[0];
+        w[1] = n[1];
+      }
+      u64 to = base + warp_inclusive(w[0] + w[1]);
+      unsigned upto_n = n[0] + n[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, upto_n, o);
+        if (lane >= o) upto_n += y;
+      }
+      to -= w[1];
+      if (to - w[0] < limit && limit <= to)
+        s.result = {to - w[0], group * kGroupBins + 2 * lane, static_cast<int>(n[0]), static_cast<int>(seen + upto_n - n[1] - n[0])};
+      if (to < limit && limit <= to + w[1])
+        s.result = {to, group * kGroupBins + 2 * lane + 1, static_cast<int>(n[1]), static_cast<int>(seen + upto_n - n[1])};
     }
     __syncthreads();
     const Result found = s.result;
-    if (found.bin < 0) return false;  // no more than k tokens: all are kept
     above = found.above;
     before = found.before;
     const bool all = found.before + found.count <= kList;  // everything down to the cut fits the list
@@ -575,14 +600,24 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
         return true;
       }
       if (rank == 0) {
-        const u64 key = block_sort(t < found.count ? s.list[t] : kNone, s.mass);
-        const float v = from_ordered(~static_cast<unsigned>(key >> 32));
-        const u64 w = t < found.count ? (kMass ? r.mass(v) : 1) : 0;
-        u64 total;
-        const u64 to = above + block_inclusive(w, s.scan, total);
+        u64 key = t < found.count ? s.list[t] : kNone, w, to;
+        if (found.count <= kFew) {  // each finds what comes before it
+          w = t < found.count ? (kMass ? r.mass(from_ordered(~static_cast<unsigned>(key >> 32))) : 1) : 0;
+          if (t < found.count) s.mass[t] = w;
+          __syncthreads();
+          to = above + w;
+          if (t < found.count)
+#pragma unroll 4
+            for (int j = 0; j < found.count; ++j) to += s.list[j] < key ? s.mass[j] : 0;
+        } else {
+          key = block_sort(key, s.mass);
+          w = t < found.count ? (kMass ? r.mass(from_ordered(~static_cast<unsigned>(key >> 32))) : 1) : 0;
+          u64 total;
+          to = above + block_inclusive(w, s.scan, total);
+        }
         if (to - w < limit && limit <= to) {
           for (int c = 0; c < ctas; ++c) {
-            *cluster.map_shared_rank(&s.cut_value, c) = v;
+            *cluster.map_shared_rank(&s.cut_value, c) = from_ordered(~static_cast<unsigned>(key >> 32));
             *cluster.map_shared_rank(&s.cut_index, c) = static_cast<int>(static_cast<unsigned>(key));
           }
         }
@@ -846,6 +881,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     }
   }
 }
+
+// two CTAs an SM at 16384 tokens: 228 KB, of which each takes one besides
+static_assert(sizeof(Shared) + (16384 + 8) * 6 <= 113 * 1024, "room");
 
 template <typename T>
 cudaError_t launch(SampleArgs a, int ctas, cudaStream_t s) {

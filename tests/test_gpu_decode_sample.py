@@ -104,6 +104,39 @@ def test_masked_rows_and_infinities(ops):
         check(ops, small, torch.tensor([0.9, 0.9], device="cuda"), **settings)
 
 
+def vectorised(x, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The rule over many rows at once, on the GPU: (tokens, log probabilities)."""
+    x, order = torch.sort(x.float(), dim=1, descending=True, stable=True)
+    t32 = [float(torch.tensor(v, dtype=F32)) for v in (temperature, top_p, min_p)]
+    mass = torch.round(torch.exp((x.double() - x[:, :1].double()) / t32[0]) * 2.0 ** 45).to(torch.int64)
+    if top_k:
+        mass[:, top_k:] = 0
+    upto = mass.cumsum(1)
+    if t32[1] < 1.0:
+        mass[upto - mass >= torch.ceil(t32[1] * upto[:, -1:].double()).to(torch.int64).clamp(min=1)] = 0
+    mass[mass < math.ceil(t32[2] * 2.0 ** 45)] = 0
+    mass = torch.zeros_like(mass).scatter_(1, order, mass)
+    upto = mass.cumsum(1)
+    total = upto[:, -1:]
+    target = torch.minimum(torch.floor(u.double()[:, None] * total.double()).to(torch.int64), total - 1)
+    token = torch.searchsorted(upto, target, right=True)
+    return token[:, 0], torch.log(mass.gather(1, token).double() / total.double())[:, 0]
+
+
+@pytest.mark.parametrize("settings", [dict(top_p=0.999, temperature=1.5), dict(top_p=0.9), dict(top_p=0.5, temperature=2.0),
+                                      dict(top_p=0.7, temperature=0.6), dict(top_k=3000), dict(top_k=20000, top_p=0.9),
+                                      dict(top_k=600, top_p=0.99, min_p=0.01), dict(min_p=0.001, temperature=3.0)])
+@pytest.mark.parametrize("vocab,dtype", [(262144, F32), (131072, F32), (131072, BF16), (20001, F32)])
+def test_cuts_in_every_place(ops, vocab, dtype, settings):
+    """Cuts deep in a row's bulk, 48 rows each: a token that one pass sees in another bin than the next pass moves a
+    cut by some ranks, which is 10^-6 of a total, so the totals are held to 10^-7 (the log's rounding and some)."""
+    x, u = logits_of(48, vocab, dtype, vocab)
+    tokens, logprobs = ops.sample_tokens(x, u, return_logprobs=True, **settings)
+    want, log = vectorised(x, u, **settings)
+    assert torch.equal(tokens, want)
+    assert ((logprobs.double() - log).abs() <= 2.0 ** -24 * log.abs() + 1e-9).all()
+
+
 def test_settings_by_row_and_64_bit_numbers(ops):
     rng = random.Random(4)
     x, _ = logits_of(40, 20000, BF16, 8)
