@@ -32,7 +32,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = kThreads;
 constexpr int kGroups = 8, kGroupBins = kBins / kGroups;  // of bins
 constexpr int kList = kThreads;       // tokens that are sorted
-constexpr int kFew = 96;              // of them, that are ranked instead (a sort takes as long as some 100)
+constexpr int kFew = 128;             // of them, that are ranked instead (a sort takes as long as some 100)
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxPart = kMaxVocab / kMaxCluster;  // tokens of a CTA
@@ -318,6 +318,36 @@ __device__ __forceinline__ void emit(const SampleArgs& a, const Row& r, int toke
 __device__ __forceinline__ void finish_list(const SampleArgs& a, const Row& r, int n, int k, u64 limit) {
   Shared& s = LB_S;
   const int t = threadIdx.x;
+  if (n <= kFew) {  // each token finds what comes before it, by value and then by index
+    const u64 key = t < n ? s.list[t] : kNone;
+    u64 m = t < n ? r.mass(from_ordered(~static_cast<unsigned>(key >> 32))) : 0, before = 0;
+    if (t < n) s.mass[t] = m;
+    __syncthreads();
+    int rank = 0;
+    if (t < n)
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const bool first = s.list[j] < key;
+        rank += first;
+        before += first ? s.mass[j] : 0;
+      }
+    if (rank >= k) m = 0;
+    if (r.top_p < 1.0) {
+      if (limit == 0) limit = share_of(r.top_p, block_sum(m, s.scan));
+      if (before >= limit) m = 0;
+    }
+    if (m < r.min_mass) m = 0;
+    const u64 total = block_sum(m, s.scan), target = target_of(r.u, total);  // (everyone has read the masses)
+    if (t < n) s.mass[t] = m;
+    __syncthreads();
+    if (m) {
+      u64 to = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) to += static_cast<unsigned>(s.list[j]) < static_cast<unsigned>(key) ? s.mass[j] : 0;
+      if (to <= target && target < to + m) emit(a, r, static_cast<int>(static_cast<unsigned>(key)), m, total);
+    }
+    return;
+  }
   const u64 key = block_sort(t < n ? s.list[t] : kNone, s.mass);
   const float x = from_ordered(~static_cast<unsigned>(key >> 32));
   const int index = static_cast<int>(static_cast<unsigned>(key));

@@ -565,50 +565,51 @@ def head_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be int32 or int64")
     _need(positions, "positions", positions.dtype, (t,), dev)
-    sides = [("q", q, q_out, q_weight)]
-    if k is not None:
-        if k.dim() != 3 or k.dtype != q.dtype or k.shape[0] != t or k.shape[2] != dim:
-            raise ValueError("k must be like q but for its number of heads")
-        sides.append(("k", k, k_out, k_weight))
-    elif k_out is not None or k_weight is not None:
-        raise ValueError("k_out and k_weight come with k")
-    weight_dtype = torch.float32
-    for name, x, out, weight in sides:
-        if x.device != dev or (x.numel() and x.stride(2) != 1):
-            raise ValueError(f"{name} must be on {dev}, its rows contiguous")
-        if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != dev
-                                or (out.numel() and (out.stride(2) != 1 or not _spread(out)))):
-            raise ValueError(f"{name}_out must be like {name}, its rows contiguous and apart")
-        if out is not None and out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and t:
-            raise ValueError(f"{name}_out must have {name}'s strides where it is {name}")
-        if weight is not None:
-            if not norm:
-                raise ValueError("weights belong to the norm")
-            if weight.dtype not in (torch.float32, q.dtype):
-                raise ValueError("weights must be float32 or of q's type")
-            _need(weight, f"{name}_weight", weight.dtype, (dim,), dev)
-            weight_dtype = weight.dtype
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError("weights must be of one type")
     if not 0.0 <= eps < math.inf:
         raise ValueError("eps must not be negative")
-    if q_out is None:
-        q_out = q.new_empty(q.shape)
-    if k is not None and k_out is None:
-        k_out = k.new_empty(k.shape)
+    q_out, q_args, q_to = _head_side("q", q, q_out, q_weight, dev, norm)
+    if k is None:
+        if k_out is not None or k_weight is not None:
+            raise ValueError("k_out and k_weight come with k")
+        kv_heads, k_args, k_to = 0, (None, 0, 0), (None, 0, 0)
+    else:
+        if k.dim() != 3 or k.dtype != q.dtype or k.shape[0] != t or k.shape[2] != dim:
+            raise ValueError("k must be like q but for its number of heads")
+        kv_heads = k.shape[1]
+        k_out, k_args, k_to = _head_side("k", k, k_out, k_weight, dev, norm)
+    weight = q_weight if q_weight is not None else k_weight
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("weights must be of one type")
     if t:
-        if k is None:
-            k_args = out_args = (None, 0, 0)
-            kv_heads = 0
-        else:
-            k_args, out_args = (k.data_ptr(), k.stride(0), k.stride(1)), (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
-            kv_heads = k.shape[1]
-        _call(dev, "lb_op_head_norm_rotary", q.data_ptr(), q.stride(0), q.stride(1), heads, *k_args, kv_heads, DTYPE_CODES[q.dtype],
+        _call(dev, "lb_op_head_norm_rotary", *q_args, heads, *k_args, kv_heads, DTYPE_CODES[q.dtype],
               t, dim, positions.data_ptr(), positions.dtype == torch.int64, rotary._t_turns.data_ptr(), rotary.rotary_dim,
               rotary.pairs == "neighbours", None if q_weight is None else q_weight.data_ptr(),
-              None if k_weight is None else k_weight.data_ptr(), DTYPE_CODES[weight_dtype], norm, eps,
-              q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *out_args)
+              None if k_weight is None else k_weight.data_ptr(), _lib.LB_F32 if weight is None else DTYPE_CODES[weight.dtype], norm, eps,
+              *q_to, *k_to)
     return q_out, k_out
+
+
+def _head_side(name: str, x: torch.Tensor, out: torch.Tensor | None, weight: torch.Tensor | None, dev: torch.device, norm: bool):
+    """Checks one of q and k; (its output, address and strides of the input, of the output)."""
+    step = x.stride()
+    if x.device != dev or (step[2] != 1 and x.numel()):
+        raise ValueError(f"{name} must be on {dev}, its rows contiguous")
+    if weight is not None:
+        if not norm:
+            raise ValueError("weights belong to the norm")
+        if weight.dtype not in (torch.float32, x.dtype):
+            raise ValueError("weights must be float32 or of q's type")
+        _need(weight, f"{name}_weight", weight.dtype, (x.shape[2],), dev)
+    if out is None:
+        out = torch.empty_like(x)  # (of a part of a product's output: contiguous)
+        to = out.stride()
+    else:
+        to = out.stride()
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != dev or (out.numel() and (to[2] != 1 or not _spread(out))):
+            raise ValueError(f"{name}_out must be like {name}, its rows contiguous and apart")
+        if out.data_ptr() == x.data_ptr() and to != step and out.numel():
+            raise ValueError(f"{name}_out must have {name}'s strides where it is {name}")
+    return out, (x.data_ptr(), step[0], step[1]), (out.data_ptr(), to[0], to[1])
 
 
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
