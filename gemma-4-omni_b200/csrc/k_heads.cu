@@ -48,11 +48,6 @@ __device__ __forceinline__ T from_float(float v) {
   else if constexpr (__is_same(T, __half)) return __float2half_rn(v);
   else return __float2bfloat16_rn(v);
 }
-template <typename T>
-struct alignas(4 * sizeof(T)) Four {
-  T v[4];
-};
-
 __device__ __forceinline__ void sin_cos(unsigned long long turns, float& s, float& c) {
   const unsigned h = static_cast<unsigned>(turns >> 32);       // 2^-32 turns
   const unsigned quadrant = (h + (1u << 29)) >> 30;            // (wraps to 0 with the turn)
@@ -77,83 +72,150 @@ __device__ __forceinline__ float weight_at(const HeadsArgs& a, const HeadsSide& 
   return a.weight_f32 ? static_cast<const float*>(s.weight)[i] : as_float(static_cast<const T*>(s.weight)[i]);
 }
 
-// The heads [first, last) of a side that this group of lanes takes, `stride` apart.
+// two 32-bit values an instruction
+typedef unsigned long long pair_t;
+__device__ __forceinline__ pair_t pair_of(float a, float b) {
+  pair_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void unpair(pair_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+  pair_t p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
+  return p;
+}
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+  pair_t p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+  return p;
+}
+template <typename T>
+__device__ __forceinline__ void load4(const T* at, uint32_t (&r)[sizeof(T)]) {  // (a register a pair of 16-bit values, or a value)
+  if constexpr (sizeof(T) == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    r[0] = v.x, r[1] = v.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void widen4(const uint32_t (&r)[sizeof(T)], pair_t (&v)[2]) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    if constexpr (sizeof(T) == 4) {
+      v[p] = pair_of(__uint_as_float(r[2 * p]), __uint_as_float(r[2 * p + 1]));
+    } else if constexpr (__is_same(T, __half)) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[p]));
+      v[p] = pair_of(f.x, f.y);
+    } else {
+      v[p] = pair_of(__uint_as_float(r[p] << 16), __uint_as_float(r[p] & 0xffff0000u));
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* at, const pair_t (&v)[2]) {
+  float a, b, c, d;
+  unpair(v[0], a, b);
+  unpair(v[1], c, d);
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(at) = make_float4(a, b, c, d);
+  } else if constexpr (__is_same(T, __half)) {
+    const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
+    *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  } else {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+    *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  }
+}
+
+// The heads [first, last) of a side that this group of lanes takes, in steps of a warp's heads.  A lane's eight values are two
+// pairs at ea and two at eb; rotated ones become v * own + other * cross, with the weights in the factors (of the token and lane, for all its
+// heads) and 1 / rms behind them.
 template <typename T, int LANES>
 __device__ __forceinline__ void walk(const HeadsArgs& a, const HeadsSide& side, int token, int first, int last, int ea, int eb,
                                      bool there, bool turned, const float (&sn)[4], const float (&cs)[4]) {
   constexpr int kStep = 32 / LANES, kAhead = sizeof(T) == 4 ? 2 : 4;
-  float wa[4], wb[4];
+  pair_t own[2][2], cross[2][2];  // [at ea, at eb][pair]
+  {
+    float w[2][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    wa[j] = there ? weight_at<T>(a, side, ea + j) : 0.0f;
-    wb[j] = there ? weight_at<T>(a, side, eb + j) : 0.0f;
+    for (int j = 0; j < 4; ++j) {
+      w[0][j] = there ? weight_at<T>(a, side, ea + j) : 0.0f;
+      w[1][j] = there ? weight_at<T>(a, side, eb + j) : 0.0f;
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (a.neighbours) {  // of a pair (v0, v1): v0 c - v1 s, v1 c + v0 s
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float c = cs[2 * e + p], s = sn[2 * e + p];
+          own[e][p] = pair_of(w[e][2 * p] * c, w[e][2 * p + 1] * c);
+          cross[e][p] = pair_of(-w[e][2 * p + 1] * s, w[e][2 * p] * s);
+        }
+      } else {
+        own[0][p] = pair_of(w[0][2 * p] * cs[2 * p], w[0][2 * p + 1] * cs[2 * p + 1]);
+        own[1][p] = pair_of(w[1][2 * p] * cs[2 * p], w[1][2 * p + 1] * cs[2 * p + 1]);
+        cross[0][p] = pair_of(-w[1][2 * p] * sn[2 * p], -w[1][2 * p + 1] * sn[2 * p + 1]);
+        cross[1][p] = pair_of(w[0][2 * p] * sn[2 * p], w[0][2 * p + 1] * sn[2 * p + 1]);
+      }
+    }
   }
-  const T* x = static_cast<const T*>(side.x) + token * side.token;
-  T* out = static_cast<T*>(side.out) + token * side.out_token;
-  const float inv_dim = 1.0f / static_cast<float>(a.dim);
   const int group = (threadIdx.x & 31) / LANES;
-  for (int h0 = first; h0 < last; h0 += kStep * kAhead) {
-    Four<T> ra[kAhead], rb[kAhead];
+  const T* x = static_cast<const T*>(side.x) + token * side.token + (first + group) * side.head;
+  T* out = static_cast<T*>(side.out) + token * side.out_token + (first + group) * side.out_head;
+  const long long x_step = kStep * side.head, out_step = kStep * side.out_head;
+  const float inv_dim = 1.0f / static_cast<float>(a.dim);
+  for (int h0 = first + group; h0 - group < last; h0 += kStep * kAhead) {  // (the warp's groups together)
+    uint32_t ra[kAhead][sizeof(T)], rb[kAhead][sizeof(T)];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int h = h0 + u * kStep + group;
-      if (there && h < last) {
-        ra[u] = *reinterpret_cast<const Four<T>*>(x + h * side.head + ea);
-        rb[u] = *reinterpret_cast<const Four<T>*>(x + h * side.head + eb);
+      if (there && h0 + u * kStep < last) {
+        load4<T>(x + ea, ra[u]);
+        load4<T>(x + eb, rb[u]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ra[u].v[j] = rb[u].v[j] = from_float<T>(0.0f);
+        for (int j = 0; j < static_cast<int>(sizeof(T)); ++j) ra[u][j] = rb[u][j] = 0;
       }
+      x += x_step;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int h = h0 + u * kStep + group;
-      float va[4], vb[4], sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        va[j] = as_float(ra[u].v[j]);
-        vb[j] = as_float(rb[u].v[j]);
-        sum = fmaf(va[j], va[j], fmaf(vb[j], vb[j], sum));
-      }
+      pair_t v[2][2];
+      widen4<T>(ra[u], v[0]);
+      widen4<T>(rb[u], v[1]);
+      float inv = 1.0f;
       if (a.norm) {
+        const pair_t two = fma2(v[0][0], v[0][0], fma2(v[0][1], v[0][1], fma2(v[1][0], v[1][0], mul2(v[1][1], v[1][1]))));
+        float lo, hi;
+        unpair(two, lo, hi);
+        float sum = lo + hi;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = __frsqrt_rn(fmaf(sum, inv_dim, a.eps));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          va[j] *= inv * wa[j];
-          vb[j] *= inv * wb[j];
-        }
+        inv = rsqrtf(fmaf(sum, inv_dim, a.eps));
       }
-      if (turned) {
-        if (a.neighbours) {
+      const pair_t inv2 = pair_of(inv, inv);
+      pair_t y[2][2];
 #pragma unroll
-          for (int j = 0; j < 4; j += 2) {
-            const float p = va[j], r = vb[j];
-            va[j] = fmaf(p, cs[j / 2], -va[j + 1] * sn[j / 2]);
-            va[j + 1] = fmaf(va[j + 1], cs[j / 2], p * sn[j / 2]);
-            vb[j] = fmaf(r, cs[2 + j / 2], -vb[j + 1] * sn[2 + j / 2]);
-            vb[j + 1] = fmaf(vb[j + 1], cs[2 + j / 2], r * sn[2 + j / 2]);
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          pair_t other = v[1 - e][p];
+          if (a.neighbours) {
+            float lo, hi;
+            unpair(v[e][p], lo, hi);
+            other = pair_of(hi, lo);
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = va[j];
-            va[j] = fmaf(p, cs[j], -vb[j] * sn[j]);
-            vb[j] = fmaf(vb[j], cs[j], p * sn[j]);
-          }
+          y[e][p] = mul2(v[e][p], own[e][p]);
+          if (turned) y[e][p] = fma2(other, cross[e][p], y[e][p]);
+          y[e][p] = mul2(y[e][p], inv2);
         }
+      if (there && h0 + u * kStep < last) {
+        store4<T>(out + ea, y[0]);
+        store4<T>(out + eb, y[1]);
       }
-      if (there && h < last) {
-        Four<T> oa, ob;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          oa.v[j] = from_float<T>(va[j]);
-          ob.v[j] = from_float<T>(vb[j]);
-        }
-        *reinterpret_cast<Four<T>*>(out + h * side.out_head + ea) = oa;
-        *reinterpret_cast<Four<T>*>(out + h * side.out_head + eb) = ob;
-      }
+      out += out_step;
     }
   }
 }
