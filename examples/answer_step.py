@@ -1,5 +1,5 @@
 """From PCM to a decoder block: the listener's soft tokens of each tick go through one
-text-decoder block over a paged 8-bit K/V cache.
+text-decoder block over a paged 8-bit K/V cache, and a token is drawn for each session at the end.
 
 Three sessions hear different seeded audio; each 80 ms tick the tower yields two
 soft tokens a session, the page directory plans where their keys and values go, the block
@@ -34,7 +34,7 @@ def main(ticks: int = 12) -> dict:
     from gemma4_omni_b200 import _lib, runtime, synthetic
     from gemma4_omni_b200.config import SMALL
     from gemma4_omni_b200.decode_ops import PageDirectory
-    from gemma4_omni_b200.decoder_block import DecoderBlock, DecoderConfig
+    from gemma4_omni_b200.decoder_block import DecoderBlock, DecoderConfig, DecoderHead
 
     torch.cuda.set_device(0)
     n = 3
@@ -59,12 +59,16 @@ def main(ticks: int = 12) -> dict:
             gone = live.pop(1)
             tower.reset_handle(gone)
             pages.release(torch.tensor([gone], dtype=torch.int32, device="cuda"))
+    head = DecoderHead.synthetic(SMALL.text_hidden, 1000, seed=5)
+    last = out.view(-1, 2, SMALL.text_hidden)[:, 1].contiguous()  # each live session's last token
+    tokens = head.sample(last, torch.full((last.shape[0],), 0.5, device="cuda"), temperature=0.8, top_k=50, top_p=0.95)
     status = {"tower": tower.status(), "cache": cache.status(), "pages": pages.status(), "plan": plan.status()}
     lengths = pages.lengths.tolist()
     tower.close()
-    return {"out": out, "lengths": lengths, "status": status}
+    return {"out": out, "lengths": lengths, "status": status, "tokens": tokens.tolist()}
 
 
 if __name__ == "__main__":
     result = main()
-    print("tokens held per session:", result["lengths"], "status:", result["status"], "output:", tuple(result["out"].shape))
+    print("tokens held per session:", result["lengths"], "status:", result["status"], "output:", tuple(result["out"].shape),
+          "tokens:", result["tokens"])
