@@ -66,7 +66,7 @@ struct Result {  // of one division into bins
 struct alignas(16) Shared {
   double power[kPowers];        // 2^(j / kPowers)
   union {
-    unsigned hist[4][kBins];    // counts; masses in limbs of 16 bits
+    alignas(16) unsigned hist[4][kBins];    // counts; masses in limbs of 16 bits
     u64 mass[kList];            // while tokens are sorted
   };
   u64 list[kList];
@@ -84,6 +84,7 @@ struct alignas(16) Shared {
   u64 above_count[kMaxCluster];
   int cut_index;
   float cut_value;
+  double scale, floor_reach;    // of the row: log2(e) / T; how far below the top min_p reaches, in octaves times T
   unsigned listed;
   int at;
 };
@@ -132,6 +133,31 @@ struct Masses {
   __device__ __forceinline__ u64 operator()(float x) const { return bits(x) & 0xfffffffffffffull; }
 };
 constexpr u64 kExponent = 0x433ull << 52;  // of 2^52
+// 2^(j / 128)
+__device__ const double powers[kPowers] = {
+    1.0, 1.0054299011128027, 1.0108892860517005, 1.016378314910953, 1.0218971486541166, 1.0274459491187637,
+    1.0330248790212284, 1.0386341019613787, 1.0442737824274138, 1.0499440858006872, 1.0556451783605572, 1.061377227289262,
+    1.0671404006768237, 1.0729348675259756, 1.0787607977571199, 1.0846183622133092, 1.0905077326652577, 1.0964290818163769,
+    1.102382583307841, 1.1083684117236787, 1.1143867425958924, 1.1204377524096067, 1.1265216186082418, 1.1326385195987192,
+    1.1387886347566916, 1.1449721444318042, 1.1511892299529827, 1.1574400736337511, 1.1637248587775775, 1.1700437696832502,
+    1.1763969916502812, 1.182784710984341, 1.189207115002721, 1.1956643920398273, 1.202156731452703, 1.2086843236265816,
+    1.215247359980469, 1.2218460329727576, 1.22848053610687, 1.2351510639369334, 1.241857812073484, 1.2486009771892048,
+    1.255380757024691, 1.2621973503942507, 1.2690509571917332, 1.275941778396392, 1.2828700160787783, 1.2898358734066657,
+    1.2968395546510096, 1.3038812651919358, 1.3109612115247644, 1.318079601266064, 1.3252366431597413, 1.3324325470831615,
+    1.339667524053303, 1.3469417862329458, 1.3542555469368927, 1.3616090206382248, 1.3690024229745905, 1.3764359707545302,
+    1.383909881963832, 1.3914243757719262, 1.3989796725383112, 1.4065759938190154, 1.4142135623730951, 1.4218926021691656,
+    1.42961333839197, 1.4373759974489824, 1.4451808069770467, 1.4530279958490526, 1.460917794180647, 1.4688504333369818,
+    1.4768261459394993, 1.4848451658727524, 1.4929077282912648, 1.5010140696264256, 1.5091644275934228, 1.5173590411982147,
+    1.5255981507445384, 1.533881997840956, 1.5422108254079407, 1.550584877685, 1.559004400237837, 1.567469639965553,
+    1.5759808451078865, 1.5845382652524937, 1.593142151342267, 1.6017927556826934, 1.6104903319492543, 1.6192351351948637,
+    1.6280274218573478, 1.6368674497669644, 1.645755478153965, 1.6546917676561943, 1.6636765803267364, 1.6727101796415966,
+    1.681792830507429, 1.6909247992693053, 1.7001063537185235, 1.709337763100463, 1.718619298122478, 1.7279512309618377,
+    1.7373338352737062, 1.746767386199169, 1.7562521603732995, 1.7657884359332727, 1.7753764925265212, 1.785016611318935,
+    1.7947090750031072, 1.804454167806624, 1.8142521755003989, 1.8241033854070534, 1.8340080864093424, 1.843966568958626,
+    1.8539791250833855, 1.864046048397789, 1.8741676341103, 1.8843441790323345, 1.8945759815869656, 1.9048633418176741,
+    1.9152065613971474, 1.925605943636125, 1.9360617934922943, 1.9465744175792332, 1.9571441241754002, 1.9677712232331759,
+    1.978456026387951, 1.9891988469672663,
+};
 
 __device__ __forceinline__ u64 warp_inclusive(u64 v) {
   const int lane = threadIdx.x & 31;
@@ -480,16 +506,18 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
     }
     __syncthreads();
     // ---- sums of groups of bins go to every CTA
+    u64 mass_here = 0;
     {
       const unsigned c = __reduce_add_sync(0xffffffffu, s.hist[0][t]);
-      u64 m = 0;
-      if constexpr (kMass) m = warp_sum64(s.hist[1][t] + (static_cast<u64>(s.hist[2][t]) << 16) + (static_cast<u64>(s.hist[3][t]) << 32));
+      if constexpr (kMass) mass_here = s.hist[1][t] + (static_cast<u64>(s.hist[2][t]) << 16) + (static_cast<u64>(s.hist[3][t]) << 32);
+      const u64 m = kMass ? warp_sum64(mass_here) : 0;
       if (lane == 0) {
         s.warp_count[warp] = c;
         s.scan[warp] = m;
       }
     }
     __syncthreads();
+    if constexpr (kMass) reinterpret_cast<u64*>(&s.hist[2][0])[t] = mass_here;  // (the limbs have been read: whole masses take their place)
     if (t < kGroups * ctas) {
       constexpr int kEach = kWarps / kGroups;
       const int g = t % kGroups, to = t / kGroups;
@@ -555,23 +583,24 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
       unsigned n[2] = {0, 0};
 #pragma unroll
       for (int q0 = 0; q0 < kMaxCluster; q0 += 4) {  // four CTAs' bins are under way at once
-        uint2 v[4][kMass ? 4 : 1];
+        uint2 c[4];
+        ulonglong2 m[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (q0 + q < ctas) {
-            const uint2* p = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&s.hist[0][0], q0 + q) + group * kGroupBins) + lane;
-#pragma unroll
-            for (int l = 0; l < (kMass ? 4 : 1); ++l) v[q][l] = p[l * (kBins / 2)];
+            const unsigned* p = cluster.map_shared_rank(&s.hist[0][0], q0 + q);
+            c[q] = reinterpret_cast<const uint2*>(p + group * kGroupBins)[lane];
+            if constexpr (kMass) m[q] = reinterpret_cast<const ulonglong2*>(p + 2 * kBins + 2 * group * kGroupBins)[lane];
           }
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (q0 + q < ctas) {
-            n[0] += v[q][0].x;
-            n[1] += v[q][0].y;
+            n[0] += c[q].x;
+            n[1] += c[q].y;
             if constexpr (kMass) {
-              w[0] += v[q][1].x + (static_cast<u64>(v[q][2].x) << 16) + (static_cast<u64>(v[q][3].x) << 32);
-              w[1] += v[q][1].y + (static_cast<u64>(v[q][2].y) << 16) + (static_cast<u64>(v[q][3].y) << 32);
+              w[0] += m[q].x;
+              w[1] += m[q].y;
             }
           }
         }
@@ -757,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   float* x = r.logits();
   float top = -INFINITY;
   const uint4* body = reinterpret_cast<const uint4*>(src + head);
-  constexpr int kAhead = 4;
+  constexpr int kAhead = sizeof(T) == 4 ? 8 : 4;
   for (int v0 = t; v0 < vecs; v0 += kThreads * kAhead) {
     uint4 raw[kAhead];
 #pragma unroll
@@ -782,7 +811,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     x[i] = logit(src[i]);
     top = fmaxf(top, x[i]);
   }
-  if (t < kPowers) s.power[t] = exp2(static_cast<double>(t) / kPowers);
+  if (t < kPowers) s.power[t] = powers[t];
 
   // ---- the row's settings and its maximum
   const float heat = fminf(a.temperature ? a.temperature[r.row] : a.temperature1, kMaxHeat);  // (NaN: the limit)
@@ -792,6 +821,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   r.top_p = p < 1.0f ? static_cast<double>(p) : 1.0;
   r.min_mass = least > 0.0f ? static_cast<u64>(ceil(static_cast<double>(fminf(least, 1.0f)) * static_cast<double>(1ull << kTop))) : 0;
   r.u = a.uniform64 ? static_cast<const double*>(a.uniform)[r.row] : static_cast<double>(static_cast<const float*>(a.uniform)[r.row]);
+  if (t == 32) {
+    s.scale = 1.4426950408889634074 / static_cast<double>(heat);
+    s.floor_reach = r.min_mass ? (kTop + 0.01 - log2(static_cast<double>(r.min_mass))) / s.scale : 0.0;  // (a hundredth of an octave to spare)
+  }
   const bool greedy = !(heat > 0.0f) || (a.temperature && a.temperature[r.row] != a.temperature[r.row]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -838,13 +871,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   }
   r.heat = heat;
   r.inv_heat = fminf(1.0f / heat, 1e30f);
-  // (where the next number below the top has no mass any more, no larger scale is needed: exponents stay above -150)
+  r.mass = {static_cast<double>(top), s.scale, top, 0.0f};
+  // Where the next number below the top has no mass any more, no larger scale is needed: exponents stay above -150.
   const double next = static_cast<double>(top) - static_cast<double>(nextafterf(top, -INFINITY));
-  r.mass = {static_cast<double>(top), fmin(1.4426950408889634074 / static_cast<double>(heat), 47.0 / next), top, 0.0f};
-  r.mass.least = __double2float_rd(static_cast<double>(top) - 47.0 / r.mass.scale);  // 2^-47 of the top's mass is 0
-  r.floor = -INFINITY;
-  if (r.min_mass)  // a hundredth of an octave to spare
-    r.floor = __double2float_rd(static_cast<double>(top) - (kTop + 0.01 - log2(static_cast<double>(r.min_mass))) / r.mass.scale);
+  if (r.mass.scale * next > 47.0) r.mass.scale = 47.0 / next;
+  r.mass.least = __double2float_rd(static_cast<double>(top) - fmax(47.0 * 0.69314718055994530942 * static_cast<double>(heat) * (1.0 + 1e-9), next));  // 2^-47 of the top's mass is 0
+  r.floor = r.min_mass ? __double2float_rd(static_cast<double>(top) - s.floor_reach) : -INFINITY;
   const int seg = ((a.part + kWarps - 1) / kWarps + 31) / 32 * 32;
   Left left{min(n, warp * seg), min(n, (warp + 1) * seg) - min(n, warp * seg), false};
   Listed listed{kList, r.k, 0};
