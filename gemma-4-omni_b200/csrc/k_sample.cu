@@ -894,8 +894,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   }
 
   // ---- the kept masses in the order of the indexes: by warps, by CTAs, and the warp with the target once more
-  if (r.min_mass) left.keep(r, [&](float v, int) { return v >= r.floor; });
   const auto mass_of = [&](float v) -> u64 {
+    if (v < r.floor) return 0;
     const u64 m = r.mass(v);
     return m >= r.min_mass ? m : 0;
   };
