@@ -53,11 +53,11 @@ struct Shape {
   static constexpr int kXBytes = NT * kBlockK * (kWide ? 2 : 1);
   static constexpr int kStage = kCodeBytes + kXBytes;
   // partial sums of the groups of four tokens that a CTA finishes, from 2, 4 or 8 CTAs
-  static constexpr int kParts = NT < 128 ? 2 * (NT / 4) * kBlockO * 16 : 0;
+  static constexpr int kParts = NT <= 64 ? 2 * (NT / 4) * kBlockO * 16 : 0;
   static constexpr int kRoom = 200 * 1024 - kParts;
   static constexpr int kStages = kRoom / kStage > 8 ? 8 : kRoom / kStage;
   static constexpr int kSmem = kStages * kStage + kParts + 1024;  // (up to 12 KB are declared beside it)
-  static constexpr int kSideD = NT == 128 ? 1 : 2, kD = 2 * kSideD;  // accumulators in the tensor memory, of a side and in all
+  static constexpr int kSideD = NT > 64 ? 1 : 2, kD = 2 * kSideD;  // accumulators in the tensor memory, of a side and in all
   static constexpr int kCols = NT / 2;                        // tokens of an adding warpgroup
   static constexpr int kSteps = kWide ? 16 : 32;              // k of an MMA
   static_assert(kD * NT <= kAColumn, "tensor memory");
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   const int kb0 = a.k_blocks * split / static_cast<int>(splits), kb1 = a.k_blocks * (split + 1) / static_cast<int>(splits);
   const int first = blockIdx.x / splits, step = gridDim.x / splits, tiles = a.o_tiles * a.t_tiles;
   const bool grouped = a.x_group != 0;
-  bool ok = true, joined = splits == 1 || NT == 128;
+  bool ok = true, joined = splits == 1 || NT > 64;
   if (!joined) cluster_arrive();
 
   if (warp < 4) {
@@ -575,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
 #pragma unroll
             for (int j0 = 0; j0 < S::kCols; j0 += 16) {
               pair_t r[8];
+              [[maybe_unused]] ulonglong2 xs{};  // x's scales of four tokens
               tmem_ld16(d + j0, r);
               if (j0 + 16 == S::kCols) {  // the sums are in registers
                 tc_fence_before();
@@ -584,6 +585,9 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 pair_t v = r[j];
+                if constexpr (!S::kWide) {
+                  if (grouped && j % 2 == 0) xs = *reinterpret_cast<const ulonglong2*>(&xs_s[ring][half * S::kCols + j0 + 2 * j]);
+                }
                 if constexpr (X == kXI8) {  // sums below 2^22, under the exponent of 3 * 2^22
                   float lo, hi;
                   unpair(v, lo, hi);
@@ -591,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
                            pair_of(-12582912.0f, -12582912.0f));
                 }
                 if constexpr (!S::kWide) {
-                  if (grouped) v = mul2(v, *reinterpret_cast<const pair_t*>(&xs_s[ring][half * S::kCols + j0 + 2 * j]));
+                  if (grouped) v = mul2(v, j % 2 ? xs.y : xs.x);
                 }
                 acc[side][j0 / 2 + j] = fma2(v, s2, acc[side][j0 / 2 + j]);
               }
@@ -615,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
         const long long pitch = a.ld_out * (a.out_dtype == LB_F32 ? 4 : 2);
         unsigned char* at = static_cast<unsigned char*>(a.out) + t0 * pitch + static_cast<long long>(o) * (a.out_dtype == LB_F32 ? 4 : 2);
         // up to 32 tokens a turn, the rest move up: a loop that stays in the instruction cache
-        constexpr int kTurn = S::kCols < 32 ? S::kCols : 32;
+        constexpr int kTurn = S::kCols % 32 == 0 ? 32 : S::kCols > 32 ? S::kCols / 2 : S::kCols;  // (48: twice 24)
         const bool whole = tile % a.o_tiles * kBlockO + kBlockO <= a.f && t0 + S::kCols <= a.m;
         const auto turn = [&](auto gelu, auto type) {
           using Out = decltype(type);
@@ -629,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
               unpair(acc[1][j / 2], u[0], u[1]);
               float gate = g[j & 1], up = u[j & 1];
               if (!S::kWide && !grouped) {
-                const float xs = __shfl_sync(0xffffffffu, j0 & 32 ? row_scale[1] : row_scale[0], j);
+                const float xs = __shfl_sync(0xffffffffu, j0 + j >= 32 ? row_scale[1] : row_scale[0], (j0 + j) & 31);
                 gate *= xs;
                 up *= xs;
               }
@@ -665,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
           cluster_wait();
           joined = true;
         }
-        if constexpr (NT < 128) {
+        if constexpr (NT <= 64) {
           const int n = static_cast<int>(splits), own = (NT / 4 + n - 1) / n, first_q = half * S::kCols / 4;
           const int live = (min(S::kCols, a.m - t0) + 3) / 4;
           int to = first_q % n, i = first_q / n;
@@ -688,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   }
   if (!ok && a.status) atomicOr(a.status, static_cast<int>(kStatusWaitTimeout));
   __syncwarp();
-  if (NT < 128 && splits > 1) {
+  if (NT <= 64 && splits > 1) {
     if (!joined) cluster_wait();
     cluster_arrive();
     cluster_wait();
@@ -769,6 +773,7 @@ template <int X>
 cudaError_t launch(const GatedArgs& a, int nt, int splits, const CUtensorMap& w_map, const CUtensorMap& x_map, cudaStream_t s) {
   if (nt == 32) return launch<X, 32>(a, splits, w_map, x_map, s);
   if (nt == 64) return launch<X, 64>(a, splits, w_map, x_map, s);
+  if (nt == 96) return launch<X, 96>(a, splits, w_map, x_map, s);
   return launch<X, 128>(a, splits, w_map, x_map, s);
 }
 
@@ -795,15 +800,15 @@ extern "C" int lb_op_w4_gated(const void* x, int64_t x_ld, int x_dtype, const fl
   a.o_tiles = (ffn + kBlockO - 1) / kBlockO;
   a.k_blocks = (k + kBlockK - 1) / kBlockK;
   // The width of a tile and the dealing out of K by an estimate of the time in tenths of a microsecond: a wave of tiles takes 4 us
-  // and for each block of K 0.67, 0.7 or 1 at 32, 64 or 128 tokens (1536 x 6144: 128 rows take 18 us as 48 tiles of 128 tokens, 14 as 96
-  // of 64; 499 rows 34 us as 192 of 128, some 43 as 384 of 64).  K is dealt out where all clusters fit the GPU at once: 2
+  // and for each block of K 0.67, 0.7, 0.85 or 1 at 32, 64, 96 or 128 tokens (1536 x 6144: 128 rows take 18 us as 48 tiles of 128
+  // tokens, 14 as 96 of 64).  K is dealt out where all clusters fit the GPU at once: 2
   // rows of 1536 x 6144 take 14 us whole, 10 in clusters of two, but 15 in clusters of three, not all of which fit.
   int nt = 0, splits = 1;
   long long best = 0;
-  for (const int width : {32, 64, 128}) {
+  for (const int width : {32, 64, 96, 128}) {
     const long long t_tiles = (m + width - 1) / width, tiles = a.o_tiles * t_tiles;
-    const int split = width == 128 ? 1 : tiles <= 16 && a.k_blocks >= 8 ? 8 : tiles <= 32 && a.k_blocks >= 4 ? 4 : tiles <= 74 && a.k_blocks >= 2 ? 2 : 1;
-    const long long time = (tiles * split + kSms - 1) / kSms * (40 + (width == 32 ? 67 : width == 64 ? 70 : 100) * ((a.k_blocks + split - 1) / split) / 10);
+    const int split = width > 64 ? 1 : tiles <= 16 && a.k_blocks >= 8 ? 8 : tiles <= 32 && a.k_blocks >= 4 ? 4 : tiles <= 74 && a.k_blocks >= 2 ? 2 : 1;
+    const long long time = (tiles * split + kSms - 1) / kSms * (40 + (width == 32 ? 67 : width == 64 ? 70 : width == 96 ? 85 : 100) * ((a.k_blocks + split - 1) / split) / 10);
     if (nt == 0 || time < best) {
       nt = width;
       splits = split;

@@ -49,7 +49,7 @@ def check(out, x, xs, weight, activation):
 @pytest.mark.parametrize("x_type,x_group", [(BF16, 0), (F16, 0), (E4M3, 0), (I8, 0), (E4M3, 128), (I8, 256)])
 @pytest.mark.parametrize("rows,k,ffn,group", [
     (1, 256, 128, 128), (2, 1536, 6144, 128), (3, 512, 100, 64), (32, 768, 129, 32), (33, 256, 300, 128), (64, 1024, 640, 64),
-    (65, 512, 130, 32), (129, 1536, 257, 128), (300, 2048, 1000, 64), (1000, 1024, 2500, 128), (40, 4096, 64, 32)])
+    (65, 512, 130, 32), (129, 1536, 257, 128), (300, 2048, 1000, 64), (1000, 1024, 2500, 128), (40, 4096, 64, 32), (480, 512, 6144, 64), (270, 256, 6000, 32)])
 def test_follows_the_definition(ops, rows, k, ffn, group, x_type, x_group):
     x, xs, w = inputs(ops, rows, k, ffn, group, x_type, x_group, rows + k)
     check(ops.w4_gated(x, w, x_scale=xs, out_dtype=F32), x, xs, w, "silu")
