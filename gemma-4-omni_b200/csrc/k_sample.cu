@@ -84,7 +84,7 @@ struct alignas(16) Shared {
   u64 above_count[kMaxCluster];
   int cut_index;
   float cut_value;
-  double scale, floor_reach;    // of the row: log2(e) / T; how far below the top min_p reaches, in octaves times T
+  double scale, reach, floor_reach;  // of the row: log2(e) / T; how far below the top the masses end, and min_p reaches
   unsigned listed;
   int at;
 };
@@ -627,13 +627,17 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
     above = found.above;
     before = found.before;
     const bool all = found.before + found.count <= kList;  // everything down to the cut fits the list
+    // the tokens of the bin and above: at level 0 by the product that the bin is the whole part of
+    const float edge = found.bin == kBins - 1 ? INFINITY : static_cast<float>(found.bin + 1);
     const auto down_to = [&](float x) {
+      if (level == 0) return __fmul_rn(__fsub_rn(r.distance(x), zone_lo), zone_bins) < edge;
       const int b = bin_of(x);
       return b == -2 || (b >= 0 && b <= found.bin);
     };
     if (all || found.count <= kList) {
       Shared& lead = *cluster.map_shared_rank(&s, 0);
-      left.keep(r, [&](float x, int) { return down_to(x); });
+      if (level == 0) left.keep(r, [&](float x, int) { return __fmul_rn(__fsub_rn(r.distance(x), zone_lo), zone_bins) < edge; });
+      else left.keep(r, [&](float x, int) { return down_to(x); });
       const float* x = r.logits() + left.base;
       const uint16_t* at = r.indexes() + left.base;
       int mine = 0;
@@ -823,6 +827,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   r.u = a.uniform64 ? static_cast<const double*>(a.uniform)[r.row] : static_cast<double>(static_cast<const float*>(a.uniform)[r.row]);
   if (t == 32) {
     s.scale = 1.4426950408889634074 / static_cast<double>(heat);
+    s.reach = 47.0 * 0.69314718055994530942 * (1.0 + 1e-9) * static_cast<double>(heat);
     s.floor_reach = r.min_mass ? (kTop + 0.01 - log2(static_cast<double>(r.min_mass))) / s.scale : 0.0;  // (a hundredth of an octave to spare)
   }
   const bool greedy = !(heat > 0.0f) || (a.temperature && a.temperature[r.row] != a.temperature[r.row]);
@@ -873,9 +878,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   r.inv_heat = fminf(1.0f / heat, 1e30f);
   r.mass = {static_cast<double>(top), s.scale, top, 0.0f};
   // Where the next number below the top has no mass any more, no larger scale is needed: exponents stay above -150.
-  const double next = static_cast<double>(top) - static_cast<double>(nextafterf(top, -INFINITY));
+  const int bits = __float_as_int(top);
+  const float below = top == 0.0f ? __int_as_float(0x80000001u) : __int_as_float(bits + (bits < 0 ? 1 : -1));
+  const double next = static_cast<double>(top) - static_cast<double>(below);
   if (r.mass.scale * next > 47.0) r.mass.scale = 47.0 / next;
-  r.mass.least = __double2float_rd(static_cast<double>(top) - fmax(47.0 * 0.69314718055994530942 * static_cast<double>(heat) * (1.0 + 1e-9), next));  // 2^-47 of the top's mass is 0
+  r.mass.least = __double2float_rd(static_cast<double>(top) - (s.reach > next ? s.reach : next));  // 2^-47 of the top's mass is 0
   r.floor = r.min_mass ? __double2float_rd(static_cast<double>(top) - s.floor_reach) : -INFINITY;
   const int seg = ((a.part + kWarps - 1) / kWarps + 31) / 32 * 32;
   Left left{min(n, warp * seg), min(n, (warp + 1) * seg) - min(n, warp * seg), false};
