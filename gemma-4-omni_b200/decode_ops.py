@@ -494,7 +494,7 @@ _PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510")
 
 
 @functools.lru_cache(maxsize=64)
-def _turns(rotary_dim: int, base: float) -> tuple[float, ...]:
+def _turns(rotary_dim: int, base: float) -> tuple[int, ...]:
     """The frequencies base ** (-2 i / rotary_dim), in turns a position, as signed 64-bit fractions of a turn."""
     with decimal.localcontext() as c:
         c.prec = 50
@@ -555,7 +555,8 @@ def head_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
 
     q [tokens, heads, dim], k [tokens, kv_heads, dim] (or None) of one type, such as views of one product's output; positions
     int32 or int64 [tokens], as a ``PagePlan`` has them.  With ``norm`` each head's values become x / sqrt(mean(x^2) + eps) *
-    weight (weights f32 or of q's type, None: 1).  ``q_out`` / ``k_out`` may be q and k themselves."""
+    weight (weights f32 or of q's type, None: 1).  ``q_out`` / ``k_out`` may be q and k themselves, and share
+    no memory with an input otherwise."""
     dev = rotary.device
     if q.dim() != 3 or q.dtype not in FLOAT_INPUTS:
         raise ValueError("q must be a float32, bfloat16 or float16 [tokens, heads, dim] tensor")

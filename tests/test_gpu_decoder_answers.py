@@ -171,3 +171,33 @@ def test_example_draws_tokens():
     # (the tower's split sums are added up in any order, so two runs' soft tokens may differ in their last bits)
     tokens = module.main(ticks=4)["tokens"]
     assert len(tokens) == 2 and all(0 <= t < 1000 for t in tokens)
+
+
+def test_offsets_beyond_32_bits(pkg):
+    """Rows 2^31 elements apart: queries, logits and the gated product's output, beside the same rows close together."""
+    from gemma4_omni_b200 import decode_ops as ops
+    room = torch.zeros((1 << 31) + (1 << 14), dtype=torch.bfloat16, device="cuda")
+
+    def far(cols):
+        return room.as_strided((2, cols), (1 << 31, 1))
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(12)
+    near = torch.randn(2, 4096, generator=g, device="cuda").to(torch.bfloat16)
+    at, r = torch.tensor([3, 70000], device="cuda"), ops.Rotary.create(128)
+    far(1024).copy_(near[:, :1024])
+    q = far(1024).unflatten(1, (8, 128))
+    want = ops.head_norm_rotary(near[:, :1024].unflatten(1, (8, 128)), None, at, r)[0]
+    assert torch.equal(ops.head_norm_rotary(q, None, at, r)[0], want)
+    ops.head_norm_rotary(q, None, at, r, q_out=q)
+    assert torch.equal(q, want)
+    far(4096).copy_(near)
+    u = torch.tensor([0.3, 0.8], device="cuda")
+    assert torch.equal(ops.sample_tokens(far(4096), u, top_p=0.9), ops.sample_tokens(near, u, top_p=0.9))
+    w = ops.Int4Weight.quantize(torch.randn(600, 256, generator=g, device="cuda"))
+    x = near[:, :256].contiguous()
+    want = ops.w4_gated(x, w)
+    ops.w4_gated(x, w, out=far(300))
+    assert torch.equal(far(300), want)
+    far(256).copy_(x)
+    assert torch.equal(ops.w4_gated(far(256), w), want)
