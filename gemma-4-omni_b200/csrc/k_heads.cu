@@ -13,9 +13,10 @@
 // once and walks over the token's heads; a head of dim values takes dim / 8 lanes, each with four neighbours
 // and the four that they are paired with.  Where tokens are few, a token's heads are dealt out to several warps.
 //
-// 16384 tokens of 32 + 8 heads of 128 in bf16 (336 MB) take 75 us, 4.5 TB/s, 68 % of the copy rate: instructions are issued in half of
-// the cycles, and 32 warps an SM with two heads each under way (64 registers) are what keeps most bytes in flight (four heads and 20
-// warps: 78 us; one head: 89).  Two tokens of 9 heads of 256 take 4.5 us in a graph, nearly all of it the launch.
+// 16384 tokens of 32 + 8 heads of 128 in bf16 (336 MB) take 60 us, 5.6 TB/s, 85 % of the copy rate, with four steps under way in each of 32
+// warps an SM (two: 66 us; one: 78).  The usual heads have kernels of their own, without branches for the other pairs, parts
+// and norms: instructions bind (with the branches 75 us).  Two tokens of 9 heads of 256 take 4.2 us in a graph, nearly all of it the
+// launch.
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 
@@ -69,6 +70,19 @@ __device__ __forceinline__ void sin_cos(unsigned long long turns, float& s, floa
 __device__ __forceinline__ unsigned long long position_of(const HeadsArgs& a, int token) {
   return a.positions64 ? static_cast<unsigned long long>(static_cast<const long long*>(a.positions)[token])
                        : static_cast<unsigned long long>(static_cast<long long>(static_cast<const int*>(a.positions)[token]));
+}
+// four neighbouring weights
+template <typename T>
+__device__ __forceinline__ void weights4(const HeadsArgs& a, const HeadsSide& s, int i, float (&w)[4]) {
+  if (!s.weight) {
+    w[0] = w[1] = w[2] = w[3] = 1.0f;
+  } else if (a.weight_f32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = static_cast<const float*>(s.weight)[i + j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = as_float(static_cast<const T*>(s.weight)[i + j]);
+  }
 }
 template <typename T>
 __device__ __forceinline__ float weight_at(const HeadsArgs& a, const HeadsSide& s, int i) {
@@ -137,21 +151,22 @@ __device__ __forceinline__ void store4(T* at, const pair_t (&v)[2]) {
 // The heads [first, last) of a side that this group of lanes takes, in steps of a warp's heads.  A lane's eight values are two
 // pairs at ea and two at eb; rotated ones become v * own + other * cross, with the weights in the factors (of the token and lane, for all its
 // heads) and 1 / rms behind them.
-template <typename T, int LANES>
+// kPlain: the usual heads (of 8 * LANES values, all rotated in halves, with norms), without branches.
+template <typename T, int LANES, bool kPlain>
 __device__ __forceinline__ void walk(const HeadsArgs& a, const HeadsSide& side, int token, int first, int last, int ea, int eb,
-                                     bool there, bool turned, const float (&sn)[4], const float (&cs)[4]) {
-  constexpr int kStep = 32 / LANES, kAhead = 2;
+                                     bool there_, bool turned_, const float (&sn)[4], const float (&cs)[4]) {
+  const bool there = kPlain || there_, turned = kPlain || turned_, neighbours = !kPlain && a.neighbours, norm = kPlain || a.norm;
+  constexpr int kStep = 32 / LANES, kAhead = kPlain && sizeof(T) == 2 ? 4 : 2;
   pair_t own[2][2], cross[2][2];  // [at ea, at eb][pair]
   {
-    float w[2][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[0][j] = there ? weight_at<T>(a, side, ea + j) : 0.0f;
-      w[1][j] = there ? weight_at<T>(a, side, eb + j) : 0.0f;
+    float w[2][4] = {};
+    if (there) {
+      weights4<T>(a, side, ea, w[0]);
+      weights4<T>(a, side, eb, w[1]);
     }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      if (a.neighbours) {  // of a pair (v0, v1): v0 c - v1 s, v1 c + v0 s
+      if (neighbours) {  // of a pair (v0, v1): v0 c - v1 s, v1 c + v0 s
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float c = cs[2 * e + p], s = sn[2 * e + p];
@@ -190,7 +205,7 @@ __device__ __forceinline__ void walk(const HeadsArgs& a, const HeadsSide& side, 
       widen4<T>(ra[u], v[0]);
       widen4<T>(rb[u], v[1]);
       float inv = 1.0f;
-      if (a.norm) {
+      if (norm) {
         const pair_t two = fma2(v[0][0], v[0][0], fma2(v[0][1], v[0][1], fma2(v[1][0], v[1][0], mul2(v[1][1], v[1][1]))));
         float lo, hi;
         unpair(two, lo, hi);
@@ -206,7 +221,7 @@ __device__ __forceinline__ void walk(const HeadsArgs& a, const HeadsSide& side, 
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           pair_t other = v[1 - e][p];
-          if (a.neighbours) {
+          if (neighbours) {
             float lo, hi;
             unpair(v[e][p], lo, hi);
             other = pair_of(hi, lo);
@@ -225,18 +240,18 @@ __device__ __forceinline__ void walk(const HeadsArgs& a, const HeadsSide& side, 
 }
 
 // LANES: lanes of a head, at least dim / 8
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kWarps * 32, 8) heads_kernel(const HeadsArgs a) {
+template <typename T, int LANES, bool kPlain>
+__global__ void __launch_bounds__(kWarps * 32, kPlain && sizeof(T) == 2 ? 8 : 4) heads_kernel(const HeadsArgs a) {
   const long long warp = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   if (warp >= static_cast<long long>(a.n_tokens) * a.slices) return;
   const int token = static_cast<int>(warp / a.slices), slice = static_cast<int>(warp - static_cast<long long>(token) * a.slices);
   constexpr int kStep = 32 / LANES;
   const int l = threadIdx.x & (LANES - 1);
-  const bool there = 8 * l < a.dim, turned = 8 * l < a.rotary;
+  const bool there = kPlain || 8 * l < a.dim, turned = kPlain || 8 * l < a.rotary;
   int ea = 8 * l, eb = 8 * l + 4;
-  if (!a.neighbours && turned) {
+  if (kPlain || (!a.neighbours && turned)) {
     ea = 4 * l;
-    eb = 4 * l + a.rotary / 2;
+    eb = 4 * l + (kPlain ? 4 * LANES : a.rotary / 2);
   }
   float sn[4] = {0.0f, 0.0f, 0.0f, 0.0f}, cs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
   if (turned) {
@@ -249,9 +264,9 @@ __global__ void __launch_bounds__(kWarps * 32, 8) heads_kernel(const HeadsArgs a
   const int from = static_cast<int>(static_cast<long long>(q_steps + k_steps) * slice / a.slices);
   const int to = static_cast<int>(static_cast<long long>(q_steps + k_steps) * (slice + 1) / a.slices);
   if (from < q_steps)
-    walk<T, LANES>(a, a.q, token, from * kStep, min(min(to, q_steps) * kStep, a.q.heads), ea, eb, there, turned, sn, cs);
+    walk<T, LANES, kPlain>(a, a.q, token, from * kStep, min(min(to, q_steps) * kStep, a.q.heads), ea, eb, there, turned, sn, cs);
   if (to > q_steps)
-    walk<T, LANES>(a, a.k, token, (max(from, q_steps) - q_steps) * kStep, min((to - q_steps) * kStep, a.k.heads), ea, eb, there,
+    walk<T, LANES, kPlain>(a, a.k, token, (max(from, q_steps) - q_steps) * kStep, min((to - q_steps) * kStep, a.k.heads), ea, eb, there,
                    turned, sn, cs);
 }
 
@@ -321,9 +336,11 @@ cudaError_t launch(HeadsArgs a, cudaStream_t s) {
   a.slices = static_cast<int>(want < steps ? want : steps);
   const long long warps = static_cast<long long>(a.n_tokens) * a.slices;
   const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
-  if (lanes == 8) heads_kernel<T, 8><<<grid, kWarps * 32, 0, s>>>(a);
-  else if (lanes == 16) heads_kernel<T, 16><<<grid, kWarps * 32, 0, s>>>(a);
-  else heads_kernel<T, 32><<<grid, kWarps * 32, 0, s>>>(a);
+  const bool plain = a.dim == 8 * lanes && a.rotary == a.dim && !a.neighbours && a.norm;
+  const auto kernel = lanes == 8    ? (plain ? heads_kernel<T, 8, true> : heads_kernel<T, 8, false>)
+                      : lanes == 16 ? (plain ? heads_kernel<T, 16, true> : heads_kernel<T, 16, false>)
+                                    : (plain ? heads_kernel<T, 32, true> : heads_kernel<T, 32, false>);
+  kernel<<<grid, kWarps * 32, 0, s>>>(a);
   return cudaGetLastError();
 }
 

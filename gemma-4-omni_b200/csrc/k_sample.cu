@@ -7,7 +7,7 @@
 //   token: the first by index with (sum of the kept masses up to it) > floor(u * their total)
 //
 // Masses are whole numbers, so that sums of them are the same in any order: no result depends on
-// which thread comes first.  They are computed in 64-bit floating point (to some 2^-52): a row has 10^5 borders between tokens,
+// which thread comes first.  They are computed in 64-bit floating point (to some 2^-49): a row has 10^5 borders between tokens,
 // and u falls between two roundings of one of them the more rarely the finer they are.  2^45 * 2^18 tokens stay below 2^63.
 //
 // The logits are read once.  A cluster of CTAs takes a row, each CTA holds its part of it in shared
