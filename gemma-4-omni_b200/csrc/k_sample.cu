@@ -19,7 +19,7 @@
 // so that every later pass goes over that alone: for top-p the sum of all masses and a look at a few distances come first, and
 // only what lies above the distance behind the cut is divided into bins.
 //
-// Measured (in graphs): one row of 131072 with top-k 64 and top-p 14.5 us, a chain of loads, five barriers of the cluster
+// Measured (in graphs): one row of 131072 with top-k 64 and top-p 14.5 us, a chain of loads, four barriers of the cluster
 // and 128 tokens that are ranked; 250 rows of 131072 in 32 bits by a share of 0.9 (9 thousand tokens kept a row) 264 us, 0.5 TB/s;
 // 1000 rows of 32003 by min-p 70 us.  Bound by instructions and barriers: some 45 instructions a token for its mass and the sums
 // (11 of them in 64 bits), as many again for the loads, the moves and the bins, and 16 warps that wait for one another. Sorting
@@ -69,6 +69,11 @@ struct Result {  // of one division into bins
   int bin, count, before;  // tokens in it and before it
 };
 
+struct Zone {  // of distances that hold a share's cut
+  u64 limit;
+  float lo, hi, top, low;  // top: the logits above are nearer than lo; low: those from it down are farther than hi
+};
+
 struct alignas(16) Shared {
   double power[kPowers];        // 2^(j / kPowers)
   union {
@@ -83,6 +88,7 @@ struct alignas(16) Shared {
   u64 group_mass[2][kGroups][kMaxCluster];
   unsigned group_count[2][kGroups][kMaxCluster];
   Result result;
+  Zone chosen;
   unsigned warp_count[kWarps];
   unsigned low[kMaxCluster], high[kMaxCluster];
   unsigned tie_count[kMaxCluster];
@@ -448,23 +454,31 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
       }
     }
     cluster.sync();
-    total = slot_sum(s.part_mass, ctas, 0, none);
-    limit = share_of(r.top_p, total);
-    // The sums are in units of 2^27, each short of its true value by less than 2^16 of them: a unit for each of 2^18 tokens and each warp.
-    const u64 want = limit >> 27;
-    float zone_hi = INFINITY, low = r.mass.least;
+    if (warp == 0) {  // (one warp for all: sixteen would take the others' issue slots)
+      limit = share_of(r.top_p, slot_sum(s.part_mass, ctas, 0, none));
+      // The sums are in units of 2^27, each short of its true value by less than 2^16 of them: a unit for each of 2^18 tokens and each
+      // warp.
+      const u64 want = limit >> 27;
+      Zone z0{limit, 0.0f, INFINITY, INFINITY, r.mass.least};
 #pragma unroll
-    for (int z = kZones - 1; z >= 0; --z) {
-      const u64 v = slot_sum(s.zone_sum[z], ctas, 0, none);
-      if (v > want) {
-        zone_hi = zone_end(z);
-        low = end[z];
+      for (int z = kZones - 1; z >= 0; --z) {
+        const u64 v = slot_sum(s.zone_sum[z], ctas, 0, none);
+        if (v > want) {
+          z0.hi = zone_end(z);
+          z0.low = end[z];
+        }
+        if (z0.lo == 0.0f && v + (1u << 16) < want) {
+          z0.lo = zone_end(z);
+          z0.top = end[z];
+        }
       }
-      if (zone_lo == 0.0f && v + (1u << 16) < want) {
-        zone_lo = zone_end(z);
-        zone_top = end[z];
-      }
+      if (lane == 0) s.chosen = z0;
     }
+    __syncthreads();
+    limit = s.chosen.limit;
+    zone_lo = s.chosen.lo;
+    zone_top = s.chosen.top;
+    const float zone_hi = s.chosen.hi, low = s.chosen.low;
     zone_bins = zone_hi < INFINITY ? kBins / (zone_hi - zone_lo) : 16.0f;
     left.keep(r, [&](float x, int) { return x > low; });
   }
@@ -538,16 +552,13 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
       if constexpr (kMass) *cluster.map_shared_rank(&s.group_mass[turn][g][rank], to) = m;
     }
     cluster.sync();
-    if (kMass && level == 0) {
-      u64 none;
-      above = slot_sum(s.above_mass, ctas, 0, none);
-      before = static_cast<int>(slot_sum(s.above_count, ctas, 0, none));
-    }
     // ---- the group that holds the cut, then its bins over the cluster: every CTA finds the bin for itself
-    int group = -1;
-    u64 base = 0;
-    unsigned seen = 0;
-    {
+    if (warp == 0) {
+      if (kMass && level == 0) {
+        u64 none;
+        above = slot_sum(s.above_mass, ctas, 0, none);
+        before = static_cast<int>(slot_sum(s.above_count, ctas, 0, none));
+      }
       // a lane has a group and every fourth CTA
       const int g = lane % kGroups;
       unsigned c = 0;
@@ -578,12 +589,11 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
       }
       const u64 to = above + (kMass ? upto_m : upto_c), mine = kMass ? m : c;
       const unsigned who = __ballot_sync(0xffffffffu, lane < kGroups && to - mine < limit && limit <= to);
-      if (who == 0) return false;  // (counts: no more than k tokens, all are kept)
-      group = __ffs(who) - 1;
-      base = __shfl_sync(0xffffffffu, to - mine, group);
-      seen = before + __shfl_sync(0xffffffffu, upto_c - c, group);
-    }
-    if (warp == 0) {  // two bins a lane
+      const int group = who ? __ffs(who) - 1 : 0;
+      const u64 base = __shfl_sync(0xffffffffu, to - mine, group);
+      const unsigned seen = before + __shfl_sync(0xffffffffu, upto_c - c, group);
+      if (who == 0 && lane == 0) s.result = {0, -1, 0, 0};
+      // two bins a lane
       static_assert(kGroupBins == 64, "two bins a lane");
       u64 w[2] = {0, 0};
       unsigned n[2] = {0, 0};
@@ -615,21 +625,22 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
         w[0] = n[0];
         w[1] = n[1];
       }
-      u64 to = base + warp_inclusive(w[0] + w[1]);
+      u64 upto = base + warp_inclusive(w[0] + w[1]);
       unsigned upto_n = n[0] + n[1];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const unsigned y = __shfl_up_sync(0xffffffffu, upto_n, o);
         if (lane >= o) upto_n += y;
       }
-      to -= w[1];
-      if (to - w[0] < limit && limit <= to)
-        s.result = {to - w[0], group * kGroupBins + 2 * lane, static_cast<int>(n[0]), static_cast<int>(seen + upto_n - n[1] - n[0])};
-      if (to < limit && limit <= to + w[1])
-        s.result = {to, group * kGroupBins + 2 * lane + 1, static_cast<int>(n[1]), static_cast<int>(seen + upto_n - n[1])};
+      upto -= w[1];
+      if (who && upto - w[0] < limit && limit <= upto)
+        s.result = {upto - w[0], group * kGroupBins + 2 * lane, static_cast<int>(n[0]), static_cast<int>(seen + upto_n - n[1] - n[0])};
+      if (who && upto < limit && limit <= upto + w[1])
+        s.result = {upto, group * kGroupBins + 2 * lane + 1, static_cast<int>(n[1]), static_cast<int>(seen + upto_n - n[1])};
     }
     __syncthreads();
     const Result found = s.result;
+    if (found.bin < 0) return false;  // (counts: no more than k tokens, all are kept)
     above = found.above;
     before = found.before;
     const bool all = found.before + found.count <= kList;  // everything down to the cut fits the list
