@@ -19,13 +19,13 @@
 // sums to the CTA that finishes the token (stores over the cluster), which adds them up in the order of K.
 //
 // Measured, 1536 x 6144 in groups of 128 (in graphs): 2 rows of e4m3 11 us (9.8 MB at 0.9 TB/s: a chain of launch, first loads, six
-// blocks of some 0.67 us, in which the widening warps set the pace, and the join), 128 rows 14, 499 rows 28, 4096 rows 162 (955
-// TFLOP/s, 57 % of the measured rate; 196 us where the power limit holds the clocks down).  What bounds the large ones is the work
-// beside the MMAs: of 5100 instructions for a tile of 128 tokens and a block of K the widening takes 35 %, sums 16 %, results 11 %;
-// the tensor pipe is busy for 44 % of the time.  A tile's results are not covered by the next one's MMAs, which stop two units
-// ahead (3.9 thousand of some 28 thousand cycles a tile).  Groups of 64 and 32 take two and four times the sums: 210 and 340 us.
+// blocks of some 0.67 us, in which the widening warps set the pace, and the join), 128 rows 14, 499 rows 27, 4096 rows 136 in bf16 (1134
+// TFLOP/s, 68 % of the measured rate; 164 us where the power limit holds the clocks down), 144 in fp16, 151 in int8, 173 in
+// e4m3.  What bounds the large ones is the work beside the MMAs: of some 5 thousand instructions for a tile of 128 tokens and a block
+// of K the widening takes a third, sums a sixth and results a tenth.  A tile's results are not covered by the next one's MMAs, which
+// stop two units ahead.  Groups of 64 and 32 take two and four times the sums: 197 and 326 us.
 // On the way (4096 rows): one lane issuing all MMAs 254 us, a warp that walks together 214, two widening warpgroups
-// instead of one 192, a warp a side for the MMAs 164 (the waits of one were as long as its MMAs).
+// instead of one 192, a warp a side for the MMAs 164 (the waits of one were as long as its MMAs), results without a loop 145.
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 #include "kernels.h"
@@ -69,6 +69,11 @@ struct Shape {
   static constexpr int kSideD = NT > 64 ? 1 : 2, kD = 2 * kSideD;  // accumulators in the tensor memory, of a side and in all
   static constexpr int kCols = NT / 2;                        // tokens of an adding warpgroup
   static constexpr int kSteps = kWide ? 16 : 32;              // k of an MMA
+  // Registers a thread by role.  Wide tiles of 16-bit operands are best with 40 and 176 (4096 x 1536 x 6144: 136 us; 48 and 168: 144);
+  // the widening of 8-bit ones holds more constants (e4m3 173 instead of 180), and narrow tiles wait for the widening (2 rows 9.9
+  // instead of 10.4).
+  static constexpr bool kMoreSums = kWide && NT > 64;
+  static constexpr int kLoadRegs = 40, kWidenRegs = kMoreSums ? 40 : 48, kAddRegs = kMoreSums ? 176 : 168;
   static_assert(kD * NT <= kAColumn, "tensor memory");
 };
 
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
   if (!joined) cluster_arrive();
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kLoadRegs));
     if (warp == 0 && lane == 0) {
       // ---------------- loads
       int st = 0;
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
     }
     __syncwarp();
   } else if (warp < kFirstAdder) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kWidenRegs));
     // ---------------- codes -> operands, a warpgroup a side; a lane has a row, and brings the row's scales too
     const int side = (warp - 4) >> 2, row = 32 * (warp & 3) + lane, groups = a.k / a.group;
     const Widen<X> widen;
@@ -550,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kAddRegs));
     // ---------------- sums and results
     const int half = (warp - kFirstAdder) >> 2, row = 32 * (warp & 3) + lane;
     const uint32_t from = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * S::kCols;
@@ -627,19 +632,20 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
         const int live = o < a.f ? a.m - t0 : 0;  // tokens from t0 on
         const long long pitch = a.ld_out * (a.out_dtype == LB_F32 ? 4 : 2);
         unsigned char* at = static_cast<unsigned char*>(a.out) + t0 * pitch + static_cast<long long>(o) * (a.out_dtype == LB_F32 ? 4 : 2);
-        // up to 32 tokens a turn, the rest move up: a loop that stays in the instruction cache
-        constexpr int kTurn = S::kCols % 32 == 0 ? 32 : S::kCols > 32 ? S::kCols / 2 : S::kCols;  // (48: twice 24)
+        // up to 32 tokens are computed before they are stored, without a branch between them.  (A loop over turns, with the rest moving up
+        // to the first registers, took 18 us more of 163 for 4096 rows of 1536 x 6144.)
         const bool whole = tile % a.o_tiles * kBlockO + kBlockO <= a.f && t0 + S::kCols <= a.m;
         const auto turn = [&](auto gelu, auto type) {
           using Out = decltype(type);
-#pragma unroll 1
+          constexpr int kTurn = S::kCols % 32 == 0 ? 32 : 16;
+#pragma unroll
           for (int j0 = 0; j0 < S::kCols; j0 += kTurn) {
             float v[kTurn];
 #pragma unroll
             for (int j = 0; j < kTurn; ++j) {
               float g[2], u[2];
-              unpair(acc[0][j / 2], g[0], g[1]);
-              unpair(acc[1][j / 2], u[0], u[1]);
+              unpair(acc[0][(j0 + j) / 2], g[0], g[1]);
+              unpair(acc[1][(j0 + j) / 2], u[0], u[1]);
               float gate = g[j & 1], up = u[j & 1];
               if (!S::kWide && !grouped) {
                 const float xs = __shfl_sync(0xffffffffu, j0 + j >= 32 ? row_scale[1] : row_scale[0], (j0 + j) & 31);
@@ -657,11 +663,6 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const GatedArgs a, c
                 if (j0 + j < live) put(reinterpret_cast<Out*>(at + j * pitch), v[j]);
             }
             at += kTurn * pitch;
-#pragma unroll
-            for (int j = 0; j + kTurn / 2 < S::kCols / 2; ++j) {
-              acc[0][j] = acc[0][j + kTurn / 2];
-              acc[1][j] = acc[1][j + kTurn / 2];
-            }
           }
         };
         const auto typed = [&](auto gelu) {
@@ -752,12 +753,12 @@ cudaError_t launch(const GatedArgs& a, int splits, const CUtensorMap& w_map, con
   cudaError_t e = ensure_smem(done, reinterpret_cast<const void*>(kernel), S::kSmem);
   if (e != cudaSuccess) return e;
   if (registers.load(std::memory_order_relaxed) == 0) {
-    // the warpgroups' shares of the registers (40 + 2 * 48 + 2 * 168 a thread of each) have to fit what the block is launched with
+    // the five warpgroups' shares of the registers have to fit what the block is launched with: more would be waited for without end
     cudaFuncAttributes f;
     if ((e = cudaFuncGetAttributes(&f, reinterpret_cast<const void*>(kernel))) != cudaSuccess) return e;
     registers.store(f.numRegs, std::memory_order_relaxed);
   }
-  if (registers.load(std::memory_order_relaxed) * 5 < 40 + 2 * 48 + 2 * 168) return cudaErrorInvalidConfiguration;
+  if (registers.load(std::memory_order_relaxed) * 5 < S::kLoadRegs + 2 * S::kWidenRegs + 2 * S::kAddRegs) return cudaErrorInvalidConfiguration;
   const int tiles = a.o_tiles * a.t_tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = static_cast<unsigned>(splits > 1 ? tiles * splits : tiles < kSms ? tiles : kSms);
