@@ -24,6 +24,7 @@
 // 1000 rows of 32003 by min-p 70 us.  Bound by instructions and barriers: some 45 instructions a token for its mass and the sums
 // (11 of them in 64 bits), as many again for the loads, the moves and the bins, and 16 warps that wait for one another. Sorting
 // or ranking fewer tokens in one CTA holds up the other seven of a row: 512 sorted took 12 thousand cycles, 128 ranked take 3.
+#include <cfloat>
 #include <cooperative_groups.h>
 
 #include "../../include/listener_b200.h"
@@ -888,8 +889,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     }
     return;
   }
-  if (top == INFINITY) {  // infinities share the draw alone: they become 0, the rest nothing
-    for (int i = t; i < n; i += kThreads) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+  // Infinities share the draw alone: they become 0, the rest nothing.  Where the numbers end within the masses' reach of the maximum (a row
+  // that a mask filled with the lowest number) nothing finite would be left for those without a mass, -infinity
+  // among them: such a row is moved up by its maximum, which is exact for numbers within a factor of two.
+  const bool infinite = top == INFINITY, low = top == -FLT_MAX || static_cast<double>(top) - s.reach < -static_cast<double>(FLT_MAX);
+  if (infinite || low) {
+    for (int i = t; i < n; i += kThreads) x[i] = low ? x[i] - top : x[i] == INFINITY ? 0.0f : -INFINITY;
     top = 0.0f;
     __syncthreads();
   }

@@ -104,6 +104,31 @@ def test_masked_rows_and_infinities(ops):
         check(ops, small, torch.tensor([0.9, 0.9], device="cuda"), **settings)
 
 
+@pytest.mark.parametrize("vocab", [300, 5000, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_of_the_lowest_numbers(ops, vocab, dtype):
+    """Rows that a mask filled with the type's lowest number, beside -inf and NaN, which have no mass at any temperature."""
+    lowest = torch.finfo(dtype).min
+    near = torch.tensor([lowest], dtype=dtype, device="cuda")
+    ups = [near]
+    for _ in range(5):
+        ups.append(torch.nextafter(ups[-1], torch.zeros_like(near)))
+    x = torch.full((6, vocab), -math.inf, dtype=dtype, device="cuda")
+    x[0, ::3] = lowest
+    x[1], x[1, 1::2] = lowest, math.nan
+    x[2, vocab - 2] = lowest
+    x[3, 5::7], x[3, 6::7] = lowest, ups[1]
+    for i, v in enumerate(ups):
+        x[4, i::11] = v
+    x[5], x[5, 7] = lowest, ups[1]
+    u = torch.tensor([0.999, 0.5, 0.9, 0.3, 0.999999, 0.7], device="cuda")
+    for settings in (dict(), dict(top_k=100), dict(top_p=0.6), dict(top_k=vocab - 10, top_p=0.9, min_p=0.1), dict(min_p=0.5),
+                     dict(temperature=0.0), dict(temperature=1e-6), dict(temperature=1e30), dict(temperature=1e30, top_p=0.5),
+                     dict(temperature=1e30, top_k=vocab // 2, top_p=0.999999)):
+        tokens = check(ops, x, u, **settings)
+        assert int(tokens[2]) == vocab - 2
+
+
 def vectorised(x, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """The rule over many rows at once, on the GPU: (tokens, log probabilities)."""
     x, order = torch.sort(x.float(), dim=1, descending=True, stable=True)
