@@ -489,10 +489,12 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
     for (int i = t; i < (kMass ? 4 : 1) * kBins; i += kThreads) (&s.hist[0][0])[i] = 0;
     if (t == 0) s.listed = 0;
     __syncthreads();
+    // In bins from the zone's beginning; infinite (of -infinity, and where a product overflows, far below any mass): in none.
+    const auto place_of = [&](float x) { return __fmul_rn(__fsub_rn(r.distance(x), zone_lo), zone_bins); };
     const auto bin_of = [&](float x) -> int {  // -1: below, -2: above
       if (level == 0) {
-        const float d = r.distance(x);
-        return d >= INFINITY ? -1 : x > zone_top ? -2 : max(0, min(kBins - 1, __float2int_rz(__fmul_rn(__fsub_rn(d, zone_lo), zone_bins))));
+        const float place = place_of(x);
+        return place >= INFINITY ? -1 : x > zone_top ? -2 : max(0, min(kBins - 1, __float2int_rz(place)));
       }
       const unsigned o = ordered(x);
       return o < lo ? -1 : o > hi ? -2 : static_cast<int>((hi - o) >> shift);
@@ -648,13 +650,13 @@ __device__ __forceinline__ bool select(const Row& r, cg::cluster_group& cluster,
     // the tokens of the bin and above: at level 0 by the product that the bin is the whole part of
     const float edge = found.bin == kBins - 1 ? INFINITY : static_cast<float>(found.bin + 1);
     const auto down_to = [&](float x) {
-      if (level == 0) return __fmul_rn(__fsub_rn(r.distance(x), zone_lo), zone_bins) < edge;
+      if (level == 0) return place_of(x) < edge;
       const int b = bin_of(x);
       return b == -2 || (b >= 0 && b <= found.bin);
     };
     if (all || found.count <= kList) {
       Shared& lead = *cluster.map_shared_rank(&s, 0);
-      if (level == 0) left.keep(r, [&](float x, int) { return __fmul_rn(__fsub_rn(r.distance(x), zone_lo), zone_bins) < edge; });
+      if (level == 0) left.keep(r, [&](float x, int) { return place_of(x) < edge; });
       else left.keep(r, [&](float x, int) { return down_to(x); });
       const float* x = r.logits() + left.base;
       const uint16_t* at = r.indexes() + left.base;

@@ -129,6 +129,29 @@ def test_rows_of_the_lowest_numbers(ops, vocab, dtype):
         assert int(tokens[2]) == vocab - 2
 
 
+@pytest.mark.parametrize("vocab", [400, 2000, 32003, 70001])
+@pytest.mark.parametrize("dtype,mask", [(F32, torch.finfo(F32).min), (F32, torch.finfo(BF16).min), (F32, -1e38), (F32, -1e37), (BF16, torch.finfo(BF16).min),
+                                        (BF16, -2e37), (F16, torch.finfo(F16).min)])
+def test_top_k_among_masked_tokens(ops, vocab, dtype, mask):
+    """Fewer tokens than top_k asks for, the rest of a mask's large finite value or -inf: cuts fall among tokens without a mass, whose
+    distance to the maximum, in bins, is a number or not."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(vocab)
+    rows = [(60, 10), (60, 200), (vocab - 5, 5), (vocab // 2, vocab // 3), (1, vocab - 1)]
+    x = torch.full((len(rows), vocab), -math.inf, dtype=dtype, device="cuda")
+    for row, (live, masked) in zip(x, rows):
+        order = torch.randperm(vocab, generator=g, device="cuda")
+        row[order[:live]] = (torch.randn(live, generator=g, device="cuda") * 2.5).to(dtype)
+        row[order[live:live + masked]] = mask
+    u = torch.tensor([0.9999, 0.5, 0.3, 0.99, 0.7], device="cuda")
+    k = torch.tensor([live + (masked + 1) // 2 for live, masked in rows], dtype=torch.int32, device="cuda")
+    for temperature in (0.8, 1.0, 1.3, 10.0):
+        check(ops, x, u, temperature=temperature, top_k=k)
+        check(ops, x, u, temperature=temperature, top_k=k, top_p=0.95, min_p=0.01)
+    check(ops, x, u, top_p=0.9999)
+    check(ops, x, u, top_k=64, top_p=1.0 - 2.0 ** -24)
+
+
 def vectorised(x, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """The rule over many rows at once, on the GPU: (tokens, log probabilities)."""
     x, order = torch.sort(x.float(), dim=1, descending=True, stable=True)
