@@ -101,8 +101,8 @@ class DecoderBlock:
             (c.heads, c.kv_heads, c.kv_heads), 1)
         at = plan.positions[:t]
         if c.fused:
-            q, k = ops.head_norm_rotary(q, k, at, self.rotary, q_weight=self.w.get("q_norm"), k_weight=self.w.get("k_norm"),
-                                        eps=c.rms_eps, norm=c.qk_norm)
+            q_norm, k_norm = (self.w["q_norm"], self.w["k_norm"]) if c.qk_norm else (None, None)
+            q, k = ops.head_norm_rotary(q, k, at, self.rotary, q_weight=q_norm, k_weight=k_norm, eps=c.rms_eps, norm=c.qk_norm)
         else:
             q, k = rotary(q, at, c.rope_base), rotary(k, at, c.rope_base)
         cache.append(k, v, plan.slots[:t])

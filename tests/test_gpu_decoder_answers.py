@@ -92,6 +92,16 @@ def test_agrees_with_the_block_in_plain_torch(parts):
             assert (x.double() - y.double()).norm() <= 0.05 * y.double().norm()
 
 
+def test_head_norms_weights_count_with_qk_norm_only(parts):
+    """A dict of weights that also holds head norms serves a block without them, as it does where rotation and gate are plain torch."""
+    normed = parts.DecoderBlock.synthetic(config(parts, qk_norm=True), seed=13)
+    cfg = replace(normed.cfg, qk_norm=False)
+    xs = rows(14, 20, 3)
+    a, _, _ = run(parts.DecoderBlock(cfg, normed.w), [xs])
+    b, _, _ = run(parts.DecoderBlock(cfg, {k: v for k, v in normed.w.items() if k not in ("q_norm", "k_norm")}), [xs])
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_ticks_one_by_one_agree_with_a_whole_chunk(parts):
     """As for the block in plain torch: 5 % of the output's norm."""
     block = parts.DecoderBlock.synthetic(config(parts, qk_norm=True), seed=5)
