@@ -490,22 +490,41 @@ def w4_gated(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | Non
     return out
 
 
-_PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510")
+_DIGITS = 400  # the 309 before the point of the largest double, 64 bits behind it, and some to spare
+
+
+@functools.lru_cache(maxsize=1)
+def _two_pi() -> decimal.Decimal:
+    """2 pi to more than _DIGITS digits, over whole numbers: pi / 4 = 4 arctan(1 / 5) - arctan(1 / 239) (Machin)."""
+    one = 10 ** (_DIGITS + 20)
+
+    def arctan(n: int) -> int:
+        term = total = one // n
+        k = 1
+        while term:
+            term //= -n * n
+            k += 2
+            total += term // k
+        return total
+
+    with decimal.localcontext() as c:
+        c.prec = _DIGITS + 20
+        return decimal.Decimal(8 * (4 * arctan(5) - arctan(239))) / one
 
 
 @functools.lru_cache(maxsize=64)
 def _turns(rotary_dim: int, base: float) -> tuple[int, ...]:
     """The frequencies base ** (-2 i / rotary_dim), in turns a position, as signed 64-bit fractions of a turn."""
     with decimal.localcontext() as c:
-        c.prec = 50
+        c.prec = 50 if base >= 1.0 else _DIGITS  # (digits before the point too)
         return tuple(_fraction(decimal.Decimal(base) ** (decimal.Decimal(-2 * i) / rotary_dim)) for i in range(rotary_dim // 2))
 
 
 def _fraction(radians: decimal.Decimal) -> int:
     """radians / (2 pi) modulo 1 as a whole number of 2^-64, in the range of int64."""
     with decimal.localcontext() as c:
-        c.prec = 400  # the whole turns of any double, and 64 bits behind the point
-        v = int((radians / (2 * _PI) * 2 ** 64).to_integral_value(decimal.ROUND_HALF_EVEN)) % 2 ** 64
+        c.prec = _DIGITS
+        v = int((radians / _two_pi() * 2 ** 64).to_integral_value(decimal.ROUND_HALF_EVEN)) % 2 ** 64
     return v - 2 ** 64 if v >= 2 ** 63 else v
 
 

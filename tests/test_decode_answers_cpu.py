@@ -1,6 +1,7 @@
 """The entries between a block's products and at its end refuse bad arguments before they touch a GPU."""
 from __future__ import annotations
 
+import decimal
 import math
 
 import pytest
@@ -46,6 +47,30 @@ def test_turns_are_the_frequencies(pkg):
         assert len(turns) == dim // 2
         for i, t in enumerate(turns):
             assert abs(t / 2.0 ** 64 * 2 * math.pi - base ** (-2.0 * i / dim)) <= 2.0 ** -51
+
+
+def test_turns_of_large_frequencies(pkg):
+    """What is left of the whole turns of any double, over whole numbers (pi by Gauss's formula to 450 digits)."""
+    from fractions import Fraction
+    from gemma4_omni_b200 import decode_ops as ops
+    one = 10 ** 460
+
+    def arctan(n):
+        return sum((-1) ** k * (one // n ** (2 * k + 1) // (2 * k + 1)) for k in range(400))
+
+    two_pi = Fraction(2 * (48 * arctan(18) + 32 * arctan(57) - 20 * arctan(239)), one)
+    assert abs(float(two_pi) - 2 * math.pi) < 1e-15
+
+    def want(radians):
+        v = round(radians * 2 ** 64 / two_pi) % 2 ** 64
+        return v - 2 ** 64 if v >= 2 ** 63 else v
+
+    for f in (0.0, 5e-324, 1e-10, 1.0, -1.0, 3.0, 1e15, 1e33, -1e40, 1e80, 2.0 ** 1000, 1.7976931348623157e308, -1.7976931348623157e308):
+        assert ops._fraction(decimal.Decimal(f)) == want(Fraction(f)), f
+    # a base below 1 has frequencies above it: 1, base ** -1/2
+    for base in (0.25, 1e-30, 1e-300):
+        root = Fraction(math.isqrt(int(10 ** 800 / Fraction(base))), 10 ** 400)
+        assert ops._turns(4, base) == (want(Fraction(1)), want(root))
 
 
 def test_wrappers_have_no_cpu_path(pkg):
