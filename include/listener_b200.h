@@ -569,8 +569,9 @@ int lb_op_sample(const void* logits, int64_t row_stride, int dtype, int rows, in
  *   out[t][o] = act(g) * u,  g = x[t] . W[o],  u = x[t] . W[ffn + o],  o < ffn
  * with W[r][k] = (n[r][k] - 8) * w_scale[r][k / group] of 2 ffn rows as in lb_op_w4_matvec, x and x_scale as there.
  * activation 0: silu, g / (1 + exp(-g)); 1: gelu, g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2.  Sums, activation
- * and product in 32 bits, rounded once to out_dtype (LB_F32, LB_BF16, LB_F16); ld_out elements between rows.  x and its rows
- * 16-byte aligned (x_ld times its type's size a multiple of 16 where m > 1), codes 16-byte aligned.
+ * and product in 32 bits, rounded once to out_dtype (LB_F32, LB_BF16, LB_F16); act(g) / g may be 0 where it is below 2^-126.
+ * ld_out elements between rows.  x and its rows 16-byte aligned
+ * (x_ld times its type's size a multiple of 16 where m > 1), codes 16-byte aligned.
  * *status (may be NULL) gets LB_DEV_WAIT_TIMEOUT if the kernel gave up on a bounded wait: out is then undefined. */
 int lb_op_w4_gated(const void* x, int64_t x_ld, int x_dtype, const float* x_scale, int x_group, int m,
                    const void* codes, const void* w_scale, int group, int ffn, int k, int activation, void* out,

@@ -103,6 +103,28 @@ def test_extreme_codes_and_scales(ops):
             assert (out[:, 2:4] == 0).all()
 
 
+@pytest.mark.parametrize("rows,k", [(2, 64), (200, 64), (3, 1024), (40, 1024), (600, 256)])
+def test_gates_far_below_zero(ops, rows, k):
+    """g and u are exact (one x, codes -8 and 1), exp is good to 2^-21, the sum, the reciprocal and the products to some steps: 2^-20 in
+    all; gelu's z is off by six roundings, 6 * 2^-24 |z| < 2^-21 |z|; a reciprocal below the normal numbers, 2^-126, may count as 0."""
+    ffn = 128
+    codes = torch.zeros(2 * ffn, k // 2, dtype=torch.uint8, device="cuda")
+    codes[ffn:] = 0x99
+    scales = torch.ones(2 * ffn, k // 32, dtype=F16, device="cuda")
+    x = torch.zeros(rows, k, dtype=BF16, device="cuda")
+    x[torch.arange(rows, device="cuda"), (torch.arange(rows, device="cuda") * 37) % k] = 1.0
+    for activation, ends in (("silu", (10.0, 104.0)), ("gelu", (3.0, 14.0))):
+        scales[:ffn] = torch.linspace(*ends, ffn, device="cuda")[:, None].div(8).to(F16)
+        w = ops.Int4Weight(codes, scales)
+        out = ops.w4_gated(x, w, activation=activation, out_dtype=F32)
+        g = scales[:ffn, 0].double() * -8
+        z = g if activation == "silu" else 2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)
+        ref = g / (1 + torch.exp(-z))
+        relative = 2.0 ** -20 + (0 if activation == "silu" else 2.0 ** -21 * z.abs())
+        assert ((out.double() - ref).abs() <= relative * ref.abs() + 2.0 ** -126 * g.abs()).all()
+        assert (out[:, z > -86] < 0).all()
+
+
 def test_rows_that_are_not_finite_stay_by_themselves(ops):
     x, _, w = inputs(ops, 40, 512, 200, 128, BF16, 0, 3)
     want = ops.w4_gated(x, w)
