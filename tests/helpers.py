@@ -146,3 +146,25 @@ def replay_oracle_trace(model, g):
         layers.append(torch.stack(lay))
         off += n
     return torch.cat(raws), torch.cat(softs), torch.cat(subs), torch.cat(layers, dim=1)
+
+
+def exact_gated_case(rows, k, ffn, group, x_type, x_group, seed, device):
+    """(x, x_scale or None, codes, scales) of a gated product whose two sums are exact in 32 bits in any order: whole numbers of x up to 3, scales of x
+    1 or 2, odd numbers of six bits (in units of 2^-12) as the weights' scales, so that the absolute terms of a sum stay
+    below k * 3 * 2 * 8 * 63 < 2^24 units for k up to 4096.  Codes times scales have up to nine bits, one more than bf16."""
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    codes = torch.randint(0, 256, (2 * ffn, k // 2), generator=g, device=device, dtype=torch.uint8)
+    scales = torch.randint(16, 32, (2 * ffn, k // group), generator=g, device=device) * 2 + 1
+    x = torch.randint(1, 4, (rows, k), generator=g, device=device) * (torch.randint(0, 2, (rows, k), generator=g, device=device) * 2 - 1)
+    xs = None
+    if x_type in (torch.int8, torch.float8_e4m3fn):
+        xs = torch.randint(1, 3, (rows, k // x_group if x_group else 1), generator=g, device=device).float()
+    assert k * 3 * 2 * 8 * 63 < 1 << 24
+    return x.float().to(x_type), xs, codes, (scales * 2.0 ** -12).to(torch.float16)
+
+
+def exact_gated_limit(ref):
+    """The error of act(g) * u for exact g and u: exp2 is good to 2^-22, its correction, the sum, the products and the store to 2^-24
+    each, the reciprocal to 2^-23, which is less than 2^-20 of the result in all."""
+    return 2.0 ** -20 * ref.abs()

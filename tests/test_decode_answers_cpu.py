@@ -73,6 +73,33 @@ def test_turns_of_large_frequencies(pkg):
         assert ops._turns(4, base) == (want(Fraction(1)), want(root))
 
 
+@pytest.mark.parametrize("k,group", [(1536, 128), (4096, 32)])
+def test_exact_gated_case_shows_small_faults(k, group):
+    """What the case of exact sums is for: weights rounded to bf16, one column left out, or the scales of two groups or rows exchanged
+    leave its bound at most outputs that they touch."""
+    import torch
+    from helpers import exact_gated_case, exact_gated_limit
+    from oracle import decode_ref
+    x, _, codes, scales = exact_gated_case(8, k, 64, group, torch.bfloat16, 0, k, "cpu")
+    weight = (torch.stack([codes & 15, codes >> 4], 2).view(128, k).double() - 8) * scales.double().repeat_interleave(group, 1)
+
+    def gated(w, x=x.double()):
+        g, u = (x @ w.t()).chunk(2, 1)
+        return g * torch.sigmoid(g) * u
+
+    ref, _ = decode_ref.gated(x, None, codes, scales, activation="silu")
+    assert ((gated(weight) - ref).abs() <= exact_gated_limit(ref) / 2 ** 20).all()
+    sums = x.double() @ weight.t()
+    assert torch.equal(sums, sums.float().double()) and torch.equal((x.float() @ weight.t().float()).double(), sums)
+    short = x.double().clone()
+    short[:, k // 2 + 1] = 0
+    turned = scales.roll(1, 1).double().repeat_interleave(group, 1)
+    rows = scales.roll(1, 0).double().repeat_interleave(group, 1)
+    for wrong in (gated(weight.bfloat16().double()), gated(weight, short), gated(weight / scales.double().repeat_interleave(group, 1) * turned),
+                  gated(weight / scales.double().repeat_interleave(group, 1) * rows)):
+        assert ((wrong - ref).abs() > exact_gated_limit(ref)).double().mean() > 0.9
+
+
 def test_wrappers_have_no_cpu_path(pkg):
     import torch
     from gemma4_omni_b200 import decode_ops as ops

@@ -10,6 +10,7 @@ import math
 import pytest
 import torch
 
+from helpers import exact_gated_case, exact_gated_limit
 from oracle import decode_ref
 
 pytestmark = pytest.mark.gpu
@@ -56,6 +57,19 @@ def test_follows_the_definition(ops, rows, k, ffn, group, x_type, x_group):
     y = ops.w4_gated(x, w, x_scale=xs, activation="gelu")
     assert y.dtype == (BF16 if x_type in TOP else x_type)
     check(y, x, xs, w, "gelu")
+
+
+@pytest.mark.parametrize("x_type,x_group", [(BF16, 0), (F16, 0), (E4M3, 0), (I8, 0), (E4M3, 256), (I8, 128)])
+@pytest.mark.parametrize("rows,k,ffn,group", [
+    (3, 4096, 200, 32), (40, 4096, 200, 128), (2, 1536, 2600, 64), (30, 1536, 2600, 128), (2, 1536, 6144, 128), (70, 2048, 3000, 32),
+    (130, 2048, 1000, 64), (300, 1536, 1500, 128), (500, 1536, 6144, 64), (1000, 4096, 1300, 128)])
+def test_sums_are_exact_where_they_can_be(ops, rows, k, ffn, group, x_type, x_group):
+    """Long sums without a rounding, over every dealing out of K and every width of a tile: what is left is the activation's error."""
+    x, xs, codes, scales = exact_gated_case(rows, k, ffn, group, x_type, x_group, rows + k, "cuda")
+    w = ops.Int4Weight(codes, scales)
+    ref, _ = decode_ref.gated(x, xs, codes, scales, activation="silu")
+    out = ops.w4_gated(x, w, x_scale=xs, out_dtype=F32)
+    assert ((out.double() - ref).abs() <= exact_gated_limit(ref)).all() and w.status() == 0
 
 
 @pytest.mark.parametrize("x_type", [BF16, F16, E4M3, I8])
