@@ -29,6 +29,7 @@
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "rows.h"
 
 namespace lb {
 namespace {
@@ -808,6 +809,8 @@ extern "C" int lb_op_w4_gated(const void* x, int64_t x_ld, int x_dtype, const fl
   if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(x) % 16 != 0 || (m > 1 && x_ld * size % 16 != 0))
     return LB_ERR_INVALID_ARGUMENT;
   if (ffn > (1 << 24) || m > (1 << 24) || x_ld > (1ll << 36)) return LB_ERR_CAPACITY;
+  const int64_t out_size = out_dtype == LB_F32 ? 4 : 2;
+  if (rows_meet({x, x_ld * size, 0, m, 1, k * size}, {out, ld_out * out_size, 0, m, 1, ffn * out_size})) return LB_ERR_INVALID_ARGUMENT;
   GatedArgs a{x_scale, static_cast<const __half*>(w_scale), out, ld_out, status, x_group == k ? 0 : x_group, m, ffn, k, group, out_dtype,
               activation, 0, 0, 0};
   a.o_tiles = (ffn + kBlockO - 1) / kBlockO;

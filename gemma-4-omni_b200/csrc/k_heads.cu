@@ -19,6 +19,7 @@
 // launch.
 #include "../../include/listener_b200.h"
 #include "common.cuh"
+#include "rows.h"
 
 namespace lb {
 namespace {
@@ -320,6 +321,20 @@ bool aligned(const HeadsSide& s, int n_tokens, int unit, int size) {
          whole(s.token, n_tokens) && whole(s.out_token, n_tokens) && whole(s.head, s.heads) && whole(s.out_head, s.heads);
 }
 
+// An output may be its own input, with the same strides; no other two share memory.
+bool apart(const HeadsArgs& a, int64_t size) {
+  const auto rows = [&](const void* at, long long token, long long head, int heads) {
+    return Rows{at, token * size, head * size, a.n_tokens, heads, a.dim * size};
+  };
+  const Rows in[2] = {rows(a.q.x, a.q.token, a.q.head, a.q.heads), rows(a.k.x, a.k.token, a.k.head, a.k.heads)};
+  const Rows out[2] = {rows(a.q.out, a.q.out_token, a.q.out_head, a.q.heads), rows(a.k.out, a.k.out_token, a.k.out_head, a.k.heads)};
+  for (int i = 0; i < 2; ++i) {
+    const bool own = in[i].at == out[i].at && (a.n_tokens == 1 || in[i].token == out[i].token) && (in[i].heads == 1 || in[i].head == out[i].head);
+    if ((!own && rows_meet(out[i], in[i])) || rows_meet(out[i], in[1 - i])) return false;
+  }
+  return !rows_meet(out[0], out[1]);
+}
+
 template <typename T>
 cudaError_t launch(HeadsArgs a, cudaStream_t s) {
   const bool fast = a.dim % 8 == 0 && a.dim <= 256 && a.rotary % 8 == 0 && aligned(a.q, a.n_tokens, 4, sizeof(T)) &&
@@ -375,6 +390,7 @@ extern "C" int lb_op_head_norm_rotary(const void* q, int64_t q_token_stride, int
   a.weight_f32 = weight_dtype == LB_F32;
   a.norm = norm != 0;
   a.eps = eps;
+  if (!apart(a, dtype == LB_F32 ? 4 : 2)) return LB_ERR_INVALID_ARGUMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == LB_F32 ? launch<float>(a, s) : dtype == LB_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
   return e == cudaSuccess ? LB_OK : LB_ERR_CUDA;

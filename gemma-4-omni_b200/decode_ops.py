@@ -460,7 +460,7 @@ def w4_gated(x: torch.Tensor, weight: Int4Weight, *, x_scale: torch.Tensor | Non
 
     ``weight`` [2 * ffn, k] has the gate's rows, then those of up.  x and ``x_scale`` as in ``w4_matvec``, from one row
     to thousands; both products, the activation ("silu", or "gelu" in its tanh form) and the product are in 32
-    bits, rounded once.  ``out_dtype`` defaults to x's type, bfloat16 for 8-bit x."""
+    bits, rounded once.  ``out_dtype`` defaults to x's type, bfloat16 for 8-bit x.  ``out`` shares no memory with x."""
     dev = weight.device
     rows, group, x_step = _product_input(x, weight, x_scale)
     if weight.out_features % 2:
@@ -575,7 +575,7 @@ def head_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     q [tokens, heads, dim], k [tokens, kv_heads, dim] (or None) of one type, such as views of one product's output; positions
     int32 or int64 [tokens], as a ``PagePlan`` has them.  With ``norm`` each head's values become x / sqrt(mean(x^2) + eps) *
     weight (weights f32 or of q's type, None: 1).  ``q_out`` / ``k_out`` may be q and k themselves, and share
-    no memory with an input otherwise."""
+    no memory with an input or one another otherwise (the call is refused)."""
     dev = rotary.device
     if q.dim() != 3 or q.dtype not in FLOAT_INPUTS:
         raise ValueError("q must be a float32, bfloat16 or float16 [tokens, heads, dim] tensor")

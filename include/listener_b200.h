@@ -538,7 +538,7 @@ int lb_op_w4_matvec(const void* x, int64_t x_ld, int x_dtype, const float* x_sca
  * turns[i] / 2^64): turns uint64 [rotary / 2] is the frequency in turns a position, as a
  * 64-bit fraction.  positions int32 [n_tokens] (positions64 != 0: int64), of any sign.  q, k and the
  * outputs of dtype (LB_F32, LB_BF16, LB_F16), strides in elements, the last dimension contiguous; an output may
- * be its input (with the same strides).  Weights [dim] of weight_dtype: LB_F32 or dtype.  All
+ * be its input (with the same strides), and shares no memory with q, k or the other output otherwise.  Weights [dim] of weight_dtype: LB_F32 or dtype.  All
  * in 32 bits, rounded once.  dim even, at most 1024, rotary even. */
 int lb_op_head_norm_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int heads, const void* k,
                            int64_t k_token_stride, int64_t k_head_stride, int kv_heads, int dtype, int n_tokens,
@@ -572,7 +572,8 @@ int lb_op_sample(const void* logits, int64_t row_stride, int dtype, int rows, in
  * and product in 32 bits, rounded once to out_dtype (LB_F32, LB_BF16, LB_F16); act(g) / g may be 0 where it is below 2^-126.
  * ld_out elements between rows.  x and its rows 16-byte aligned
  * (x_ld times its type's size a multiple of 16 where m > 1), codes 16-byte aligned.
- * *status (may be NULL) gets LB_DEV_WAIT_TIMEOUT if the kernel gave up on a bounded wait: out is then undefined. */
+ * out shares no memory with x.  *status (may be NULL) gets LB_DEV_WAIT_TIMEOUT if the kernel gave up on a bounded wait: out is then
+ * undefined. */
 int lb_op_w4_gated(const void* x, int64_t x_ld, int x_dtype, const float* x_scale, int x_group, int m,
                    const void* codes, const void* w_scale, int group, int ffn, int k, int activation, void* out,
                    int64_t ld_out, int out_dtype, int32_t* status, void* stream);

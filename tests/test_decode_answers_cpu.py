@@ -35,6 +35,42 @@ def test_refusals(lib, name, good, changes):
         assert getattr(lib, name)(*args) == -1, (at, value)
 
 
+Q, K, Y, Z = (i * (P << 8) for i in range(1, 5))  # addresses apart
+
+
+@pytest.mark.parametrize("name,good,changes", [
+    ("lb_op_head_norm_rotary",
+     [Q, 640, 64, 8, Q + 1024, 640, 64, 2, 1, 4, 64, P, 0, P, 64, 0, P, P, 0, 1, 1e-6, Y, 512, 64, Z, 128, 64, None],
+     # an output over an input in part, over the other one's, over the other output
+     [{21: Q + 128}, {21: Q, 22: 512}, {21: Q - 2}, {24: Q}, {24: Q + 1024 + 640 * 2 * 3 + 126}, {21: Q + 1024}, {24: Y + 3 * 1024 + 1022},
+      {24: Y, 25: 512}, {21: Q, 22: 640, 24: Q + 1022}, {2: 0, 21: Q, 22: 640, 23: 0, 24: Q, 26: 0}]),
+    ("lb_op_w4_gated", [Q, 256, 1, None, 0, 4, P, P, 64, 100, 256, 0, Y, 100, 1, None, None],
+     [{12: Q}, {12: Q + 2046}, {12: Q - 799}, {13: 256, 12: Q + 512 - 2}, {13: 256, 12: Q + 256}, {14: 0, 12: Q - 1599}, {5: 1, 12: Q + 511}]),
+])
+def test_refusals_of_outputs_that_share_memory(lib, name, good, changes):
+    for change in changes:
+        args = list(good)
+        for at, value in change.items():
+            args[at] = value
+        assert getattr(lib, name)(*args) == -1, change
+
+
+@pytest.mark.parametrize("name,good,changes", [
+    ("lb_op_head_norm_rotary",
+     [Q, 512, 64, 8, K, 128, 64, 2, 1, 1, 64, P, 0, P, 64, 0, P, P, 0, 1, 1e-6, Y, 512, 64, Z, 128, 64, None],
+     [(0, None), (3, 0), (4, None), (7, -1), (8, 2), (9, 0), (10, 0), (10, 63), (10, 1026), (11, None), (13, None), (14, 66), (14, 31),
+      (18, 2), (20, -1.0), (20, math.nan), (21, None), (24, None)]),
+    ("lb_op_w4_gated", [Q, 256, 1, None, 0, 4, P, P, 64, 100, 256, 0, Y, 100, 1, None, None],
+     [(0, None), (0, Q + 2), (1, 255), (1, 257), (2, 0), (2, 4), (3, P), (4, 128), (5, 0), (6, None), (6, P + 8), (7, None), (8, 16), (8, 256),
+      (9, 0), (10, 0), (10, 100), (11, 2), (11, -1), (12, None), (13, 99), (14, 2), (14, 4)]),
+])
+def test_refusals_of_calls_that_share_no_memory(lib, name, good, changes):
+    for at, value in changes:
+        args = list(good)
+        args[at] = value
+        assert getattr(lib, name)(*args) == -1, (at, value)
+
+
 def test_capacity(lib):
     assert lib.lb_op_sample(P, 300000, 1, 2, 262145, P, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None, None) == -4
 

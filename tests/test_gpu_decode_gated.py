@@ -214,3 +214,16 @@ def test_refusals(ops):
                 lambda: ops.w4_gated(h, w, out=torch.zeros(1, 64, device="cuda").expand(4, 64))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_an_output_over_x_is_refused(ops):
+    from gemma4_omni_b200._lib import ListenerLibError
+    x, _, w = inputs(ops, 9, 256, 128, 64, BF16, 0, 9)
+    want = ops.w4_gated(x, w)
+    room = torch.zeros(9, 512, dtype=BF16, device="cuda")
+    room[:, :256] = x
+    for bad in (room[:, :128], room[:, 200:328], room.view(-1)[:9 * 128].view(9, 128), room.view(F32)[:, 64:192]):
+        with pytest.raises(ListenerLibError):
+            ops.w4_gated(room[:, :256], w, out=bad)
+    assert torch.equal(room[:, :256], x)
+    assert torch.equal(ops.w4_gated(room[:, :256], w, out=room[:, 256:384]), want)

@@ -173,3 +173,83 @@ def test_graph_streams_and_refusals(ops):
                 lambda: setattr(r, "turns", r.turns[:3])):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_outputs_that_share_memory_are_refused(ops):
+    """Parts of one buffer: beside one another they may be inputs and outputs in any way, over one another only an input's own output."""
+    r = ops.Rotary.create(64)
+    at = torch.arange(5, device="cuda", dtype=torch.int32)
+    room = torch.randn(5, 20, 64, device="cuda").to(BF16)
+    q, k = room[:, :6], room[:, 6:8]
+    want = ops.head_norm_rotary(q, k, at, r)
+    before = room.clone()
+    for bad in (dict(q_out=room[:, 1:7]), dict(q_out=room[:, 2:8]), dict(k_out=room[:, 5:7]), dict(k_out=room[:, :2]), dict(q_out=room[:, 7:13]),
+                dict(q_out=room[:, 8:14], k_out=room[:, 13:15]), dict(q_out=room.view(5, 10, 128)[:, 2:8, :64]),
+                dict(q_out=room.view(-1)[32:32 + 5 * 6 * 64].view(5, 6, 64))):
+        with pytest.raises(ValueError):
+            ops.head_norm_rotary(q, k, at, r, **bad)
+    with pytest.raises(ValueError):
+        ops.head_norm_rotary(q, q, at, r, q_out=q)
+    assert torch.equal(room, before)
+    for good in (dict(q_out=room[:, 8:14], k_out=room[:, 14:16]), dict(q_out=room.view(5, 10, 128)[:, 4:, :64], k_out=room[:, 9:12:2]), dict(k_out=k),
+                 dict(q_out=q), dict(q_out=q, k_out=k)):
+        room.copy_(before)
+        got = ops.head_norm_rotary(q, k, at, r, **good)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_outputs_that_share_memory_are_refused(ops):
+    """Parts of one buffer: beside one another they may be inputs and outputs in any way, over one another only an input's own output."""
+    from gemma4_omni_b200._lib import ListenerLibError
+    r = ops.Rotary.create(64)
+    at = torch.arange(5, device="cuda", dtype=torch.int32)
+    room = torch.randn(5, 20, 64, device="cuda").to(BF16)
+    q, k = room[:, :6], room[:, 6:8]
+    want = ops.head_norm_rotary(q, k, at, r)
+    before = room.clone()
+    for bad in (dict(q_out=room[:, 1:7]), dict(q_out=room[:, 2:8]), dict(k_out=room[:, 5:7]), dict(k_out=room[:, :2]), dict(q_out=room[:, 7:13]),
+                dict(q_out=room[:, 8:14], k_out=room[:, 13:15]), dict(q_out=room.view(5, 10, 128)[:, 2:8, :64]),
+                dict(q_out=room.view(-1)[32:32 + 5 * 6 * 64].view(5, 6, 64))):
+        with pytest.raises(ListenerLibError):
+            ops.head_norm_rotary(q, k, at, r, **bad)
+    with pytest.raises(ListenerLibError):
+        ops.head_norm_rotary(q, q, at, r, q_out=q)
+    assert torch.equal(room, before)
+    for good in (dict(q_out=room[:, 8:14], k_out=room[:, 14:16]), dict(q_out=room.view(5, 10, 128)[:, 4:, :64], k_out=room[:, 9:12:2]), dict(k_out=k),
+                 dict(q_out=q), dict(q_out=q, k_out=k)):
+        room.copy_(before)
+        got = ops.head_norm_rotary(q, k, at, r, **good)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_layouts_in_one_buffer(ops):
+    """Inputs and outputs at random places of one buffer, with one step between tokens: refused where any value is shared, right otherwise.
+    (Rows of another alignment take another kernel: twice the bound above with |a| + |b| <= 2 sqrt(8), less than 2^-15.)"""
+    import random
+    from gemma4_omni_b200._lib import ListenerLibError
+    rng, r, dim = random.Random(6), ops.Rotary.create(8), 8
+    room = torch.randn(4000, device="cuda")
+    numbers = torch.arange(4000)
+    at = torch.arange(3, device="cuda", dtype=torch.int32)
+    done = {True: 0, False: 0}
+    for _ in range(400):
+        token = rng.choice([40, 64, 100, 300])
+        hq, hk = rng.randint(1, 4), rng.randint(1, 2)
+        places = []
+        for heads in (hq, hk, hq, hk):
+            head = rng.choice([8, 8, 12, 16, 24])
+            places.append(((3, heads, dim), (token, head, 1), rng.randint(0, 300)))
+        if token < max(p[1][1] * (p[0][1] - 1) + dim for p in places):
+            continue
+        sets = [set(numbers.as_strided(*p).flatten().tolist()) for p in places]
+        bad = bool(sets[2] & (sets[0] | sets[1]) or sets[3] & (sets[0] | sets[1] | sets[2]))
+        q, k, q_out, k_out = (room.as_strided(*p) for p in places)
+        want = ops.head_norm_rotary(q.clone(), k.clone(), at, r)
+        if bad:
+            with pytest.raises((ValueError, ListenerLibError)):  # (the first for one that begins where its input does, with other strides)
+                ops.head_norm_rotary(q, k, at, r, q_out=q_out, k_out=k_out)
+        else:
+            ops.head_norm_rotary(q, k, at, r, q_out=q_out, k_out=k_out)
+            assert (q_out - want[0]).abs().max() <= 2.0 ** -15 and (k_out - want[1]).abs().max() <= 2.0 ** -15
+        done[bad] += 1
+    assert min(done.values()) > 30
