@@ -3,10 +3,10 @@
 //   (a, b) -> (a cos t - b sin t, b cos t + a sin t),   t = position * frequency_i
 // for the first `rotary` values of a head, paired as halves (i, i + rotary / 2) or neighbours (2 i, 2 i + 1).
 //
-// Angles are exact up to their last rounding at any position: a frequency is a 64-bit fraction of a turn, its
-// product with the position modulo 2^64 is the fraction of a turn that is left, and no bit of it is lost before the
-// quadrant is taken off.  sin and cos of what is left (at most pi / 4) are their Taylor series up to x^9 and x^10
-// (first terms left out: 2e-9 and 2e-10).
+// Angles: a frequency is a fraction of a turn, rounded to 2^-64, and its product with the position modulo 2^64 is the fraction of a turn
+// that is left, exactly.  So an angle is off by at most 2^-65 turns times the position (4e-10 at 2^31, 2e-7 at 2^40, 2e-4 at 2^50) and
+// 2^-32 turns (1.5e-9), as the upper half of its bits goes on to the sines.  sin and cos of what is left of a quadrant (at most pi / 4) are
+// their Taylor series up to x^9 and x^10 (first terms left out: 2e-9 and 2e-10).
 //
 // The pass is bound by its bytes: a value is read once, kept in registers through sum, norm and
 // rotation (all in 32 bits) and rounded once.  A warp takes a token, turns its angles into sines

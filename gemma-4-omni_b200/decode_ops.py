@@ -531,8 +531,8 @@ def _fraction(radians: decimal.Decimal) -> int:
 class Rotary:
     """The frequencies of a position rotation of heads of ``dim`` values.
 
-    ``turns`` int64 [rotary_dim / 2]: frequencies in turns a position, as 64-bit fractions, so that the angle of any
-    position is exact.  ``pairs``: "halves" pairs value i with i + rotary_dim / 2, "neighbours" 2 i with 2 i + 1;
+    ``turns`` int64 [rotary_dim / 2]: frequencies in turns a position, as 64-bit fractions, of which no whole turns are left
+    over; an angle is good to 2e-9 radians and 2e-19 times the position (2e-7 at 2^40).  ``pairs``: "halves" pairs value i with i + rotary_dim / 2, "neighbours" 2 i with 2 i + 1;
     values from rotary_dim on are not rotated."""
 
     turns = _exchangeable("turns", torch.int64, lambda r: (r.rotary_dim // 2,), 8)

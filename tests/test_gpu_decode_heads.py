@@ -116,6 +116,25 @@ def test_values_of_the_ends(ops):
     assert torch.equal(y[1], ops.head_norm_rotary(x[1:2], None, at[1:2], r, norm=False)[0][0])
 
 
+def test_far_positions_against_the_frequencies(ops):
+    """The angle's own bound: 2^-65 turns times the position for the frequency's rounding, 2^-32 turns for the bits that are dropped; beside it
+    six roundings of 2^-24 (sines 3, the products and sums)."""
+    import decimal
+    pi = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803")
+    at = [12345, (1 << 31) - 1, -(1 << 31), (1 << 40) + 3, -(1 << 44) - 7, (1 << 50) + 11]
+    with decimal.localcontext() as c:
+        c.prec = 80
+        angles = [[float((p * decimal.Decimal(10000) ** (decimal.Decimal(-2 * i) / 64)) % (2 * pi)) for i in range(32)] for p in at]
+    angle = torch.tensor(angles, dtype=torch.float64, device="cuda")
+    x = torch.randn(len(at), 1, 64, generator=gen(8), device="cuda")
+    y, _ = ops.head_norm_rotary(x, None, torch.tensor(at, device="cuda"), ops.Rotary.create(64), norm=False)
+    a, b = x[:, 0, :32].double(), x[:, 0, 32:].double()
+    ref = torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], 1)
+    off = 2 * math.pi * (torch.tensor(at, dtype=torch.float64, device="cuda").abs() * 2.0 ** -65 + 2.0 ** -32)[:, None] + 6 * 2.0 ** -24
+    size = (a.abs() + b.abs()).repeat(1, 2)
+    assert ((y[:, 0].double() - ref).abs() <= off * size).all()
+
+
 def test_rotation_keeps_scores_of_equal_distances(ops):
     """q at p + d and k at p have the same product for every p: 2 dim products of values good to some 2^-22."""
     g = gen(5)
