@@ -18,14 +18,15 @@
 // Few tokens: the tiles of outputs are fewer than the SMs, so K is dealt out to the CTAs of a cluster.  Each sends its partial
 // sums to the CTA that finishes the token (stores over the cluster), which adds them up in the order of K.
 //
-// Measured, 1536 x 6144 in groups of 128 (in graphs): 2 rows of e4m3 11 us (9.8 MB at 0.9 TB/s: a chain of launch, first loads, six
-// blocks of some 0.67 us, in which the widening warps set the pace, and the join), 128 rows 14, 499 rows 27, 4096 rows 136 in bf16 (1134
-// TFLOP/s, 68 % of the measured rate; 164 us where the power limit holds the clocks down), 144 in fp16, 151 in int8, 173 in
-// e4m3.  What bounds the large ones is the work beside the MMAs: of some 5 thousand instructions for a tile of 128 tokens and a block
-// of K the widening takes a third, sums a sixth and results a tenth.  A tile's results are not covered by the next one's MMAs, which
-// stop two units ahead.  Groups of 64 and 32 take two and four times the sums: 197 and 326 us.
-// On the way (4096 rows): one lane issuing all MMAs 254 us, a warp that walks together 214, two widening warpgroups
-// instead of one 192, a warp a side for the MMAs 164 (the waits of one were as long as its MMAs), results without a loop 145.
+// Measured, 1536 x 6144 in groups of 128 (calls in one graph, weights out of L2): 2 rows of e4m3 12.1 us (9.8 MB at 0.8 TB/s: a
+// chain of launch, first loads, six blocks of some 0.67 us, in which the widening warps set the pace, and the join; weights in L2
+// 11.2), of bf16 10.8; bf16: 128 rows 15.4, 499 rows 28, 4096 rows 143 (1081 TFLOP/s, 65 % of the measured rate; 162 us where the
+// power limit holds the clocks down); 4096 rows in fp16 153, int8 156, e4m3 178, with x's scales in groups of 128 213 and 206.
+// What bounds the large ones is the work beside the MMAs: of some 5 thousand instructions for a tile of 128 tokens and a block of K
+// the widening takes a third, sums a sixth and results a tenth.  A tile's results are not covered by the next one's MMAs, which
+// stop two units ahead.  Groups of 64 and 32 take two and four times the sums: 204 and 327 us. On the way (4096 rows, the steps'
+// own times): one lane issuing all MMAs 254 us, a warp that walks together 214, two widening warpgroups instead of one 192, a warp
+// a side for the MMAs 164 (the waits of one were as long as its MMAs), results without a loop 145.
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 #include "kernels.h"
@@ -70,9 +71,9 @@ struct Shape {
   static constexpr int kSideD = NT > 64 ? 1 : 2, kD = 2 * kSideD;  // accumulators in the tensor memory, of a side and in all
   static constexpr int kCols = NT / 2;                        // tokens of an adding warpgroup
   static constexpr int kSteps = kWide ? 16 : 32;              // k of an MMA
-  // Registers a thread by role.  Wide tiles of 16-bit operands are best with 40 and 176 (4096 x 1536 x 6144: 136 us; 48 and 168: 144);
-  // the widening of 8-bit ones holds more constants (e4m3 173 instead of 180), and narrow tiles wait for the widening (2 rows 9.9
-  // instead of 10.4).
+  // Registers a thread by role.  Wide tiles of 16-bit operands are best with 40 and 176 (4096 x 1536 x 6144 in bf16: 6 % less than with 48
+  // and 168); the widening of 8-bit ones holds more constants (e4m3: 4 % less the other way), and narrow tiles wait for the widening (2 rows:
+  // 5 % less).
   static constexpr bool kMoreSums = kWide && NT > 64;
   static constexpr int kLoadRegs = 40, kWidenRegs = kMoreSums ? 40 : 48, kAddRegs = kMoreSums ? 176 : 168;
   static_assert(kD * NT <= kAColumn, "tensor memory");
@@ -815,10 +816,11 @@ extern "C" int lb_op_w4_gated(const void* x, int64_t x_ld, int x_dtype, const fl
               activation, 0, 0, 0};
   a.o_tiles = (ffn + kBlockO - 1) / kBlockO;
   a.k_blocks = (k + kBlockK - 1) / kBlockK;
-  // The width of a tile and the dealing out of K by an estimate of the time in tenths of a microsecond: a wave of tiles takes 4 us
-  // and for each block of K 0.67, 0.7, 0.85 or 1 at 32, 64, 96 or 128 tokens (1536 x 6144: 128 rows take 18 us as 48 tiles of 128
-  // tokens, 14 as 96 of 64).  K is dealt out where all clusters fit the GPU at once: 2
-  // rows of 1536 x 6144 take 14 us whole, 10 in clusters of two, but 15 in clusters of three, not all of which fit.
+  // The width of a tile and the dealing out of K by an estimate of the time in tenths of a microsecond: a wave of tiles takes 4
+  // us and for each block of K 0.67, 0.7, 0.85 or 1 at 32, 64, 96 or 128 tokens (1536 x 6144 in groups of 128, bf16, where all
+  // five were measured: 128 rows as 48 tiles of 128 tokens take 1.3 times as long as 96 of 64; finer groups and 8-bit x cost more at
+  // each width, which the estimate leaves out).  K is dealt out where all clusters fit the GPU at once: 2 rows of 1536 x
+  // 6144 take 1.4 times as long whole as in clusters of two, and 1.5 times in clusters of three, not all of which fit.
   int nt = 0, splits = 1;
   long long best = 0;
   for (const int width : {32, 64, 96, 128}) {

@@ -3,20 +3,23 @@
 //   (a, b) -> (a cos t - b sin t, b cos t + a sin t),   t = position * frequency_i
 // for the first `rotary` values of a head, paired as halves (i, i + rotary / 2) or neighbours (2 i, 2 i + 1).
 //
-// Angles: a frequency is a fraction of a turn, rounded to 2^-64, and its product with the position modulo 2^64 is the fraction of a turn
-// that is left, exactly.  So an angle is off by at most 2^-65 turns times the position (4e-10 at 2^31, 2e-7 at 2^40, 2e-4 at 2^50) and
-// 2^-32 turns (1.5e-9), as the upper half of its bits goes on to the sines.  sin and cos of what is left of a quadrant (at most pi / 4) are
-// their Taylor series up to x^9 and x^10 (first terms left out: 2e-9 and 2e-10).
+// Angles: a frequency is a fraction of a turn, rounded to 2^-64, and its product with the position modulo 2^64 is the fraction of a
+// turn that is left, exactly.  So an angle is off by at most 2^-65 turns times the position (4e-10 at 2^31, 2e-7 at 2^40, 2e-4 at
+// 2^50) and 2^-32 turns (1.5e-9), as the upper half of its bits goes on to the sines.  sin and cos of what is left of a quadrant
+// (at most pi / 4) are their Taylor series up to x^9 and x^10 (first terms left out: 2e-9 and 2e-10).
 //
 // The pass is bound by its bytes: a value is read once, kept in registers through sum, norm and
 // rotation (all in 32 bits) and rounded once.  A warp takes a token, turns its angles into sines
 // once and walks over the token's heads; a head of dim values takes dim / 8 lanes, each with four neighbours
 // and the four that they are paired with.  Where tokens are few, a token's heads are dealt out to several warps.
 //
-// 16384 tokens of 32 + 8 heads of 128 in bf16 (336 MB) take 60 us, 5.6 TB/s, 85 % of the copy rate, with four steps under way in each of 32
-// warps an SM (two: 66 us; one: 78).  The usual heads have kernels of their own, without branches for the other pairs, parts
-// and norms: instructions bind (with the branches 75 us).  Two tokens of 9 heads of 256 take 4.2 us in a graph, nearly all of it the
-// launch.
+// 16384 tokens of 32 + 8 heads of 128 in bf16 (336 MB) take 58 us, 5.8 TB/s, 88 % of the copy rate, with four steps under way in
+// each of 32 warps an SM (two: 66 us; one: 78).  The usual heads have kernels of their own, without branches for the other pairs,
+// parts and norms (a third fewer instructions; with the branches 75 us).  What is left is waiting for loads (6.5 of 13 cycles
+// between a warp's instructions).  8 + 1 heads of 256 (151 MB) take 36 us, 4.2 TB/s: these kernels hold 16 or, at 256, 68 bytes of
+// registers in local memory.  Values of 32 bits, a quarter rotated in neighbours, 3001 tokens of 16 + 4 heads of 64 (31 MB): 11.5
+// us, 2.7 TB/s, some 20 warps an SM with two loads ahead each. The kernel for any size takes 81 us for 8192 tokens of 8 + 1 heads
+// of 512 (1.9 TB/s).  Two tokens of 9 heads of 256 take 2.8 us among others in a graph, nearly all of it the launch.
 #include "../../include/listener_b200.h"
 #include "common.cuh"
 #include "rows.h"

@@ -19,11 +19,13 @@
 // so that every later pass goes over that alone: for top-p the sum of all masses and a look at a few distances come first, and
 // only what lies above the distance behind the cut is divided into bins.
 //
-// Measured (in graphs): one row of 131072 with top-k 64 and top-p 14.5 us, a chain of loads, four barriers of the cluster
-// and 128 tokens that are ranked; 250 rows of 131072 in 32 bits by a share of 0.9 (9 thousand tokens kept a row) 264 us, 0.5 TB/s;
-// 1000 rows of 32003 by min-p 70 us.  Bound by instructions and barriers: some 45 instructions a token for its mass and the sums
-// (11 of them in 64 bits), as many again for the loads, the moves and the bins, and 16 warps that wait for one another. Sorting
-// or ranking fewer tokens in one CTA holds up the other seven of a row: 512 sorted took 12 thousand cycles, 128 ranked take 3.
+// Measured (calls in one graph, logits out of L2): one row of 131072 with top-k 64 and top-p 13.1 us, a chain of loads, four
+// barriers of the cluster and 128 tokens that are ranked; 250 rows of 131072 in 32 bits by a share of 0.9 (9 thousand tokens kept a
+// row) 260 us, 0.5 TB/s, with top-k 50 too 122, unfiltered 102, greedy 58 (2.3 TB/s); 1000 rows of 32003 by min-p 68 us.  Beyond
+// 131072 tokens a CTA holds twice as many and an SM one CTA instead of two: 125 rows of 262144 in bf16 by that share 401 us (250 of
+// 131072: 275), one row as above 17.2.  Bound by instructions and barriers: some 45 instructions a token for its mass and the sums
+// (11 of them in 64 bits), as many again for the loads, the moves and the bins, and 16 warps that wait for one another. Sorting or
+// ranking fewer tokens in one CTA holds up the other seven of a row: 512 sorted took 12 thousand cycles, 128 ranked take 3.
 #include <cfloat>
 #include <cooperative_groups.h>
 
@@ -47,7 +49,8 @@ constexpr int kTop = 45;              // log2 of the largest mass
 constexpr int kPowers = 128;
 constexpr float kMaxHeat = 1e30f;     // so that 47 octaves stay inside the 32-bit numbers
 constexpr unsigned long long kNone = ~0ull;
-// Distances to the maximum, in units of T, between which a share's cut is looked for first.
+// Distances to the maximum, in units of T, between which a share's cut is looked for first.  Where it lies nearer or farther the bins
+// start at the maximum or reach 32 units down; the result is the same, more tokens are put into bins.
 constexpr int kZones = 4;
 __host__ __device__ constexpr float zone_end(int z) { return z == 0 ? 4.0f : z == 1 ? 8.0f : z == 2 ? 11.0f : 14.0f; }
 

@@ -119,7 +119,8 @@ class DecoderBlock:
 
 
 class DecoderHead:
-    """The end of a decoder: norm, the vocabulary's product, and the draw of a token for each row.
+    """The end of a decoder: norm, the vocabulary's product, and the draw of a token for each row.  The normed rows are e4m3 with a
+    scale a row (``rms_norm8``), as before a block's products: logits of 16-bit rows are the caller's own ``w4_matvec``.
     ``norm`` f32 [hidden], ``vocab`` [vocab, hidden] as ``Int4Weight``."""
 
     def __init__(self, norm: torch.Tensor, vocab: ops.Int4Weight, *, rms_eps: float = 1e-6):
