@@ -538,9 +538,10 @@ int lb_op_w4_matvec(const void* x, int64_t x_ld, int x_dtype, const float* x_sca
  * turns[i] / 2^64): turns uint64 [rotary / 2] is the frequency in turns a position, as a
  * 64-bit fraction.  positions int32 [n_tokens] (positions64 != 0: int64), of any sign.  q, k and the
  * outputs of dtype (LB_F32, LB_BF16, LB_F16), strides in elements, the last dimension contiguous; an output may
- * be its input (with the same strides), and shares no memory with q, k or the other output otherwise.  Weights [dim] of weight_dtype: LB_F32 or dtype.  All
- * in 32 bits, rounded once; so are the squares: values beyond some 2^59 have the mean's root infinite and become 0, and below 2^-63 they
- * count as 0 in it.  dim even, at most 1024, rotary even. */
+ * be its input (with the same strides), and shares no memory with q, k or the other output otherwise.  Weights
+ * [dim] of weight_dtype: LB_F32 or dtype.  All in 32 bits, rounded once; so are the squares: heads with values
+ * beyond some 2^59 overflow there (0 or NaN comes out), and values below 2^-63 do not count in the mean.
+ * dim even, at most 1024, rotary even. */
 int lb_op_head_norm_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int heads, const void* k,
                            int64_t k_token_stride, int64_t k_head_stride, int kv_heads, int dtype, int n_tokens,
                            int dim, const void* positions, int positions64, const uint64_t* turns, int rotary,
